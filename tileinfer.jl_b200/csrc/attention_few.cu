@@ -1,0 +1,433 @@
+// Attention of a few new tokens of every sequence over the paged cache, in bfloat16: the step that tests a drafted run. The new tokens'
+// keys and values are in the cache already; token i of a sequence's T stands at position L - T + i, and sees the keys up to itself (and, with a
+// window, the window's last ones only).
+//
+//   out[i, h] = sum_j softmax_j(scale q[i, h] k[j]) v[j], over the visible j.
+//
+// Bound by reading the cache once, so the T x (query heads per KV head) rows that share a KV head are the rows of the MMA tiles (slabs of 16,
+// 32 or 64), and the work is shared out by length: the units, 64-key tiles of all (sequence, KV head, slab), are numbered in that order, and every
+// resident block takes an equal run of them, whatever the sequences' lengths. A block that does a whole item writes its rows; the parts of an
+// item that several blocks share are left in 32-bit (maximum, sum, unnormalised output) and joined by a second kernel in ascending order.
+//
+// Four warps share a tile out as MT groups of 16 rows x 4 / MT groups of keys. Scores, the running maximum and sum, and the output stand in
+// 32-bit; P is rounded to bfloat16 as the operand of P V alone (its sum is not), O once. A tile's keys and values beyond the sequence's end or
+// before the first visible key may hold anything: their scores are replaced and their values zeroed.
+#include "common.cuh"
+#include "mma_util.cuh"
+
+#define AF_PAGE 64
+#define AF_THREADS 128
+#define AF_MAX_SEQS 1024
+
+struct FewShape {
+    int T, L, first, t0, tiles, slabs;                       // new tokens, length, first visible key, first tile, tiles, slabs of rows
+};
+__device__ __forceinline__ FewShape few_shape(int T, int L, int window, int group, int M) {
+    FewShape s;
+    s.T = T; s.L = L;
+    s.first = window > 0 ? max(0, L - T - window + 1) : 0;
+    s.t0 = s.first / AF_PAGE;
+    s.tiles = T > 0 && L > 0 ? (L + AF_PAGE - 1) / AF_PAGE - s.t0 : 0;
+    s.slabs = (T * group + M - 1) / M;
+    return s;
+}
+// The blocks' runs: block c of G takes the units [U c / G, U (c + 1) / G), none of them empty (G at most U).
+__device__ __forceinline__ long long few_low(long long U, int c, int G) { return U * c / G; }
+__device__ __forceinline__ int few_owner(long long U, long long u, int G) { return (int)(((u + 1) * G - 1) / U); }
+
+// The joining kernel's part of the work space: [0] units in all, [1 + b] units of the sequences before b.
+template <int D> struct FewSmem {
+    static constexpr int STAGES = D <= 128 ? 3 : 2;
+    static constexpr int TILE = AF_PAGE * D;
+    static constexpr size_t BYTES = (size_t)STAGES * 2 * TILE * sizeof(bf16);
+};
+
+template <int D, int MT>
+__global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_kernel(bf16* out, const bf16* q, const bf16* k_cache, const bf16* v_cache,
+                                                                                     const int* block_table, int table_stride, const int* seq_slots,
+                                                                                     const int* cu, const int* kv_lens, float* ws_o, float* ws_ml,
+                                                                                     long long* units, float scale_log2e, int B, int nq, int nkv, int window) {
+    constexpr int M = 16 * MT, WK = 4 / MT, KS = D / 16, NT = D / 8, CPR = D / 8;
+    typedef FewSmem<D> SM;
+    extern __shared__ __align__(128) unsigned char af_smem[];
+    __shared__ long long s_units[AF_MAX_SEQS + 1];
+    __shared__ long long s_scan[AF_THREADS / 32];
+    __shared__ float s_ml[WK][M][2];
+    bf16* ring = reinterpret_cast<bf16*>(af_smem);
+    const int group = nq / nkv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int wr = warp % MT, wk = warp / MT;
+
+    // Units before every sequence.
+    long long carry = 0;
+    for (int b0 = 0; b0 < B; b0 += AF_THREADS) {
+        const int b = b0 + threadIdx.x;
+        long long v = 0;
+        if (b < B) {
+            const FewShape s = few_shape(__ldcg(cu + b + 1) - __ldcg(cu + b), __ldcg(kv_lens + b), window, group, M);
+            v = (long long)s.tiles * s.slabs * nkv;
+        }
+        const long long own = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        __syncthreads();
+        if (lane == 31) s_scan[warp] = v;
+        __syncthreads();
+        long long before = carry;
+        for (int w = 0; w < AF_THREADS / 32; ++w) {
+            if (w < warp) before += s_scan[w];
+            carry += s_scan[w];
+        }
+        if (b < B) s_units[b] = before + v - own;
+    }
+    if (threadIdx.x == 0) s_units[B] = carry;
+    __syncthreads();
+    const long long U = s_units[B];
+    const int G = (int)min((long long)gridDim.x, U);
+    if ((int)blockIdx.x >= max(G, 1)) return;                // more blocks than units
+    const long long lo = G > 0 ? few_low(U, blockIdx.x, G) : 0, hi = G > 0 ? few_low(U, blockIdx.x + 1, G) : 0;
+
+    struct Place {
+        FewShape s;
+        int b, kvh, slab, tile;                              // tile counts from the first visible one
+    };
+    auto locate = [&](long long u) {
+        Place p;
+        int a = 0, z = B;                                    // the last sequence with units before it <= u and units of its own
+        while (z - a > 1) {
+            const int mid = (a + z) >> 1;
+            if (s_units[mid] <= u) a = mid; else z = mid;
+        }
+        p.b = a;
+        p.s = few_shape(__ldcg(cu + a + 1) - __ldcg(cu + a), __ldcg(kv_lens + a), window, group, M);
+        const int v = (int)(u - s_units[a]), item = v / p.s.tiles;
+        p.tile = v - item * p.s.tiles;
+        p.kvh = item / p.s.slabs;
+        p.slab = item - p.kvh * p.s.slabs;
+        return p;
+    };
+
+    // What is asked for next: its place, and its page one tile ahead of its copies.
+    bool waited = false;
+    auto wait_once = [&] {
+        if (!waited) { pdl_enter(); waited = true; }
+    };
+    long long next_u = lo;
+    Place next{};
+    int next_page = 0;
+    const int* next_table = nullptr;
+    auto enter = [&] {
+        if (next_u < hi) {
+            next = locate(next_u);
+            next_table = block_table + (size_t)__ldcg(seq_slots + next.b) * table_stride + next.s.t0;
+            next_page = __ldcg(next_table + next.tile);
+        }
+    };
+    enter();
+    int fill = 0;
+    auto issue = [&] {
+        if (next_u < hi) {
+            // Tiles with new keys were written by the kernel before this one; the others stand since earlier steps.
+            if ((next.s.t0 + next.tile + 1) * AF_PAGE > next.s.L - next.s.T) wait_once();
+            const size_t base = ((size_t)next_page * nkv + next.kvh) * SM::TILE;
+            bf16* dst = ring + (size_t)fill * 2 * SM::TILE;
+            for (int c = threadIdx.x; c < AF_PAGE * CPR; c += AF_THREADS) {
+                const int row = c / CPR, cc = c % CPR;
+                const unsigned at = (row * CPR + swz<D>(row, cc)) * 8;
+                cp_async16(smem_u32(dst + at), k_cache + base + (size_t)c * 8);
+                cp_async16(smem_u32(dst + SM::TILE + at), v_cache + base + (size_t)c * 8);
+            }
+            ++next_u;
+            if (++next.tile == next.s.tiles) enter();
+            else if (next_u < hi) next_page = __ldcg(next_table + next.tile);
+        }
+        fill = fill == SM::STAGES - 1 ? 0 : fill + 1;
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < SM::STAGES - 1; ++s) issue();
+    wait_once();
+    if (blockIdx.x == 0)                                     // for the joining kernel
+        for (int b = threadIdx.x; b <= B; b += AF_THREADS) units[b] = s_units[b];
+
+    int stage = 0;
+    long long u = lo;
+    while (u < hi) {
+        // One segment: the tiles of one item that lie in this block's run.
+        const Place at = locate(u);
+        const FewShape& s = at.s;
+        const long long seg_end = min(hi, u + (s.tiles - at.tile));
+        const int rows = s.T * group, first_token = __ldcg(cu + at.b);
+        int pos[2], low[2];
+        const bf16* qrow[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = at.slab * M + wr * 16 + g + 8 * h, i = r / group;
+            const bool real = r < rows;
+            pos[h] = real ? s.L - s.T + i : -1;
+            low[h] = window > 0 ? max(0, pos[h] - window + 1) : 0;
+            qrow[h] = real ? q + ((size_t)(first_token + i) * nq + (size_t)at.kvh * group + (r - i * group)) * D : nullptr;
+        }
+        unsigned qf[KS][4];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = ks * 16 + 2 * t;
+            qf[ks][0] = qrow[0] != nullptr ? __ldcg(reinterpret_cast<const unsigned*>(qrow[0] + d)) : 0u;
+            qf[ks][1] = qrow[1] != nullptr ? __ldcg(reinterpret_cast<const unsigned*>(qrow[1] + d)) : 0u;
+            qf[ks][2] = qrow[0] != nullptr ? __ldcg(reinterpret_cast<const unsigned*>(qrow[0] + d + 8)) : 0u;
+            qf[ks][3] = qrow[1] != nullptr ? __ldcg(reinterpret_cast<const unsigned*>(qrow[1] + d + 8)) : 0u;
+        }
+        float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+
+        int tile = s.t0 + at.tile;
+        for (; u < seg_end; ++u, ++tile) {
+            cp_async_wait<SM::STAGES - 2>();
+            __syncthreads();
+            issue();                                         // into the stage that the tile before has left
+            bf16* kt = ring + (size_t)stage * 2 * SM::TILE;
+            bf16* vt = kt + SM::TILE;
+            stage = stage == SM::STAGES - 1 ? 0 : stage + 1;
+            const int key_base = tile * AF_PAGE;
+            if (key_base + AF_PAGE > s.L || key_base < s.first) {          // values that nobody sees may be infinite or NaN: 0 x those is NaN
+                for (int c = threadIdx.x; c < AF_PAGE * CPR; c += AF_THREADS) {
+                    const int row = c / CPR, key = key_base + row;
+                    if (key >= s.L || key < s.first) *reinterpret_cast<uint4*>(vt + c * 8) = make_uint4(0, 0, 0, 0);
+                }
+                __syncthreads();
+            }
+            float sc[2 * MT][4];
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
+            const int mat = lane >> 3, r8 = lane & 7;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int nb = 0; nb < MT; ++nb) {
+                    const int row = (wk * MT + nb) * 16 + (mat >> 1) * 8 + r8;
+                    unsigned kb[4];
+                    ldmatrix_x4(kb, smem_u32(kt + (row * CPR + swz<D>(row, 2 * ks + (mat & 1))) * 8));
+                    mma16816(sc[2 * nb], qf[ks], kb[0], kb[1]);
+                    mma16816(sc[2 * nb + 1], qf[ks], kb[2], kb[3]);
+                }
+            float mx0 = -INFINITY, mx1 = -INFINITY;
+            const bool edge = key_base + AF_PAGE > s.L - s.T + 1 || (window > 0 && key_base < s.L - window);
+            const int key0 = key_base + wk * MT * 16 + 2 * t;
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int key = key0 + 8 * i + j;
+                    const bool ok0 = !edge || (key <= pos[0] && key >= low[0]), ok1 = !edge || (key <= pos[1] && key >= low[1]);
+                    sc[i][j] = ok0 ? sc[i][j] * scale_log2e : -INFINITY;
+                    sc[i][2 + j] = ok1 ? sc[i][2 + j] * scale_log2e : -INFINITY;
+                    mx0 = fmaxf(mx0, sc[i][j]);
+                    mx1 = fmaxf(mx1, sc[i][2 + j]);
+                }
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+            const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+            const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
+            const float c0 = exp2f(m0 - b0), c1 = exp2f(m1 - b1);
+            m0 = n0; m1 = n1;
+            l0 *= c0; l1 *= c1;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) { o[i][0] *= c0; o[i][1] *= c0; o[i][2] *= c1; o[i][3] *= c1; }
+#pragma unroll
+            for (int nb = 0; nb < MT; ++nb) {
+                unsigned pf[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float* x = sc[2 * nb + h];
+                    x[0] = exp2f(x[0] - b0); x[1] = exp2f(x[1] - b0); x[2] = exp2f(x[2] - b1); x[3] = exp2f(x[3] - b1);
+                    l0 += x[0] + x[1];
+                    l1 += x[2] + x[3];
+                    pf[2 * h] = pack_bf16(x[0], x[1]);
+                    pf[2 * h + 1] = pack_bf16(x[2], x[3]);
+                }
+                const int row = (wk * MT + nb) * 16 + (mat & 1) * 8 + r8;
+#pragma unroll
+                for (int c = 0; c < NT; c += 2) {
+                    unsigned vb[4];
+                    ldmatrix_x4_trans(vb, smem_u32(vt + (row * CPR + swz<D>(row, c + (mat >> 1))) * 8));
+                    mma16816(o[c], pf, vb[0], vb[1]);
+                    mma16816(o[c + 1], pf, vb[2], vb[3]);
+                }
+            }
+        }
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+
+        // The warps' shares of the keys joined, in the stage that the segment's last tile leaves (it is filled again only after the next
+        // tile's barrier): row r of key group k at [k][r], its columns turned by 8 r so that a quad's neighbours meet other banks.
+        __syncthreads();
+        float* mg = reinterpret_cast<float*>(ring + (size_t)(stage == 0 ? SM::STAGES - 1 : stage - 1) * 2 * SM::TILE);
+        {
+            float* a = mg + (size_t)(wk * M + wr * 16 + g) * D;
+            float* b = a + 8 * D;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const int col = ((i + g) % NT) * 8 + 2 * t;
+                *reinterpret_cast<float2*>(a + col) = make_float2(o[i][0], o[i][1]);
+                *reinterpret_cast<float2*>(b + col) = make_float2(o[i][2], o[i][3]);
+            }
+            if (t == 0) {
+                s_ml[wk][wr * 16 + g][0] = m0; s_ml[wk][wr * 16 + g][1] = l0;
+                s_ml[wk][wr * 16 + g + 8][0] = m1; s_ml[wk][wr * 16 + g + 8][1] = l1;
+            }
+        }
+        __syncthreads();
+        const bool whole = seg_end - (u - (long long)(tile - s.t0 - at.tile)) == s.tiles && at.tile == 0;
+        const size_t slot = (size_t)blockIdx.x * 2 + (u - (tile - s.t0 - at.tile) == lo ? 0 : 1);
+        const int here = min(M, rows - at.slab * M);
+        for (int e = threadIdx.x; e < here * D; e += AF_THREADS) {
+            const int r = e / D, d = e - r * D, col = (d + 8 * (r & 7)) % D;
+            float mm = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < WK; ++k) mm = fmaxf(mm, s_ml[k][r][0]);
+            const float base = mm == -INFINITY ? 0.f : mm;
+            float sum = 0.f, acc = 0.f;
+#pragma unroll
+            for (int k = 0; k < WK; ++k) {
+                const float f = exp2f(s_ml[k][r][0] - base);
+                sum += s_ml[k][r][1] * f;
+                acc += mg[(size_t)(k * M + r) * D + col] * f;
+            }
+            if (whole) {
+                const int row = at.slab * M + r, i = row / group;
+                out[((size_t)(first_token + i) * nq + (size_t)at.kvh * group + (row - i * group)) * D + d] = __float2bfloat16_rn(sum > 0.f ? acc / sum : 0.f);
+            } else {
+                ws_o[(slot * M + r) * D + d] = acc;
+                if (d == 0) { ws_ml[(slot * M + r) * 2] = mm; ws_ml[(slot * M + r) * 2 + 1] = sum; }
+            }
+        }
+    }
+    cp_async_wait<0>();
+}
+
+// The parts of a row that several blocks share, in ascending order: a block a (new token, head). Rows of items that one block did are done; rows
+// without keys get zeros.
+__global__ void attention_few_join_kernel(bf16* out, const int* cu, const int* kv_lens, const float* ws_o, const float* ws_ml, const long long* units,
+                                          int B, int nq, int nkv, int D, int M, int window, int blocks) {
+    const int b = blockIdx.y, i = blockIdx.x / nq, head = blockIdx.x % nq, group = nq / nkv;
+    const int first_token = __ldcg(cu + b), T = __ldcg(cu + b + 1) - first_token;
+    const int L = __ldcg(kv_lens + b);
+    pdl_enter();
+    if (i >= T) return;
+    const FewShape s = few_shape(T, L, window, group, M);
+    bf16* dst = out + ((size_t)(first_token + i) * nq + head) * D;
+    if (s.tiles == 0) {
+        for (int d = threadIdx.x; d < D; d += blockDim.x) dst[d] = __float2bfloat16_rn(0.f);
+        return;
+    }
+    const long long U = __ldcg(units + B);
+    const int G = (int)min((long long)blocks, U);
+    const int kvh = head / group, row = i * group + head % group, slab = row / M, r = row % M;
+    const long long u0 = __ldcg(units + b) + (long long)(kvh * s.slabs + slab) * s.tiles;
+    const int c0 = few_owner(U, u0, G), c1 = few_owner(U, u0 + s.tiles - 1, G);
+    if (c0 == c1) return;
+    auto slot = [&](int c) { return ((size_t)c * 2 + (few_low(U, c, G) >= u0 ? 0 : 1)) * M + r; };
+    // The maximum over the parts by a warp's lanes (every warp for itself), then the parts in ascending order.
+    float mm = -INFINITY;
+    for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32) mm = fmaxf(mm, __ldcg(ws_ml + slot(c) * 2));
+    mm = warp_max(mm);
+    const float base = mm == -INFINITY ? 0.f : mm;
+    for (int d = threadIdx.x; d < D; d += blockDim.x) {
+        float sum = 0.f, acc = 0.f;
+        for (int c = c0; c <= c1; c += 4) {
+            float m[4], l[4], v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool ok = c + k <= c1;
+                const size_t at = slot(ok ? c + k : c1);
+                m[k] = ok ? __ldcg(ws_ml + at * 2) : -INFINITY;
+                l[k] = __ldcg(ws_ml + at * 2 + 1);
+                v[k] = __ldcg(ws_o + at * D + d);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float f = exp2f(m[k] - base);
+                sum = fmaf(l[k], f, sum);
+                acc = fmaf(v[k], f, acc);
+            }
+        }
+        dst[d] = __float2bfloat16_rn(sum > 0.f ? acc / sum : 0.f);
+    }
+}
+
+static int few_rows(int max_rows, int D) { return D > 128 || max_rows <= 16 ? 16 : max_rows <= 32 ? 32 : 64; }
+static int few_blocks(int D) { return (D <= 128 ? 2 : 1) * ti_sm_count(); }
+
+// Bytes of the work space: 64-bit words for the units before each sequence, then two slots of rows a block.
+extern "C" long long ti_attention_few_workspace(int B, int max_new, int nq, int nkv, int D) {
+    if (B <= 0 || max_new <= 0 || nq <= 0 || nkv <= 0 || D <= 0) return 0;
+    const long long M = few_rows(max_new * (nq / nkv), D), slots = 2LL * few_blocks(D);
+    return 8LL * (AF_MAX_SEQS + 2) + slots * M * (D + 2) * 4;
+}
+
+template <int D, int MT>
+static int launch_few(bf16* out, const bf16* q, const bf16* k, const bf16* v, const int* table, int table_stride, const int* seq_slots, const int* cu,
+                      const int* kv_lens, void* ws, float scale, int B, int nq, int nkv, int max_new, int window, cudaStream_t stream) {
+    static bool configured = false;
+    if (!configured) {
+        cudaError_t e = cudaFuncSetAttribute(attention_few_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FewSmem<D>::BYTES);
+        if (e != cudaSuccess) return ti_fail("attention_few: %s", cudaGetErrorString(e));
+        configured = true;
+    }
+    constexpr int M = 16 * MT;
+    const int G = few_blocks(D);
+    long long* units = (long long*)ws;
+    float* ws_o = (float*)(units + AF_MAX_SEQS + 2);
+    float* ws_ml = ws_o + (size_t)2 * G * M * D;
+    ti_launch(attention_few_kernel<D, MT>, dim3(G), dim3(AF_THREADS), FewSmem<D>::BYTES, stream, out, q, k, v, table, table_stride, seq_slots, cu, kv_lens,
+              ws_o, ws_ml, units, scale * 1.4426950408889634f, B, nq, nkv, window);
+    if (int rc = ti_check_launch("attention_few")) return rc;
+    ti_launch(attention_few_join_kernel, dim3(max_new * nq, B), dim3(D <= 32 ? 32 : D <= 64 ? 64 : 128), 0, stream, out, cu, kv_lens, ws_o, ws_ml, units, B, nq, nkv, D, M,
+              window, G);
+    return ti_check_launch("attention_few_join");
+}
+
+// q [tokens, nq, D] and out [tokens, nq * D]; the tokens of sequence b are cu[b] to cu[b + 1], at most max_new; kv_lens[b] its length with them; its
+// pages are row seq_slots[b] of block_table. `ws`: ti_attention_few_workspace bytes, 16-byte aligned. Returns 2 for sizes outside what it takes.
+extern "C" int ti_attention_few(void* out, const void* q, const void* k_cache, const void* v_cache, const int* block_table, int table_stride,
+                                const int* seq_slots, const int* cu, const int* kv_lens, void* ws, long long ws_bytes, float scale, int B, int nq,
+                                int nkv, int D, int page_size, int max_new, int window, cudaStream_t stream) {
+    if (B == 0 || max_new == 0) return 0;
+    TI_REQUIRE(B > 0 && max_new > 0 && nq > 0 && nkv > 0 && D > 0 && window >= 0, "attention_few: %d sequences, %d new tokens, %d / %d heads of %d", B,
+               max_new, nq, nkv, D);
+    if (page_size != AF_PAGE || nq % nkv != 0 || B > AF_MAX_SEQS || (long long)max_new * nq > 65535LL * 1024 || nq / nkv > 1024) {
+        ti_fail("attention_few takes pages of %d and at most %d sequences; got pages of %d, %d sequences, %d / %d heads", AF_PAGE, AF_MAX_SEQS, page_size,
+                B, nq, nkv);
+        return 2;
+    }
+    TI_REQUIRE(ws != nullptr && aligned16(ws) && ws_bytes >= ti_attention_few_workspace(B, max_new, nq, nkv, D), "attention_few: work space of %lld bytes, %lld needed",
+               ws_bytes, ti_attention_few_workspace(B, max_new, nq, nkv, D));
+    const int M = few_rows(max_new * (nq / nkv), D);
+#define AF_LAUNCH(d, mt) \
+    return launch_few<d, mt>((bf16*)out, (const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_table, table_stride, seq_slots, cu, kv_lens, ws, \
+                             scale, B, nq, nkv, max_new, window, stream)
+#define AF_CASE(d)                          \
+    case d:                                 \
+        if (M == 16) AF_LAUNCH(d, 1);       \
+        if (M == 32) AF_LAUNCH(d, 2);       \
+        AF_LAUNCH(d, 4);
+    switch (D) {
+        AF_CASE(16) AF_CASE(32) AF_CASE(48) AF_CASE(64) AF_CASE(80) AF_CASE(96) AF_CASE(112) AF_CASE(128)
+        case 256: AF_LAUNCH(256, 1);
+        default:
+            ti_fail("attention_few has no instance for head size %d", D);
+            return 2;
+    }
+#undef AF_CASE
+#undef AF_LAUNCH
+}

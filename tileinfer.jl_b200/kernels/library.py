@@ -91,7 +91,7 @@ _SIGNATURES = {
 }
 
 
-_KERNELS_PER_CALL = {"ti_memory_chunks": 3, "ti_ssm_chunks": 3, "ti_ssm_chunks_tc": 3}
+_KERNELS_PER_CALL = {"ti_attention_few": 2, "ti_memory_chunks": 3, "ti_ssm_chunks": 3, "ti_ssm_chunks_tc": 3}
 
 
 def lib():
@@ -123,6 +123,10 @@ def lib():
     wrapped.ti_expert_plan_max_tiles = handle.ti_expert_plan_max_tiles
     handle.ti_memory_chunk_pitch.restype, handle.ti_memory_chunk_pitch.argtypes = c_int, [c_int, c_int]
     wrapped.ti_memory_chunk_pitch = handle.ti_memory_chunk_pitch
+    for name, args in (("ti_attention_few_workspace", [_I] * 5), ("ti_verify_drafts_workspace", [_I])):
+        fn = getattr(handle, name)
+        fn.restype, fn.argtypes = c_longlong, args
+        setattr(wrapped, name, fn)
     wrapped.handle = handle
     for name, args in _SIGNATURES.items():
         fn = getattr(handle, name)
@@ -255,4 +259,15 @@ _SIGNATURES.update({
     "ti_ssm_chunks": [_P, _P, _L, _I, _I, _I, _P, _L, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
     "ti_ssm_chunks_tc": [_P, _P, _L, _I, _I, _I, _P, _L, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P],
     "ti_ssm_gate_norm": [_P, _P, _P, _L, _P, _F, _I, _I, _I, _I, _P],
+})
+
+# Drafts and their test: products with weights of 4 bits, attention of a few new tokens, probabilities, which drafted tokens stand.
+_SIGNATURES.update({
+    "ti_linear4": [_P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _F, _F, _I, _P],
+    "ti_quantize4": [_P, _L, _I, _P, _P, _I, _P, _I, _I, _I, _P],
+    "ti_attention_few": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _L, _F, _I, _I, _I, _I, _I, _I, _I, _P],
+    "ti_probabilities": [_P, _L, _P, _L, _I, _I, _F, _I, _F, _P],
+    "ti_verify_drafts": [_P, _P, _P, _L, _L, _P, _L, _L, _P, _P, _P, _I, _I, _I, _P, _P, _P],
+    "ti_match_drafts": [_P, _P, _P, _P, _P, _I, _I, _P],
+    "ti_uniforms": [_P, _P, _P, _I, _I, _P],
 })

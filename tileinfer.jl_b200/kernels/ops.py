@@ -951,3 +951,167 @@ def ssm_gate_norm(out, y, z, w, eps, parts):
     _need(out, "out"); _need(y, "y", torch.float32); _need(z, "z", out.dtype, contiguous=False); _need(w, "w", out.dtype)
     check(lib().ti_ssm_gate_norm(out.data_ptr(), y.data_ptr(), z.data_ptr(), z.stride(0), w.data_ptr(), eps, parts, out.shape[0], out.shape[1],
                                  dtype_code(out.dtype), _stream()), "ssm_gate_norm")
+
+
+# ---------------------------------------------------------------- drafts of a few tokens and their test
+LINEAR4_GROUPS = (32, 64, 128)
+
+
+def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0.0, 0.0)):
+    """y [n, out] = x [n, in] Wᵀ for W[o, k] = (code - zero) * scale: ``codes`` [out, in / 8] int32 hold eight consecutive k a word (the even
+    ones in its low half, the odd ones in its high half, four bits each in ascending order), ``scales`` [in / group, out] of x's type for groups of
+    32, 64 or 128 k, ``zeros`` [in / group, out] uint8, or 8 for all. 32-bit sums, rounded once; with ``EPI_F32_OUT`` y is float32 and the sums
+    are not rounded. Made for steps of few tokens; any number is taken. ``quantize4`` makes the codes."""
+    for t, name, dtype in ((x, "x", None), (y, "y", None), (codes, "codes", torch.int32), (scales, "scales", x.dtype)):
+        _need(t, name, dtype, contiguous=name in ("codes", "scales"))
+    code = dtype_code(x.dtype)
+    if x.dim() != 2 or y.dim() != 2 or codes.dim() != 2 or scales.dim() != 2:
+        raise KernelError("linear4: x, y, codes and scales have two dimensions")
+    (n, k), (out, words), (groups, so) = x.shape, codes.shape, scales.shape
+    if words * 8 != k or so != out or groups < 1 or k % groups or k // groups not in LINEAR4_GROUPS or tuple(y.shape) != (n, out):
+        raise KernelError(f"linear4: x {tuple(x.shape)}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)}, y {tuple(y.shape)} do not fit "
+                          f"(groups of {', '.join(map(str, LINEAR4_GROUPS))})")
+    if (n and k and x.stride(1) != 1) or (n and out and y.stride(1) != 1):
+        raise KernelError("linear4: rows of x and y must be dense")
+    if zeros is not None:
+        _need(zeros, "zeros", torch.uint8)
+        if zeros.shape != scales.shape:
+            raise KernelError(f"linear4: zeros {tuple(zeros.shape)} for scales {tuple(scales.shape)}")
+    if y.dtype != (torch.float32 if epilogue == EPI_F32_OUT else x.dtype):
+        raise KernelError(f"linear4: output must be {torch.float32 if epilogue == EPI_F32_OUT else x.dtype}")
+    check(lib().ti_linear4(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), n, out, k,
+                           k // groups, epilogue, act[0], act[1], act[2], act[3], code, _stream()), "linear4")
+
+
+def quantize4(codes, scales, w, zeros=None):
+    """The codes, scales and (where ``zeros`` is given) zeros that ``linear4`` takes, from a matrix w [out, in] (float32 or bfloat16), each group
+    rounded to the nearest code: without zeros scale = max |w| / 7, with them (max - min) / 15 over the group and 0."""
+    _need(w, "w", contiguous=False); _need(codes, "codes", torch.int32); _need(scales, "scales")
+    if w.dim() != 2 or codes.dim() != 2 or scales.dim() != 2:
+        raise KernelError("quantize4: w, codes and scales have two dimensions")
+    (out, k), groups = w.shape, scales.shape[0]
+    if (out and k and w.stride(1) != 1) or tuple(codes.shape) != (out, k // 8) or scales.shape[1] != out or groups < 1 or k % groups or \
+            k // groups not in LINEAR4_GROUPS:
+        raise KernelError(f"quantize4: w {tuple(w.shape)}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)} do not fit "
+                          f"(groups of {', '.join(map(str, LINEAR4_GROUPS))})")
+    if zeros is not None:
+        _need(zeros, "zeros", torch.uint8)
+        if zeros.shape != scales.shape:
+            raise KernelError(f"quantize4: zeros {tuple(zeros.shape)} for scales {tuple(scales.shape)}")
+    check(lib().ti_quantize4(w.data_ptr(), w.stride(0), dtype_code(w.dtype), codes.data_ptr(), scales.data_ptr(), dtype_code(scales.dtype), _ptr(zeros),
+                             out, k, k // groups, _stream()), "quantize4")
+
+
+_few_ws = {}
+
+
+def _workspace(kind: str, nbytes: int, device, zeroed: bool = False) -> torch.Tensor:
+    """At least ``nbytes`` of the kind's work space for the current stream (calls on one stream follow one another), grown on demand."""
+    key = (kind, device, _stream())
+    ws = _few_ws.get(key)
+    if ws is None or ws.numel() < nbytes:
+        make = torch.zeros if zeroed else torch.empty
+        ws = _few_ws[key] = make(max(nbytes, 4096), dtype=torch.uint8, device=device)
+    return ws
+
+
+def attention_few_workspace(seqs: int, max_new: int, nq: int, nkv: int, head_dim: int) -> int:
+    """Bytes of work space that ``attention_few`` needs."""
+    return int(lib().ti_attention_few_workspace(seqs, max_new, nq, nkv, head_dim))
+
+
+def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, kv_lens, scale, nq, nkv, head_dim, page_size, max_new, window=0,
+                  workspace=None) -> None:
+    """Attention of a few new tokens of every sequence over its pages, which hold the new tokens' keys and values already: the tokens
+    cu_seqlens[b] to cu_seqlens[b + 1] of q [n, nq, head_dim] (at most ``max_new`` of them, or none) are the last of the kv_lens[b] positions of the
+    sequence in slot seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out [n, nq * head_dim]. bfloat16 (the
+    32-bit path's sums do not depend on how a step is cut: ``attention_plain``). The work is shared out by the sequences' lengths on the device.
+    ``workspace``: ``attention_few_workspace`` bytes (uint8); without it one kept per stream."""
+    for t, name in ((out, "out"), (q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache")):
+        _need(t, name, torch.bfloat16)
+    for t, name in ((block_table, "block_table"), (seq_slots, "seq_slots"), (cu_seqlens, "cu_seqlens"), (kv_lens, "kv_lens")):
+        _need(t, name, torch.int32, contiguous=name != "block_table")
+    seqs, n = kv_lens.numel(), q.shape[0]
+    if nkv < 1 or nq < 1 or nq % nkv or head_dim < 1 or max_new < 0 or window < 0:
+        raise KernelError(f"attention_few: {nq} query heads on {nkv}, head size {head_dim}, {max_new} new tokens, window {window}")
+    if q.numel() != n * nq * head_dim or out.numel() != q.numel() or k_cache.shape != v_cache.shape or \
+            tuple(k_cache.shape[-3:]) != (nkv, page_size, head_dim) or cu_seqlens.numel() != seqs + 1 or seq_slots.numel() != seqs or \
+            block_table.dim() != 2 or (block_table.numel() and block_table.stride(1) != 1):
+        raise KernelError(f"attention_few: q {tuple(q.shape)}, out {tuple(out.shape)}, pages {tuple(k_cache.shape)}, {seqs} sequences, table "
+                          f"{tuple(block_table.shape)} do not fit {nq} / {nkv} heads of {head_dim} on pages of {page_size}")
+    if n == 0 or seqs == 0:
+        return
+    if workspace is None:
+        workspace = _workspace("attention_few", attention_few_workspace(seqs, max_new, nq, nkv, head_dim), q.device)
+    check(lib().ti_attention_few(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                                 seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), workspace.data_ptr(), workspace.numel(), scale, seqs, nq,
+                                 nkv, head_dim, page_size, max_new, window or 0, _stream()), "attention_few")
+
+
+def probabilities(out, logits, temperature, top_k=0, top_p=1.0):
+    """out [rows, vocab] = what ``sample`` draws from with these settings: exp((l - max) / temperature) over the ``top_k`` best (ties to the smaller
+    id; 0: all), then over the smallest best-first prefix whose mass reaches ``top_p``, divided by its sum; 0 elsewhere. A logit of -inf or NaN has
+    probability 0. float32; rows of both may be strided."""
+    _need(logits, "logits", torch.float32, contiguous=False); _need(out, "out", torch.float32, contiguous=False)
+    if logits.dim() != 2 or out.shape != logits.shape or (logits.numel() and (logits.stride(1) != 1 or out.stride(1) != 1)):
+        raise KernelError(f"probabilities: logits {tuple(logits.shape)} with strides {logits.stride()}, out {tuple(out.shape)} with {out.stride()}")
+    check(lib().ti_probabilities(out.data_ptr(), out.stride(0), logits.data_ptr(), logits.stride(0), logits.shape[0], logits.shape[1], temperature,
+                                 top_k, top_p, _stream()), "probabilities")
+
+
+def _need_run(accepted, tokens, drafts, counts, what):
+    """Checks what both tests of drafts share; returns (sequences, drafts)."""
+    for t, name in ((accepted, "accepted"), (tokens, "tokens"), (drafts, "drafts"), (counts, "counts")):
+        if t is not None:
+            _need(t, name, torch.int32)
+    if drafts.dim() != 2:
+        raise KernelError(f"{what}: drafts {tuple(drafts.shape)} (sequences, drafts)")
+    seqs, k = drafts.shape
+    if accepted.numel() != seqs or tuple(tokens.shape) != (seqs, k + 1) or (counts is not None and counts.numel() != seqs):
+        raise KernelError(f"{what}: accepted {tuple(accepted.shape)}, tokens {tuple(tokens.shape)} for drafts {tuple(drafts.shape)}")
+    return seqs, k
+
+
+def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None):
+    """Which drafted tokens stand: ``drafts`` [seqs, k] int32, drawn from the draft's probabilities ``q`` [seqs, k, vocab] (None: certain ones, as a
+    greedy draft's), against the model's ``p`` [seqs, k + 1, vocab], with ``uniforms`` [seqs, k + 1] in [0, 1). Draft i stands while
+    uniforms[i] * q[i, d] < p[i, d]; accepted[seq] is how many do, and tokens [seqs, k + 1] gets them, the token after them (by the last uniform
+    number, in ascending order of ids, from max(p - q, 0) at the first refusal, from p after the last draft where all stand; in 2^-40 fixed
+    point) and then -1. ``counts`` [seqs] int32: how many of a sequence's drafts there are (the rest of its row is not read). float32; p and q may
+    have any strides but for a dense last dimension. A row of p without weight gives the token -1."""
+    seqs, k = _need_run(accepted, tokens, drafts, counts, "verify_drafts")
+    _need(p, "p", torch.float32, contiguous=False); _need(uniforms, "uniforms", torch.float32)
+    vocab = p.shape[-1]
+    if tuple(p.shape) != (seqs, k + 1, vocab) or tuple(uniforms.shape) != (seqs, k + 1) or (p.numel() and p.stride(2) != 1):
+        raise KernelError(f"verify_drafts: p {tuple(p.shape)}, uniforms {tuple(uniforms.shape)} for drafts {tuple(drafts.shape)}")
+    q_args = (None, 0, 0)
+    if q is not None:
+        _need(q, "q", torch.float32, contiguous=False)
+        if tuple(q.shape) != (seqs, k, vocab) or (q.numel() and q.stride(2) != 1):
+            raise KernelError(f"verify_drafts: q {tuple(q.shape)} for p {tuple(p.shape)}")
+        q_args = (q.data_ptr(), q.stride(0), q.stride(1)) if k else q_args
+    if seqs == 0:
+        return
+    sums = _workspace("verify_sums", int(lib().ti_verify_drafts_workspace(seqs)), p.device)
+    tickets = _workspace("verify_tickets", 4 * seqs, p.device, zeroed=True)
+    check(lib().ti_verify_drafts(accepted.data_ptr(), tokens.data_ptr(), p.data_ptr(), p.stride(0), p.stride(1), *q_args, drafts.data_ptr(),
+                                 uniforms.data_ptr(), _ptr(counts), seqs, k, vocab, sums.data_ptr(), tickets.data_ptr(), _stream()), "verify_drafts")
+
+
+def match_drafts(accepted, tokens, chosen, drafts, counts=None):
+    """Which drafted tokens are the model's own greedy choices: ``chosen`` [seqs, k + 1] int32 (``argmax`` of its logits) against ``drafts`` [seqs, k].
+    accepted and tokens as in ``verify_drafts``; the token after the accepted ones is the model's choice there."""
+    seqs, k = _need_run(accepted, tokens, drafts, counts, "match_drafts")
+    _need(chosen, "chosen", torch.int32)
+    if tuple(chosen.shape) != (seqs, k + 1):
+        raise KernelError(f"match_drafts: chosen {tuple(chosen.shape)} for drafts {tuple(drafts.shape)}")
+    check(lib().ti_match_drafts(accepted.data_ptr(), tokens.data_ptr(), chosen.data_ptr(), drafts.data_ptr(), _ptr(counts), seqs, k, _stream()),
+          "match_drafts")
+
+
+def uniforms(out, seeds, counters):
+    """out [rows, m] float32: the sampler's next m uniform numbers of each row's (seed, counter); the counters move on by m."""
+    _need(out, "out", torch.float32); _need(seeds, "seeds", torch.int32); _need(counters, "counters", torch.int32)
+    if out.dim() != 2 or seeds.numel() != out.shape[0] or counters.numel() != out.shape[0]:
+        raise KernelError(f"uniforms: out {tuple(out.shape)} for {seeds.numel()} seeds, {counters.numel()} counters")
+    check(lib().ti_uniforms(out.data_ptr(), seeds.data_ptr(), counters.data_ptr(), out.shape[0], out.shape[1], _stream()), "uniforms")
