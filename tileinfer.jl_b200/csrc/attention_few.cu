@@ -12,7 +12,7 @@
 // Four warps share a tile out as MT groups of 16 rows x 4 / MT groups of keys. Scores, the running maximum and sum, and the output stand in
 // 32-bit; P is rounded to bfloat16 as the operand of P V alone (its sum is not), O once. A tile's keys and values beyond the sequence's end or
 // before the first visible key may hold anything: their scores are replaced and their values zeroed.
-#include "common.cuh"
+#include "even_runs.cuh"
 #include "mma_util.cuh"
 
 #define AF_PAGE 64
@@ -31,10 +31,6 @@ __device__ __forceinline__ FewShape few_shape(int T, int L, int window, int grou
     s.slabs = (T * group + M - 1) / M;
     return s;
 }
-// The blocks' runs: block c of G takes the units [U c / G, U (c + 1) / G), none of them empty (G at most U).
-__device__ __forceinline__ long long few_low(long long U, int c, int G) { return U * c / G; }
-__device__ __forceinline__ int few_owner(long long U, long long u, int G) { return (int)(((u + 1) * G - 1) / U); }
-
 // The joining kernel's part of the work space: [0] units in all, [1 + b] units of the sequences before b.
 template <int D> struct FewSmem {
     static constexpr int STAGES = D <= 128 ? 3 : 2;
@@ -88,7 +84,7 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
     const long long U = s_units[B];
     const int G = (int)min((long long)gridDim.x, U);
     if ((int)blockIdx.x >= max(G, 1)) return;                // more blocks than units
-    const long long lo = G > 0 ? few_low(U, blockIdx.x, G) : 0, hi = G > 0 ? few_low(U, blockIdx.x + 1, G) : 0;
+    const long long lo = G > 0 ? run_low(U, blockIdx.x, G) : 0, hi = G > 0 ? run_low(U, blockIdx.x + 1, G) : 0;
 
     struct Place {
         FewShape s;
@@ -334,9 +330,9 @@ __global__ void attention_few_join_kernel(bf16* out, const int* cu, const int* k
     const int G = (int)min((long long)blocks, U);
     const int kvh = head / group, row = i * group + head % group, slab = row / M, r = row % M;
     const long long u0 = __ldcg(units + b) + (long long)(kvh * s.slabs + slab) * s.tiles;
-    const int c0 = few_owner(U, u0, G), c1 = few_owner(U, u0 + s.tiles - 1, G);
+    const int c0 = run_owner(U, u0, G), c1 = run_owner(U, u0 + s.tiles - 1, G);
     if (c0 == c1) return;
-    auto slot = [&](int c) { return ((size_t)c * 2 + (few_low(U, c, G) >= u0 ? 0 : 1)) * M + r; };
+    auto slot = [&](int c) { return (size_t)run_slot(U, c, G, u0) * M + r; };
     // The maximum over the parts by a warp's lanes (every warp for itself), then the parts in ascending order.
     float mm = -INFINITY;
     for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32) mm = fmaxf(mm, __ldcg(ws_ml + slot(c) * 2));

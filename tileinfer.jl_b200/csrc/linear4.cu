@@ -6,37 +6,11 @@
 // Exactness: code - zero is a whole number of at most 15 and exact in bfloat16. A group's products x (code - zero) are summed in 32-bit,
 // the sum is multiplied by the group's scale in 32-bit, and the groups' sums are added in 32-bit; the result is rounded once. Nothing is
 // rounded to fewer bits before that (a weight (code - zero) * scale rounded to bfloat16 would cost as much again as the output's rounding).
-#include "common.cuh"
+#include "linear4.cuh"
 #include "mma_util.cuh"
 
-#define L4_EPI_NONE 0
-#define L4_EPI_XIELU 1
-#define L4_EPI_F32_OUT 2
-
-// Two of a word's codes as bfloat16 pairs, less the zero: 0x4300 | c is 128 + c in bfloat16 (its step is 1 there), and taking 128 + zero off is exact.
-__device__ __forceinline__ unsigned widen_pair(unsigned w, unsigned shift, __nv_bfloat162 base) {
-    const unsigned c = ((w >> shift) & 0x000F000Fu) | 0x43004300u;
-    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&c), base);
-    return *reinterpret_cast<const unsigned*>(&v);
-}
-
-__device__ __forceinline__ void store_result(void* y, long long ldy, int token, int row, float s, int epilogue, const XieluParams& act, bool y32) {
-    if (epilogue == L4_EPI_F32_OUT || (y32 && epilogue == L4_EPI_NONE)) {
-        ((float*)y)[(size_t)token * ldy + row] = s;
-        return;
-    }
-    if (y32) {
-        ((float*)y)[(size_t)token * ldy + row] = epilogue == L4_EPI_XIELU ? xielu_value<float>(s, act) : gelu_epilogue(s, epilogue);
-        return;
-    }
-    float v = rnd<bf16>(s);
-    if (epilogue == L4_EPI_XIELU) v = xielu_value<bf16>(v, act);
-    if (epilogue >= TI_EPI_GELU_ERF) v = gelu_epilogue(v, epilogue);
-    ((bf16*)y)[(size_t)token * ldy + row] = __float2bfloat16_rn(v);
-}
-
-// ------------------------------------------------------------------------------ bfloat16, up to 16 tokens at once
-// Bound by reading the codes once. The rows are shared out evenly among the resident blocks (in fours), the k of a block's rows among its
+// ------------------------------------------------------------------------------ bfloat16, eight tokens at once
+// Bound by reading the codes once (and by the eleven instructions that widen a word of them, seven on a pipe of half rate). The rows are shared out evenly among the resident blocks (in fours), the k of a block's rows among its
 // warps in stretches of 256: a warp keeps its stretch's tokens in registers as MMA operands and streams [16 rows, 256 k] pieces (2 KB, a
 // 128-byte line of every row) through a ring of its own in shared memory, so no barrier stands in the loop; the warps' sums are added once per
 // pass over the rows. A word of codes feeds two MMAs as the rows' operand; the k of the two operands are permuted alike, and so that an MMA's
@@ -60,81 +34,109 @@ __device__ __forceinline__ void cp_async4(unsigned dst, const void* src) {
 // The place of 16-byte piece p of row r: the rows that one phase of a 4-, 8- or 16-byte read covers fall into different banks.
 __device__ __forceinline__ int l4_place(int r, int p) { return p ^ (((r & 1) << 2) | (r & 2) | ((r & 4) >> 2)); }
 
-template <int NT, int GROUP>
+template <int GROUP>
 __global__ void __launch_bounds__(L4_WARPS * 32, 2) linear4_kernel(const unsigned* __restrict__ codes, const bf16* __restrict__ scales,
                                                                    const unsigned char* __restrict__ zeros, const bf16* x, long long ldx, void* y,
                                                                    long long ldy, int n, int out, int K, int passes, bool x_wide, bool s_wide,
                                                                    int epilogue, XieluParams act, bool y32) {
     typedef L4Piece<GROUP> P;
     constexpr int WORDS = GROUP / 32;                        // consecutive words a thread takes
+    constexpr int S_EACH = (P::GROUPS * 8 + 31) / 32, Z_EACH = (P::GROUPS * 4 + 31) / 32;
     extern __shared__ __align__(128) unsigned char l4_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     unsigned char* ring = l4_smem + (size_t)warp * L4_STAGES * P::BYTES;
-    const int token0 = blockIdx.y * 8 * NT;
+    const int token0 = blockIdx.y * 8;
     const int stretches = (K + L4_KC - 1) / L4_KC, groups = K / GROUP;
     const int mine = warp < stretches ? (stretches - warp + L4_WARPS - 1) / L4_WARPS : 0;
     const int fours = (out + 3) >> 2;
+    // Rows lane / 8 + 4 u of a piece: u turns one bit of the place of a 16-byte piece.
+    const int place0 = l4_place(lane >> 3, lane & 7) * 16, place1 = l4_place((lane >> 3) + 4, lane & 7) * 16;
+    const int read_at = g * 128 + l4_place(g, (t * WORDS) >> 2) * 16 + ((t * WORDS) & 3) * 4;
     bool waited = false;
 
+#pragma unroll 1
     for (int pass = 0; pass < passes; ++pass) {
         const long long share = (long long)pass * gridDim.x + blockIdx.x, shares = (long long)passes * gridDim.x;
         const int r0 = 4 * (int)(fours * share / shares), r1 = min(out, 4 * (int)(fours * (share + 1) / shares));
         const int tiles = (r1 - r0 + 15) >> 4;
-        // The pieces in the order of their use: the tiles of a stretch, stretch after stretch; each into the ring's next place.
-        int next_s = 0, next_m = 0, next_at = 0, at = 0;
-        auto issue = [&]() {
-            if (next_s < mine) {
-                unsigned char* dst = ring + next_at;
-                const int stretch = warp + next_s * L4_WARPS, base = r0 + 16 * next_m;
-                next_at = next_at == (L4_STAGES - 1) * P::BYTES ? 0 : next_at + P::BYTES;
-                if (++next_m == tiles) { next_m = 0; ++next_s; }
+        // The pieces in the order of their use: the tiles of a stretch, stretch after stretch; each into the ring's next place. Addresses move
+        // on by sums: `code` is this lane's first row and 16 bytes of the next piece, `scale` and `zero` its part of the scales and zeros.
+        int next_m = 0, left = mine, next_at = 0, at = 0, next_word = warp * (L4_KC / 8) + 4 * (lane & 7), rows_left = r1 - r0 - (lane >> 3);
+        const unsigned* code = codes + (size_t)(r0 + (lane >> 3)) * (K >> 3) + next_word;
+        auto table_at = [&](auto* table, int e, int per, int wide) {                     // entry e of a stretch's `per` entries a group
+            return table + (size_t)min((mine - left) * L4_WARPS * P::GROUPS + warp * P::GROUPS + e / per, groups - 1) * out + r0 + wide * (e % per);
+        };
+        const bf16* scale[S_EACH];
+        const unsigned char* zero[Z_EACH];
+        auto seek = [&] {
+            if (!s_wide) return;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int r = u * 4 + (lane >> 3), p = lane & 7, word = stretch * (L4_KC / 8) + 4 * p;
-                    if (base + r < r1 && word * 8 < K)
-                        cp_async16(smem_u32(dst + r * 128 + l4_place(r, p) * 16), codes + (size_t)(base + r) * (K >> 3) + word);
-                }
-                const int group0 = stretch * P::GROUPS;
+            for (int k = 0; k < S_EACH; ++k) scale[k] = table_at(scales, lane + 32 * k, 8, 2);
+            if (zeros == nullptr) return;
+#pragma unroll
+            for (int k = 0; k < Z_EACH; ++k) zero[k] = table_at(zeros, lane + 32 * k, 4, 4);
+        };
+        auto issue = [&]() {
+            if (left > 0) {
+                unsigned char* dst = ring + next_at;
+                const unsigned to = smem_u32(dst) + (lane >> 3) * 128;
+                const bool inside = next_word * 8 < K;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (inside && 4 * u < rows_left) cp_async16(to + u * 512 + ((u & 1) ? place1 : place0), code + (size_t)(4 * u) * (K >> 3));
                 if (s_wide) {
-                    for (int e = lane; e < P::GROUPS * 8; e += 32) {
-                        const int grp = min(group0 + (e >> 3), groups - 1), r = base + 2 * (e & 7);
-                        if (r < r1) cp_async4(smem_u32(dst + P::CODES + e * 4), scales + (size_t)grp * out + r);
+#pragma unroll
+                    for (int k = 0; k < S_EACH; ++k) {
+                        const int e = lane + 32 * k;
+                        if (e < P::GROUPS * 8 && 16 * next_m + 2 * (e & 7) < r1 - r0) cp_async4(smem_u32(dst + P::CODES + e * 4), scale[k] + 16 * next_m);
                     }
-                    if (zeros != nullptr)
-                        for (int e = lane; e < P::GROUPS * 4; e += 32) {
-                            const int grp = min(group0 + (e >> 2), groups - 1), r = base + 4 * (e & 3);
-                            if (r < r1) cp_async4(smem_u32(dst + P::CODES + P::SCALES + e * 4), zeros + (size_t)grp * out + r);
+                    if (zeros != nullptr) {
+#pragma unroll
+                        for (int k = 0; k < Z_EACH; ++k) {
+                            const int e = lane + 32 * k;
+                            if (e < P::GROUPS * 4 && 16 * next_m + 4 * (e & 3) < r1 - r0)
+                                cp_async4(smem_u32(dst + P::CODES + P::SCALES + e * 4), zero[k] + 16 * next_m);
                         }
+                    }
                 } else {
                     for (int e = lane; e < P::GROUPS * 16; e += 32) {
-                        const int grp = min(group0 + (e >> 4), groups - 1), r = base + (e & 15);
-                        if (r < r1) {
-                            reinterpret_cast<bf16*>(dst + P::CODES)[e] = scales[(size_t)grp * out + r];
-                            if (zeros != nullptr) dst[P::CODES + P::SCALES + e] = zeros[(size_t)grp * out + r];
+                        const bf16* from = table_at(scales, e, 16, 1) + 16 * next_m;
+                        if (16 * next_m + (e & 15) < r1 - r0) {
+                            reinterpret_cast<bf16*>(dst + P::CODES)[e] = *from;
+                            if (zeros != nullptr) dst[P::CODES + P::SCALES + e] = *(table_at(zeros, e, 16, 1) + 16 * next_m);
                         }
                     }
+                }
+                next_at = next_at == (L4_STAGES - 1) * P::BYTES ? 0 : next_at + P::BYTES;
+                code += (size_t)16 * (K >> 3);
+                rows_left -= 16;
+                if (++next_m == tiles) {
+                    next_m = 0;
+                    --left;
+                    next_word += L4_WARPS * (L4_KC / 8);
+                    code += L4_WARPS * (L4_KC / 8) - (size_t)(16 * tiles) * (K >> 3);
+                    rows_left += 16 * tiles;
+                    seek();
                 }
             }
             cp_async_commit();
         };
+        seek();
 #pragma unroll
         for (int i = 0; i < L4_STAGES - 1; ++i) issue();
         if (!waited) { pdl_enter(); waited = true; }         // codes and scales are no result of a step: only the tokens are waited for
 
-        float acc[L4_MT][NT][4];
+        float acc[L4_MT][4];
 #pragma unroll
         for (int m = 0; m < L4_MT; ++m)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+            for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
 
         for (int s = 0; s < mine; ++s) {
-            // The stretch's tokens: word w of the thread's words holds k = 8 w to 8 w + 7 of token g (+ 8 j).
-            uint4 xv[NT][8];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int token = token0 + g + 8 * j;
+            // The stretch's tokens: word w of the thread's words holds eight k of token g.
+            uint4 xv[8];
+            {
+                const int token = token0 + g;
 #pragma unroll
                 for (int w = 0; w < 8; ++w) {
                     const int word = (w / WORDS) * (GROUP / 8) + t * WORDS + w % WORDS, k = (warp + s * L4_WARPS) * L4_KC + 8 * word;
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(L4_WARPS * 32, 2) linear4_kernel(const unsigne
                                            e[6] | (unsigned)e[7] << 16);
                         }
                     }
-                    xv[j][w] = v;
+                    xv[w] = v;
                 }
             }
 #pragma unroll
@@ -164,17 +166,12 @@ __global__ void __launch_bounds__(L4_WARPS * 32, 2) linear4_kernel(const unsigne
                 const bf16* sc = reinterpret_cast<const bf16*>(src + P::CODES);
 #pragma unroll
                 for (int q = 0; q < P::GROUPS; ++q) {
-                    float part[NT][4];
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) part[j][c] = 0.f;
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
                     unsigned lo[WORDS], hi[WORDS];
                     {
                         // This group's words of rows g and g + 8: GROUP / 2 bytes a row from byte q * GROUP / 2, thread t's from t * 4 WORDS on.
-                        const int byte = q * (GROUP / 2) + t * 4 * WORDS, p = byte >> 4, in = byte & 15;
-                        const unsigned* a = reinterpret_cast<const unsigned*>(src + g * 128 + l4_place(g, p) * 16 + in);
-                        const unsigned* b = reinterpret_cast<const unsigned*>(src + (g + 8) * 128 + l4_place(g, p) * 16 + in);
+                        const unsigned* a = reinterpret_cast<const unsigned*>(src + (read_at ^ (q * (GROUP / 32) * 16)));
+                        const unsigned* b = a + 8 * 32;
                         if (WORDS == 4) {
                             const uint4 va = *reinterpret_cast<const uint4*>(a), vb = *reinterpret_cast<const uint4*>(b);
                             lo[0] = va.x; lo[1 % WORDS] = va.y; lo[2 % WORDS] = va.z; lo[3 % WORDS] = va.w;
@@ -185,10 +182,10 @@ __global__ void __launch_bounds__(L4_WARPS * 32, 2) linear4_kernel(const unsigne
                             hi[0] = vb.x; hi[1 % WORDS] = vb.y;
                         } else { lo[0] = *a; hi[0] = *b; }
                     }
-                    __nv_bfloat162 base_lo = __floats2bfloat162_rn(136.f, 136.f), base_hi = base_lo;
+                    unsigned base_lo = 0x43084308u, base_hi = base_lo;                   // 128 + zero, twice
                     if (zeros != nullptr) {
-                        base_lo = __float2bfloat162_rn(128.f + (float)src[P::CODES + P::SCALES + q * 16 + g]);
-                        base_hi = __float2bfloat162_rn(128.f + (float)src[P::CODES + P::SCALES + q * 16 + g + 8]);
+                        base_lo = src[P::CODES + P::SCALES + q * 16 + g] * 0x00010001u + 0x43004300u;
+                        base_hi = src[P::CODES + P::SCALES + q * 16 + g + 8] * 0x00010001u + 0x43004300u;
                     }
 #pragma unroll
                     for (int w = 0; w < WORDS; ++w) {
@@ -196,58 +193,49 @@ __global__ void __launch_bounds__(L4_WARPS * 32, 2) linear4_kernel(const unsigne
                                                    widen_pair(hi[w], 4, base_hi)},
                                                   {widen_pair(lo[w], 8, base_lo), widen_pair(hi[w], 8, base_hi), widen_pair(lo[w], 12, base_lo),
                                                    widen_pair(hi[w], 12, base_hi)}};
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            mma16816(part[j], a[0], xv[j][q * WORDS + w].x, xv[j][q * WORDS + w].y);
-                            mma16816(part[j], a[1], xv[j][q * WORDS + w].z, xv[j][q * WORDS + w].w);
-                        }
+                        mma16816(part, a[0], xv[q * WORDS + w].x, xv[q * WORDS + w].y);
+                        mma16816(part, a[1], xv[q * WORDS + w].z, xv[q * WORDS + w].w);
                     }
                     const float s_lo = to_f32(sc[q * 16 + g]), s_hi = to_f32(sc[q * 16 + g + 8]);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        acc[m][j][0] = fmaf(s_lo, part[j][0], acc[m][j][0]);
-                        acc[m][j][1] = fmaf(s_lo, part[j][1], acc[m][j][1]);
-                        acc[m][j][2] = fmaf(s_hi, part[j][2], acc[m][j][2]);
-                        acc[m][j][3] = fmaf(s_hi, part[j][3], acc[m][j][3]);
-                    }
+                    acc[m][0] = fmaf(s_lo, part[0], acc[m][0]);
+                    acc[m][1] = fmaf(s_lo, part[1], acc[m][1]);
+                    acc[m][2] = fmaf(s_hi, part[2], acc[m][2]);
+                    acc[m][3] = fmaf(s_hi, part[3], acc[m][3]);
                 }
             }
         }
         // The warps' sums in ascending order of the warps, through the ring's memory.
         cp_async_wait<0>();
         __syncthreads();
-        float* red = reinterpret_cast<float*>(l4_smem);      // [warp][tile][j][lane][4]
+        float* red = reinterpret_cast<float*>(l4_smem);      // [warp][tile][lane][4]
 #pragma unroll
         for (int m = 0; m < L4_MT; ++m)
             if (m < tiles)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    *reinterpret_cast<float4*>(red + ((((size_t)warp * L4_MT + m) * NT + j) * 32 + lane) * 4) =
-                        make_float4(acc[m][j][0], acc[m][j][1], acc[m][j][2], acc[m][j][3]);
+                *reinterpret_cast<float4*>(red + (((size_t)warp * L4_MT + m) * 32 + lane) * 4) = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
         __syncthreads();
         const int used = min(L4_WARPS, stretches);
-        for (int e = threadIdx.x; e < tiles * NT * 128; e += L4_WARPS * 32) {
-            const int l = (e & 127) >> 2, c = e & 3, j = (e >> 7) % NT, m = (e >> 7) / NT;
-            const int row = r0 + 16 * m + (l >> 2) + ((c & 2) ? 8 : 0), token = token0 + 8 * j + 2 * (l & 3) + (c & 1);
+        for (int e = threadIdx.x; e < tiles * 128; e += L4_WARPS * 32) {
+            const int l = (e & 127) >> 2, c = e & 3, m = e >> 7;
+            const int row = r0 + 16 * m + (l >> 2) + ((c & 2) ? 8 : 0), token = token0 + 2 * (l & 3) + (c & 1);
             if (row >= r1 || token >= n) continue;
             float sum = 0.f;
-            for (int w = 0; w < used; ++w) sum += red[((((size_t)w * L4_MT + m) * NT + j) * 32 + l) * 4 + c];
+            for (int w = 0; w < used; ++w) sum += red[(((size_t)w * L4_MT + m) * 32 + l) * 4 + c];
             store_result(y, ldy, token, row, sum, epilogue, act, y32);
         }
         __syncthreads();                                     // the ring is filled again
     }
 }
 
-template <int NT, int GROUP>
+template <int GROUP>
 static int launch_linear4(const void* codes, const void* scales, const void* zeros, const void* x, long long ldx, void* y, long long ldy, int n,
                           int out, int K, int epilogue, XieluParams act, bool y32, cudaStream_t stream) {
     typedef L4Piece<GROUP> P;
-    constexpr size_t ring = (size_t)L4_WARPS * L4_STAGES * P::BYTES, red = (size_t)L4_WARPS * L4_MT * NT * 128 * sizeof(float);
+    constexpr size_t ring = (size_t)L4_WARPS * L4_STAGES * P::BYTES, red = (size_t)L4_WARPS * L4_MT * 128 * sizeof(float);
     constexpr size_t smem = ring > red ? ring : red;
     static_assert(smem <= 113 * 1024, "two blocks per SM");
     static bool configured = false;
     if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(linear4_kernel<NT, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = cudaFuncSetAttribute(linear4_kernel<GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return ti_fail("linear4: %s", cudaGetErrorString(e));
         configured = true;
     }
@@ -256,7 +244,7 @@ static int launch_linear4(const void* codes, const void* scales, const void* zer
     const int passes = (fours + blocks * (4 * L4_MT) - 1) / (blocks * (4 * L4_MT));
     const bool x_wide = aligned16(x) && ldx % 8 == 0;
     const bool s_wide = out % 4 == 0 && (uintptr_t)scales % 4 == 0 && (uintptr_t)zeros % 4 == 0;
-    ti_launch(linear4_kernel<NT, GROUP>, dim3(blocks, (n + 8 * NT - 1) / (8 * NT)), dim3(L4_WARPS * 32), smem, stream, (const unsigned*)codes,
+    ti_launch(linear4_kernel<GROUP>, dim3(blocks, (n + 7) / 8), dim3(L4_WARPS * 32), smem, stream, (const unsigned*)codes,
               (const bf16*)scales, (const unsigned char*)zeros, (const bf16*)x, ldx, y, ldy, n, out, K, passes, x_wide, s_wide, epilogue, act, y32);
     return ti_check_launch("linear4");
 }
@@ -335,19 +323,23 @@ __global__ void __launch_bounds__(L4F_WARPS * 32) linear4_f32_kernel(const unsig
     }
 }
 
+// Which of the two bfloat16 kernels: eight tokens at a time, each time over all codes, or up to 64 tokens through shared memory (linear4_wide.cu),
+// whose blocks share tiles and need a second kernel to join them. us, eights / shared memory: 16 tokens x 21,504 x 4,096 31 / 26, x 2,048 x 2,048
+// 8.8 / 7.2, x 1,024 x 1,024 5.7 / 5.8, x 512 x 4,096 5.7 / 8.4; 24 tokens x 512 x 4,096 9.5 / 9.2; 64 tokens x 320 x 256 7.3 / 13.4.
+extern "C" int ti_linear4_shared(int n, int out, int K) { return n > 8 && (long long)((n + 7) / 8) * out * K > (1LL << 22); }
+
 // codes [out, K / 8] words, scales [K / group, out] of x's type, zeros [K / group, out] bytes or null; y [n, ldy] of x's type, or 32-bit sums
-// that are not rounded (epilogue 2).
+// that are not rounded (epilogue 2). `parts`: ti_linear4_parts(n, out, K) bytes (null where that is 0); `status`: the word of bounded waits.
 extern "C" int ti_linear4(void* y, long long ldy, const void* x, long long ldx, const void* codes, const void* scales, const void* zeros, int n,
-                          int out, int K, int group, int epilogue, float alpha_p, float alpha_n, float beta, float eps, int dtype,
-                          cudaStream_t stream) {
+                          int out, int K, int group, int epilogue, float alpha_p, float alpha_n, float beta, float eps, int dtype, void* parts,
+                          int* status, cudaStream_t stream) {
     if (n == 0 || out == 0) return 0;
     TI_REQUIRE(n > 0 && out > 0 && K > 0, "linear4: %d tokens, %d x %d", n, out, K);
     TI_REQUIRE(group == 32 || group == 64 || group == 128, "linear4: groups of %d (32, 64 or 128)", group);
     TI_REQUIRE(K % group == 0, "linear4: %d inputs are not whole groups of %d", K, group);
     TI_REQUIRE(aligned16(codes), "linear4: the codes must be 16-byte aligned");
     TI_REQUIRE(dtype == TI_F32 || dtype == TI_BF16, "linear4: unknown element type code %d", dtype);
-    TI_REQUIRE(epilogue == L4_EPI_NONE || epilogue == L4_EPI_XIELU || epilogue == L4_EPI_F32_OUT || (epilogue >= TI_EPI_GELU_ERF && epilogue <= TI_EPI_LAST),
-               "linear4: unknown epilogue %d", epilogue);
+    TI_REQUIRE(linear4_epilogue_known(epilogue), "linear4: unknown epilogue %d", epilogue);
     const XieluParams act{alpha_p, alpha_n, beta, eps};
     if (dtype == TI_F32) {
         TI_REQUIRE((n + L4F_TOKENS - 1) / L4F_TOKENS <= 65535, "linear4: %d tokens in one launch", n);
@@ -357,17 +349,14 @@ extern "C" int ti_linear4(void* y, long long ldy, const void* x, long long ldx, 
                   x_wide, epilogue, act);
         return ti_check_launch("linear4");
     }
+    // Rows of x that TMA does not take go eight tokens at a time, too.
+    if (ti_linear4_shared(n, out, K) && aligned16(x) && ldx % 8 == 0)
+        return linear4_wide(y, ldy, x, ldx, codes, scales, zeros, n, out, K, group, epilogue, act, parts, status, stream);
     TI_REQUIRE((n + 7) / 8 <= 65535, "linear4: %d tokens in one launch", n);
-#define L4_CASE(nt, grp) return launch_linear4<nt, grp>(codes, scales, zeros, x, ldx, y, ldy, n, out, K, epilogue, act, epilogue == L4_EPI_F32_OUT, stream)
-    if (n <= 8) {
-        if (group == 32) L4_CASE(1, 32);
-        if (group == 64) L4_CASE(1, 64);
-        L4_CASE(1, 128);
-    }
-    if (group == 32) L4_CASE(2, 32);
-    if (group == 64) L4_CASE(2, 64);
-    L4_CASE(2, 128);
-#undef L4_CASE
+    const bool y32 = epilogue == L4_EPI_F32_OUT;
+    if (group == 32) return launch_linear4<32>(codes, scales, zeros, x, ldx, y, ldy, n, out, K, epilogue, act, y32, stream);
+    if (group == 64) return launch_linear4<64>(codes, scales, zeros, x, ldx, y, ldy, n, out, K, epilogue, act, y32, stream);
+    return launch_linear4<128>(codes, scales, zeros, x, ldx, y, ldy, n, out, K, epilogue, act, y32, stream);
 }
 
 // ------------------------------------------------------------------------------ the codes of a matrix

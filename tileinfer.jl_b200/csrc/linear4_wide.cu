@@ -1,0 +1,337 @@
+// Products with weights of 4 bits whose tokens come through shared memory, up to 64 at once: see linear4.cu for what is computed.
+//
+// A stage holds [256 rows, 256 k] of codes, the tokens of these k (both by TMA, in swizzled rows of 128 bytes) and the rows' scales and zeros; the
+// block's warps take 16 or 32 rows each. A lane's word of codes (8 consecutive k of a row) feeds two MMAs as the rows' operand, 32 consecutive k at a
+// time, so an MMA's k lie in one group; the k of both operands are permuted alike. Rows and tokens stand in the MMAs in bit-reversed order, which
+// spreads every phase of a swizzled read over all banks.
+//
+// What bounds it: reading the codes once (up to 16 tokens), then mma.sync: 9 cycles a scheduler for 16 rows x 16 k x 8 tokens, 26 for the codes' eleven
+// instructions a word, seven of them on a pipe of half rate. (Weights widened into tensor memory as tcgen05.mma's operand, with a group's sum
+// read back from there, took 165 us for 16 and 245 us for 64 tokens x 131,072 x 4,096: a chain of five hand-overs between warps, 100 to 250 cycles
+// each, for every 128 k.)
+//
+// The units of work, [256 rows, 256 k], are numbered along k, then over the rows (and the tokens in sixty-fours), and every SM takes an equal run of them
+// (even_runs.cuh). Parts of a tile that several blocks share go to the work space; a second kernel adds them in the blocks' order.
+#include "linear4.cuh"
+#include "even_runs.cuh"
+#include "mma_util.cuh"
+#include "tcgen05.cuh"
+#include "tensor_map.h"
+
+namespace {
+using namespace tc;
+
+constexpr int KC = 256, ROWS = 256, CODES = ROWS * KC / 2;
+
+// Tokens in eights (NT), warps and tiles of 16 rows a warp (MT): few tokens leave registers for many warps, many make an operand's reading worth 32 rows.
+template <int NT, int GROUP> struct Shape {
+    static constexpr int N = 8 * NT, MT = NT <= 8 ? 1 : 2, WARPS = ROWS / (16 * MT), THREADS = 32 * WARPS, GROUPS = KC / GROUP;
+    static constexpr int X = N * KC * 2;
+    // Per group the 16-byte pieces of memory that hold its scales (zeros), wherever they begin: the place of the first in its piece is what its address says.
+    static constexpr int PIECES = 2 * ROWS / 16 + 1, ZERO_PIECES = ROWS / 16 + 1, SCALES = GROUPS * 16 * (PIECES + ZERO_PIECES);
+    static constexpr int BYTES = (CODES + X + SCALES + 1023) / 1024 * 1024;
+    static constexpr int FIT = (224 * 1024) / BYTES, STAGES = FIT > 5 ? 5 : FIT;
+};
+
+struct Args {
+    const bf16* scales;
+    const unsigned char* zeros;
+    void* y;
+    long long ldy;
+    float* parts;                                            // [slot][N tokens][256 rows]
+    int* status;
+    int n, out, groups, steps, chunks;                       // steps of 256 k; chunks of N tokens
+    long long units;
+    int epilogue;
+    XieluParams act;
+    bool y32;
+};
+
+__device__ __forceinline__ void copy16(unsigned dst, uintptr_t src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// MMAs that the compiler may move (their results are functions of their operands), so that the next words' loads and widening stand between them.
+__device__ __forceinline__ void mma_more(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ int reversed3(int g) { return ((g & 1) << 2) | (g & 2) | ((g & 4) >> 2); }
+
+template <int NT, int GROUP>
+__global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_kernel(const __grid_constant__ CUtensorMap map_codes,
+                                                                                    const __grid_constant__ CUtensorMap map_x, const Args p) {
+    typedef Shape<NT, GROUP> S;
+    constexpr int MT = S::MT, N = S::N;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* tiles = smem_dyn + ((1024u - (smem_addr(smem_dyn) & 1023u)) & 1023u);
+    const unsigned stages = smem_addr(tiles);
+    __shared__ __align__(8) unsigned long long bars[S::STAGES];
+    const unsigned full0 = smem_addr(bars);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = reversed3(lane >> 2), t = lane & 3;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::STAGES; ++s) mbar_init(full0 + 8 * s, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    const int G = gridDim.x, steps = p.steps;
+    const long long U = p.units, lo = run_low(U, blockIdx.x, G), hi = run_low(U, blockIdx.x + 1, G);
+    // Item = 256 rows x a chunk of tokens; the chunks of one stretch of rows follow one another, so its codes are read from memory once.
+    const uintptr_t s_end = (uintptr_t)(p.scales + (size_t)p.groups * p.out), z_end = (uintptr_t)(p.zeros + (size_t)p.groups * p.out);
+    // A thread's pieces of a step's scales and zeros: which group of the step, which piece.
+    constexpr int S_EACH = (S::GROUPS * S::PIECES + S::THREADS - 1) / S::THREADS;
+    int s_group[S_EACH], s_piece[S_EACH];
+#pragma unroll
+    for (int k = 0; k < S_EACH; ++k) {
+        const int e = threadIdx.x + k * S::THREADS;
+        s_group[k] = e < S::GROUPS * S::PIECES ? e / S::PIECES : 1 << 30;
+        s_piece[k] = 16 * (e % S::PIECES);
+    }
+    const int z_e = S::THREADS - 1 - threadIdx.x;
+    const int z_group = p.zeros != nullptr && z_e < S::GROUPS * S::ZERO_PIECES ? z_e / S::ZERO_PIECES : 1 << 30, z_piece = 16 * (z_e % S::ZERO_PIECES);
+    // What is asked for next.
+    long long next_u = lo, next_item = lo / steps;
+    int next_step = (int)(lo - next_item * steps), fill = 0, next_row = (int)(next_item / p.chunks) * ROWS, next_token = (int)(next_item % p.chunks) * N;
+    auto ask_codes = [&](int slot, int step, int row) {      // one thread
+        const unsigned bar = full0 + 8 * slot, dst = stages + slot * S::BYTES;
+        mbar_expect_tx(bar, CODES + N * KC * 2);
+        tma_load_2d(dst, &map_codes, step * (KC / 4), row, bar);
+    };
+    auto ask = [&](bool codes) {
+        if (next_u < hi) {
+            const unsigned dst = stages + fill * S::BYTES;
+            if (threadIdx.x == 0) {
+                if (codes) ask_codes(fill, next_step, next_row);
+#pragma unroll
+                for (int a = 0; a < KC / 64; ++a) tma_load_2d(dst + CODES + a * (S::X / 4), &map_x, next_step * KC + a * 64, next_token, full0 + 8 * fill);
+            }
+            const int left = p.groups - next_step * S::GROUPS;
+            const size_t first = (size_t)(next_step * S::GROUPS) * p.out + next_row;
+#pragma unroll
+            for (int k = 0; k < S_EACH; ++k)
+                if (s_group[k] < left) {
+                    const uintptr_t from = ((uintptr_t)(p.scales + first + (size_t)s_group[k] * p.out) & ~(uintptr_t)15) + s_piece[k];
+                    if (from < s_end) copy16(dst + CODES + S::X + (threadIdx.x + k * S::THREADS) * 16, from);
+                }
+            if (z_group < left) {
+                const uintptr_t from = ((uintptr_t)(p.zeros + first + (size_t)z_group * p.out) & ~(uintptr_t)15) + z_piece;
+                if (from < z_end) copy16(dst + CODES + S::X + S::GROUPS * S::PIECES * 16 + z_e * 16, from);
+            }
+            ++next_u;
+            if (++next_step == steps) {
+                next_step = 0;
+                ++next_item;
+                next_row = (int)(next_item / p.chunks) * ROWS;
+                next_token = (int)(next_item % p.chunks) * N;
+            }
+        }
+        fill = fill == S::STAGES - 1 ? 0 : fill + 1;
+        cp_async_commit();
+    };
+    // Codes are no result of a step: the first ones are asked for before the wait for the kernel before.
+    if (threadIdx.x == 0) {
+        long long item = next_item;
+        int step = next_step;
+        for (int s = 0; s < S::STAGES - 1 && lo + s < hi; ++s) {
+            ask_codes(s, step, (int)(item / p.chunks) * ROWS);
+            if (++step == steps) { step = 0; ++item; }
+        }
+    }
+    pdl_enter();
+#pragma unroll 1
+    for (int s = 0; s < S::STAGES - 1; ++s) ask(false);
+
+    float acc[MT][NT][4];
+    auto clear = [&] {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[m][j][c] = 0.f;
+    };
+    clear();
+    long long item = lo / steps;
+    int step = (int)(lo - item * steps), stage = 0, row0 = (int)(item / p.chunks) * ROWS;
+    unsigned phase = 0;
+    bool ok = true;
+    // A lane's places in a stage at its first 32 k: the swizzle turns bits 4 to 6 by the row's lowest three (bit-reversed order: g).
+    const unsigned code_at = (warp * MT * 16 + g) * 128 + (g << 4) + 4 * t, x_at = CODES + g * 128 + ((t ^ g) << 4);
+    for (long long u = lo; u < hi; ++u) {
+        cp_async_wait<S::STAGES - 2>();
+        ok = __syncthreads_and(mbar_wait(full0 + 8 * stage, phase, p.status, 16));
+        if (!ok) break;
+        ask(true);                                           // into the stage that every warp has left
+        const unsigned char* src = tiles + stage * S::BYTES;
+        if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
+        const int here = min(S::GROUPS, p.groups - step * S::GROUPS);
+        // Where the step's scales and zeros begin in their first pieces: low bits of addresses, moving on by a row of the tables a group.
+        unsigned s_low = (unsigned)(uintptr_t)p.scales + 2u * ((unsigned)(step * S::GROUPS) * (unsigned)p.out + (unsigned)row0);
+        unsigned z_low = (unsigned)(uintptr_t)p.zeros + (unsigned)(step * S::GROUPS) * (unsigned)p.out + (unsigned)row0;
+        const unsigned char *scales = src + CODES + S::X + 2 * (warp * MT * 16 + g), *zeros = src + CODES + S::X + S::GROUPS * S::PIECES * 16 + warp * MT * 16 + g;
+        unsigned chunk = 0;                                  // 32 k: a 16-byte piece of a row of codes, four of a row of tokens
+#pragma unroll 1
+        for (int q = 0; q < here; ++q) {
+            float part[MT][NT][4];
+            unsigned base[MT][2];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const unsigned z = p.zeros != nullptr ? zeros[(z_low & 15) + 16 * m + 8 * h] : 8u;
+                    base[m][h] = z * 0x00010001u + 0x43004300u;                          // 128 + zero, twice
+                }
+            auto block = [&](bool first) {
+                const unsigned char *rows = src + (code_at ^ (chunk << 4)), *x = src + (x_at ^ ((chunk & 1) << 6)) + (chunk >> 1) * (S::X / 4);
+                uint4 b[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) b[j] = *reinterpret_cast<const uint4*>(x + j * 1024);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const unsigned lo_w = *reinterpret_cast<const unsigned*>(rows + m * 2048), hi_w = *reinterpret_cast<const unsigned*>(rows + m * 2048 + 1024);
+                    const unsigned lo_b = base[m][0], hi_b = base[m][1];
+                    const unsigned a0[4] = {widen_pair(lo_w, 0, lo_b), widen_pair(hi_w, 0, hi_b), widen_pair(lo_w, 4, lo_b), widen_pair(hi_w, 4, hi_b)};
+                    const unsigned a1[4] = {widen_pair(lo_w, 8, lo_b), widen_pair(hi_w, 8, hi_b), widen_pair(lo_w, 12, lo_b), widen_pair(hi_w, 12, hi_b)};
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        if (first) mma_first(part[m][j], a0, b[j].x, b[j].y);
+                        else mma_more(part[m][j], a0, b[j].x, b[j].y);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) mma_more(part[m][j], a1, b[j].z, b[j].w);
+                }
+                ++chunk;
+            };
+            block(true);
+            if (NT <= 2) {
+#pragma unroll
+                for (int i = 1; i < GROUP / 32; ++i) block(false);
+            } else {                                         // many MMAs a block of k: its code once, for the instruction cache
+#pragma unroll 1
+                for (int i = 1; i < GROUP / 32; ++i) block(false);
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const float s_lo = to_f32(*reinterpret_cast<const bf16*>(scales + (s_low & 15) + 32 * m));
+                const float s_hi = to_f32(*reinterpret_cast<const bf16*>(scales + (s_low & 15) + 32 * m + 16));
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    acc[m][j][0] = fmaf(s_lo, part[m][j][0], acc[m][j][0]);
+                    acc[m][j][1] = fmaf(s_lo, part[m][j][1], acc[m][j][1]);
+                    acc[m][j][2] = fmaf(s_hi, part[m][j][2], acc[m][j][2]);
+                    acc[m][j][3] = fmaf(s_hi, part[m][j][3], acc[m][j][3]);
+                }
+            }
+            scales += S::PIECES * 16; zeros += S::ZERO_PIECES * 16;
+            s_low += 2u * (unsigned)p.out; z_low += (unsigned)p.out;
+        }
+        if (step + 1 == steps || u + 1 == hi) {              // the item's end, or this run's
+            const long long u0 = item * steps;
+            const bool whole = u0 >= lo && u0 + steps <= hi;
+            const int token0 = (int)(item % p.chunks) * N;
+            float* part = p.parts + (size_t)run_slot(U, blockIdx.x, G, u0) * N * ROWS;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        // A thread's columns 2 t and 2 t + 1 are tokens in bit-reversed order, its rows g and g + 8.
+                        const int r = (warp * MT + m) * 16 + g + ((c & 2) ? 8 : 0), token = 8 * j + reversed3(2 * t + (c & 1));
+                        if (token0 + token >= p.n || row0 + r >= p.out) continue;
+                        if (whole) store_result(p.y, p.ldy, token0 + token, row0 + r, acc[m][j][c], p.epilogue, p.act, p.y32);
+                        else part[(size_t)token * ROWS + r] = acc[m][j][c];
+                    }
+            clear();
+        }
+        if (++step == steps) { step = 0; ++item; row0 = (int)(item / p.chunks) * ROWS; }
+    }
+    cp_async_wait<0>();
+    if (!ok) drain_after_timeout();                          // a wait ran out: let what is in flight land
+}
+
+// The parts of 256 rows that several blocks share, in the blocks' order: blocks of (128 rows, eight tokens), a thread a row and two tokens.
+constexpr int JOIN_TOKENS = 8, JOIN_ROWS = 128;
+__global__ void __launch_bounds__(512) linear4_join_kernel(const Args p, int N, int G) {
+    const int slot = threadIdx.x >> 7, r = (blockIdx.x & 1) * JOIN_ROWS + (threadIdx.x & 127), first = blockIdx.y * JOIN_TOKENS, chunk = first / N;
+    const long long item = (long long)(blockIdx.x >> 1) * p.chunks + chunk, u0 = item * p.steps;
+    const int c0 = run_owner(p.units, u0, G), c1 = run_owner(p.units, u0 + p.steps - 1, G), row = (blockIdx.x >> 1) * ROWS + r;
+    pdl_enter();
+    if (c0 == c1 || row >= p.out) return;
+    const int token = first + 2 * slot;
+    const float* part = p.parts + (size_t)(token - chunk * N) * ROWS + r;
+    float s0 = 0.f, s1 = 0.f;
+    for (int c = c0; c <= c1; c += 6) {
+        float a[6], b[6];
+#pragma unroll
+        for (int k = 0; k < 6; ++k) {
+            const bool ok = c + k <= c1;
+            const float* src = part + (size_t)run_slot(p.units, ok ? c + k : c1, G, u0) * N * ROWS;
+            a[k] = ok && token < p.n ? __ldcg(src) : 0.f;
+            b[k] = ok && token + 1 < p.n ? __ldcg(src + ROWS) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 6; ++k) { s0 += a[k]; s1 += b[k]; }
+    }
+    if (token < p.n) store_result(p.y, p.ldy, token, row, s0, p.epilogue, p.act, p.y32);
+    if (token + 1 < p.n) store_result(p.y, p.ldy, token + 1, row, s1, p.epilogue, p.act, p.y32);
+}
+
+int tokens_at_once(int n) { return n <= 16 ? 16 : n <= 32 ? 32 : 64; }
+
+template <int NT, int GROUP> int launch(const CUtensorMap& codes, const CUtensorMap& x, const Args& a, cudaStream_t stream) {
+    typedef Shape<NT, GROUP> S;
+    constexpr size_t smem = (size_t)S::STAGES * S::BYTES + 1024;
+    static_assert(S::STAGES >= 3, "stages");
+    static bool configured = false;
+    if (!configured) {
+        cudaError_t e = cudaFuncSetAttribute(linear4_wide_kernel<NT, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return ti_fail("linear4_wide: %s", cudaGetErrorString(e));
+        configured = true;
+    }
+    const int blocks = (int)(a.units < ti_sm_count() ? a.units : ti_sm_count());
+    ti_launch(linear4_wide_kernel<NT, GROUP>, dim3(blocks), dim3(S::THREADS), smem, stream, codes, x, a);
+    if (int rc = ti_check_launch("linear4_wide")) return rc;
+    if (a.units % blocks == 0 && (a.units / blocks) % a.steps == 0) return 0;            // every run ends with an item: no parts
+    ti_launch(linear4_join_kernel, dim3(2 * ((a.out + ROWS - 1) / ROWS), (a.n + JOIN_TOKENS - 1) / JOIN_TOKENS), dim3(512), 0, stream, a, 8 * NT, blocks);
+    return ti_check_launch("linear4_join");
+}
+
+}  // namespace
+
+// Bytes of the work space for parts: 0 where the product takes none.
+extern "C" long long ti_linear4_parts(int n, int out, int K) {
+    return ti_linear4_shared(n, out, K) ? 2LL * ti_sm_count() * tokens_at_once(n) * ROWS * 4 : 0;
+}
+
+int linear4_wide(void* y, long long ldy, const void* x, long long ldx, const void* codes, const void* scales, const void* zeros, int n, int out, int K,
+                 int group, int epilogue, XieluParams act, void* parts, int* status, cudaStream_t stream) {
+    TI_REQUIRE(parts != nullptr && status != nullptr, "linear4: work space missing");
+    const int N = tokens_at_once(n);
+    CUtensorMap map_codes, map_x;
+    {   // The codes as [out, K / 4] numbers of 16 bits, moved as they are.
+        const unsigned long long dims[2] = {(unsigned long long)K / 4, (unsigned long long)out}, strides[1] = {(unsigned long long)K / 2};
+        const unsigned box[2] = {KC / 4, ROWS};
+        if (int rc = ti_tensor_map_bf16(&map_codes, codes, 2, dims, strides, box, true)) return rc;
+        const unsigned long long x_dims[2] = {(unsigned long long)K, (unsigned long long)n}, x_strides[1] = {(unsigned long long)ldx * 2};
+        const unsigned x_box[2] = {64, (unsigned)N};
+        if (int rc = ti_tensor_map_bf16(&map_x, x, 2, x_dims, x_strides, x_box, true)) return rc;
+    }
+    Args a;
+    a.scales = (const bf16*)scales; a.zeros = (const unsigned char*)zeros;
+    a.y = y; a.ldy = ldy; a.parts = (float*)parts; a.status = status;
+    a.n = n; a.out = out; a.groups = K / group; a.steps = (K + KC - 1) / KC; a.chunks = (n + N - 1) / N;
+    a.units = (long long)((out + ROWS - 1) / ROWS) * a.chunks * a.steps;
+    a.epilogue = epilogue; a.act = act; a.y32 = epilogue == L4_EPI_F32_OUT;
+#define L4_GROUPS(nt)                                                  \
+    if (group == 32) return launch<nt, 32>(map_codes, map_x, a, stream); \
+    if (group == 64) return launch<nt, 64>(map_codes, map_x, a, stream); \
+    return launch<nt, 128>(map_codes, map_x, a, stream);
+    if (N == 16) { L4_GROUPS(2) }
+    if (N == 32) { L4_GROUPS(4) }
+    L4_GROUPS(8)
+#undef L4_GROUPS
+}

@@ -11,6 +11,7 @@ from . import library as _library
 
 from . import ops
 from .library import KernelError, add_launches, check, lib
+from .ops import check_status, status_word
 
 GEMV_MAX_TOKENS = 8          # from 9 tokens on the tensor-core product is faster (measured per layer: 151 against 162 us at 12 tokens)
 _sm_count = 0
@@ -60,26 +61,6 @@ def linear(lin, x, out, epilogue, act, allow_partials=False):
     if k % 8 == 0 and k >= 8 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0:
         return _tcgen05(lin, x, out, epilogue, act, allow_partials)
     return None
-
-
-_status = None
-
-
-def status_word() -> torch.Tensor:
-    """Device word that kernels with bounded waits write a code to when a wait runs out."""
-    global _status
-    if _status is None:
-        _status = torch.zeros(1, dtype=torch.int32, device="cuda")
-    return _status
-
-
-def check_status() -> None:
-    """Raise if a kernel gave up on a wait since the last check (costs one device read)."""
-    if _status is not None:
-        code = int(_status.item())
-        if code:
-            _status.zero_()
-            raise KernelError(f"a tensor-core kernel gave up waiting on a barrier (waits {[i for i in range(31) if code >> i & 1]}); its results are invalid")
 
 
 def tc_splits(out_features: int, in_features: int, n: int) -> int:

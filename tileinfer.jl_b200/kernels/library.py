@@ -40,8 +40,17 @@ def current_stream() -> int:
     current stream (looking that up costs more than a launch, so a pass looks it up once)."""
     if pinned_stream is not None:
         return pinned_stream
+    return _lookup()
+
+
+def _lookup() -> int:
+    """torch's current stream on the current device: 0.2 us by its raw handle, 3.4 by way of a stream object."""
+    global _lookup
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    torch.cuda.current_stream()                              # sets CUDA up
+    raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
+    _lookup = (lambda: raw(device())) if raw is not None and device is not None else (lambda: torch.cuda.current_stream().cuda_stream)
+    return _lookup()
 
 
 class stream_scope:
@@ -49,9 +58,8 @@ class stream_scope:
 
     def __enter__(self):
         global pinned_stream
-        import torch
         self.before = pinned_stream
-        pinned_stream = torch.cuda.current_stream().cuda_stream
+        pinned_stream = _lookup()
         return self
 
     def __exit__(self, *exc):
@@ -123,7 +131,7 @@ def lib():
     wrapped.ti_expert_plan_max_tiles = handle.ti_expert_plan_max_tiles
     handle.ti_memory_chunk_pitch.restype, handle.ti_memory_chunk_pitch.argtypes = c_int, [c_int, c_int]
     wrapped.ti_memory_chunk_pitch = handle.ti_memory_chunk_pitch
-    for name, args in (("ti_attention_few_workspace", [_I] * 5), ("ti_verify_drafts_workspace", [_I])):
+    for name, args in (("ti_attention_few_workspace", [_I] * 5), ("ti_verify_drafts_workspace", [_I]), ("ti_linear4_parts", [_I] * 3)):
         fn = getattr(handle, name)
         fn.restype, fn.argtypes = c_longlong, args
         setattr(wrapped, name, fn)
@@ -263,7 +271,7 @@ _SIGNATURES.update({
 
 # Drafts and their test: products with weights of 4 bits, attention of a few new tokens, probabilities, which drafted tokens stand.
 _SIGNATURES.update({
-    "ti_linear4": [_P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _F, _F, _I, _P],
+    "ti_linear4": [_P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _F, _F, _I, _P, _P, _P],
     "ti_quantize4": [_P, _L, _I, _P, _P, _I, _P, _I, _I, _I, _P],
     "ti_attention_few": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _L, _F, _I, _I, _I, _I, _I, _I, _I, _P],
     "ti_probabilities": [_P, _L, _P, _L, _I, _I, _F, _I, _F, _P],

@@ -33,6 +33,26 @@ def _stream() -> int:
     return _library.current_stream()
 
 
+_status = None
+
+
+def status_word() -> torch.Tensor:
+    """Device word that kernels with bounded waits write a code to when a wait runs out."""
+    global _status
+    if _status is None:
+        _status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    return _status
+
+
+def check_status() -> None:
+    """Raise if a kernel gave up on a wait since the last check (costs one device read)."""
+    if _status is not None:
+        code = int(_status.item())
+        if code:
+            _status.zero_()
+            raise KernelError(f"a tensor-core kernel gave up waiting on a barrier (waits {[i for i in range(31) if code >> i & 1]}); its results are invalid")
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -979,8 +999,13 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
             raise KernelError(f"linear4: zeros {tuple(zeros.shape)} for scales {tuple(scales.shape)}")
     if y.dtype != (torch.float32 if epilogue == EPI_F32_OUT else x.dtype):
         raise KernelError(f"linear4: output must be {torch.float32 if epilogue == EPI_F32_OUT else x.dtype}")
+    stream = _stream()
+    parts = status = None
+    if n > 8 and code == BF16:
+        parts = _workspace("linear4", int(lib().ti_linear4_parts(n, out, k)), x.device, stream).data_ptr()
+        status = status_word().data_ptr()
     check(lib().ti_linear4(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), n, out, k,
-                           k // groups, epilogue, act[0], act[1], act[2], act[3], code, _stream()), "linear4")
+                           k // groups, epilogue, act[0], act[1], act[2], act[3], code, parts, status, stream), "linear4")
 
 
 def quantize4(codes, scales, w, zeros=None):
@@ -1005,9 +1030,9 @@ def quantize4(codes, scales, w, zeros=None):
 _few_ws = {}
 
 
-def _workspace(kind: str, nbytes: int, device, zeroed: bool = False) -> torch.Tensor:
-    """At least ``nbytes`` of the kind's work space for the current stream (calls on one stream follow one another), grown on demand."""
-    key = (kind, device, _stream())
+def _workspace(kind: str, nbytes: int, device, stream: int, zeroed: bool = False) -> torch.Tensor:
+    """At least ``nbytes`` of the kind's work space for ``stream`` (calls on one stream follow one another), grown on demand."""
+    key = (kind, device, stream)
     ws = _few_ws.get(key)
     if ws is None or ws.numel() < nbytes:
         make = torch.zeros if zeroed else torch.empty
@@ -1041,11 +1066,12 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
                           f"{tuple(block_table.shape)} do not fit {nq} / {nkv} heads of {head_dim} on pages of {page_size}")
     if n == 0 or seqs == 0:
         return
+    stream = _stream()
     if workspace is None:
-        workspace = _workspace("attention_few", attention_few_workspace(seqs, max_new, nq, nkv, head_dim), q.device)
+        workspace = _workspace("attention_few", attention_few_workspace(seqs, max_new, nq, nkv, head_dim), q.device, stream)
     check(lib().ti_attention_few(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
                                  seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), workspace.data_ptr(), workspace.numel(), scale, seqs, nq,
-                                 nkv, head_dim, page_size, max_new, window or 0, _stream()), "attention_few")
+                                 nkv, head_dim, page_size, max_new, window or 0, stream), "attention_few")
 
 
 def probabilities(out, logits, temperature, top_k=0, top_p=1.0):
@@ -1092,10 +1118,11 @@ def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None):
         q_args = (q.data_ptr(), q.stride(0), q.stride(1)) if k else q_args
     if seqs == 0:
         return
-    sums = _workspace("verify_sums", int(lib().ti_verify_drafts_workspace(seqs)), p.device)
-    tickets = _workspace("verify_tickets", 4 * seqs, p.device, zeroed=True)
+    stream = _stream()
+    sums = _workspace("verify_sums", int(lib().ti_verify_drafts_workspace(seqs)), p.device, stream)
+    tickets = _workspace("verify_tickets", 4 * seqs, p.device, stream, zeroed=True)
     check(lib().ti_verify_drafts(accepted.data_ptr(), tokens.data_ptr(), p.data_ptr(), p.stride(0), p.stride(1), *q_args, drafts.data_ptr(),
-                                 uniforms.data_ptr(), _ptr(counts), seqs, k, vocab, sums.data_ptr(), tickets.data_ptr(), _stream()), "verify_drafts")
+                                 uniforms.data_ptr(), _ptr(counts), seqs, k, vocab, sums.data_ptr(), tickets.data_ptr(), stream), "verify_drafts")
 
 
 def match_drafts(accepted, tokens, chosen, drafts, counts=None):
