@@ -17,8 +17,6 @@
 #define DV_WARPS (DV_THREADS / 32)
 #define DV_MAX_CHUNKS 256
 
-__device__ __forceinline__ u64 fixed_weight(float w) { return __float2ull_rn(fminf(fmaxf(w, 0.f), 1.f) * 1099511627776.0f); }   // NaN: 0
-
 // Inclusive scan over the block of one value per thread; `scratch`: DV_WARPS + 1 words, free again after the next barrier.
 __device__ __forceinline__ u64 dv_scan(u64 v, u64* scratch, u64& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -76,54 +74,53 @@ __global__ void __launch_bounds__(DV_THREADS) verify_drafts_kernel(int* accepted
     const bool differs = stand < count;
     const float* qr = differs && qb != nullptr ? qb + (size_t)stand * q_row : nullptr;
     const int without = differs && qb == nullptr ? __ldcg(drafts + (size_t)b * K + stand) : -1;
-    auto rest = [&](int v, float pv, float qv) { return fixed_weight(v == without ? pv - 1.f : pv - qv); };
+    auto rest = [&](int v, float pv, float qv) { return fixed_parts(v == without ? pv - 1.f : pv - qv); };
+    // Four neighbours of both rows, 0 beyond the end.
+    auto load4 = [&](int v, int end, float4& a, float4& c) {
+        a = c = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (v + 3 < end) {
+            a = __ldcg(reinterpret_cast<const float4*>(pr + v));
+            if (qr != nullptr) c = __ldcg(reinterpret_cast<const float4*>(qr + v));
+        } else if (v < end) {
+            a.x = __ldcg(pr + v);
+            if (v + 1 < end) a.y = __ldcg(pr + v + 1);
+            if (v + 2 < end) a.z = __ldcg(pr + v + 2);
+            if (qr != nullptr) {
+                c.x = __ldcg(qr + v);
+                if (v + 1 < end) c.y = __ldcg(qr + v + 1);
+                if (v + 2 < end) c.z = __ldcg(qr + v + 2);
+            }
+        }
+    };
 
     const int lo = min(vocab, chunk * per), hi = min(vocab, lo + per);
     const bool wide = ((uintptr_t)pr & 15) == 0 && ((uintptr_t)qr & 15) == 0;
-    u64 part = 0, whole = 0;
+    u64 part = 0;
     if (wide) {
         for (int v0 = lo + 4 * threadIdx.x; v0 < hi; v0 += 16 * DV_THREADS) {
             float4 a[4], c[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int v = v0 + u * 4 * DV_THREADS;
-                a[u] = c[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (v + 3 < hi) {
-                    a[u] = __ldcg(reinterpret_cast<const float4*>(pr + v));
-                    if (qr != nullptr) c[u] = __ldcg(reinterpret_cast<const float4*>(qr + v));
-                } else if (v < hi) {
-                    a[u].x = __ldcg(pr + v);
-                    if (v + 1 < hi) a[u].y = __ldcg(pr + v + 1);
-                    if (v + 2 < hi) a[u].z = __ldcg(pr + v + 2);
-                    if (qr != nullptr) {
-                        c[u].x = __ldcg(qr + v);
-                        if (v + 1 < hi) c[u].y = __ldcg(qr + v + 1);
-                        if (v + 2 < hi) c[u].z = __ldcg(qr + v + 2);
-                    }
-                }
-            }
+            for (int u = 0; u < 4; ++u) load4(v0 + u * 4 * DV_THREADS, hi, a[u], c[u]);
+            int high = 0, low = 0;                           // sixteen of them fit 32 bits
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int v = v0 + u * 4 * DV_THREADS;
-                part += rest(v, a[u].x, c[u].x) + rest(v + 1, a[u].y, c[u].y) + rest(v + 2, a[u].z, c[u].z) + rest(v + 3, a[u].w, c[u].w);
-                whole += fixed_weight(a[u].x) + fixed_weight(a[u].y) + fixed_weight(a[u].z) + fixed_weight(a[u].w);
+                const Fixed f0 = rest(v, a[u].x, c[u].x), f1 = rest(v + 1, a[u].y, c[u].y), f2 = rest(v + 2, a[u].z, c[u].z), f3 = rest(v + 3, a[u].w, c[u].w);
+                high += f0.high + f1.high + f2.high + f3.high;
+                low += f0.low + f1.low + f2.low + f3.low;
             }
+            part += (u64)(((long long)high << 20) + low);
         }
     } else {
         for (int v = lo + threadIdx.x; v < hi; v += DV_THREADS) {
-            const float a = __ldcg(pr + v);
-            part += rest(v, a, qr != nullptr ? __ldcg(qr + v) : 0.f);
-            whole += fixed_weight(a);
+            const Fixed f = rest(v, __ldcg(pr + v), qr != nullptr ? __ldcg(qr + v) : 0.f);
+            part += (u64)(((long long)f.high << 20) + f.low);
         }
     }
-    u64 part_sum, whole_sum;
+    u64 part_sum;
     dv_scan(part, scratch, part_sum);
-    __syncthreads();
-    dv_scan(whole, scratch, whole_sum);
     if (threadIdx.x == 0) {
-        u64* mine = sums + ((size_t)b * chunks + chunk) * 2;
-        mine[0] = part_sum;
-        mine[1] = whole_sum;
+        sums[(size_t)b * chunks + chunk] = part_sum;
         __threadfence();
         s_last = atomicAdd(&tickets[b], 1u) == (unsigned)chunks - 1;
         s_found = -1;
@@ -134,43 +131,72 @@ __global__ void __launch_bounds__(DV_THREADS) verify_drafts_kernel(int* accepted
 
     // The stretch that holds the target, a thread a stretch.
     const bool in = (int)threadIdx.x < chunks;
-    const u64* all = sums + ((size_t)b * chunks + threadIdx.x) * 2;
-    u64 w_part = in ? __ldcg(all) : 0, w_whole = in ? __ldcg(all + 1) : 0, total, p_total;
+    u64 w_part = in ? __ldcg(sums + (size_t)b * chunks + threadIdx.x) : 0, total;
     u64 through = dv_scan(w_part, scratch, total);
-    __syncthreads();
-    const u64 p_through = dv_scan(w_whole, scratch, p_total);
-    const bool plain = total == 0;                            // no weight in the differences (or none to take off)
-    if (plain) { total = p_total; through = p_through; w_part = w_whole; }
     const float u = __ldcg(uniforms + (size_t)b * (K + 1) + K);
     const u32 r24 = (u32)fminf(fmaxf(u, 0.f) * 16777216.f, 16777215.f);
+    const bool plain = total == 0;                            // no weight in the differences (or none to take off): the weights of p itself
+    if (plain) {
+        u64 whole = 0;
+        for (int v = threadIdx.x; v < vocab; v += DV_THREADS) whole += fixed_weight(__ldcg(pr + v));
+        __syncthreads();
+        dv_scan(whole, scratch, total);
+    }
     u64 target = draw_target(total, r24);
     if (target == 0) target = 1;
     __shared__ u64 s_before;
-    if (in && through >= target && through - w_part < target) { s_found = (int)threadIdx.x; s_before = through - w_part; }
+    if (threadIdx.x == 0 && plain) { s_found = total ? 0 : -1; s_before = 0; }           // searched from its beginning
+    if (!plain && in && through >= target && through - w_part < target) { s_found = (int)threadIdx.x; s_before = through - w_part; }
     __syncthreads();
     int next = -1;
     if (s_found >= 0) {                                       // uniform over the block
-        const int first = s_found * per, end = min(vocab, first + per), mine = (per + DV_THREADS - 1) / DV_THREADS;
-        const int v0 = first + (int)threadIdx.x * mine, v1 = min(end, v0 + mine);
-        const u64 before = s_before;
-        auto weight = [&](int v) {
-            const float a = __ldcg(pr + v);
-            return plain ? fixed_weight(a) : rest(v, a, qr != nullptr ? __ldcg(qr + v) : 0.f);
-        };
-        u64 sum = 0, all_in;
-        for (int v = v0; v < v1; ++v) sum += weight(v);
-        u64 cum = before + dv_scan(sum, scratch, all_in) - sum;
+        int v0 = s_found * per;
+        const int end = plain ? vocab : min(vocab, v0 + per);
+        u64 cum = s_before;
         __syncthreads();
-        if (cum < target && cum + sum >= target) {            // one thread
-            int v = v0;
-            for (; v < v1; ++v) {
-                cum += weight(v);
-                if (cum >= target) break;
+        // Sixteen tokens a thread at a time, in runs of four: the runs' sums scanned in order, then the run that reaches the target.
+        for (; v0 < end && next < 0; v0 += 16 * DV_THREADS) {
+            u64 w[4][4], sum[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int v = v0 + (k * DV_THREADS + (int)threadIdx.x) * 4;
+                float4 a, c;
+                if (wide) load4(v, end, a, c);
+                else {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        e[i] = v + i < end ? __ldcg(pr + v + i) : 0.f;
+                        e[4 + i] = v + i < end && qr != nullptr ? __ldcg(qr + v + i) : 0.f;
+                    }
+                    a = make_float4(e[0], e[1], e[2], e[3]); c = make_float4(e[4], e[5], e[6], e[7]);
+                }
+                const float av[4] = {a.x, a.y, a.z, a.w}, cv[4] = {c.x, c.y, c.z, c.w};
+                sum[k] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const Fixed f = plain ? fixed_parts(av[i]) : rest(v + i, av[i], cv[i]);
+                    w[k][i] = (u64)(((long long)f.high << 20) + f.low);
+                    sum[k] += w[k][i];
+                }
             }
-            s_found = v;
+            if (threadIdx.x == 0) s_found = -1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                u64 all_in, before = cum + dv_scan(sum[k], scratch, all_in) - sum[k];
+                if (before < target && before + sum[k] >= target) {                      // one thread
+                    int i = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (before < target) { before += w[k][e]; i = e; }
+                    s_found = v0 + (k * DV_THREADS + (int)threadIdx.x) * 4 + i;
+                }
+                cum += all_in;
+            }
+            __syncthreads();
+            next = s_found;
+            __syncthreads();
         }
-        __syncthreads();
-        next = s_found;
     }
     for (int i = threadIdx.x; i <= K; i += DV_THREADS)
         tokens[(size_t)b * (K + 1) + i] = i < stand ? __ldcg(drafts + (size_t)b * K + i) : i == stand ? next : -1;
@@ -180,16 +206,15 @@ __global__ void __launch_bounds__(DV_THREADS) verify_drafts_kernel(int* accepted
     }
 }
 
-// Stretches of a row: of at least 1,024 tokens, about eight blocks to an SM in all.
+// Stretches of a row: 1,024 tokens while that fills no more than two blocks to an SM, 4,096 (what a block looks through at once) beyond.
 static int verify_chunks(int seqs, int vocab) {
     int chunks = (vocab + 1023) / 1024;
-    const int most = (8 * ti_sm_count() + seqs - 1) / seqs;
-    if (chunks > most) chunks = most;
+    if ((long long)chunks * seqs > 2LL * ti_sm_count()) chunks = (vocab + 4095) / 4096;
     if (chunks > DV_MAX_CHUNKS) chunks = DV_MAX_CHUNKS;
-    return chunks < 1 ? 1 : chunks;
+    return chunks;
 }
 
-extern "C" long long ti_verify_drafts_workspace(int seqs) { return seqs > 0 ? (long long)seqs * DV_MAX_CHUNKS * 16 : 0; }
+extern "C" long long ti_verify_drafts_workspace(int seqs) { return seqs > 0 ? (long long)seqs * DV_MAX_CHUNKS * 8 : 0; }
 
 // p [B, K + 1, vocab] and q [B, K, vocab] (or null) float with strides in elements, drafts [B, K], uniforms [B, K + 1], counts [B] or null; sums:
 // ti_verify_drafts_workspace bytes; tickets [B] words that are zero before the first launch (the kernel leaves them zero).

@@ -8,20 +8,33 @@
 // the sums in the order of the ranks. A filter is a radix select over the 56-bit key (descending logit, then id): a pass counts (or adds the 2^40
 // fixed-point masses of) the digits of the keys that are still in question, every block adds up its share of the bins over the cluster, and the one
 // whose share holds the target names the digit; a pass whose bin is kept whole ends it.
+// The best few (up to half as many as there are groups of eight threads, what sampling mostly asks for) need none of that: the top_k-th largest of the
+// groups' maxima bounds the row's top_k-th largest from below, the few tokens that reach it are exchanged, and each finds its rank by comparisons.
 #include "sampling_rule.cuh"
 
 #define PB_THREADS 512
 #define PB_WARPS (PB_THREADS / 32)
 #define PB_BINS 2048
 #define PB_HELD 16384                // logits of a block's share that are held
+#define PB_TOPS (PB_THREADS / 8)     // groups of eight threads of a block
+#define PB_BEST 512                  // tokens that reach the bound, of a block and of the row (both lists lie where the bins do)
 
-// exp((l - max) / T) with 1 / T as the sum of two 32-bit numbers: the rounding of the quotient alone, not of 1 / T as well.
+// exp((l - max) / T) = 2^((l - max) log2(e) / T), the factor as the sum of two 32-bit numbers: the rounding of the product alone, not of the factor as
+// well. What lies below 2^-126 becomes 0; a masked logit's difference, -inf or NaN, is held to a finite one. (expf with its range reduction took
+// 18 instructions of a token where this takes five, and instructions bounded the kernel.)
 struct Temper {
-    float inv, rest;
+    float inv;                                               // 1 / T, for the sampler's weights
+    float factor, rest;                                      // log2(e) / T
 };
 __device__ __forceinline__ float tempered(float l, float maxl, const Temper& t) {
-    const float d = l == maxl ? 0.f : fmaxf(l - maxl, -3e38f);           // (+inf) - (+inf) too; -inf times the rest would be +inf or NaN
-    return expf(fmaf(d, t.inv, d * t.rest));
+    const float d = fmaxf(l - maxl, -3e38f);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(d, t.factor, d * t.rest)));
+    return e;
+}
+__device__ __forceinline__ float logit_of(u64 key) {         // desc_key's inverse
+    const u32 asc = ~(u32)(key >> SM_ID_BITS);
+    return __uint_as_float((asc & 0x80000000u) ? asc ^ 0x80000000u : ~asc);
 }
 
 // Inclusive scan over the block; `scratch`: PB_WARPS words.
@@ -47,13 +60,17 @@ __device__ __forceinline__ u64 pb_scan(u64 v, u64* scratch, u64& total) {
 }
 
 template <int C>
-__global__ void __launch_bounds__(PB_THREADS) probabilities_kernel(float* out, long long ldo, const float* logits, long long ld, int vocab, int per,
+__global__ void __launch_bounds__(PB_THREADS, 3) probabilities_kernel(float* out, long long ldo, const float* logits, long long ld, int vocab, int per,
                                                                    Temper temper, int top_k, float top_p, bool held, bool masses) {
     extern __shared__ __align__(16) unsigned char pb_smem[];
     __shared__ float scratch[33];
     __shared__ u64 scan[PB_WARPS];
-    __shared__ float x_max, x_sum;                           // this block's, for the cluster
+    __shared__ float x_tops[PB_TOPS], x_sum;                 // this block's, for the cluster
     __shared__ u64 x_total, x_found[3];
+    __shared__ u32 x_best;
+    __shared__ __align__(16) float tops[PB_TOPS * C];
+    __shared__ float bar;
+    __shared__ u32 first_of[C + 1];
     float* copy = reinterpret_cast<float*>(pb_smem);
     u32* hist = reinterpret_cast<u32*>(pb_smem + (held ? (size_t)per * 4 : 0));          // counts, or the low halves of masses; then the high ones
     const unsigned rank = C > 1 ? cluster_rank() : 0u;
@@ -78,32 +95,59 @@ __global__ void __launch_bounds__(PB_THREADS) probabilities_kernel(float* out, l
         }
         __syncthreads();
     }
-    // f(place in the share, logit) over the share; NaN counts as masked.
+    // f(place in the share, logit) over the share; `each` takes NaN for a masked logit, `each_raw` leaves that to f.
     const float* src = held ? copy : row + lo;
     const bool wide = held || row_wide;
     auto clean = [](float l) { return l == l ? l : -INFINITY; };
-    auto each = [&](auto f) {
+    auto each_raw = [&](auto f) {
         const int n4 = wide ? n >> 2 : 0;
+#pragma unroll 2
         for (int i = threadIdx.x; i < n4; i += PB_THREADS) {
             const float4 v = reinterpret_cast<const float4*>(src)[i];
-            f(4 * i, clean(v.x)); f(4 * i + 1, clean(v.y)); f(4 * i + 2, clean(v.z)); f(4 * i + 3, clean(v.w));
+            f(4 * i, v.x); f(4 * i + 1, v.y); f(4 * i + 2, v.z); f(4 * i + 3, v.w);
         }
-        for (int i = 4 * n4 + threadIdx.x; i < n; i += PB_THREADS) f(i, clean(src[i]));
+        for (int i = 4 * n4 + threadIdx.x; i < n; i += PB_THREADS) f(i, src[i]);
     };
+    auto each = [&](auto f) { each_raw([&](int i, float l) { f(i, clean(l)); }); };
 
+    // The groups' maxima: of warps where few best are asked for, of eight threads else.
+    const int group_log = top_k <= PB_WARPS * C / 2 || top_k >= vocab ? 5 : 3, tops_here = PB_THREADS >> group_log, tops_all = tops_here * C;
     float maxl = -INFINITY;
-    each([&](int, float l) { maxl = fmaxf(maxl, l); });
-    maxl = block_max(maxl, scratch);
-    if (C > 1) {
-        if (threadIdx.x == 0) x_max = maxl;
-        sync_cluster();
+    each_raw([&](int, float l) { maxl = fmaxf(maxl, l); });
 #pragma unroll
-        for (int r = 0; r < C; ++r) maxl = fmaxf(maxl, ld_remote(&x_max, (unsigned)r));
+    for (int o = 1; o < 32; o <<= 1)
+        if (o < (1 << group_log)) maxl = fmaxf(maxl, __shfl_xor_sync(0xffffffffu, maxl, o));
+    if ((threadIdx.x & ((1 << group_log) - 1)) == 0) x_tops[threadIdx.x >> group_log] = maxl;
+    if (threadIdx.x == 0) x_best = 0;
+    sync_cluster();
+    maxl = -INFINITY;
+    if ((int)threadIdx.x < tops_all) {                       // every group's maximum of the whole row
+        const int i = threadIdx.x, from = i >> (9 - group_log);
+        tops[i] = maxl = C > 1 ? ld_remote(&x_tops[i & (tops_here - 1)], (unsigned)from) : x_tops[i];
     }
-
+    maxl = block_max(maxl, scratch);
+    // Equal infinities are a difference of 0 (and a choice among them alone): the row as its logits' signs.
+    const bool endless = maxl == INFINITY;
     u64 bound = ~0ull;
     auto key_of = [&](int i, float l) { return ((u64)desc_key(l) << SM_ID_BITS) | (u64)(u32)(lo + i); };
-    auto mass = [&](float l) { return l == maxl ? 1ull << 40 : token_weight(W_MASS, l, maxl, temper.inv); };
+    // The sampler's weight of a token (token_weight), by parts of 32 bits.
+    auto parts_of = [&](float l) { return fixed_parts(l == maxl ? 1.f : expf((l - maxl) * temper.inv)); };
+    auto mass = [&](float l) { const Fixed f = parts_of(l); return (u64)(((long long)f.high << 20) + f.low); };
+    auto mass_of_kept = [&] {                                // the whole cluster's, of the keys up to `bound`
+        u64 local = 0, total;
+        each([&](int i, float l) {
+            if (bound == ~0ull || key_of(i, l) <= bound) local += mass(l);
+        });
+        pb_scan(local, scan, total);
+        if (C > 1) {
+            if (threadIdx.x == 0) x_total = total;           // the selection before has been read: its last barrier stands behind
+            sync_cluster();
+            total = 0;
+#pragma unroll
+            for (int r = 0; r < C; ++r) total += ld_remote(&x_total, (unsigned)r);
+        }
+        return total;
+    };
     auto select = [&](bool by_mass, u64 target) {
         auto width = [](int pass) { return pass < 2 ? 11 : pass == 2 ? 10 : 8; };        // the logit's 32 bits, then the id's 24
         u64 prefix = 0, base = 0;
@@ -171,47 +215,158 @@ __global__ void __launch_bounds__(PB_THREADS) probabilities_kernel(float* out, l
         }
         bound = ((prefix + 1) << shift) - 1;
     };
-    if (top_k > 0 && top_k < vocab && maxl > -INFINITY) select(false, (u64)top_k);
-    if (top_p < 1.f && maxl > -INFINITY) {
-        u64 local = 0, total;
-        each([&](int i, float l) {
-            if (key_of(i, l) <= bound) local += mass(l);
-        });
-        pb_scan(local, scan, total);
-        if (C > 1) {
-            if (threadIdx.x == 0) x_total = total;           // the selection before has been read: its last barrier stands behind
-            sync_cluster();
-            total = 0;
-#pragma unroll
-            for (int r = 0; r < C; ++r) total += ld_remote(&x_total, (unsigned)r);
-        }
-        const u64 target = (u64)ceil((double)top_p * (double)total);
-        select(true, target ? target : 1);
-    }
-
+    auto number = [&](float l) { return endless ? (l == maxl ? 1.f : 0.f) : tempered(l, maxl, temper); };
     float sum = 0.f;
-    const bool cut = bound != ~0ull;
-    each([&](int i, float l) {
-        if (!cut || key_of(i, l) <= bound) sum += tempered(l, maxl, temper);
-    });
-    sum = block_sum(sum, scratch);
-    if (C > 1) {
-        if (threadIdx.x == 0) x_sum = sum;
-        sync_cluster();
-        sum = 0.f;
+    bool summed = false;
+    const bool by_count = top_k > 0 && top_k < vocab, by_mass = top_p < 1.f;
+    auto mass_target = [&](u64 total) {
+        const u64 x = (u64)ceil((double)top_p * (double)total);
+        return x ? x : 1ull;
+    };
+    if ((by_count || by_mass) && maxl > -INFINITY) {
+        const int want = by_count ? top_k : tops_all / 2;    // for a prefix by mass alone: as many as the groups' maxima give
+        bool few = want <= tops_all / 2 && want > 0;
+        if (few) {
+            const u64 row_mass = by_count ? 0 : mass_of_kept();
+            u64* mine = reinterpret_cast<u64*>(hist);
+            u64* all = mine + PB_BEST;
+            if ((int)threadIdx.x < tops_all) {
+                const float v = tops[threadIdx.x];
+                int rank = 0;
+                for (int i = 0; i < tops_all; i += 4) {
+                    const float4 o = *reinterpret_cast<const float4*>(tops + i);
+                    const int me = (int)threadIdx.x - i;
+                    rank += (o.x > v || (o.x == v && 0 < me)) + (o.y > v || (o.y == v && 1 < me)) + (o.z > v || (o.z == v && 2 < me)) +
+                            (o.w > v || (o.w == v && 3 < me));
+                }
+                if (rank == want - 1) bar = v;
+            }
+            __syncthreads();
+            const float least = bar;
+            each_raw([&](int i, float l) {
+                if (l >= least) {
+                    const u32 at = atomicAdd(&x_best, 1u);
+                    if (at < PB_BEST) mine[at] = key_of(i, l);
+                }
+            });
+            sync_cluster();
+            if (threadIdx.x < 32) {                          // where every block's tokens begin in the row's list
+                const u32 here = (int)threadIdx.x < C ? (C > 1 ? ld_remote(&x_best, threadIdx.x) : x_best) : 0u;
+                u32 through = here;
 #pragma unroll
-        for (int r = 0; r < C; ++r) sum += ld_remote(&x_sum, (unsigned)r);
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");            // this block reads no other's memory any more
+                for (int o = 1; o < C; o <<= 1) {
+                    const u32 before = __shfl_up_sync(0xffffffffu, through, o);
+                    if ((int)threadIdx.x >= o) through += before;
+                }
+                if ((int)threadIdx.x < C) first_of[threadIdx.x + 1] = through;
+                if (threadIdx.x == 0) first_of[0] = 0;
+            }
+            __syncthreads();
+            const int total = (int)first_of[C];
+            few = total <= PB_BEST && total >= want;         // the same for the whole cluster (NaN may leave too few)
+            if (few) {
+                for (int i = threadIdx.x; i < total; i += PB_THREADS) {
+                    int r = 0;
+#pragma unroll
+                    for (int k = 1; k < C; ++k) r += (u32)i >= first_of[k];
+                    all[i] = C > 1 ? ld_remote(&mine[(u32)i - first_of[r]], (unsigned)r) : mine[i];
+                }
+                __syncthreads();
+                // Keys differ, so ranks do: what is added is added in the order of the ranks, not of the tokens' arrival. Four threads a key.
+                u64 keys[PB_BEST * 4 / PB_THREADS];
+                int ranks[PB_BEST * 4 / PB_THREADS];
+#pragma unroll
+                for (int k = 0; k < PB_BEST * 4 / PB_THREADS; ++k) {
+                    const int c = k * (PB_THREADS / 4) + ((int)threadIdx.x >> 2);
+                    keys[k] = ~0ull;
+                    ranks[k] = 0;
+                    if (k * (PB_THREADS / 4) < total) {
+                        if (c < total) {
+                            keys[k] = all[c];
+                            for (int i = threadIdx.x & 3; i < total; i += 4) ranks[k] += all[i] < keys[k];
+                        }
+                        ranks[k] += __shfl_xor_sync(0xffffffffu, ranks[k], 1);
+                        ranks[k] += __shfl_xor_sync(0xffffffffu, ranks[k], 2);
+                    }
+                }
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < PB_BEST * 4 / PB_THREADS; ++k)
+                    if (k * (PB_THREADS / 4) + ((int)threadIdx.x >> 2) < total && (threadIdx.x & 3) == 0) all[ranks[k]] = keys[k];
+                __syncthreads();
+                int kept = by_count ? top_k : total;
+                const u64 key = (int)threadIdx.x < kept ? all[threadIdx.x] : 0;
+                if (by_mass) {
+                    const u64 m = (int)threadIdx.x < kept ? mass(logit_of(key)) : 0;
+                    u64 listed;
+                    const u64 through = pb_scan(m, scan, listed), target = mass_target(by_count ? listed : row_mass);
+                    if (threadIdx.x == 0) x_found[0] = 0;
+                    __syncthreads();
+                    if (through >= target && through - m < target) x_found[0] = threadIdx.x + 1;
+                    __syncthreads();
+                    kept = (int)x_found[0];
+                    few = kept > 0;                          // else the prefix reaches beyond the list
+                }
+                if (few) {
+                    bound = all[kept - 1];
+                    sum = block_sum((int)threadIdx.x < kept ? number(logit_of(key)) : 0.f, scratch);
+                    summed = true;
+                }
+            }
+            sync_cluster();                                  // nobody reads another's list any more
+        }
+        if (!few) {
+            if (by_count) select(false, (u64)top_k);
+            if (by_mass) select(true, mass_target(mass_of_kept()));
+        }
     }
-    const float scale = maxl == -INFINITY ? 0.f : __fdiv_rn(1.f, sum);
-    auto value = [&](int i, float l) { return scale > 0.f && (!cut || key_of(i, l) <= bound) ? tempered(l, maxl, temper) * scale : 0.f; };
+    const bool cut = bound != ~0ull;
+    const float least_kept = cut ? logit_of(bound) : -INFINITY;          // (a bin kept whole ends with its last key: NaN there compares as nothing)
+    if (!summed) {
+        // Without filters the numbers themselves take their logits' places.
+        if (!cut && held) {
+            const int n4 = (n + 3) >> 2;                     // the copy's end is padded to whole vectors: beyond the share it is not used
+#pragma unroll 2
+            for (int i = threadIdx.x; i < n4; i += PB_THREADS) {
+                float4 v = reinterpret_cast<const float4*>(copy)[i];
+                v.x = number(v.x); v.y = number(v.y); v.z = number(v.z); v.w = number(v.w);
+                reinterpret_cast<float4*>(copy)[i] = v;
+                if (4 * i + 3 < n) sum += (v.x + v.y) + (v.z + v.w);
+                else sum += v.x + (4 * i + 1 < n ? v.y : 0.f) + (4 * i + 2 < n ? v.z : 0.f);
+            }
+        } else {
+            each([&](int i, float l) {
+                if (!cut || key_of(i, l) <= bound) sum += number(l);
+            });
+        }
+        sum = block_sum(sum, scratch);
+        if (C > 1) {
+            if (threadIdx.x == 0) x_sum = sum;
+            sync_cluster();
+            sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < C; ++r) sum += ld_remote(&x_sum, (unsigned)r);
+        }
+    }
+    if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");     // this block reads no other's memory any more
+    const float scale = __fdiv_rn(1.f, sum);
     const int n4 = wide && out_wide ? n >> 2 : 0;
-    for (int i = threadIdx.x; i < n4; i += PB_THREADS) {
-        const float4 v = reinterpret_cast<const float4*>(src)[i];
-        *reinterpret_cast<float4*>(p + lo + 4 * i) = make_float4(value(4 * i, clean(v.x)), value(4 * i + 1, clean(v.y)), value(4 * i + 2, clean(v.z)),
-                                                                 value(4 * i + 3, clean(v.w)));
-    }
-    for (int i = 4 * n4 + threadIdx.x; i < n; i += PB_THREADS) p[lo + i] = value(i, clean(src[i]));
+    auto write = [&](auto value) {
+#pragma unroll 2
+        for (int i = threadIdx.x; i < n4; i += PB_THREADS) {
+            const float4 v = reinterpret_cast<const float4*>(src)[i];
+            *reinterpret_cast<float4*>(p + lo + 4 * i) = make_float4(value(4 * i, v.x), value(4 * i + 1, v.y), value(4 * i + 2, v.z), value(4 * i + 3, v.w));
+        }
+        for (int i = 4 * n4 + threadIdx.x; i < n; i += PB_THREADS) p[lo + i] = value(i, src[i]);
+    };
+    if (maxl == -INFINITY) write([&](int, float) { return 0.f; });
+    else if (!cut && held) write([&](int, float e) { return e * scale; });
+    else if (!cut) write([&](int, float l) { return number(l) * scale; });
+    else write([&](int i, float l) {
+        l = clean(l);
+        if (l < least_kept) return 0.f;                      // all but a few end here
+        return key_of(i, l) <= bound ? number(l) * scale : 0.f;
+    });
     if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");       // nor any other this one's
 }
 
@@ -251,8 +406,8 @@ extern "C" int ti_probabilities(float* out, long long ldo, const float* logits, 
     TI_REQUIRE(temperature > 0.f, "probabilities: temperature must be > 0");
     TI_REQUIRE(top_k >= 0, "probabilities: top_k must be >= 0");
     TI_REQUIRE(top_p > 0.f && top_p <= 1.f, "probabilities: top_p must be in (0, 1]");
-    const double inv = 1.0 / (double)temperature;
-    const Temper temper{(float)inv, (float)(inv - (double)(float)inv)};
+    const double factor = 1.4426950408889634 / (double)temperature;
+    const Temper temper{1.0f / temperature, (float)factor, (float)(factor - (double)(float)factor)};
     // As few blocks a row as can hold it; more while the rows leave SMs idle and a share stays above 2,048.
     int share = 1;
     while (share < 8 && ((vocab + share - 1) / share > PB_HELD || (n_rows * share * 2 <= ti_sm_count() && vocab / share > 4096))) share *= 2;
