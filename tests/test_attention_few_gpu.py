@@ -177,7 +177,7 @@ def test_refusals(ops):
     ops.attention_few(**base)
     ws = torch.empty(16, dtype=torch.uint8, device="cuda")
     for change in (dict(q=d["q"].float()), dict(q=d["q"].cpu()), dict(out=base["out"][:1]), dict(nkv=3), dict(nq=6), dict(head_dim=32), dict(page_size=32),
-                   dict(kv_lens=d["lens"].long()), dict(cu_seqlens=d["cu"][:1]), dict(seq_slots=d["table"][0]), dict(workspace=ws), dict(window=-1),
+                   dict(kv_lens=d["lens"].long()), dict(cu_seqlens=d["cu"][:1]), dict(seq_slots=d["table"][0]), dict(workspace=ws), dict(window=-1), dict(scale=0.0), dict(scale=-1.0),
                    dict(v_cache=d["v"][:1]), dict(max_new=-1), dict(q=d["q"].transpose(0, 1).contiguous().transpose(0, 1)), dict(block_table=d["table"][0])):
         with pytest.raises(ops.KernelError):
             ops.attention_few(**{**base, **change})

@@ -14,6 +14,8 @@
 // before the first visible key may hold anything: their scores are replaced and their values zeroed.
 #include "even_runs.cuh"
 #include "mma_util.cuh"
+#include "tcgen05.cuh"
+#include "tensor_map.h"
 
 #define AF_PAGE 64
 #define AF_THREADS 128
@@ -35,21 +37,40 @@ __device__ __forceinline__ FewShape few_shape(int T, int L, int window, int grou
 template <int D> struct FewSmem {
     static constexpr int STAGES = D <= 128 ? 3 : 2;
     static constexpr int TILE = AF_PAGE * D;
-    static constexpr size_t BYTES = (size_t)STAGES * 2 * TILE * sizeof(bf16);
+    // Heads of whole 64 elements come by TMA, as columns of [64 keys, 64 elements] in rows of 128 swizzled bytes; others by 16-byte copies.
+    static constexpr bool TMA = D % 64 == 0;
+    static constexpr size_t BYTES = (size_t)STAGES * 2 * TILE * sizeof(bf16) + (TMA ? 1024 : 0);
 };
+// The 16-byte piece c of key `row` in a tile, in elements.
+template <int D> __device__ __forceinline__ int few_at(int row, int c) {
+    if (FewSmem<D>::TMA) return (c >> 3) * (AF_PAGE * 64) + row * 64 + (((c & 7) ^ (row & 7)) << 3);
+    return (row * (D / 8) + swz<D>(row, c)) * 8;
+}
+// Below 2^-126: 0.
+__device__ __forceinline__ float power2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 template <int D, int MT>
-__global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_kernel(bf16* out, const bf16* q, const bf16* k_cache, const bf16* v_cache,
-                                                                                     const int* block_table, int table_stride, const int* seq_slots,
+__global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                                     const __grid_constant__ CUtensorMap map_v, bf16* out, const bf16* q,
+                                                                                     const bf16* k_cache, const bf16* v_cache, const int* block_table, int table_stride, const int* seq_slots,
                                                                                      const int* cu, const int* kv_lens, float* ws_o, float* ws_ml,
-                                                                                     long long* units, float scale_log2e, int B, int nq, int nkv, int window) {
+                                                                                     long long* units, int* status, float scale_log2e, int B, int nq, int nkv, int window) {
     constexpr int M = 16 * MT, WK = 4 / MT, KS = D / 16, NT = D / 8, CPR = D / 8;
     typedef FewSmem<D> SM;
     extern __shared__ __align__(128) unsigned char af_smem[];
     __shared__ long long s_units[AF_MAX_SEQS + 1];
     __shared__ long long s_scan[AF_THREADS / 32];
     __shared__ float s_ml[WK][M][2];
-    bf16* ring = reinterpret_cast<bf16*>(af_smem);
+    __shared__ __align__(8) unsigned long long s_full[SM::STAGES];
+    bf16* ring = reinterpret_cast<bf16*>(af_smem + (SM::TMA ? (1024u - (smem_u32(af_smem) & 1023u)) & 1023u : 0u));
+    if (SM::TMA && threadIdx.x == 0) {                       // the barriers below stand between this and the first use
+        for (int s = 0; s < SM::STAGES; ++s) tc::mbar_init(smem_u32(s_full + s), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     const int group = nq / nkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int wr = warp % MT, wk = warp / MT;
@@ -128,20 +149,32 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
         if (next_u < hi) {
             // Tiles with new keys were written by the kernel before this one; the others stand since earlier steps.
             if ((next.s.t0 + next.tile + 1) * AF_PAGE > next.s.L - next.s.T) wait_once();
-            const size_t base = ((size_t)next_page * nkv + next.kvh) * SM::TILE;
             bf16* dst = ring + (size_t)fill * 2 * SM::TILE;
-            for (int c = threadIdx.x; c < AF_PAGE * CPR; c += AF_THREADS) {
-                const int row = c / CPR, cc = c % CPR;
-                const unsigned at = (row * CPR + swz<D>(row, cc)) * 8;
-                cp_async16(smem_u32(dst + at), k_cache + base + (size_t)c * 8);
-                cp_async16(smem_u32(dst + SM::TILE + at), v_cache + base + (size_t)c * 8);
+            if (SM::TMA) {
+                if (threadIdx.x == 0) {
+                    const unsigned bar = smem_u32(s_full + fill);
+                    const int row = (next_page * nkv + next.kvh) * AF_PAGE;
+                    tc::mbar_expect_tx(bar, 2 * SM::TILE * sizeof(bf16));
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) {
+                        tc::tma_load_2d(smem_u32(dst + c * (AF_PAGE * 64)), &map_k, c * 64, row, bar);
+                        tc::tma_load_2d(smem_u32(dst + SM::TILE + c * (AF_PAGE * 64)), &map_v, c * 64, row, bar);
+                    }
+                }
+            } else {
+                const size_t base = ((size_t)next_page * nkv + next.kvh) * SM::TILE;
+                for (int c = threadIdx.x; c < AF_PAGE * CPR; c += AF_THREADS) {
+                    const int at = few_at<D>(c / CPR, c % CPR);
+                    cp_async16(smem_u32(dst + at), k_cache + base + (size_t)c * 8);
+                    cp_async16(smem_u32(dst + SM::TILE + at), v_cache + base + (size_t)c * 8);
+                }
             }
             ++next_u;
             if (++next.tile == next.s.tiles) enter();
             else if (next_u < hi) next_page = __ldcg(next_table + next.tile);
         }
         fill = fill == SM::STAGES - 1 ? 0 : fill + 1;
-        cp_async_commit();
+        if (!SM::TMA) cp_async_commit();
     };
 #pragma unroll
     for (int s = 0; s < SM::STAGES - 1; ++s) issue();
@@ -150,8 +183,10 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
         for (int b = threadIdx.x; b <= B; b += AF_THREADS) units[b] = s_units[b];
 
     int stage = 0;
+    unsigned phase = 0;
+    bool ok = true;
     long long u = lo;
-    while (u < hi) {
+    while (ok && u < hi) {
         // One segment: the tiles of one item that lie in this block's run.
         const Place at = locate(u);
         const FewShape& s = at.s;
@@ -184,18 +219,24 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
 
         int tile = s.t0 + at.tile;
         for (; u < seg_end; ++u, ++tile) {
-            cp_async_wait<SM::STAGES - 2>();
-            __syncthreads();
+            if (SM::TMA) {
+                ok = __syncthreads_and(tc::mbar_wait(smem_u32(s_full + stage), phase, status, 28));
+                if (!ok) break;
+            } else {
+                cp_async_wait<SM::STAGES - 2>();
+                __syncthreads();
+            }
             issue();                                         // into the stage that the tile before has left
             bf16* kt = ring + (size_t)stage * 2 * SM::TILE;
             bf16* vt = kt + SM::TILE;
-            stage = stage == SM::STAGES - 1 ? 0 : stage + 1;
+            if (++stage == SM::STAGES) { stage = 0; phase ^= 1; }
             const int key_base = tile * AF_PAGE;
             if (key_base + AF_PAGE > s.L || key_base < s.first) {          // values that nobody sees may be infinite or NaN: 0 x those is NaN
                 for (int c = threadIdx.x; c < AF_PAGE * CPR; c += AF_THREADS) {
                     const int row = c / CPR, key = key_base + row;
-                    if (key >= s.L || key < s.first) *reinterpret_cast<uint4*>(vt + c * 8) = make_uint4(0, 0, 0, 0);
+                    if (key >= s.L || key < s.first) *reinterpret_cast<uint4*>(vt + few_at<D>(row, c % CPR)) = make_uint4(0, 0, 0, 0);
                 }
+                if (SM::TMA) tc::fence_async_smem();
                 __syncthreads();
             }
             float sc[2 * MT][4];
@@ -210,42 +251,50 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
                 for (int nb = 0; nb < MT; ++nb) {
                     const int row = (wk * MT + nb) * 16 + (mat >> 1) * 8 + r8;
                     unsigned kb[4];
-                    ldmatrix_x4(kb, smem_u32(kt + (row * CPR + swz<D>(row, 2 * ks + (mat & 1))) * 8));
+                    ldmatrix_x4(kb, smem_u32(kt + few_at<D>(row, 2 * ks + (mat & 1))));
                     mma16816(sc[2 * nb], qf[ks], kb[0], kb[1]);
                     mma16816(sc[2 * nb + 1], qf[ks], kb[2], kb[3]);
                 }
+            // Maxima of the unscaled scores (the scale, which is positive, is taken with the exponent); a tile at the run's or the window's edge has
+            // its scores replaced first.
             float mx0 = -INFINITY, mx1 = -INFINITY;
-            const bool edge = key_base + AF_PAGE > s.L - s.T + 1 || (window > 0 && key_base < s.L - window);
-            const int key0 = key_base + wk * MT * 16 + 2 * t;
+            if (key_base + AF_PAGE > s.L - s.T + 1 || (window > 0 && key_base < s.L - window)) {
+                const int key0 = key_base + wk * MT * 16 + 2 * t;
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i)
+                for (int i = 0; i < 2 * MT; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int key = key0 + 8 * i + j;
-                    const bool ok0 = !edge || (key <= pos[0] && key >= low[0]), ok1 = !edge || (key <= pos[1] && key >= low[1]);
-                    sc[i][j] = ok0 ? sc[i][j] * scale_log2e : -INFINITY;
-                    sc[i][2 + j] = ok1 ? sc[i][2 + j] * scale_log2e : -INFINITY;
-                    mx0 = fmaxf(mx0, sc[i][j]);
-                    mx1 = fmaxf(mx1, sc[i][2 + j]);
-                }
+                    for (int j = 0; j < 2; ++j) {
+                        const int key = key0 + 8 * i + j;
+                        if (key > pos[0] || key < low[0]) sc[i][j] = -INFINITY;
+                        if (key > pos[1] || key < low[1]) sc[i][2 + j] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i) {
+                mx0 = fmaxf(mx0, fmaxf(sc[i][0], sc[i][1]));
+                mx1 = fmaxf(mx1, fmaxf(sc[i][2], sc[i][3]));
+            }
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
             mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
             mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-            const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+            const float n0 = fmaxf(m0, mx0 * scale_log2e), n1 = fmaxf(m1, mx1 * scale_log2e);
             const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-            const float c0 = exp2f(m0 - b0), c1 = exp2f(m1 - b1);
-            m0 = n0; m1 = n1;
-            l0 *= c0; l1 *= c1;
+            if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {             // most tiles leave the maxima, and then the sums, as they are
+                const float c0 = power2(m0 - b0), c1 = power2(m1 - b1);
+                l0 *= c0; l1 *= c1;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) { o[i][0] *= c0; o[i][1] *= c0; o[i][2] *= c1; o[i][3] *= c1; }
+                for (int i = 0; i < NT; ++i) { o[i][0] *= c0; o[i][1] *= c0; o[i][2] *= c1; o[i][3] *= c1; }
+            }
+            m0 = n0; m1 = n1;
 #pragma unroll
             for (int nb = 0; nb < MT; ++nb) {
                 unsigned pf[4];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float* x = sc[2 * nb + h];
-                    x[0] = exp2f(x[0] - b0); x[1] = exp2f(x[1] - b0); x[2] = exp2f(x[2] - b1); x[3] = exp2f(x[3] - b1);
+                    x[0] = power2(fmaf(x[0], scale_log2e, -b0)); x[1] = power2(fmaf(x[1], scale_log2e, -b0));
+                    x[2] = power2(fmaf(x[2], scale_log2e, -b1)); x[3] = power2(fmaf(x[3], scale_log2e, -b1));
                     l0 += x[0] + x[1];
                     l1 += x[2] + x[3];
                     pf[2 * h] = pack_bf16(x[0], x[1]);
@@ -255,12 +304,13 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
 #pragma unroll
                 for (int c = 0; c < NT; c += 2) {
                     unsigned vb[4];
-                    ldmatrix_x4_trans(vb, smem_u32(vt + (row * CPR + swz<D>(row, c + (mat >> 1))) * 8));
+                    ldmatrix_x4_trans(vb, smem_u32(vt + few_at<D>(row, c + (mat >> 1))));
                     mma16816(o[c], pf, vb[0], vb[1]);
                     mma16816(o[c + 1], pf, vb[2], vb[3]);
                 }
             }
         }
+        if (!ok) break;
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
 
@@ -307,8 +357,10 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
                 if (d == 0) { ws_ml[(slot * M + r) * 2] = mm; ws_ml[(slot * M + r) * 2 + 1] = sum; }
             }
         }
+        if (SM::TMA) tc::fence_async_smem();                 // TMA fills this memory after the next barrier
     }
-    cp_async_wait<0>();
+    if (!SM::TMA) cp_async_wait<0>();
+    if (!ok) tc::drain_after_timeout();                      // a wait ran out: let what is in flight land
 }
 
 // The parts of a row that several blocks share, in ascending order: a block a (new token, head). Rows of items that one block did are done; rows
@@ -333,31 +385,40 @@ __global__ void attention_few_join_kernel(bf16* out, const int* cu, const int* k
     const int c0 = run_owner(U, u0, G), c1 = run_owner(U, u0 + s.tiles - 1, G);
     if (c0 == c1) return;
     auto slot = [&](int c) { return (size_t)run_slot(U, c, G, u0) * M + r; };
-    // The maximum over the parts by a warp's lanes (every warp for itself), then the parts in ascending order.
+    // The parts' weights, worked out by a thread each; their outputs are asked for eight at a time meanwhile, and added in ascending order.
+    extern __shared__ float weight[];
+    __shared__ float s_max[4], s_sum[4];
+    const int parts = c1 - c0 + 1, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     float mm = -INFINITY;
-    for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32) mm = fmaxf(mm, __ldcg(ws_ml + slot(c) * 2));
+    for (int c = threadIdx.x; c < parts; c += blockDim.x) mm = fmaxf(mm, __ldcg(ws_ml + slot(c0 + c) * 2));
     mm = warp_max(mm);
+    if ((threadIdx.x & 31) == 0) s_max[warp] = mm;
+    __syncthreads();
+    for (int w = 0; w < warps; ++w) mm = fmaxf(mm, s_max[w]);
     const float base = mm == -INFINITY ? 0.f : mm;
+    float sum = 0.f;
+    for (int c = threadIdx.x; c < parts; c += blockDim.x) {
+        const size_t at = slot(c0 + c);
+        const float f = exp2f(__ldcg(ws_ml + at * 2) - base);
+        weight[c] = f;
+        sum = fmaf(__ldcg(ws_ml + at * 2 + 1), f, sum);
+    }
+    sum = warp_sum(sum);
+    if ((threadIdx.x & 31) == 0) s_sum[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
+    for (int w = 0; w < warps; ++w) sum += s_sum[w];
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
     for (int d = threadIdx.x; d < D; d += blockDim.x) {
-        float sum = 0.f, acc = 0.f;
-        for (int c = c0; c <= c1; c += 4) {
-            float m[4], l[4], v[4];
+        float acc = 0.f;
+        for (int c = 0; c < parts; c += 16) {
+            float v[16];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool ok = c + k <= c1;
-                const size_t at = slot(ok ? c + k : c1);
-                m[k] = ok ? __ldcg(ws_ml + at * 2) : -INFINITY;
-                l[k] = __ldcg(ws_ml + at * 2 + 1);
-                v[k] = __ldcg(ws_o + at * D + d);
-            }
+            for (int k = 0; k < 16; ++k) v[k] = c + k < parts ? __ldcg(ws_o + slot(c0 + c + k) * D + d) : 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float f = exp2f(m[k] - base);
-                sum = fmaf(l[k], f, sum);
-                acc = fmaf(v[k], f, acc);
-            }
+            for (int k = 0; k < 16; ++k) acc = fmaf(v[k], c + k < parts ? weight[c + k] : 0.f, acc);
         }
-        dst[d] = __float2bfloat16_rn(sum > 0.f ? acc / sum : 0.f);
+        dst[d] = __float2bfloat16_rn(acc * inv);
     }
 }
 
@@ -373,7 +434,7 @@ extern "C" long long ti_attention_few_workspace(int B, int max_new, int nq, int 
 
 template <int D, int MT>
 static int launch_few(bf16* out, const bf16* q, const bf16* k, const bf16* v, const int* table, int table_stride, const int* seq_slots, const int* cu,
-                      const int* kv_lens, void* ws, float scale, int B, int nq, int nkv, int max_new, int window, cudaStream_t stream) {
+                      const int* kv_lens, void* ws, int* status, float scale, int B, int nq, int nkv, int max_new, int pages, int window, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
         cudaError_t e = cudaFuncSetAttribute(attention_few_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FewSmem<D>::BYTES);
@@ -385,25 +446,38 @@ static int launch_few(bf16* out, const bf16* q, const bf16* k, const bf16* v, co
     long long* units = (long long*)ws;
     float* ws_o = (float*)(units + AF_MAX_SEQS + 2);
     float* ws_ml = ws_o + (size_t)2 * G * M * D;
-    ti_launch(attention_few_kernel<D, MT>, dim3(G), dim3(AF_THREADS), FewSmem<D>::BYTES, stream, out, q, k, v, table, table_stride, seq_slots, cu, kv_lens,
-              ws_o, ws_ml, units, scale * 1.4426950408889634f, B, nq, nkv, window);
+    CUtensorMap map_k = {}, map_v = {};
+    if (FewSmem<D>::TMA) {
+        const unsigned long long dims[2] = {(unsigned long long)D, (unsigned long long)pages * nkv * AF_PAGE}, strides[1] = {(unsigned long long)D * 2};
+        const unsigned box[2] = {64, AF_PAGE};
+        if (int rc = ti_tensor_map_bf16(&map_k, k, 2, dims, strides, box, true)) return rc;
+        if (int rc = ti_tensor_map_bf16(&map_v, v, 2, dims, strides, box, true)) return rc;
+    }
+    ti_launch(attention_few_kernel<D, MT>, dim3(G), dim3(AF_THREADS), FewSmem<D>::BYTES, stream, map_k, map_v, out, q, k, v, table, table_stride, seq_slots, cu,
+              kv_lens, ws_o, ws_ml, units, status, scale * 1.4426950408889634f, B, nq, nkv, window);
     if (int rc = ti_check_launch("attention_few")) return rc;
-    ti_launch(attention_few_join_kernel, dim3(max_new * nq, B), dim3(D <= 32 ? 32 : D <= 64 ? 64 : 128), 0, stream, out, cu, kv_lens, ws_o, ws_ml, units, B, nq, nkv, D, M,
+    ti_launch(attention_few_join_kernel, dim3(max_new * nq, B), dim3(D <= 32 ? 32 : D <= 64 ? 64 : 128), (size_t)G * sizeof(float), stream, out, cu, kv_lens, ws_o, ws_ml, units, B, nq, nkv, D, M,
               window, G);
     return ti_check_launch("attention_few_join");
 }
 
 // q [tokens, nq, D] and out [tokens, nq * D]; the tokens of sequence b are cu[b] to cu[b + 1], at most max_new; kv_lens[b] its length with them; its
-// pages are row seq_slots[b] of block_table. `ws`: ti_attention_few_workspace bytes, 16-byte aligned. Returns 2 for sizes outside what it takes.
+// pages are row seq_slots[b] of block_table (of a pool of `pages`). `status`: the word of bounded waits. `ws`: ti_attention_few_workspace bytes, 16-byte aligned. Returns 2 for sizes outside what it takes.
 extern "C" int ti_attention_few(void* out, const void* q, const void* k_cache, const void* v_cache, const int* block_table, int table_stride,
-                                const int* seq_slots, const int* cu, const int* kv_lens, void* ws, long long ws_bytes, float scale, int B, int nq,
-                                int nkv, int D, int page_size, int max_new, int window, cudaStream_t stream) {
+                                const int* seq_slots, const int* cu, const int* kv_lens, void* ws, long long ws_bytes, int* status, float scale, int B, int nq,
+                                int nkv, int D, int page_size, int max_new, int pages, int window, cudaStream_t stream) {
     if (B == 0 || max_new == 0) return 0;
     TI_REQUIRE(B > 0 && max_new > 0 && nq > 0 && nkv > 0 && D > 0 && window >= 0, "attention_few: %d sequences, %d new tokens, %d / %d heads of %d", B,
                max_new, nq, nkv, D);
+    TI_REQUIRE(scale > 0.f, "attention_few: scale must be positive");
     if (page_size != AF_PAGE || nq % nkv != 0 || B > AF_MAX_SEQS || (long long)max_new * nq > 65535LL * 1024 || nq / nkv > 1024) {
         ti_fail("attention_few takes pages of %d and at most %d sequences; got pages of %d, %d sequences, %d / %d heads", AF_PAGE, AF_MAX_SEQS, page_size,
                 B, nq, nkv);
+        return 2;
+    }
+    TI_REQUIRE(status != nullptr && aligned16(k_cache) && aligned16(v_cache), "attention_few: pages must be 16-byte aligned");
+    if ((long long)pages * nkv * AF_PAGE > 0x7fffffffLL) {
+        ti_fail("attention_few: a pool of %d pages of %d heads has more than 2^31 rows", pages, nkv);
         return 2;
     }
     TI_REQUIRE(ws != nullptr && aligned16(ws) && ws_bytes >= ti_attention_few_workspace(B, max_new, nq, nkv, D), "attention_few: work space of %lld bytes, %lld needed",
@@ -411,7 +485,7 @@ extern "C" int ti_attention_few(void* out, const void* q, const void* k_cache, c
     const int M = few_rows(max_new * (nq / nkv), D);
 #define AF_LAUNCH(d, mt) \
     return launch_few<d, mt>((bf16*)out, (const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_table, table_stride, seq_slots, cu, kv_lens, ws, \
-                             scale, B, nq, nkv, max_new, window, stream)
+                             status, scale, B, nq, nkv, max_new, pages, window, stream)
 #define AF_CASE(d)                          \
     case d:                                 \
         if (M == 16) AF_LAUNCH(d, 1);       \

@@ -273,7 +273,7 @@ _SIGNATURES.update({
 _SIGNATURES.update({
     "ti_linear4": [_P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _F, _F, _I, _P, _P, _P],
     "ti_quantize4": [_P, _L, _I, _P, _P, _I, _P, _I, _I, _I, _P],
-    "ti_attention_few": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _L, _F, _I, _I, _I, _I, _I, _I, _I, _P],
+    "ti_attention_few": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _L, _P, _F, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "ti_probabilities": [_P, _L, _P, _L, _I, _I, _F, _I, _F, _P],
     "ti_verify_drafts": [_P, _P, _P, _L, _L, _P, _L, _L, _P, _P, _P, _I, _I, _I, _P, _P, _P],
     "ti_match_drafts": [_P, _P, _P, _P, _P, _I, _I, _P],

@@ -1070,8 +1070,9 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
     if workspace is None:
         workspace = _workspace("attention_few", attention_few_workspace(seqs, max_new, nq, nkv, head_dim), q.device, stream)
     check(lib().ti_attention_few(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                                 seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), workspace.data_ptr(), workspace.numel(), scale, seqs, nq,
-                                 nkv, head_dim, page_size, max_new, window or 0, stream), "attention_few")
+                                 seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                                 status_word().data_ptr(), scale, seqs, nq, nkv, head_dim, page_size, max_new, k_cache.shape[0], window or 0, stream),
+          "attention_few")
 
 
 def probabilities(out, logits, temperature, top_k=0, top_p=1.0):
