@@ -107,11 +107,12 @@ def test_windows(ops, window):
     check(ops, [(6, 1500), (6, 7), (3, 64), (16, 700)], 8, 4, 128, window, seed=window)
 
 
-def test_many_sequences_of_unequal_lengths(ops):
+@pytest.mark.parametrize("seqs", [300, 513, 1030])
+def test_many_sequences_of_unequal_lengths(ops, seqs):
     g = torch.Generator().manual_seed(4)
     runs = []
-    for _ in range(300):
-        length = int(torch.randint(1, 500, (1,), generator=g))
+    for _ in range(seqs):
+        length = int(torch.randint(1, 300, (1,), generator=g))
         runs.append((int(torch.randint(0, min(length, 6) + 1, (1,), generator=g)), length))
     check(ops, runs, 4, 2, 32)
 

@@ -19,7 +19,7 @@
 
 #define AF_PAGE 64
 #define AF_THREADS 128
-#define AF_MAX_SEQS 1024
+#define AF_MAX_SEQS 512                  // of one launch: their lengths, slots and units stand in shared memory
 
 struct FewShape {
     int T, L, first, t0, tiles, slabs;                       // new tokens, length, first visible key, first tile, tiles, slabs of rows
@@ -33,7 +33,6 @@ __device__ __forceinline__ FewShape few_shape(int T, int L, int window, int grou
     s.slabs = (T * group + M - 1) / M;
     return s;
 }
-// The joining kernel's part of the work space: [0] units in all, [1 + b] units of the sequences before b.
 template <int D> struct FewSmem {
     static constexpr int STAGES = D <= 128 ? 3 : 2;
     static constexpr int TILE = AF_PAGE * D;
@@ -58,12 +57,12 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
                                                                                      const __grid_constant__ CUtensorMap map_v, bf16* out, const bf16* q,
                                                                                      const bf16* k_cache, const bf16* v_cache, const int* block_table, int table_stride, const int* seq_slots,
                                                                                      const int* cu, const int* kv_lens, float* ws_o, float* ws_ml,
-                                                                                     long long* units, int* status, float scale_log2e, int B, int nq, int nkv, int window) {
+                                                                                     unsigned* units, int* status, float scale_log2e, int B, int nq, int nkv, int window) {
     constexpr int M = 16 * MT, WK = 4 / MT, KS = D / 16, NT = D / 8, CPR = D / 8;
     typedef FewSmem<D> SM;
     extern __shared__ __align__(128) unsigned char af_smem[];
-    __shared__ long long s_units[AF_MAX_SEQS + 1];
-    __shared__ long long s_scan[AF_THREADS / 32];
+    __shared__ unsigned s_units[AF_MAX_SEQS + 1], s_scan[AF_THREADS / 32];
+    __shared__ int s_cu[AF_MAX_SEQS + 1], s_len[AF_MAX_SEQS], s_slot[AF_MAX_SEQS];
     __shared__ float s_ml[WK][M][2];
     __shared__ __align__(8) unsigned long long s_full[SM::STAGES];
     bf16* ring = reinterpret_cast<bf16*>(af_smem + (SM::TMA ? (1024u - (smem_u32(af_smem) & 1023u)) & 1023u : 0u));
@@ -76,24 +75,29 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
     const int wr = warp % MT, wk = warp / MT;
 
     // Units before every sequence.
-    long long carry = 0;
+    unsigned carry = 0;
     for (int b0 = 0; b0 < B; b0 += AF_THREADS) {
         const int b = b0 + threadIdx.x;
-        long long v = 0;
+        unsigned v = 0;
         if (b < B) {
-            const FewShape s = few_shape(__ldcg(cu + b + 1) - __ldcg(cu + b), __ldcg(kv_lens + b), window, group, M);
-            v = (long long)s.tiles * s.slabs * nkv;
+            const int at = __ldcg(cu + b), end = __ldcg(cu + b + 1), len = __ldcg(kv_lens + b);
+            s_slot[b] = __ldcg(seq_slots + b);
+            s_cu[b] = at;
+            if (b == B - 1) s_cu[B] = end;
+            s_len[b] = len;
+            const FewShape s = few_shape(end - at, len, window, group, M);
+            v = (unsigned)(s.tiles * s.slabs * nkv);
         }
-        const long long own = v;
+        const unsigned own = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, v, o);
+            const unsigned u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
         }
         __syncthreads();
         if (lane == 31) s_scan[warp] = v;
         __syncthreads();
-        long long before = carry;
+        unsigned before = carry;
         for (int w = 0; w < AF_THREADS / 32; ++w) {
             if (w < warp) before += s_scan[w];
             carry += s_scan[w];
@@ -102,16 +106,16 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
     }
     if (threadIdx.x == 0) s_units[B] = carry;
     __syncthreads();
-    const long long U = s_units[B];
-    const int G = (int)min((long long)gridDim.x, U);
-    if ((int)blockIdx.x >= max(G, 1)) return;                // more blocks than units
-    const long long lo = G > 0 ? run_low(U, blockIdx.x, G) : 0, hi = G > 0 ? run_low(U, blockIdx.x + 1, G) : 0;
+    const unsigned U = s_units[B], G = min(gridDim.x, U);
+    if (blockIdx.x >= max(G, 1u)) return;                    // more blocks than units
+    const Runs runs(U, max(G, 1u));
+    const unsigned lo = runs.low(blockIdx.x), hi = runs.low(blockIdx.x + 1);
 
     struct Place {
         FewShape s;
         int b, kvh, slab, tile;                              // tile counts from the first visible one
     };
-    auto locate = [&](long long u) {
+    auto locate = [&](unsigned u) {
         Place p;
         int a = 0, z = B;                                    // the last sequence with units before it <= u and units of its own
         while (z - a > 1) {
@@ -119,7 +123,7 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
             if (s_units[mid] <= u) a = mid; else z = mid;
         }
         p.b = a;
-        p.s = few_shape(__ldcg(cu + a + 1) - __ldcg(cu + a), __ldcg(kv_lens + a), window, group, M);
+        p.s = few_shape(s_cu[a + 1] - s_cu[a], s_len[a], window, group, M);
         const int v = (int)(u - s_units[a]), item = v / p.s.tiles;
         p.tile = v - item * p.s.tiles;
         p.kvh = item / p.s.slabs;
@@ -132,14 +136,14 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
     auto wait_once = [&] {
         if (!waited) { pdl_enter(); waited = true; }
     };
-    long long next_u = lo;
+    unsigned next_u = lo;
     Place next{};
     int next_page = 0;
     const int* next_table = nullptr;
     auto enter = [&] {
         if (next_u < hi) {
             next = locate(next_u);
-            next_table = block_table + (size_t)__ldcg(seq_slots + next.b) * table_stride + next.s.t0;
+            next_table = block_table + (size_t)s_slot[next.b] * table_stride + next.s.t0;
             next_page = __ldcg(next_table + next.tile);
         }
     };
@@ -185,13 +189,13 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
     int stage = 0;
     unsigned phase = 0;
     bool ok = true;
-    long long u = lo;
+    unsigned u = lo;
     while (ok && u < hi) {
         // One segment: the tiles of one item that lie in this block's run.
         const Place at = locate(u);
         const FewShape& s = at.s;
-        const long long seg_end = min(hi, u + (s.tiles - at.tile));
-        const int rows = s.T * group, first_token = __ldcg(cu + at.b);
+        const unsigned seg_begin = u, seg_end = min(hi, u + (unsigned)(s.tiles - at.tile));
+        const int rows = s.T * group, first_token = s_cu[at.b];
         int pos[2], low[2];
         const bf16* qrow[2];
 #pragma unroll
@@ -333,8 +337,8 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
             }
         }
         __syncthreads();
-        const bool whole = seg_end - (u - (long long)(tile - s.t0 - at.tile)) == s.tiles && at.tile == 0;
-        const size_t slot = (size_t)blockIdx.x * 2 + (u - (tile - s.t0 - at.tile) == lo ? 0 : 1);
+        const bool whole = (int)(seg_end - seg_begin) == s.tiles;
+        const size_t slot = (size_t)blockIdx.x * 2 + (seg_begin == lo ? 0 : 1);
         const int here = min(M, rows - at.slab * M);
         for (int e = threadIdx.x; e < here * D; e += AF_THREADS) {
             const int r = e / D, d = e - r * D, col = (d + 8 * (r & 7)) % D;
@@ -363,73 +367,77 @@ __global__ void __launch_bounds__(AF_THREADS, D <= 128 ? 2 : 1) attention_few_ke
     if (!ok) tc::drain_after_timeout();                      // a wait ran out: let what is in flight land
 }
 
-// The parts of a row that several blocks share, in ascending order: a block a (new token, head). Rows of items that one block did are done; rows
-// without keys get zeros.
-__global__ void attention_few_join_kernel(bf16* out, const int* cu, const int* kv_lens, const float* ws_o, const float* ws_ml, const long long* units,
-                                          int B, int nq, int nkv, int D, int M, int window, int blocks) {
-    const int b = blockIdx.y, i = blockIdx.x / nq, head = blockIdx.x % nq, group = nq / nkv;
-    const int first_token = __ldcg(cu + b), T = __ldcg(cu + b + 1) - first_token;
-    const int L = __ldcg(kv_lens + b);
+// The parts of the rows that several blocks share, in ascending order: a warp a row, four elements a lane; blocks of (four rows, KV head, sequence).
+// Rows of items that one block did are done; rows without keys get zeros. What bounds it is one dependent load after another, so a row's maxima, sums
+// and first outputs are asked for together, and all blocks are resident at once (512 threads a block: 22 us for 64 sequences, some 6 beside the kernel before).
+#define AF_JOIN_ROWS 4
+__global__ void __launch_bounds__(32 * AF_JOIN_ROWS) attention_few_join_kernel(bf16* out, const int* cu, const int* kv_lens, const float* ws_o,
+                                                                               const float* ws_ml, const unsigned* units, int B, int nq, int nkv, int D,
+                                                                               int M, int window, int blocks) {
+    const int b = blockIdx.z, kvh = blockIdx.y, group = nq / nkv, lane = threadIdx.x & 31, row = blockIdx.x * AF_JOIN_ROWS + (threadIdx.x >> 5);
+    const int first_token = __ldcg(cu + b), T = __ldcg(cu + b + 1) - first_token, L = __ldcg(kv_lens + b);
     pdl_enter();
-    if (i >= T) return;
+    const unsigned U = __ldcg(units + B), before = __ldcg(units + b);
+    if (row >= T * group) return;
     const FewShape s = few_shape(T, L, window, group, M);
-    bf16* dst = out + ((size_t)(first_token + i) * nq + head) * D;
+    const int i = row / group;
+    bf16* dst = out + ((size_t)(first_token + i) * nq + (size_t)kvh * group + (row - i * group)) * D;
     if (s.tiles == 0) {
-        for (int d = threadIdx.x; d < D; d += blockDim.x) dst[d] = __float2bfloat16_rn(0.f);
+        for (int d = lane; d < D; d += 32) dst[d] = __float2bfloat16_rn(0.f);
         return;
     }
-    const long long U = __ldcg(units + B);
-    const int G = (int)min((long long)blocks, U);
-    const int kvh = head / group, row = i * group + head % group, slab = row / M, r = row % M;
-    const long long u0 = __ldcg(units + b) + (long long)(kvh * s.slabs + slab) * s.tiles;
-    const int c0 = run_owner(U, u0, G), c1 = run_owner(U, u0 + s.tiles - 1, G);
+    const Runs runs(U, min((unsigned)blocks, U));
+    const int slab = row / M, in = row - slab * M;
+    const unsigned u0 = before + (unsigned)((kvh * s.slabs + slab) * s.tiles), c0 = runs.owner(u0), c1 = runs.owner(u0 + s.tiles - 1);
     if (c0 == c1) return;
-    auto slot = [&](int c) { return (size_t)run_slot(U, c, G, u0) * M + r; };
-    // The parts' weights, worked out by a thread each; their outputs are asked for eight at a time meanwhile, and added in ascending order.
-    extern __shared__ float weight[];
-    __shared__ float s_max[4], s_sum[4];
-    const int parts = c1 - c0 + 1, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    float mm = -INFINITY;
-    for (int c = threadIdx.x; c < parts; c += blockDim.x) mm = fmaxf(mm, __ldcg(ws_ml + slot(c0 + c) * 2));
+    const int parts = (int)(c1 - c0 + 1);
+    // A run that begins before the item holds its part in the second slot: the first part alone may.
+    const size_t first = (size_t)runs.slot(c0, u0) * M + in, others = (size_t)2 * c0 * M + in;
+    auto at = [&](int c) { return c == 0 ? first : others + (size_t)2 * c * M; };
+    const float2* ml = reinterpret_cast<const float2*>(ws_ml);
+    float2 mine = lane < parts ? __ldcg(ml + at(lane)) : make_float2(-INFINITY, 0.f);
+    float mm = mine.x;
+    for (int c = 32 + lane; c < parts; c += 32) mm = fmaxf(mm, __ldcg(ml + at(c)).x);
     mm = warp_max(mm);
-    if ((threadIdx.x & 31) == 0) s_max[warp] = mm;
-    __syncthreads();
-    for (int w = 0; w < warps; ++w) mm = fmaxf(mm, s_max[w]);
     const float base = mm == -INFINITY ? 0.f : mm;
-    float sum = 0.f;
-    for (int c = threadIdx.x; c < parts; c += blockDim.x) {
-        const size_t at = slot(c0 + c);
-        const float f = exp2f(__ldcg(ws_ml + at * 2) - base);
-        weight[c] = f;
-        sum = fmaf(__ldcg(ws_ml + at * 2 + 1), f, sum);
-    }
-    sum = warp_sum(sum);
-    if ((threadIdx.x & 31) == 0) s_sum[warp] = sum;
-    __syncthreads();
-    sum = 0.f;
-    for (int w = 0; w < warps; ++w) sum += s_sum[w];
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    for (int d = threadIdx.x; d < D; d += blockDim.x) {
-        float acc = 0.f;
-        for (int c = 0; c < parts; c += 16) {
-            float v[16];
+    for (int d0 = 0; d0 < D; d0 += 128) {
+        const int d = d0 + 4 * lane;
+        const bool on = d < D;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+        for (int c32 = 0; c32 < parts; c32 += 32) {
+            if (c32 > 0 || d0 > 0) mine = c32 + lane < parts ? __ldcg(ml + at(c32 + lane)) : make_float2(-INFINITY, 0.f);
+            const float f = exp2f(mine.x - base);
+            sum += warp_sum(mine.y * f);
+            for (int c = 0; c < 32 && c32 + c < parts; c += 8) {
+                float4 v[8];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = c + k < parts ? __ldcg(ws_o + slot(c0 + c + k) * D + d) : 0.f;
+                for (int k = 0; k < 8; ++k)
+                    v[k] = on && c32 + c + k < parts ? __ldcg(reinterpret_cast<const float4*>(ws_o + at(c32 + c + k) * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) acc = fmaf(v[k], c + k < parts ? weight[c + k] : 0.f, acc);
+                for (int k = 0; k < 8; ++k) {
+                    const float w = __shfl_sync(0xffffffffu, f, c + k);
+                    acc.x = fmaf(v[k].x, w, acc.x); acc.y = fmaf(v[k].y, w, acc.y); acc.z = fmaf(v[k].z, w, acc.z); acc.w = fmaf(v[k].w, w, acc.w);
+                }
+            }
         }
-        dst[d] = __float2bfloat16_rn(acc * inv);
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        if (on) {
+            const __nv_bfloat162 lo2 = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi2 = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+            reinterpret_cast<__nv_bfloat162*>(dst + d)[0] = lo2;
+            reinterpret_cast<__nv_bfloat162*>(dst + d)[1] = hi2;
+        }
     }
 }
 
 static int few_rows(int max_rows, int D) { return D > 128 || max_rows <= 16 ? 16 : max_rows <= 32 ? 32 : 64; }
 static int few_blocks(int D) { return (D <= 128 ? 2 : 1) * ti_sm_count(); }
 
-// Bytes of the work space: 64-bit words for the units before each sequence, then two slots of rows a block.
+// Bytes of the work space: the units before each sequence, then two slots of rows a block.
 extern "C" long long ti_attention_few_workspace(int B, int max_new, int nq, int nkv, int D) {
     if (B <= 0 || max_new <= 0 || nq <= 0 || nkv <= 0 || D <= 0) return 0;
     const long long M = few_rows(max_new * (nq / nkv), D), slots = 2LL * few_blocks(D);
-    return 8LL * (AF_MAX_SEQS + 2) + slots * M * (D + 2) * 4;
+    return 4LL * (AF_MAX_SEQS + 4) + slots * M * (D + 2) * 4;
 }
 
 template <int D, int MT>
@@ -443,8 +451,8 @@ static int launch_few(bf16* out, const bf16* q, const bf16* k, const bf16* v, co
     }
     constexpr int M = 16 * MT;
     const int G = few_blocks(D);
-    long long* units = (long long*)ws;
-    float* ws_o = (float*)(units + AF_MAX_SEQS + 2);
+    unsigned* units = (unsigned*)ws;
+    float* ws_o = (float*)(units + AF_MAX_SEQS + 4);
     float* ws_ml = ws_o + (size_t)2 * G * M * D;
     CUtensorMap map_k = {}, map_v = {};
     if (FewSmem<D>::TMA) {
@@ -456,8 +464,8 @@ static int launch_few(bf16* out, const bf16* q, const bf16* k, const bf16* v, co
     ti_launch(attention_few_kernel<D, MT>, dim3(G), dim3(AF_THREADS), FewSmem<D>::BYTES, stream, map_k, map_v, out, q, k, v, table, table_stride, seq_slots, cu,
               kv_lens, ws_o, ws_ml, units, status, scale * 1.4426950408889634f, B, nq, nkv, window);
     if (int rc = ti_check_launch("attention_few")) return rc;
-    ti_launch(attention_few_join_kernel, dim3(max_new * nq, B), dim3(D <= 32 ? 32 : D <= 64 ? 64 : 128), (size_t)G * sizeof(float), stream, out, cu, kv_lens, ws_o, ws_ml, units, B, nq, nkv, D, M,
-              window, G);
+    ti_launch(attention_few_join_kernel, dim3((max_new * (nq / nkv) + AF_JOIN_ROWS - 1) / AF_JOIN_ROWS, nkv, B), dim3(32 * AF_JOIN_ROWS), 0, stream, out, cu,
+              kv_lens, ws_o, ws_ml, units, B, nq, nkv, D, M, window, G);
     return ti_check_launch("attention_few_join");
 }
 
@@ -470,9 +478,11 @@ extern "C" int ti_attention_few(void* out, const void* q, const void* k_cache, c
     TI_REQUIRE(B > 0 && max_new > 0 && nq > 0 && nkv > 0 && D > 0 && window >= 0, "attention_few: %d sequences, %d new tokens, %d / %d heads of %d", B,
                max_new, nq, nkv, D);
     TI_REQUIRE(scale > 0.f, "attention_few: scale must be positive");
-    if (page_size != AF_PAGE || nq % nkv != 0 || B > AF_MAX_SEQS || (long long)max_new * nq > 65535LL * 1024 || nq / nkv > 1024) {
-        ti_fail("attention_few takes pages of %d and at most %d sequences; got pages of %d, %d sequences, %d / %d heads", AF_PAGE, AF_MAX_SEQS, page_size,
-                B, nq, nkv);
+    const int M = few_rows(max_new * (nq / nkv), D);
+    const long long slabs = (max_new * (long long)(nq / nkv) + M - 1) / M;
+    if (page_size != AF_PAGE || nq % nkv != 0 || nkv > 65535 || slabs * nkv * table_stride * (B < AF_MAX_SEQS ? B : AF_MAX_SEQS) >= 1LL << 31) {
+        ti_fail("attention_few takes pages of %d and fewer than 2^31 tiles of %d keys; got pages of %d, %d sequences of up to %d pages, %d new tokens, %d / %d heads",
+                AF_PAGE, AF_PAGE, page_size, B, table_stride, max_new, nq, nkv);
         return 2;
     }
     TI_REQUIRE(status != nullptr && aligned16(k_cache) && aligned16(v_cache), "attention_few: pages must be 16-byte aligned");
@@ -482,22 +492,28 @@ extern "C" int ti_attention_few(void* out, const void* q, const void* k_cache, c
     }
     TI_REQUIRE(ws != nullptr && aligned16(ws) && ws_bytes >= ti_attention_few_workspace(B, max_new, nq, nkv, D), "attention_few: work space of %lld bytes, %lld needed",
                ws_bytes, ti_attention_few_workspace(B, max_new, nq, nkv, D));
-    const int M = few_rows(max_new * (nq / nkv), D);
+    for (int b0 = 0; b0 < B; b0 += AF_MAX_SEQS) {            // the sequences in turns of as many as a launch takes
+        const int n = B - b0 < AF_MAX_SEQS ? B - b0 : AF_MAX_SEQS;
+        int rc;
 #define AF_LAUNCH(d, mt) \
-    return launch_few<d, mt>((bf16*)out, (const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_table, table_stride, seq_slots, cu, kv_lens, ws, \
-                             status, scale, B, nq, nkv, max_new, pages, window, stream)
-#define AF_CASE(d)                          \
-    case d:                                 \
-        if (M == 16) AF_LAUNCH(d, 1);       \
-        if (M == 32) AF_LAUNCH(d, 2);       \
-        AF_LAUNCH(d, 4);
-    switch (D) {
-        AF_CASE(16) AF_CASE(32) AF_CASE(48) AF_CASE(64) AF_CASE(80) AF_CASE(96) AF_CASE(112) AF_CASE(128)
-        case 256: AF_LAUNCH(256, 1);
-        default:
-            ti_fail("attention_few has no instance for head size %d", D);
-            return 2;
+    rc = launch_few<d, mt>((bf16*)out, (const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, block_table, table_stride, seq_slots + b0, cu + b0, kv_lens + b0, ws, \
+                             status, scale, n, nq, nkv, max_new, pages, window, stream)
+#define AF_CASE(d)                                   \
+    case d:                                          \
+        if (M == 16) AF_LAUNCH(d, 1);                \
+        else if (M == 32) AF_LAUNCH(d, 2);           \
+        else AF_LAUNCH(d, 4);                        \
+        break;
+        switch (D) {
+            AF_CASE(16) AF_CASE(32) AF_CASE(48) AF_CASE(64) AF_CASE(80) AF_CASE(96) AF_CASE(112) AF_CASE(128)
+            case 256: AF_LAUNCH(256, 1); break;
+            default:
+                ti_fail("attention_few has no instance for head size %d", D);
+                return 2;
+        }
+        if (rc) return rc;
     }
+    return 0;
 #undef AF_CASE
 #undef AF_LAUNCH
 }

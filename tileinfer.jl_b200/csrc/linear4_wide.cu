@@ -41,7 +41,7 @@ struct Args {
     float* parts;                                            // [slot][N tokens][256 rows]
     int* status;
     int n, out, groups, steps, chunks;                       // steps of 256 k; chunks of N tokens
-    long long units;
+    unsigned units;
     int epilogue;
     XieluParams act;
     bool y32;
@@ -77,8 +77,9 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    const int G = gridDim.x, steps = p.steps;
-    const long long U = p.units, lo = run_low(U, blockIdx.x, G), hi = run_low(U, blockIdx.x + 1, G);
+    const unsigned steps = p.steps;
+    const Runs runs(p.units, gridDim.x);
+    const unsigned lo = runs.low(blockIdx.x), hi = runs.low(blockIdx.x + 1);
     // Item = 256 rows x a chunk of tokens; the chunks of one stretch of rows follow one another, so its codes are read from memory once.
     const uintptr_t s_end = (uintptr_t)(p.scales + (size_t)p.groups * p.out), z_end = (uintptr_t)(p.zeros + (size_t)p.groups * p.out);
     // A thread's pieces of a step's scales and zeros: which group of the step, which piece.
@@ -93,8 +94,8 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
     const int z_e = S::THREADS - 1 - threadIdx.x;
     const int z_group = p.zeros != nullptr && z_e < S::GROUPS * S::ZERO_PIECES ? z_e / S::ZERO_PIECES : 1 << 30, z_piece = 16 * (z_e % S::ZERO_PIECES);
     // What is asked for next.
-    long long next_u = lo, next_item = lo / steps;
-    int next_step = (int)(lo - next_item * steps), fill = 0, next_row = (int)(next_item / p.chunks) * ROWS, next_token = (int)(next_item % p.chunks) * N;
+    unsigned next_u = lo, next_item = lo / steps;
+    int next_step = lo - next_item * steps, fill = 0, next_row = next_item / p.chunks * ROWS, next_token = next_item % p.chunks * N;
     auto ask_codes = [&](int slot, int step, int row) {      // one thread
         const unsigned bar = full0 + 8 * slot, dst = stages + slot * S::BYTES;
         mbar_expect_tx(bar, CODES + N * KC * 2);
@@ -121,11 +122,11 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
                 if (from < z_end) copy16(dst + CODES + S::X + S::GROUPS * S::PIECES * 16 + z_e * 16, from);
             }
             ++next_u;
-            if (++next_step == steps) {
+            if (++next_step == (int)steps) {
                 next_step = 0;
                 ++next_item;
-                next_row = (int)(next_item / p.chunks) * ROWS;
-                next_token = (int)(next_item % p.chunks) * N;
+                next_row = next_item / p.chunks * ROWS;
+                next_token = next_item % p.chunks * N;
             }
         }
         fill = fill == S::STAGES - 1 ? 0 : fill + 1;
@@ -133,11 +134,11 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
     };
     // Codes are no result of a step: the first ones are asked for before the wait for the kernel before.
     if (threadIdx.x == 0) {
-        long long item = next_item;
+        unsigned item = next_item;
         int step = next_step;
         for (int s = 0; s < S::STAGES - 1 && lo + s < hi; ++s) {
-            ask_codes(s, step, (int)(item / p.chunks) * ROWS);
-            if (++step == steps) { step = 0; ++item; }
+            ask_codes(s, step, item / p.chunks * ROWS);
+            if (++step == (int)steps) { step = 0; ++item; }
         }
     }
     pdl_enter();
@@ -154,13 +155,13 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
                 for (int c = 0; c < 4; ++c) acc[m][j][c] = 0.f;
     };
     clear();
-    long long item = lo / steps;
-    int step = (int)(lo - item * steps), stage = 0, row0 = (int)(item / p.chunks) * ROWS;
+    unsigned item = lo / steps;
+    int step = lo - item * steps, stage = 0, row0 = item / p.chunks * ROWS;
     unsigned phase = 0;
     bool ok = true;
     // A lane's places in a stage at its first 32 k: the swizzle turns bits 4 to 6 by the row's lowest three (bit-reversed order: g).
     const unsigned code_at = (warp * MT * 16 + g) * 128 + (g << 4) + 4 * t, x_at = CODES + g * 128 + ((t ^ g) << 4);
-    for (long long u = lo; u < hi; ++u) {
+    for (unsigned u = lo; u < hi; ++u) {
         cp_async_wait<S::STAGES - 2>();
         ok = __syncthreads_and(mbar_wait(full0 + 8 * stage, phase, p.status, 16));
         if (!ok) break;
@@ -228,11 +229,11 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
             scales += S::PIECES * 16; zeros += S::ZERO_PIECES * 16;
             s_low += 2u * (unsigned)p.out; z_low += (unsigned)p.out;
         }
-        if (step + 1 == steps || u + 1 == hi) {              // the item's end, or this run's
-            const long long u0 = item * steps;
+        if (step + 1 == (int)steps || u + 1 == hi) {              // the item's end, or this run's
+            const unsigned u0 = item * steps;
             const bool whole = u0 >= lo && u0 + steps <= hi;
-            const int token0 = (int)(item % p.chunks) * N;
-            float* part = p.parts + (size_t)run_slot(U, blockIdx.x, G, u0) * N * ROWS;
+            const int token0 = item % p.chunks * N;
+            float* part = p.parts + (size_t)runs.slot(blockIdx.x, u0) * N * ROWS;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
                     }
             clear();
         }
-        if (++step == steps) { step = 0; ++item; row0 = (int)(item / p.chunks) * ROWS; }
+        if (++step == (int)steps) { step = 0; ++item; row0 = item / p.chunks * ROWS; }
     }
     cp_async_wait<0>();
     if (!ok) drain_after_timeout();                          // a wait ran out: let what is in flight land
@@ -257,19 +258,20 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
 constexpr int JOIN_TOKENS = 8, JOIN_ROWS = 128;
 __global__ void __launch_bounds__(512) linear4_join_kernel(const Args p, int N, int G) {
     const int slot = threadIdx.x >> 7, r = (blockIdx.x & 1) * JOIN_ROWS + (threadIdx.x & 127), first = blockIdx.y * JOIN_TOKENS, chunk = first / N;
-    const long long item = (long long)(blockIdx.x >> 1) * p.chunks + chunk, u0 = item * p.steps;
-    const int c0 = run_owner(p.units, u0, G), c1 = run_owner(p.units, u0 + p.steps - 1, G), row = (blockIdx.x >> 1) * ROWS + r;
+    const Runs runs(p.units, G);
+    const unsigned u0 = ((blockIdx.x >> 1) * p.chunks + chunk) * p.steps, c0 = runs.owner(u0), c1 = runs.owner(u0 + p.steps - 1);
+    const int row = (blockIdx.x >> 1) * ROWS + r;
     pdl_enter();
     if (c0 == c1 || row >= p.out) return;
     const int token = first + 2 * slot;
     const float* part = p.parts + (size_t)(token - chunk * N) * ROWS + r;
     float s0 = 0.f, s1 = 0.f;
-    for (int c = c0; c <= c1; c += 6) {
+    for (unsigned c = c0; c <= c1; c += 6) {
         float a[6], b[6];
 #pragma unroll
         for (int k = 0; k < 6; ++k) {
             const bool ok = c + k <= c1;
-            const float* src = part + (size_t)run_slot(p.units, ok ? c + k : c1, G, u0) * N * ROWS;
+            const float* src = part + (size_t)runs.slot(ok ? c + k : c1, u0) * N * ROWS;
             a[k] = ok && token < p.n ? __ldcg(src) : 0.f;
             b[k] = ok && token + 1 < p.n ? __ldcg(src + ROWS) : 0.f;
         }
@@ -292,7 +294,7 @@ template <int NT, int GROUP> int launch(const CUtensorMap& codes, const CUtensor
         if (e != cudaSuccess) return ti_fail("linear4_wide: %s", cudaGetErrorString(e));
         configured = true;
     }
-    const int blocks = (int)(a.units < ti_sm_count() ? a.units : ti_sm_count());
+    const int blocks = (int)a.units < ti_sm_count() ? (int)a.units : ti_sm_count();
     ti_launch(linear4_wide_kernel<NT, GROUP>, dim3(blocks), dim3(S::THREADS), smem, stream, codes, x, a);
     if (int rc = ti_check_launch("linear4_wide")) return rc;
     if (a.units % blocks == 0 && (a.units / blocks) % a.steps == 0) return 0;            // every run ends with an item: no parts
@@ -324,7 +326,9 @@ int linear4_wide(void* y, long long ldy, const void* x, long long ldx, const voi
     a.scales = (const bf16*)scales; a.zeros = (const unsigned char*)zeros;
     a.y = y; a.ldy = ldy; a.parts = (float*)parts; a.status = status;
     a.n = n; a.out = out; a.groups = K / group; a.steps = (K + KC - 1) / KC; a.chunks = (n + N - 1) / N;
-    a.units = (long long)((out + ROWS - 1) / ROWS) * a.chunks * a.steps;
+    const long long units = (long long)((out + ROWS - 1) / ROWS) * a.chunks * a.steps;
+    TI_REQUIRE(units < (1LL << 31), "linear4: %d tokens x %d x %d are too many units of work", n, out, K);
+    a.units = (unsigned)units;
     a.epilogue = epilogue; a.act = act; a.y32 = epilogue == L4_EPI_F32_OUT;
 #define L4_GROUPS(nt)                                                  \
     if (group == 32) return launch<nt, 32>(map_codes, map_x, a, stream); \
