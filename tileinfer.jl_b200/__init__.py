@@ -9,5 +9,5 @@ CUDA kernels (``csrc``, loaded by ``kernels``).
 __version__ = "0.2.0"
 
 from .api import generate, generation_defaults, load_model            # noqa: E402
-from .engine import Engine                                            # noqa: E402
+from .engine import Draft, Engine                                     # noqa: E402
 from .sampling import SamplingParams                                  # noqa: E402

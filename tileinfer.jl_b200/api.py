@@ -9,7 +9,7 @@ import json
 import os
 from typing import Callable, List, Optional, Sequence, Union
 
-from .engine import Engine
+from .engine import Draft, Engine
 from .engine.generate import generate as _generate
 from .sampling import SamplingParams
 
@@ -50,10 +50,11 @@ def generation_defaults(model_dir: str, engine: Engine):
 
 def generate(model: Engine, prompts: Union[Sequence[int], Sequence[Sequence[int]]], max_new_tokens: int = 256,
              sampling: SamplingParams = SamplingParams(), stop_ids: Optional[Sequence[int]] = None, seed: int = 0,
-             on_token: Optional[Callable[[int, int], None]] = None):
+             on_token: Optional[Callable[[int, int], None]] = None, draft: Optional[Draft] = None):
     """Generate up to ``max_new_tokens`` tokens for one prompt (a list of ids; returns a list) or for
-    several (a list of lists; returns a list of lists). Stop tokens are not returned."""
+    several (a list of lists; returns a list of lists). Stop tokens are not returned. ``draft``: ``Draft(model, tokens=4)``, the
+    model with its matrices in 4 bits, which proposes a few tokens that the model then tests in one step."""
     single = len(prompts) > 0 and isinstance(prompts[0], int)
     out = _generate(model, [prompts] if single else prompts, max_new_tokens=max_new_tokens, sampling=sampling,
-                    stop_ids=stop_ids, seed=seed, on_token=on_token)
+                    stop_ids=stop_ids, seed=seed, on_token=on_token, draft=draft)
     return out[0] if single else out

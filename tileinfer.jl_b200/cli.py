@@ -68,9 +68,10 @@ OPTIONS: Dict[str, Option] = {o.name: o for o in (
     Option("backend", ("fast", "plain"), "fast", "tensor-core kernels or the plain reference kernels"),
     Option("dtype", ("bfloat16", "float32"), "bfloat16", "element type of weights, activations and cache"),
     Option("max-seqs", int, 8, "sequences per batch at most"),
+    Option("draft", int, 0, "tokens to draft a step with the model's matrices in 4 bits, for the model to test (0: none)"),
     Option("stop-ids", token_ids, None, "stop tokens instead of the configuration's EOS ids (\"\" for none)"),
 )}
-GENERATION = ("max-tokens", "max-context", "temperature", "top-k", "top-p", "seed", "backend", "dtype", "max-seqs", "stop-ids")
+GENERATION = ("max-tokens", "max-context", "temperature", "top-k", "top-p", "seed", "backend", "dtype", "max-seqs", "draft", "stop-ids")
 
 
 @dataclass(frozen=True)
@@ -143,6 +144,16 @@ def load_for_generation(model_dir: str, values):
     return engine, sampling, pick("stop-ids", stop), pick("seed", random.getrandbits(32))
 
 
+def load_draft(engine, values):
+    """The draft that ``--draft`` asks for, or None."""
+    from .engine import Draft
+    return Draft(engine, values["draft"]) if values["draft"] else None
+
+
+def drafted(draft) -> str:
+    return "" if draft is None else f"; {draft.stood} of {draft.drafted} drafted tokens stood"
+
+
 def cmd_run(positional, values) -> None:
     from .api import generate
     model_dir, prompt = positional
@@ -150,10 +161,11 @@ def cmd_run(positional, values) -> None:
     if not ids:
         raise ArgumentError("the prompt has no token ids")
     engine, sampling, stop, seed = load_for_generation(model_dir, values)
+    draft = load_draft(engine, values)
     stats = GenerationStats(sys.stdout)
-    out = generate(engine, ids, max_new_tokens=values["max-tokens"], sampling=sampling, stop_ids=stop, seed=seed, on_token=stats)
+    out = generate(engine, ids, max_new_tokens=values["max-tokens"], sampling=sampling, stop_ids=stop, seed=seed, on_token=stats, draft=draft)
     print(flush=True)
-    print(f"[{len(ids)} prompt tokens, {len(out)} generated; {stats.summary(len(out))}]", file=sys.stderr)
+    print(f"[{len(ids)} prompt tokens, {len(out)} generated; {stats.summary(len(out))}{drafted(draft)}]", file=sys.stderr)
 
 
 def cmd_generate(positional, values) -> None:
@@ -164,14 +176,15 @@ def cmd_generate(positional, values) -> None:
     if not prompts:
         raise ArgumentError("no prompts")
     engine, sampling, stop, seed = load_for_generation(model_dir, values)
+    draft = load_draft(engine, values)
     stats = GenerationStats()
     outs = generate(engine, prompts, max_new_tokens=values["max-tokens"], sampling=sampling, stop_ids=stop, seed=seed,
-                    on_token=stats)
+                    on_token=stats, draft=draft)
     for o in outs:
         print(" ".join(str(t) for t in o))
     total = sum(len(o) for o in outs)
     print(f"[{sum(len(p) for p in prompts)} prompt tokens in {len(prompts)} prompts, {total} generated; "
-          f"{stats.summary(total)}]", file=sys.stderr)
+          f"{stats.summary(total)}{drafted(draft)}]", file=sys.stderr)
 
 
 def cmd_random(positional, values) -> None:

@@ -14,6 +14,7 @@ own.
 """
 from __future__ import annotations
 
+import copy
 import json
 import os
 from typing import Dict, List, Optional, Sequence, Tuple
@@ -57,6 +58,12 @@ class Engine:
                            max_seqs=max_seqs, page_size=page_size, max_seq_len=max_context,
                            share=self.model.cache_shares(), max_step_tokens=int(max_step_tokens))
         self.max_step_tokens = int(max_step_tokens)
+        self.use_graphs = graphs
+        self.vocab_size = self.spec.vocab_size
+        self._start_planning()
+
+    def _start_planning(self) -> None:
+        """A planner for this engine's steps, and no graphs yet."""
         self.planner = StepPlanner(self.cache, self.max_step_tokens, self.device)
         self.planner.runtime = self.rt
         # A mixer may want tables of its own in the metadata of one-token steps: the first mixer of each paged
@@ -71,11 +78,9 @@ class Engine:
             plan = mixer.decode_plan(self.cache.groups[view.group_index]) if hasattr(mixer, "decode_plan") else None
             if plan is not None:
                 self.planner.attach_plan(self.cache.groups[view.group_index], plan)
-        self.use_graphs = graphs
         self._graphs: Dict[int, object] = {}
         self._logits: Dict[int, torch.Tensor] = {}
         self._graph_launches: Dict[int, int] = {}
-        self.vocab_size = self.spec.vocab_size
 
     # ---- construction
     @classmethod
@@ -95,6 +100,17 @@ class Engine:
         device = require_cuda(kw.get("device", "cuda"))
         tensors = random_tensors(tensor_declarations(config.model_spec()), seed, dtype=torch.bfloat16, device=str(device))
         return cls(config, tensors, **kw)
+
+    def twin(self, model) -> "Engine":
+        """An engine that runs ``model`` on THIS engine's sequences: the same cache, lengths and scratch buffers, with step metadata and graphs of
+        its own. The model's layers ask for the same storage (a copy of this engine's with other matrices). Steps of the two follow one another on
+        one stream; what either writes, the other reads."""
+        if model.cache_requests() != self.model.cache_requests():
+            raise ValueError("a twin's layers ask for the same storage as the engine's")
+        other = copy.copy(self)
+        other.model = model
+        other._start_planning()
+        return other
 
     # ---- sequences
     def new_sequence(self) -> int:
@@ -116,7 +132,7 @@ class Engine:
 
     # ---- the step
     def step(self, entries: Sequence[Tuple[int, Sequence[int]]], want: Optional[Sequence[Sequence[int]]] = None,
-             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+             out: Optional[torch.Tensor] = None, few: bool = False) -> torch.Tensor:
         """Run ``entries`` = [(slot, next tokens)] as one batch; returns float32 logits
         ``[wanted, vocab]`` in the order of the entries and of ``want`` (offsets into each entry's
         tokens, in any order; default: each entry's last token).
@@ -124,7 +140,10 @@ class Engine:
         A step of one token per sequence that wants exactly those tokens' logits is replayed from a CUDA
         graph and returns the graph's own output buffer, one per batch size: the next such step of the same
         batch size overwrites it, so ``clone()`` what must outlive it (or pass ``out``, which is always
-        written by launches of its own). Every other step returns a fresh tensor."""
+        written by launches of its own). Every other step returns a fresh tensor.
+
+        ``few``: the sequences bring a few tokens each (drafted runs, say): their attention is shared out over the GPU by the lengths of
+        their caches, where a prompt's is by its tokens."""
         entries = [(int(s), list(t)) for s, t in entries]
         if want is None:
             want = [[len(t) - 1] for _, t in entries]
@@ -153,11 +172,12 @@ class Engine:
             return self._decode_step(entries, want)
         logits = out if out is not None else torch.empty((n_want, self.vocab_size), dtype=torch.float32, device=self.device)
         with nvtx_range("prefill" if not decode else "step"):
-            return self._general_step(entries, want, logits, n_total)
+            return self._general_step(entries, want, logits, n_total, few)
 
-    def _general_step(self, entries, want, logits, n_total):
+    def _general_step(self, entries, want, logits, n_total, few=False):
         if n_total <= self.max_step_tokens:
             ctx = self.planner.plan(entries, want)
+            ctx.few = few
             self.model.forward(ctx, self.cache, logits)
             for s, t in entries:
                 self.cache.advance(s, len(t))

@@ -16,6 +16,7 @@ from dataclasses import dataclass
 from typing import Callable, List, Optional, Sequence
 
 from ..sampling import DeviceSampler, SamplingParams, sequence_seed
+from .drafting import decode_batch_drafted
 
 
 @dataclass
@@ -60,9 +61,12 @@ def finished(token: int, generated: int, max_new_tokens: int, stop_ids) -> str:
 
 def generate(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int = 256,
              sampling: SamplingParams = SamplingParams(), stop_ids: Optional[Sequence[int]] = None, seed: int = 0,
-             on_token: Optional[Callable[[int, int], None]] = None) -> List[List[int]]:
+             on_token: Optional[Callable[[int, int], None]] = None, draft=None) -> List[List[int]]:
     """New token ids of every request, without stop tokens. ``on_token(request, id)`` is called
-    for each new token. ``stop_ids`` defaults to the configuration's EOS ids; ``[]`` disables them."""
+    for each new token. ``stop_ids`` defaults to the configuration's EOS ids; ``[]`` disables them. ``draft``: a
+    ``drafting.Draft`` of this engine whose tokens the model tests, several a step."""
+    if draft is not None and draft.engine is not engine:
+        raise ValueError("the draft was made for another engine")
     stop = set(engine.spec.eos_token_ids if stop_ids is None else stop_ids)
     prompts = [list(p) for p in prompts]
     results: List[List[int]] = [[] for _ in prompts]
@@ -77,7 +81,10 @@ def generate(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int = 256
         try:
             sampler.reset([sequence_seed(seed, r) for r in batch])
             logits = engine.step([(slots[r], prompts[r]) for r in batch])
-            decode_batch(engine, sampler, sampling, list(batch), slots, logits, results, max_new_tokens, stop, on_token)
+            if draft is not None:
+                decode_batch_drafted(engine, draft, sampling, seed, list(batch), slots, logits, results, max_new_tokens, stop, on_token)
+            else:
+                decode_batch(engine, sampler, sampling, list(batch), slots, logits, results, max_new_tokens, stop, on_token)
             engine.check_health()
         finally:
             for r in list(slots):

@@ -56,6 +56,8 @@ class StepContext:
     max_q_len: int = 0
     max_kv_len: int = 0
     runtime: object = None              # scratch buffers for kernels that need a workspace
+    # The sequences bring a few tokens each (a drafted run): attention is shared out by the lengths of their caches.
+    few: bool = False
 
     def group(self, index: int) -> GroupMeta:
         return self.groups[index]

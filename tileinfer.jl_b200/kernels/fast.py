@@ -337,6 +337,13 @@ def attention(out, q, cache, meta, step, spec, sink=None, chunk=0, distance_bias
     [heads] float32: a slope by distance taken off, times log2(e). ``keep``: beside a window, the first ``keep`` positions stay visible."""
     if q.dtype != torch.bfloat16:
         return False
+    if getattr(step, "few", False) and not step.is_decode and sink is None and not (chunk or distance_bias2 is not None or cap or slopes2 is not None or keep) and \
+            spec.head_dim in ops.FEW_HEAD_DIMS and cache.page_size == ops.FEW_PAGE:
+        bytes_ = ops.attention_few_workspace(step.n_seqs, step.max_q_len, spec.num_heads, spec.num_kv_heads, spec.head_dim)
+        ops.attention_few(out, q, cache.k, cache.v, meta.block_table, step.seq_slots, step.cu_seqlens, step.kv_lens, spec.scale, spec.num_heads,
+                          spec.num_kv_heads, spec.head_dim, cache.page_size, step.max_q_len, window=spec.window or 0,
+                          workspace=step.runtime.buffer("attention.few", (bytes_,), torch.uint8))
+        return True
     # The entry points with a sink take it as one more argument before the stream; without a sink the plain ones are called.
     extra = (sink.data_ptr(),) if sink is not None else ()
     L = lib()

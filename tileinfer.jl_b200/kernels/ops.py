@@ -977,11 +977,17 @@ def ssm_gate_norm(out, y, z, w, eps, parts):
 LINEAR4_GROUPS = (32, 64, 128)
 
 
-def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0.0, 0.0)):
+def linear4_workspace(n: int, out_features: int, in_features: int) -> int:
+    """Bytes of work space that ``linear4`` needs for n bfloat16 tokens (0: none)."""
+    return int(lib().ti_linear4_parts(n, out_features, in_features)) if n > 8 else 0
+
+
+def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0.0, 0.0), workspace=None):
     """y [n, out] = x [n, in] Wᵀ for W[o, k] = (code - zero) * scale: ``codes`` [out, in / 8] int32 hold eight consecutive k a word (the even
     ones in its low half, the odd ones in its high half, four bits each in ascending order), ``scales`` [in / group, out] of x's type for groups of
     32, 64 or 128 k, ``zeros`` [in / group, out] uint8, or 8 for all. 32-bit sums, rounded once; with ``EPI_F32_OUT`` y is float32 and the sums
-    are not rounded. Made for steps of few tokens; any number is taken. ``quantize4`` makes the codes."""
+    are not rounded. Made for steps of few tokens; any number is taken. ``quantize4`` makes the codes. ``workspace``: ``linear4_workspace`` bytes
+    (uint8); without it one kept per stream."""
     for t, name, dtype in ((x, "x", None), (y, "y", None), (codes, "codes", torch.int32), (scales, "scales", x.dtype)):
         _need(t, name, dtype, contiguous=name in ("codes", "scales"))
     code = dtype_code(x.dtype)
@@ -1002,7 +1008,13 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
     stream = _stream()
     parts = status = None
     if n > 8 and code == BF16:
-        parts = _workspace("linear4", int(lib().ti_linear4_parts(n, out, k)), x.device, stream).data_ptr()
+        need = linear4_workspace(n, out, k)
+        if need:
+            if workspace is None:
+                workspace = _workspace("linear4", need, x.device, stream)
+            elif workspace.numel() < need or not workspace.is_cuda:
+                raise KernelError(f"linear4: work space of {workspace.numel()} bytes, {need} needed")
+            parts = workspace.data_ptr()
         status = status_word().data_ptr()
     check(lib().ti_linear4(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), n, out, k,
                            k // groups, epilogue, act[0], act[1], act[2], act[3], code, parts, status, stream), "linear4")
@@ -1038,6 +1050,9 @@ def _workspace(kind: str, nbytes: int, device, stream: int, zeroed: bool = False
         make = torch.zeros if zeroed else torch.empty
         ws = _few_ws[key] = make(max(nbytes, 4096), dtype=torch.uint8, device=device)
     return ws
+
+
+FEW_HEAD_DIMS, FEW_PAGE = (16, 32, 48, 64, 80, 96, 112, 128, 256), 64        # what attention_few takes
 
 
 def attention_few_workspace(seqs: int, max_new: int, nq: int, nkv: int, head_dim: int) -> int:

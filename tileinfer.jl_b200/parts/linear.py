@@ -40,3 +40,32 @@ class Linear:
                 return done
         ops.gemm_plain(out, x, self.weight, ops.EPI_F32_OUT)
         return out
+
+
+class Linear4(Linear):
+    """The same product with a matrix of 4 bits a weight, made from another's: codes with a scale (and, asked for, a zero) per group of ``group``
+    inputs, or of the largest smaller group that divides them. Nothing of the other is kept; there is no ``weight``."""
+
+    def __init__(self, other: Linear, group: int = 128, zeros: bool = False):
+        fit = next((g for g in sorted(ops.LINEAR4_GROUPS, reverse=True) if g <= group and other.in_features % g == 0), None)
+        if fit is None:
+            raise ValueError(f"{other.name}: {other.in_features} inputs do not divide into groups of {', '.join(map(str, ops.LINEAR4_GROUPS))} up to {group}")
+        self.rt, self.name, self.partials_name = other.rt, other.name, other.partials_name
+        self.out_features, self.in_features, w = other.out_features, other.in_features, other.weight
+        groups = self.in_features // fit
+        self.codes = torch.empty(self.out_features, self.in_features // 8, dtype=torch.int32, device=w.device)
+        self.scales = torch.empty(groups, self.out_features, dtype=w.dtype, device=w.device)
+        self.zeros = torch.empty(groups, self.out_features, dtype=torch.uint8, device=w.device) if zeros else None
+        ops.quantize4(self.codes, self.scales, w, self.zeros)
+
+    def forward(self, x: torch.Tensor, out: torch.Tensor, epilogue: int = ops.EPI_NONE, act=(0.0, 0.0, 0.0, 0.0), allow_partials: bool = False):
+        ops.linear4(out, x, self.codes, self.scales, self.zeros, epilogue, act, self._workspace(x.shape[0]))
+        return out
+
+    def forward_f32(self, x: torch.Tensor, out: torch.Tensor):
+        ops.linear4(out, x, self.codes, self.scales, self.zeros, ops.EPI_F32_OUT, workspace=self._workspace(x.shape[0]))
+        return out
+
+    def _workspace(self, n: int):
+        need = ops.linear4_workspace(n, self.out_features, self.in_features) if self.rt.dtype == torch.bfloat16 else 0
+        return self.rt.buffer("linear4.parts", (need,), torch.uint8) if need else None

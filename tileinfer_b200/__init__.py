@@ -11,5 +11,5 @@ __path__ = [_os.path.join(_os.path.dirname(_os.path.dirname(_os.path.abspath(__f
 __version__ = "0.2.0"
 
 from .api import generate, generation_defaults, load_model            # noqa: E402
-from .engine import Engine                                            # noqa: E402
+from .engine import Draft, Engine                                     # noqa: E402
 from .sampling import SamplingParams                                  # noqa: E402
