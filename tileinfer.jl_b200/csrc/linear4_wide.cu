@@ -1,7 +1,8 @@
-// Products with weights of 4 bits whose tokens come through shared memory, up to 64 at once: see linear4.cu for what is computed.
+// Products with weights of 4 bits whose tokens come through shared memory, up to 32 at once: see linear4.cu for what is computed.
 //
-// A stage holds [256 rows, 256 k] of codes, the tokens of these k (both by TMA, in swizzled rows of 128 bytes) and the rows' scales and zeros; the
-// block's warps take 16 or 32 rows each. A lane's word of codes (8 consecutive k of a row) feeds two MMAs as the rows' operand, 32 consecutive k at a
+// A stage holds [256 rows, 256 k] of codes, the tokens of these k (both by TMA, in swizzled rows of 128 bytes) and the rows' scales and zeros; one warp
+// asks for them (a thread of a computing warp that did so held up its warp and then all), sixteen take 16 rows each and go through the stages on their
+// own: no barrier of the block stands in the loop. A lane's word of codes (8 consecutive k of a row) feeds two MMAs as the rows' operand, 32 consecutive k at a
 // time, so an MMA's k lie in one group; the k of both operands are permuted alike. Rows and tokens stand in the MMAs in bit-reversed order, which
 // spreads every phase of a swizzled read over all banks.
 //
@@ -10,7 +11,7 @@
 // read back from there, took 165 us for 16 and 245 us for 64 tokens x 131,072 x 4,096: a chain of five hand-overs between warps, 100 to 250 cycles
 // each, for every 128 k.)
 //
-// The units of work, [256 rows, 256 k], are numbered along k, then over the rows (and the tokens in sixty-fours), and every SM takes an equal run of them
+// The units of work, [256 rows, 256 k], are numbered along k, then over the rows (and the tokens in thirty-twos), and every SM takes an equal run of them
 // (even_runs.cuh). Parts of a tile that several blocks share go to the work space; a second kernel adds them in the blocks' order.
 #include "linear4.cuh"
 #include "even_runs.cuh"
@@ -23,12 +24,12 @@ using namespace tc;
 
 constexpr int KC = 256, ROWS = 256, CODES = ROWS * KC / 2;
 
-// Tokens in eights (NT), warps and tiles of 16 rows a warp (MT): few tokens leave registers for many warps, many make an operand's reading worth 32 rows.
+// Tokens in eights (NT); sixteen computing warps of 16 rows, and the one that asks.
 template <int NT, int GROUP> struct Shape {
-    static constexpr int N = 8 * NT, MT = NT <= 8 ? 1 : 2, WARPS = ROWS / (16 * MT), THREADS = 32 * WARPS, GROUPS = KC / GROUP;
+    static constexpr int N = 8 * NT, WARPS = ROWS / 16, THREADS = 32 * (WARPS + 1), GROUPS = KC / GROUP;
     static constexpr int X = N * KC * 2;
     // Per group the 16-byte pieces of memory that hold its scales (zeros), wherever they begin: the place of the first in its piece is what its address says.
-    static constexpr int PIECES = 2 * ROWS / 16 + 1, ZERO_PIECES = ROWS / 16 + 1, SCALES = GROUPS * 16 * (PIECES + ZERO_PIECES);
+    static constexpr int S_ROW = 2 * ROWS + 16, Z_ROW = ROWS + 16, SCALES = GROUPS * (S_ROW + Z_ROW);
     static constexpr int BYTES = (CODES + X + SCALES + 1023) / 1024 * 1024;
     static constexpr int FIT = (224 * 1024) / BYTES, STAGES = FIT > 5 ? 5 : FIT;
 };
@@ -47,8 +48,10 @@ struct Args {
     bool y32;
 };
 
-__device__ __forceinline__ void copy16(unsigned dst, uintptr_t src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// Both addresses and the size are multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(unsigned dst, uintptr_t src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 // MMAs that the compiler may move (their results are functions of their operands), so that the next words' loads and widening stand between them.
 __device__ __forceinline__ void mma_more(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
@@ -65,15 +68,15 @@ template <int NT, int GROUP>
 __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_kernel(const __grid_constant__ CUtensorMap map_codes,
                                                                                     const __grid_constant__ CUtensorMap map_x, const Args p) {
     typedef Shape<NT, GROUP> S;
-    constexpr int MT = S::MT, N = S::N;
+    constexpr int N = S::N;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* tiles = smem_dyn + ((1024u - (smem_addr(smem_dyn) & 1023u)) & 1023u);
     const unsigned stages = smem_addr(tiles);
-    __shared__ __align__(8) unsigned long long bars[S::STAGES];
-    const unsigned full0 = smem_addr(bars);
+    __shared__ __align__(8) unsigned long long bars[2 * S::STAGES];
+    const unsigned full0 = smem_addr(bars), empty0 = full0 + 8 * S::STAGES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = reversed3(lane >> 2), t = lane & 3;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::STAGES; ++s) mbar_init(full0 + 8 * s, 1);
+        for (int s = 0; s < S::STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, S::WARPS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -81,78 +84,68 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
     const Runs runs(p.units, gridDim.x);
     const unsigned lo = runs.low(blockIdx.x), hi = runs.low(blockIdx.x + 1);
     // Item = 256 rows x a chunk of tokens; the chunks of one stretch of rows follow one another, so its codes are read from memory once.
-    const uintptr_t s_end = (uintptr_t)(p.scales + (size_t)p.groups * p.out), z_end = (uintptr_t)(p.zeros + (size_t)p.groups * p.out);
-    // A thread's pieces of a step's scales and zeros: which group of the step, which piece.
-    constexpr int S_EACH = (S::GROUPS * S::PIECES + S::THREADS - 1) / S::THREADS;
-    int s_group[S_EACH], s_piece[S_EACH];
-#pragma unroll
-    for (int k = 0; k < S_EACH; ++k) {
-        const int e = threadIdx.x + k * S::THREADS;
-        s_group[k] = e < S::GROUPS * S::PIECES ? e / S::PIECES : 1 << 30;
-        s_piece[k] = 16 * (e % S::PIECES);
-    }
-    const int z_e = S::THREADS - 1 - threadIdx.x;
-    const int z_group = p.zeros != nullptr && z_e < S::GROUPS * S::ZERO_PIECES ? z_e / S::ZERO_PIECES : 1 << 30, z_piece = 16 * (z_e % S::ZERO_PIECES);
-    // What is asked for next.
-    unsigned next_u = lo, next_item = lo / steps;
-    int next_step = lo - next_item * steps, fill = 0, next_row = next_item / p.chunks * ROWS, next_token = next_item % p.chunks * N;
-    auto ask_codes = [&](int slot, int step, int row) {      // one thread
-        const unsigned bar = full0 + 8 * slot, dst = stages + slot * S::BYTES;
-        mbar_expect_tx(bar, CODES + N * KC * 2);
-        tma_load_2d(dst, &map_codes, step * (KC / 4), row, bar);
-    };
-    auto ask = [&](bool codes) {
-        if (next_u < hi) {
-            const unsigned dst = stages + fill * S::BYTES;
-            if (threadIdx.x == 0) {
-                if (codes) ask_codes(fill, next_step, next_row);
-#pragma unroll
-                for (int a = 0; a < KC / 64; ++a) tma_load_2d(dst + CODES + a * (S::X / 4), &map_x, next_step * KC + a * 64, next_token, full0 + 8 * fill);
+    pdl_launch_dependents();
+    if (warp == S::WARPS) {
+        // ---------------------------------------------------------------- asking: a lane a copy
+        // A group's scales and zeros come as the 16-byte pieces that hold them: whole ones, none beyond the last with a byte of the tables.
+        const int q = lane & 7;                              // lanes 0 to 7: codes and tokens, 8 to 15: scales, 16 to 23: zeros of group q
+        const bool is_scale = (lane >> 3) == 1 && q < S::GROUPS, is_zero = (lane >> 3) == 2 && q < S::GROUPS && p.zeros != nullptr;
+        const unsigned char* table = is_zero ? p.zeros : reinterpret_cast<const unsigned char*>(p.scales);
+        const unsigned width = is_zero ? 1 : 2, most = is_zero ? S::Z_ROW : S::S_ROW;
+        const unsigned to = CODES + S::X + (is_zero ? S::GROUPS * S::S_ROW + q * S::Z_ROW : q * S::S_ROW);
+        const uintptr_t end = ((uintptr_t)table + (size_t)p.groups * p.out * width + 15) & ~(uintptr_t)15;
+        unsigned item = lo / steps, phase = 0;
+        int step = lo - item * steps, slot = 0;
+        int row = item / p.chunks * ROWS, token = item % p.chunks * N;
+        bool waited = false;
+        for (unsigned u = lo; u < hi; ++u) {
+            const unsigned bar = full0 + 8 * slot, dst = stages + slot * S::BYTES;
+            if (u >= lo + S::STAGES && !__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * slot, phase ^ 1, p.status, 17))) break;
+            unsigned bytes = 0;
+            uintptr_t from = 0;
+            if ((is_scale || is_zero) && step * S::GROUPS + q < p.groups) {
+                from = ((uintptr_t)table + ((size_t)(step * S::GROUPS + q) * p.out + row) * width) & ~(uintptr_t)15;
+                bytes = end - from < most ? (unsigned)(end - from) : most;
             }
-            const int left = p.groups - next_step * S::GROUPS;
-            const size_t first = (size_t)(next_step * S::GROUPS) * p.out + next_row;
-#pragma unroll
-            for (int k = 0; k < S_EACH; ++k)
-                if (s_group[k] < left) {
-                    const uintptr_t from = ((uintptr_t)(p.scales + first + (size_t)s_group[k] * p.out) & ~(uintptr_t)15) + s_piece[k];
-                    if (from < s_end) copy16(dst + CODES + S::X + (threadIdx.x + k * S::THREADS) * 16, from);
+            const unsigned all = __reduce_add_sync(0xffffffffu, bytes);
+            if (lane == 0) mbar_expect_tx(bar, CODES + N * KC * 2 + all);
+            __syncwarp();
+            if (lane == 0) tma_load_2d(dst, &map_codes, step * (KC / 4), row, bar);
+            if (bytes) bulk_load(dst + to, from, bytes, bar);
+            // Weights are no result of a step: the first stages' are asked for before the wait for the kernel before.
+            if (waited && lane >= 1 && lane <= KC / 64)
+                tma_load_2d(dst + CODES + (lane - 1) * (S::X / 4), &map_x, step * KC + (lane - 1) * 64, token, bar);
+            if (!waited && (u + 1 == hi || u + 1 == lo + S::STAGES)) {
+                pdl_wait();
+                waited = true;
+                if (lane >= 1 && lane <= KC / 64) {
+                    unsigned at = lo / steps;
+                    int s = lo - at * steps;
+                    for (unsigned v = lo; v <= u; ++v) {
+                        tma_load_2d(stages + (v - lo) * S::BYTES + CODES + (lane - 1) * (S::X / 4), &map_x, s * KC + (lane - 1) * 64, at % p.chunks * N, full0 + 8 * (v - lo));
+                        if (++s == (int)steps) { s = 0; ++at; }
+                    }
                 }
-            if (z_group < left) {
-                const uintptr_t from = ((uintptr_t)(p.zeros + first + (size_t)z_group * p.out) & ~(uintptr_t)15) + z_piece;
-                if (from < z_end) copy16(dst + CODES + S::X + S::GROUPS * S::PIECES * 16 + z_e * 16, from);
             }
-            ++next_u;
-            if (++next_step == (int)steps) {
-                next_step = 0;
-                ++next_item;
-                next_row = next_item / p.chunks * ROWS;
-                next_token = next_item % p.chunks * N;
+            if (++slot == S::STAGES) { slot = 0; phase ^= 1; }
+            if (++step == (int)steps) {
+                step = 0;
+                ++item;
+                row = item / p.chunks * ROWS;
+                token = item % p.chunks * N;
             }
         }
-        fill = fill == S::STAGES - 1 ? 0 : fill + 1;
-        cp_async_commit();
-    };
-    // Codes are no result of a step: the first ones are asked for before the wait for the kernel before.
-    if (threadIdx.x == 0) {
-        unsigned item = next_item;
-        int step = next_step;
-        for (int s = 0; s < S::STAGES - 1 && lo + s < hi; ++s) {
-            ask_codes(s, step, item / p.chunks * ROWS);
-            if (++step == (int)steps) { step = 0; ++item; }
-        }
+        if (*reinterpret_cast<volatile int*>(p.status) != 0) drain_after_timeout();      // a wait ran out: let what is in flight land
+        return;
     }
-    pdl_enter();
-#pragma unroll 1
-    for (int s = 0; s < S::STAGES - 1; ++s) ask(false);
+    pdl_wait();                                              // y may still be read by the kernel before
 
-    float acc[MT][NT][4];
+    float acc[NT][4];
     auto clear = [&] {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[m][j][c] = 0.f;
+            for (int c = 0; c < 4; ++c) acc[j][c] = 0.f;
     };
     clear();
     unsigned item = lo / steps;
@@ -160,98 +153,79 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
     unsigned phase = 0;
     bool ok = true;
     // A lane's places in a stage at its first 32 k: the swizzle turns bits 4 to 6 by the row's lowest three (bit-reversed order: g).
-    const unsigned code_at = (warp * MT * 16 + g) * 128 + (g << 4) + 4 * t, x_at = CODES + g * 128 + ((t ^ g) << 4);
+    const unsigned code_at = (warp * 16 + g) * 128 + (g << 4) + 4 * t, x_at = CODES + g * 128 + ((t ^ g) << 4);
     for (unsigned u = lo; u < hi; ++u) {
-        cp_async_wait<S::STAGES - 2>();
-        ok = __syncthreads_and(mbar_wait(full0 + 8 * stage, phase, p.status, 16));
+        ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * stage, phase, p.status, 16));
         if (!ok) break;
-        ask(true);                                           // into the stage that every warp has left
         const unsigned char* src = tiles + stage * S::BYTES;
-        if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
         const int here = min(S::GROUPS, p.groups - step * S::GROUPS);
         // Where the step's scales and zeros begin in their first pieces: low bits of addresses, moving on by a row of the tables a group.
         unsigned s_low = (unsigned)(uintptr_t)p.scales + 2u * ((unsigned)(step * S::GROUPS) * (unsigned)p.out + (unsigned)row0);
         unsigned z_low = (unsigned)(uintptr_t)p.zeros + (unsigned)(step * S::GROUPS) * (unsigned)p.out + (unsigned)row0;
-        const unsigned char *scales = src + CODES + S::X + 2 * (warp * MT * 16 + g), *zeros = src + CODES + S::X + S::GROUPS * S::PIECES * 16 + warp * MT * 16 + g;
+        const unsigned char *scales = src + CODES + S::X + 2 * (warp * 16 + g), *zeros = src + CODES + S::X + S::GROUPS * S::S_ROW + warp * 16 + g;
         unsigned chunk = 0;                                  // 32 k: a 16-byte piece of a row of codes, four of a row of tokens
 #pragma unroll 1
         for (int q = 0; q < here; ++q) {
-            float part[MT][NT][4];
-            unsigned base[MT][2];
+            float part[NT][4];
+            unsigned base[2];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const unsigned z = p.zeros != nullptr ? zeros[(z_low & 15) + 16 * m + 8 * h] : 8u;
-                    base[m][h] = z * 0x00010001u + 0x43004300u;                          // 128 + zero, twice
-                }
+            for (int h = 0; h < 2; ++h) {
+                const unsigned z = p.zeros != nullptr ? zeros[(z_low & 15) + 8 * h] : 8u;
+                base[h] = z * 0x00010001u + 0x43004300u;     // 128 + zero, twice
+            }
             auto block = [&](bool first) {
                 const unsigned char *rows = src + (code_at ^ (chunk << 4)), *x = src + (x_at ^ ((chunk & 1) << 6)) + (chunk >> 1) * (S::X / 4);
                 uint4 b[NT];
 #pragma unroll
                 for (int j = 0; j < NT; ++j) b[j] = *reinterpret_cast<const uint4*>(x + j * 1024);
+                const unsigned lo_w = *reinterpret_cast<const unsigned*>(rows), hi_w = *reinterpret_cast<const unsigned*>(rows + 1024);
+                const unsigned a0[4] = {widen_pair(lo_w, 0, base[0]), widen_pair(hi_w, 0, base[1]), widen_pair(lo_w, 4, base[0]), widen_pair(hi_w, 4, base[1])};
+                const unsigned a1[4] = {widen_pair(lo_w, 8, base[0]), widen_pair(hi_w, 8, base[1]), widen_pair(lo_w, 12, base[0]), widen_pair(hi_w, 12, base[1])};
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const unsigned lo_w = *reinterpret_cast<const unsigned*>(rows + m * 2048), hi_w = *reinterpret_cast<const unsigned*>(rows + m * 2048 + 1024);
-                    const unsigned lo_b = base[m][0], hi_b = base[m][1];
-                    const unsigned a0[4] = {widen_pair(lo_w, 0, lo_b), widen_pair(hi_w, 0, hi_b), widen_pair(lo_w, 4, lo_b), widen_pair(hi_w, 4, hi_b)};
-                    const unsigned a1[4] = {widen_pair(lo_w, 8, lo_b), widen_pair(hi_w, 8, hi_b), widen_pair(lo_w, 12, lo_b), widen_pair(hi_w, 12, hi_b)};
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        if (first) mma_first(part[m][j], a0, b[j].x, b[j].y);
-                        else mma_more(part[m][j], a0, b[j].x, b[j].y);
-                    }
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) mma_more(part[m][j], a1, b[j].z, b[j].w);
+                for (int j = 0; j < NT; ++j) {
+                    if (first) mma_first(part[j], a0, b[j].x, b[j].y);
+                    else mma_more(part[j], a0, b[j].x, b[j].y);
                 }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) mma_more(part[j], a1, b[j].z, b[j].w);
                 ++chunk;
             };
             block(true);
-            if (NT <= 2) {
 #pragma unroll
-                for (int i = 1; i < GROUP / 32; ++i) block(false);
-            } else {                                         // many MMAs a block of k: its code once, for the instruction cache
-#pragma unroll 1
-                for (int i = 1; i < GROUP / 32; ++i) block(false);
+            for (int i = 1; i < GROUP / 32; ++i) block(false);
+            const float s_lo = to_f32(*reinterpret_cast<const bf16*>(scales + (s_low & 15))), s_hi = to_f32(*reinterpret_cast<const bf16*>(scales + (s_low & 15) + 16));
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                acc[j][0] = fmaf(s_lo, part[j][0], acc[j][0]);
+                acc[j][1] = fmaf(s_lo, part[j][1], acc[j][1]);
+                acc[j][2] = fmaf(s_hi, part[j][2], acc[j][2]);
+                acc[j][3] = fmaf(s_hi, part[j][3], acc[j][3]);
             }
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const float s_lo = to_f32(*reinterpret_cast<const bf16*>(scales + (s_low & 15) + 32 * m));
-                const float s_hi = to_f32(*reinterpret_cast<const bf16*>(scales + (s_low & 15) + 32 * m + 16));
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    acc[m][j][0] = fmaf(s_lo, part[m][j][0], acc[m][j][0]);
-                    acc[m][j][1] = fmaf(s_lo, part[m][j][1], acc[m][j][1]);
-                    acc[m][j][2] = fmaf(s_hi, part[m][j][2], acc[m][j][2]);
-                    acc[m][j][3] = fmaf(s_hi, part[m][j][3], acc[m][j][3]);
-                }
-            }
-            scales += S::PIECES * 16; zeros += S::ZERO_PIECES * 16;
+            scales += S::S_ROW; zeros += S::Z_ROW;
             s_low += 2u * (unsigned)p.out; z_low += (unsigned)p.out;
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty0 + 8 * stage);
+        if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
         if (step + 1 == (int)steps || u + 1 == hi) {              // the item's end, or this run's
             const unsigned u0 = item * steps;
             const bool whole = u0 >= lo && u0 + steps <= hi;
             const int token0 = item % p.chunks * N;
             float* part = p.parts + (size_t)runs.slot(blockIdx.x, u0) * N * ROWS;
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        // A thread's columns 2 t and 2 t + 1 are tokens in bit-reversed order, its rows g and g + 8.
-                        const int r = (warp * MT + m) * 16 + g + ((c & 2) ? 8 : 0), token = 8 * j + reversed3(2 * t + (c & 1));
-                        if (token0 + token >= p.n || row0 + r >= p.out) continue;
-                        if (whole) store_result(p.y, p.ldy, token0 + token, row0 + r, acc[m][j][c], p.epilogue, p.act, p.y32);
-                        else part[(size_t)token * ROWS + r] = acc[m][j][c];
-                    }
+                for (int c = 0; c < 4; ++c) {
+                    // A thread's columns 2 t and 2 t + 1 are tokens in bit-reversed order, its rows g and g + 8.
+                    const int r = warp * 16 + g + ((c & 2) ? 8 : 0), token = 8 * j + reversed3(2 * t + (c & 1));
+                    if (token0 + token >= p.n || row0 + r >= p.out) continue;
+                    if (whole) store_result(p.y, p.ldy, token0 + token, row0 + r, acc[j][c], p.epilogue, p.act, p.y32);
+                    else part[(size_t)token * ROWS + r] = acc[j][c];
+                }
             clear();
         }
         if (++step == (int)steps) { step = 0; ++item; row0 = item / p.chunks * ROWS; }
     }
-    cp_async_wait<0>();
-    if (!ok) drain_after_timeout();                          // a wait ran out: let what is in flight land
 }
 
 // The parts of 256 rows that several blocks share, in the blocks' order: blocks of (128 rows, eight tokens), a thread a row and two tokens.
@@ -282,7 +256,7 @@ __global__ void __launch_bounds__(512) linear4_join_kernel(const Args p, int N, 
     if (token + 1 < p.n) store_result(p.y, p.ldy, token + 1, row, s1, p.epilogue, p.act, p.y32);
 }
 
-int tokens_at_once(int n) { return n <= 16 ? 16 : n <= 32 ? 32 : 64; }
+int tokens_at_once(int n) { return n <= 16 ? 16 : 32; }
 
 template <int NT, int GROUP> int launch(const CUtensorMap& codes, const CUtensorMap& x, const Args& a, cudaStream_t stream) {
     typedef Shape<NT, GROUP> S;
@@ -335,7 +309,6 @@ int linear4_wide(void* y, long long ldy, const void* x, long long ldx, const voi
     if (group == 64) return launch<nt, 64>(map_codes, map_x, a, stream); \
     return launch<nt, 128>(map_codes, map_x, a, stream);
     if (N == 16) { L4_GROUPS(2) }
-    if (N == 32) { L4_GROUPS(4) }
-    L4_GROUPS(8)
+    L4_GROUPS(4)
 #undef L4_GROUPS
 }
