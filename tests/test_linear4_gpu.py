@@ -61,7 +61,8 @@ def test_sizes(ops, dtype, group, n, out, groups):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("n,out,k,group,with_zeros", [(1, 6144, 4096, 128, True), (3, 4096, 21504, 64, False), (12, 2051, 8192, 128, True),
-                                                      (2, 50257, 512, 32, True), (40, 4096, 4096, 128, False), (64, 3001, 2048, 32, True)])
+                                                      (2, 50257, 512, 32, True), (40, 4096, 4096, 128, False), (64, 3001, 2048, 32, True), (5, 2051, 8192, 32, True),
+                                                      (1, 2600, 8320, 64, True), (8, 2048, 9216, 128, False)])
 def test_layer_sizes(ops, dtype, n, out, k, group, with_zeros):
     check(ops, n, out, k, group, dtype, with_zeros)
 

@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(512) linear4_join_kernel(const Args p, int N, 
     if (token + 1 < p.n) store_result(p.y, p.ldy, token + 1, row, s1, p.epilogue, p.act, p.y32);
 }
 
-int tokens_at_once(int n) { return n <= 16 ? 16 : 32; }
+int tokens_at_once(int n) { return n <= 8 ? 8 : n <= 16 ? 16 : 32; }
 
 template <int NT, int GROUP> int launch(const CUtensorMap& codes, const CUtensorMap& x, const Args& a, cudaStream_t stream) {
     typedef Shape<NT, GROUP> S;
@@ -308,6 +308,7 @@ int linear4_wide(void* y, long long ldy, const void* x, long long ldx, const voi
     if (group == 32) return launch<nt, 32>(map_codes, map_x, a, stream); \
     if (group == 64) return launch<nt, 64>(map_codes, map_x, a, stream); \
     return launch<nt, 128>(map_codes, map_x, a, stream);
+    if (N == 8) { L4_GROUPS(1) }
     if (N == 16) { L4_GROUPS(2) }
     L4_GROUPS(4)
 #undef L4_GROUPS

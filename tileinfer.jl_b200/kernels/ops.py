@@ -979,7 +979,7 @@ LINEAR4_GROUPS = (32, 64, 128)
 
 def linear4_workspace(n: int, out_features: int, in_features: int) -> int:
     """Bytes of work space that ``linear4`` needs for n bfloat16 tokens (0: none)."""
-    return int(lib().ti_linear4_parts(n, out_features, in_features)) if n > 8 else 0
+    return int(lib().ti_linear4_parts(n, out_features, in_features))
 
 
 def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0.0, 0.0), workspace=None):
@@ -1007,15 +1007,13 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
         raise KernelError(f"linear4: output must be {torch.float32 if epilogue == EPI_F32_OUT else x.dtype}")
     stream = _stream()
     parts = status = None
-    if n > 8 and code == BF16:
-        need = linear4_workspace(n, out, k)
-        if need:
-            if workspace is None:
-                workspace = _workspace("linear4", need, x.device, stream)
-            elif workspace.numel() < need or not workspace.is_cuda:
-                raise KernelError(f"linear4: work space of {workspace.numel()} bytes, {need} needed")
-            parts = workspace.data_ptr()
-        status = status_word().data_ptr()
+    need = linear4_workspace(n, out, k) if code == BF16 else 0
+    if need:
+        if workspace is None:
+            workspace = _workspace("linear4", need, x.device, stream)
+        elif workspace.numel() < need or not workspace.is_cuda:
+            raise KernelError(f"linear4: work space of {workspace.numel()} bytes, {need} needed")
+        parts, status = workspace.data_ptr(), status_word().data_ptr()
     check(lib().ti_linear4(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), n, out, k,
                            k // groups, epilogue, act[0], act[1], act[2], act[3], code, parts, status, stream), "linear4")
 
