@@ -15,6 +15,7 @@ from . import library as _library
 from .library import KernelError, check, lib
 
 F32, BF16 = 0, 1
+_F32, _I32, _U8, _BF16 = torch.float32, torch.int32, torch.uint8, torch.bfloat16
 EPI_NONE, EPI_XIELU, EPI_F32_OUT = 0, 1, 2
 EPI_GELU_ERF, EPI_GELU_TANH = 4, 5          # GELU of the rounded sum, exact or tanh form (3: raw partial sums, inside the library)
 EPI_RELU2 = 6                               # max(rounded sum, 0)^2
@@ -977,9 +978,15 @@ def ssm_gate_norm(out, y, z, w, eps, parts):
 LINEAR4_GROUPS = (32, 64, 128)
 
 
+_linear4_need = {}
+
+
 def linear4_workspace(n: int, out_features: int, in_features: int) -> int:
     """Bytes of work space that ``linear4`` needs for n bfloat16 tokens (0: none)."""
-    return int(lib().ti_linear4_parts(n, out_features, in_features))
+    need = _linear4_need.get((n, out_features, in_features))
+    if need is None:
+        need = _linear4_need[n, out_features, in_features] = int(lib().ti_linear4_parts(n, out_features, in_features))
+    return need
 
 
 def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0.0, 0.0), workspace=None):
@@ -988,23 +995,26 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
     32, 64 or 128 k, ``zeros`` [in / group, out] uint8, or 8 for all. 32-bit sums, rounded once; with ``EPI_F32_OUT`` y is float32 and the sums
     are not rounded. Made for steps of few tokens; any number is taken. ``quantize4`` makes the codes. ``workspace``: ``linear4_workspace`` bytes
     (uint8); without it one kept per stream."""
-    for t, name, dtype in ((x, "x", None), (y, "y", None), (codes, "codes", torch.int32), (scales, "scales", x.dtype)):
-        _need(t, name, dtype, contiguous=name in ("codes", "scales"))
-    code = dtype_code(x.dtype)
-    if x.dim() != 2 or y.dim() != 2 or codes.dim() != 2 or scales.dim() != 2:
-        raise KernelError("linear4: x, y, codes and scales have two dimensions")
-    (n, k), (out, words), (groups, so) = x.shape, codes.shape, scales.shape
-    if words * 8 != k or so != out or groups < 1 or k % groups or k // groups not in LINEAR4_GROUPS or tuple(y.shape) != (n, out):
-        raise KernelError(f"linear4: x {tuple(x.shape)}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)}, y {tuple(y.shape)} do not fit "
-                          f"(groups of {', '.join(map(str, LINEAR4_GROUPS))})")
-    if (n and k and x.stride(1) != 1) or (n and out and y.stride(1) != 1):
-        raise KernelError("linear4: rows of x and y must be dense")
-    if zeros is not None:
-        _need(zeros, "zeros", torch.uint8)
-        if zeros.shape != scales.shape:
-            raise KernelError(f"linear4: zeros {tuple(zeros.shape)} for scales {tuple(scales.shape)}")
-    if y.dtype != (torch.float32 if epilogue == EPI_F32_OUT else x.dtype):
-        raise KernelError(f"linear4: output must be {torch.float32 if epilogue == EPI_F32_OUT else x.dtype}")
+    dtype = x.dtype
+    # One expression while all is well (a draft's step makes hundreds of these calls); what is wrong is looked for afterwards.
+    try:
+        (n, k), (out, words), (groups, columns) = x.shape, codes.shape, scales.shape
+        fits = x.is_cuda and y.is_cuda and codes.is_cuda and scales.is_cuda and codes.dtype is _I32 and scales.dtype is dtype and \
+            codes.is_contiguous() and scales.is_contiguous() and words * 8 == k and columns == out and y.shape == (n, out) and \
+            groups > 0 and k == groups * (group := k // groups) and group in LINEAR4_GROUPS and \
+            y.dtype is (_F32 if epilogue == EPI_F32_OUT else dtype) and (x.stride(1) == 1 or not n) and (y.stride(1) == 1 or not n * out) and \
+            (zeros is None or (zeros.is_cuda and zeros.dtype is _U8 and zeros.shape == scales.shape and zeros.is_contiguous()))
+    except ValueError:
+        raise KernelError("linear4: x, codes and scales have two dimensions") from None
+    if not fits:
+        for t, name, want in ((x, "x", None), (y, "y", None), (codes, "codes", _I32), (scales, "scales", dtype)):
+            _need(t, name, want, contiguous=name in ("codes", "scales"))
+        if zeros is not None:
+            _need(zeros, "zeros", _U8)
+        raise KernelError(f"linear4: x {tuple(x.shape)} {x.stride()}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)}, zeros "
+                          f"{None if zeros is None else tuple(zeros.shape)}, y {tuple(y.shape)} {y.stride()} of {y.dtype} do not fit (groups of "
+                          f"{', '.join(map(str, LINEAR4_GROUPS))}, dense rows, y of x's type or float32 with EPI_F32_OUT)")
+    code = dtype_code(dtype)
     stream = _stream()
     parts = status = None
     need = linear4_workspace(n, out, k) if code == BF16 else 0
@@ -1014,8 +1024,10 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
         elif workspace.numel() < need or not workspace.is_cuda:
             raise KernelError(f"linear4: work space of {workspace.numel()} bytes, {need} needed")
         parts, status = workspace.data_ptr(), status_word().data_ptr()
-    check(lib().ti_linear4(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), n, out, k,
-                           k // groups, epilogue, act[0], act[1], act[2], act[3], code, parts, status, stream), "linear4")
+    rc = lib().ti_linear4(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(),
+                          None if zeros is None else zeros.data_ptr(), n, out, k, group, epilogue, *act, code, parts, status, stream)
+    if rc:
+        check(rc, "linear4")
 
 
 def quantize4(codes, scales, w, zeros=None):
@@ -1065,18 +1077,21 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
     sequence in slot seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out [n, nq * head_dim]. bfloat16 (the
     32-bit path's sums do not depend on how a step is cut: ``attention_plain``). The work is shared out by the sequences' lengths on the device.
     ``workspace``: ``attention_few_workspace`` bytes (uint8); without it one kept per stream."""
-    for t, name in ((out, "out"), (q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache")):
-        _need(t, name, torch.bfloat16)
-    for t, name in ((block_table, "block_table"), (seq_slots, "seq_slots"), (cu_seqlens, "cu_seqlens"), (kv_lens, "kv_lens")):
-        _need(t, name, torch.int32, contiguous=name != "block_table")
     seqs, n = kv_lens.numel(), q.shape[0]
-    if nkv < 1 or nq < 1 or nq % nkv or head_dim < 1 or max_new < 0 or window < 0:
-        raise KernelError(f"attention_few: {nq} query heads on {nkv}, head size {head_dim}, {max_new} new tokens, window {window}")
-    if q.numel() != n * nq * head_dim or out.numel() != q.numel() or k_cache.shape != v_cache.shape or \
-            tuple(k_cache.shape[-3:]) != (nkv, page_size, head_dim) or cu_seqlens.numel() != seqs + 1 or seq_slots.numel() != seqs or \
-            block_table.dim() != 2 or (block_table.numel() and block_table.stride(1) != 1):
+    fits = out.dtype is _BF16 and q.dtype is _BF16 and k_cache.dtype is _BF16 and v_cache.dtype is _BF16 and out.is_cuda and q.is_cuda and \
+        k_cache.is_cuda and v_cache.is_cuda and out.is_contiguous() and q.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous() and \
+        block_table.dtype is _I32 and seq_slots.dtype is _I32 and cu_seqlens.dtype is _I32 and kv_lens.dtype is _I32 and block_table.is_cuda and \
+        seq_slots.is_cuda and cu_seqlens.is_cuda and kv_lens.is_cuda and seq_slots.is_contiguous() and cu_seqlens.is_contiguous() and \
+        kv_lens.is_contiguous() and nkv > 0 and nq > 0 and nq % nkv == 0 and head_dim > 0 and max_new >= 0 and window >= 0 and \
+        q.numel() == n * nq * head_dim == out.numel() and k_cache.shape == v_cache.shape and k_cache.shape[-3:] == (nkv, page_size, head_dim) and \
+        cu_seqlens.numel() == seqs + 1 and seq_slots.numel() == seqs and block_table.dim() == 2 and (not block_table.numel() or block_table.stride(1) == 1)
+    if not fits:
+        for t, name in ((out, "out"), (q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache")):
+            _need(t, name, _BF16)
+        for t, name in ((block_table, "block_table"), (seq_slots, "seq_slots"), (cu_seqlens, "cu_seqlens"), (kv_lens, "kv_lens")):
+            _need(t, name, _I32, contiguous=name != "block_table")
         raise KernelError(f"attention_few: q {tuple(q.shape)}, out {tuple(out.shape)}, pages {tuple(k_cache.shape)}, {seqs} sequences, table "
-                          f"{tuple(block_table.shape)} do not fit {nq} / {nkv} heads of {head_dim} on pages of {page_size}")
+                          f"{tuple(block_table.shape)}, {max_new} new tokens, window {window} do not fit {nq} / {nkv} heads of {head_dim} on pages of {page_size}")
     if n == 0 or seqs == 0:
         return
     stream = _stream()
@@ -1099,17 +1114,23 @@ def probabilities(out, logits, temperature, top_k=0, top_p=1.0):
                                  top_k, top_p, _stream()), "probabilities")
 
 
-def _need_run(accepted, tokens, drafts, counts, what):
-    """Checks what both tests of drafts share; returns (sequences, drafts)."""
+def _run_fits(accepted, tokens, drafts, counts, seqs, k) -> bool:
+    """What both tests of drafts ask of what they share."""
+    return accepted.is_cuda and accepted.dtype is _I32 and accepted.numel() == seqs and accepted.is_contiguous() and \
+        tokens.is_cuda and tokens.dtype is _I32 and tokens.shape == (seqs, k + 1) and tokens.is_contiguous() and \
+        drafts.is_cuda and drafts.dtype is _I32 and drafts.is_contiguous() and \
+        (counts is None or (counts.is_cuda and counts.dtype is _I32 and counts.numel() == seqs and counts.is_contiguous()))
+
+
+def _refuse_run(what, accepted, tokens, drafts, counts, **others):
     for t, name in ((accepted, "accepted"), (tokens, "tokens"), (drafts, "drafts"), (counts, "counts")):
         if t is not None:
-            _need(t, name, torch.int32)
-    if drafts.dim() != 2:
-        raise KernelError(f"{what}: drafts {tuple(drafts.shape)} (sequences, drafts)")
-    seqs, k = drafts.shape
-    if accepted.numel() != seqs or tuple(tokens.shape) != (seqs, k + 1) or (counts is not None and counts.numel() != seqs):
-        raise KernelError(f"{what}: accepted {tuple(accepted.shape)}, tokens {tuple(tokens.shape)} for drafts {tuple(drafts.shape)}")
-    return seqs, k
+            _need(t, name, _I32)
+    said = {"accepted": accepted, "tokens": tokens, "drafts": drafts, "counts": counts, **others}
+    raise KernelError(f"{what}: " + ", ".join(f"{name} {tuple(t.shape)} {t.dtype}" for name, t in said.items() if t is not None) + " do not fit")
+
+
+_verify_bytes = {}
 
 
 def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None):
@@ -1119,33 +1140,46 @@ def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None):
     number, in ascending order of ids, from max(p - q, 0) at the first refusal, from p after the last draft where all stand; in 2^-40 fixed
     point) and then -1. ``counts`` [seqs] int32: how many of a sequence's drafts there are (the rest of its row is not read). float32; p and q may
     have any strides but for a dense last dimension. A row of p without weight gives the token -1."""
-    seqs, k = _need_run(accepted, tokens, drafts, counts, "verify_drafts")
-    _need(p, "p", torch.float32, contiguous=False); _need(uniforms, "uniforms", torch.float32)
-    vocab = p.shape[-1]
-    if tuple(p.shape) != (seqs, k + 1, vocab) or tuple(uniforms.shape) != (seqs, k + 1) or (p.numel() and p.stride(2) != 1):
-        raise KernelError(f"verify_drafts: p {tuple(p.shape)}, uniforms {tuple(uniforms.shape)} for drafts {tuple(drafts.shape)}")
     q_args = (None, 0, 0)
-    if q is not None:
-        _need(q, "q", torch.float32, contiguous=False)
-        if tuple(q.shape) != (seqs, k, vocab) or (q.numel() and q.stride(2) != 1):
-            raise KernelError(f"verify_drafts: q {tuple(q.shape)} for p {tuple(p.shape)}")
-        q_args = (q.data_ptr(), q.stride(0), q.stride(1)) if k else q_args
+    try:
+        (seqs, k), vocab = drafts.shape, p.shape[-1]
+        fits = _run_fits(accepted, tokens, drafts, counts, seqs, k) and p.is_cuda and p.dtype is _F32 and p.shape == (seqs, k + 1, vocab) and \
+            (p.stride(2) == 1 or not seqs * vocab) and uniforms.is_cuda and uniforms.dtype is _F32 and uniforms.shape == (seqs, k + 1) and \
+            uniforms.is_contiguous()
+        if fits and q is not None:
+            fits = q.is_cuda and q.dtype is _F32 and q.shape == (seqs, k, vocab) and (not seqs * k * vocab or q.stride(2) == 1)
+            q_args = (q.data_ptr(), q.stride(0), q.stride(1)) if k else q_args
+    except (ValueError, IndexError):
+        fits = False
+    if not fits:
+        _refuse_run("verify_drafts", accepted, tokens, drafts, counts, p=p, q=q, uniforms=uniforms)
     if seqs == 0:
         return
     stream = _stream()
-    sums = _workspace("verify_sums", int(lib().ti_verify_drafts_workspace(seqs)), p.device, stream)
-    tickets = _workspace("verify_tickets", 4 * seqs, p.device, stream, zeroed=True)
-    check(lib().ti_verify_drafts(accepted.data_ptr(), tokens.data_ptr(), p.data_ptr(), p.stride(0), p.stride(1), *q_args, drafts.data_ptr(),
-                                 uniforms.data_ptr(), _ptr(counts), seqs, k, vocab, sums.data_ptr(), tickets.data_ptr(), stream), "verify_drafts")
+    # The tickets (zero before and after every call), then the stretches' sums.
+    head = (4 * seqs + 15) // 16 * 16
+    need = _verify_bytes.get(seqs)
+    if need is None:
+        need = _verify_bytes[seqs] = head + int(lib().ti_verify_drafts_workspace(seqs))
+    # The place of the sums depends on the number of sequences: a work space is kept for each.
+    ws = _workspace(("verify", seqs), need, p.device, stream, zeroed=True).data_ptr()
+    rc = lib().ti_verify_drafts(accepted.data_ptr(), tokens.data_ptr(), p.data_ptr(), p.stride(0), p.stride(1), *q_args, drafts.data_ptr(),
+                                uniforms.data_ptr(), None if counts is None else counts.data_ptr(), seqs, k, vocab, ws + head, ws, stream)
+    if rc:
+        check(rc, "verify_drafts")
 
 
 def match_drafts(accepted, tokens, chosen, drafts, counts=None):
     """Which drafted tokens are the model's own greedy choices: ``chosen`` [seqs, k + 1] int32 (``argmax`` of its logits) against ``drafts`` [seqs, k].
     accepted and tokens as in ``verify_drafts``; the token after the accepted ones is the model's choice there."""
-    seqs, k = _need_run(accepted, tokens, drafts, counts, "match_drafts")
-    _need(chosen, "chosen", torch.int32)
-    if tuple(chosen.shape) != (seqs, k + 1):
-        raise KernelError(f"match_drafts: chosen {tuple(chosen.shape)} for drafts {tuple(drafts.shape)}")
+    try:
+        seqs, k = drafts.shape
+        fits = _run_fits(accepted, tokens, drafts, counts, seqs, k) and chosen.is_cuda and chosen.dtype is _I32 and chosen.shape == (seqs, k + 1) and \
+            chosen.is_contiguous()
+    except ValueError:
+        fits = False
+    if not fits:
+        _refuse_run("match_drafts", accepted, tokens, drafts, counts, chosen=chosen)
     check(lib().ti_match_drafts(accepted.data_ptr(), tokens.data_ptr(), chosen.data_ptr(), drafts.data_ptr(), _ptr(counts), seqs, k, _stream()),
           "match_drafts")
 
