@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(L4F_WARPS * 32) linear4_f32_kernel(const unsig
 extern "C" int ti_linear4_shared(int n, int out, int K) {
     const long long weights = (long long)out * K;
     if (n <= 8) return weights >= 1LL << 28 || (weights >= 1LL << 24 && K >= 8192);
-    return (long long)((n + 7) / 8) * weights > 1LL << 22;
+    return (long long)((n + 7) / 8) * weights >= 1LL << 21;
 }
 
 // codes [out, K / 8] words, scales [K / group, out] of x's type, zeros [K / group, out] bytes or null; y [n, ldy] of x's type, or 32-bit sums

@@ -6,10 +6,12 @@
 // time, so an MMA's k lie in one group; the k of both operands are permuted alike. Rows and tokens stand in the MMAs in bit-reversed order, which
 // spreads every phase of a swizzled read over all banks.
 //
-// What bounds it: reading the codes once (up to 16 tokens), then mma.sync: 9 cycles a scheduler for 16 rows x 16 k x 8 tokens, 26 for the codes' eleven
-// instructions a word, seven of them on a pipe of half rate. (Weights widened into tensor memory as tcgen05.mma's operand, with a group's sum
-// read back from there, took 165 us for 16 and 245 us for 64 tokens x 131,072 x 4,096: a chain of five hand-overs between warps, 100 to 250 cycles
-// each, for every 128 k.)
+// What bounds it: reading the codes once (up to 16 tokens: 131,072 x 4,096 without the arithmetic takes 51 us for 8 tokens, with it 70), then mma.sync: 8 cycles a
+// scheduler for 16 rows x 16 k x 8 tokens, 10 beside other instructions, and 26 for the codes' eleven instructions a word, seven of them on a pipe of half
+// rate. 131,072 x 4,096: 70 us for 8 tokens, 82 for 16, 118 for 32, 222 for 64. Other forms took longer: weights widened into tensor memory as tcgen05.mma's operand with a
+// group's sum read back from there (165 us for 16, 245 for 64), the same with codes as float16 of 2^-24 (five instructions a word, tokens brought to
+// float16 by a kernel ahead: 108 and 419), float16 with mma.sync (66 us for 8 tokens, but 137 for 32 and a launch more on small weights), e4m3
+// (its operands are widened again by 20 cycles an MMA), eight warps of 32 rows (the tokens read half as often: 137 for 32), 64 tokens at once (271).
 //
 // The units of work, [256 rows, 256 k], are numbered along k, then over the rows (and the tokens in thirty-twos), and every SM takes an equal run of them
 // (even_runs.cuh). Parts of a tile that several blocks share go to the work space; a second kernel adds them in the blocks' order.
@@ -31,7 +33,9 @@ template <int NT, int GROUP> struct Shape {
     // Per group the 16-byte pieces of memory that hold its scales (zeros), wherever they begin: the place of the first in its piece is what its address says.
     static constexpr int S_ROW = 2 * ROWS + 16, Z_ROW = ROWS + 16, SCALES = GROUPS * (S_ROW + Z_ROW);
     static constexpr int BYTES = (CODES + X + SCALES + 1023) / 1024 * 1024;
-    static constexpr int FIT = (224 * 1024) / BYTES, STAGES = FIT > 5 ? 5 : FIT;
+    // A warp's results on their way out, sixteen tokens of 16 rows at a time (24 apart: no two lanes of a write meet in a bank).
+    static constexpr int OUT_ROW = 24, OUT_EIGHTS = NT < 2 ? NT : 2, OUT = OUT_EIGHTS * 8 * OUT_ROW * 4, OUTS = WARPS * OUT;
+    static constexpr int FIT = (226 * 1024 - OUTS) / BYTES, STAGES = FIT > 5 ? 5 : FIT;
 };
 
 struct Args {
@@ -164,8 +168,10 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
         unsigned z_low = (unsigned)(uintptr_t)p.zeros + (unsigned)(step * S::GROUPS) * (unsigned)p.out + (unsigned)row0;
         const unsigned char *scales = src + CODES + S::X + 2 * (warp * 16 + g), *zeros = src + CODES + S::X + S::GROUPS * S::S_ROW + warp * 16 + g;
         unsigned chunk = 0;                                  // 32 k: a 16-byte piece of a row of codes, four of a row of tokens
-#pragma unroll 1
-        for (int q = 0; q < here; ++q) {
+        // The groups of a step side by side: 131,072 x 4,096 and 8 tokens 79 us in turn, 72 so; 16 tokens 94 and 86.
+#pragma unroll
+        for (int q = 0; q < S::GROUPS; ++q) {
+            if (q >= here) break;
             float part[NT][4];
             unsigned base[2];
 #pragma unroll
@@ -212,33 +218,60 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
             const bool whole = u0 >= lo && u0 + steps <= hi;
             const int token0 = item % p.chunks * N;
             float* part = p.parts + (size_t)runs.slot(blockIdx.x, u0) * N * ROWS;
+            if (!whole) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    // A thread's columns 2 t and 2 t + 1 are tokens in bit-reversed order, its rows g and g + 8.
-                    const int r = warp * 16 + g + ((c & 2) ? 8 : 0), token = 8 * j + reversed3(2 * t + (c & 1));
-                    if (token0 + token >= p.n || row0 + r >= p.out) continue;
-                    if (whole) store_result(p.y, p.ldy, token0 + token, row0 + r, acc[j][c], p.epilogue, p.act, p.y32);
-                    else part[(size_t)token * ROWS + r] = acc[j][c];
+                    for (int c = 0; c < 4; ++c) {
+                        // A thread's columns 2 t and 2 t + 1 are tokens in bit-reversed order, its rows g and g + 8.
+                        const int r = warp * 16 + g + ((c & 2) ? 8 : 0), token = 8 * j + reversed3(2 * t + (c & 1));
+                        if (token0 + token < p.n && row0 + r < p.out) part[(size_t)token * ROWS + r] = acc[j][c];
+                    }
+            } else {
+                // Through shared memory to a loop: the code of all epilogues once per sixteen tokens, not once per result (131,072 x 4,096, 64 tokens: 274 us
+                // with it unrolled, 244 so).
+                float* mine = reinterpret_cast<float*>(tiles + S::STAGES * S::BYTES + warp * S::OUT);
+                const int row = warp * 16 + (lane & 15), tokens = min(N, p.n - token0);
+#pragma unroll
+                for (int j0 = 0; j0 < NT; j0 += S::OUT_EIGHTS) {
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < S::OUT_EIGHTS; ++j)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) mine[(8 * j + reversed3(2 * t + (c & 1))) * S::OUT_ROW + g + ((c & 2) ? 8 : 0)] = acc[j0 + j][c];
+                    __syncwarp();
+                    const int first = 8 * j0, last = min(first + 8 * S::OUT_EIGHTS, tokens);
+                    if (row0 + row >= p.out) continue;
+#pragma unroll 1
+                    for (int e = first + (lane >> 4); e < last; e += 2)
+                        store_result(p.y, p.ldy, token0 + e, row0 + row, mine[(e - first) * S::OUT_ROW + (lane & 15)], p.epilogue, p.act, p.y32);
                 }
+            }
             clear();
         }
         if (++step == (int)steps) { step = 0; ++item; row0 = item / p.chunks * ROWS; }
     }
 }
 
-// The parts of 256 rows that several blocks share, in the blocks' order: blocks of (128 rows, eight tokens), a thread a row and two tokens.
-constexpr int JOIN_TOKENS = 8, JOIN_ROWS = 128;
-__global__ void __launch_bounds__(512) linear4_join_kernel(const Args p, int N, int G) {
-    const int slot = threadIdx.x >> 7, r = (blockIdx.x & 1) * JOIN_ROWS + (threadIdx.x & 127), first = blockIdx.y * JOIN_TOKENS, chunk = first / N;
+// The parts of 256 rows that several blocks share, in the blocks' order: blocks of (128 rows, two tokens), a thread a row: small enough to stand beside
+// a product's block (2,048 x 9,216 and 8 tokens 8 us; in blocks of 512 threads, which find no registers beside it, 10.7).
+constexpr int JOIN_TOKENS = 2, JOIN_ROWS = 128;
+__global__ void __launch_bounds__(JOIN_ROWS) linear4_join_kernel(const Args p, int N, int G, bool by_cuts) {
+    const int r = (blockIdx.x & 1) * JOIN_ROWS + threadIdx.x, which = blockIdx.x >> 1;
     const Runs runs(p.units, G);
-    const unsigned u0 = ((blockIdx.x >> 1) * p.chunks + chunk) * p.steps, c0 = runs.owner(u0), c1 = runs.owner(u0 + p.steps - 1);
-    const int row = (blockIdx.x >> 1) * ROWS + r;
+    // The items, or, where those are more, the cuts between runs (131,072 x 4,096 and 64 tokens 251 us, 222 by cuts): a cut's item is that cut's if no cut
+    // before lies in it.
+    unsigned tile = which, chunk = blockIdx.z;
+    if (by_cuts) {
+        const unsigned cut = runs.low(which + 1) / p.steps;
+        tile = cut / p.chunks;
+        chunk = cut - tile * p.chunks;
+    }
+    const unsigned u0 = (tile * p.chunks + chunk) * p.steps, c0 = runs.owner(u0), c1 = runs.owner(u0 + p.steps - 1);
+    const int row = tile * ROWS + r, token0 = chunk * N, token = token0 + blockIdx.y * JOIN_TOKENS;
     pdl_enter();
-    if (c0 == c1 || row >= p.out) return;
-    const int token = first + 2 * slot;
-    const float* part = p.parts + (size_t)(token - chunk * N) * ROWS + r;
+    if (c0 == c1 || (by_cuts && c0 != (unsigned)which) || row >= p.out || token >= p.n) return;
+    const float* part = p.parts + (size_t)(token - token0) * ROWS + r;
     float s0 = 0.f, s1 = 0.f;
     for (unsigned c = c0; c <= c1; c += 6) {
         float a[6], b[6];
@@ -260,7 +293,7 @@ int tokens_at_once(int n) { return n <= 8 ? 8 : n <= 16 ? 16 : 32; }
 
 template <int NT, int GROUP> int launch(const CUtensorMap& codes, const CUtensorMap& x, const Args& a, cudaStream_t stream) {
     typedef Shape<NT, GROUP> S;
-    constexpr size_t smem = (size_t)S::STAGES * S::BYTES + 1024;
+    constexpr size_t smem = (size_t)S::STAGES * S::BYTES + S::OUTS + 1024;
     static_assert(S::STAGES >= 3, "stages");
     static bool configured = false;
     if (!configured) {
@@ -272,7 +305,10 @@ template <int NT, int GROUP> int launch(const CUtensorMap& codes, const CUtensor
     ti_launch(linear4_wide_kernel<NT, GROUP>, dim3(blocks), dim3(S::THREADS), smem, stream, codes, x, a);
     if (int rc = ti_check_launch("linear4_wide")) return rc;
     if (a.units % blocks == 0 && (a.units / blocks) % a.steps == 0) return 0;            // every run ends with an item: no parts
-    ti_launch(linear4_join_kernel, dim3(2 * ((a.out + ROWS - 1) / ROWS), (a.n + JOIN_TOKENS - 1) / JOIN_TOKENS), dim3(512), 0, stream, a, 8 * NT, blocks);
+    const int tiles = (a.out + ROWS - 1) / ROWS;
+    const bool by_cuts = (long long)tiles * a.chunks > blocks - 1 || a.chunks > 65535;
+    ti_launch(linear4_join_kernel, dim3(2 * (by_cuts ? blocks - 1 : tiles), ((a.n < 8 * NT ? a.n : 8 * NT) + JOIN_TOKENS - 1) / JOIN_TOKENS, by_cuts ? 1 : a.chunks),
+              dim3(JOIN_ROWS), 0, stream, a, 8 * NT, blocks, by_cuts);
     return ti_check_launch("linear4_join");
 }
 
