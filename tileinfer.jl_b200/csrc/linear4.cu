@@ -325,12 +325,13 @@ __global__ void __launch_bounds__(L4F_WARPS * 32) linear4_f32_kernel(const unsig
 
 // Which of the two bfloat16 kernels: eight tokens at a time, each time over all codes, or up to 32 tokens through shared memory (linear4_wide.cu), whose
 // blocks take equal runs of units and need a second kernel to join shared tiles. Up to eight tokens the first reads a block's tokens once per
-// stretch of k, for few rows that is most of its work: it is left to short k. us, eights / shared memory: 1 token x 21,504 x 4,096 14.5 / 18.4,
-// x 6,144 x 4,096 7.4 / 8.8, x 2,048 x 9,216 10.3 / 7.6, x 4,096 x 21,504 22.6 / 19.7, x 131,072 x 4,096 84 / 78; 16 tokens x 21,504 x 4,096 31 / 20.5,
-// x 2,048 x 2,048 8.8 / 5.6, x 1,024 x 1,024 5.7 / 5.8; 24 tokens x 512 x 4,096 9.5 / 7.2; 64 tokens x 320 x 256 7.3 / 13.
+// stretch of k, for few rows that is most of its work: it is left to short k. us, eights / shared memory: 1 token x 21,504 x 4,096 14.6 / 17.1,
+// x 6,144 x 4,096 7.4 / 8.3, x 12,856 x 8,000 18.5 / 20.3, x 65,536 x 2,048 24.1 / 22.8, x 131,072 x 4,096 84 / 70; x 1,024 x 8,192 9.2 / 7.7, x 200 x 11,904
+// 8.9 / 7.9; 16 tokens x 21,504 x 4,096 31 / 18.9, x 1,024 x 1,024 5.7 / 4.9, x 512 x 512 2.9 / 5.2; 32 tokens x 1,024 x 1,024 11.2 / 6.4, x 320 x 2,048
+// 6.1 / 6.9; 64 tokens x 512 x 512 11 / 6.5.
 extern "C" int ti_linear4_shared(int n, int out, int K) {
     const long long weights = (long long)out * K;
-    if (n <= 8) return weights >= 1LL << 28 || (weights >= 1LL << 24 && K >= 8192);
+    if (n <= 8) return weights >= 1LL << 27 || (weights >= 1LL << 21 && K >= 8192);
     return (long long)((n + 7) / 8) * weights >= 1LL << 21;
 }
 
