@@ -1065,9 +1065,16 @@ def _workspace(kind: str, nbytes: int, device, stream: int, zeroed: bool = False
 FEW_HEAD_DIMS, FEW_PAGE = (16, 32, 48, 64, 80, 96, 112, 128, 256), 64        # what attention_few takes
 
 
+_attention_few_need = {}
+
+
 def attention_few_workspace(seqs: int, max_new: int, nq: int, nkv: int, head_dim: int) -> int:
     """Bytes of work space that ``attention_few`` needs."""
-    return int(lib().ti_attention_few_workspace(seqs, max_new, nq, nkv, head_dim))
+    key = (seqs, max_new, nq, nkv, head_dim)
+    need = _attention_few_need.get(key)
+    if need is None:
+        need = _attention_few_need[key] = int(lib().ti_attention_few_workspace(*key))
+    return need
 
 
 def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, kv_lens, scale, nq, nkv, head_dim, page_size, max_new, window=0,
@@ -1097,10 +1104,11 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
     stream = _stream()
     if workspace is None:
         workspace = _workspace("attention_few", attention_few_workspace(seqs, max_new, nq, nkv, head_dim), q.device, stream)
-    check(lib().ti_attention_few(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                                 seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), workspace.data_ptr(), workspace.numel(),
-                                 status_word().data_ptr(), scale, seqs, nq, nkv, head_dim, page_size, max_new, k_cache.shape[0], window or 0, stream),
-          "attention_few")
+    rc = lib().ti_attention_few(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                                seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                                status_word().data_ptr(), scale, seqs, nq, nkv, head_dim, page_size, max_new, k_cache.shape[0], window or 0, stream)
+    if rc:
+        check(rc, "attention_few")
 
 
 def probabilities(out, logits, temperature, top_k=0, top_p=1.0):
