@@ -1,15 +1,16 @@
 """Drafts of a few tokens, tested by the model in one step.
 
 A :class:`Draft` is the engine's own model with its matrices in 4 bits, run on the same sequences: a draft's step reads a quarter of the weights. In a
-round it continues every sequence by up to ``tokens`` tokens, one step each; the sequences are cut back, and the model runs the drafted tokens through one
-step of its own, which writes their keys and values over the draft's and gives the logits at every place. The longest run of drafted tokens that
-stands is kept, with one token more: at temperature 0 a drafted token stands while it is the model's own choice, else by the test of
-``ops.verify_drafts``, so that every token is distributed as one sampled from the model (not the same token as without a draft: the
-uniform numbers are used up in another order). Sequences that cannot be cut back (recurrent states, windows) take no draft.
+round it continues every sequence by up to ``tokens`` tokens (by no more than its budget leaves), one step each; the sequences are cut back, and the
+model runs the drafted tokens through one step of its own, which writes their keys and values over the draft's and gives the logits at every
+place. The longest run of drafted tokens that stands is kept, with one token more: at temperature 0 a drafted token stands while it is the model's
+own choice, else by the test of ``ops.verify_drafts``, so that every token is distributed as one sampled from the model (not the same token as
+without a draft: the uniform numbers are used up in another order). Sequences that cannot be cut back (recurrent states, windows) take no draft.
 """
 from __future__ import annotations
 
 import copy
+from itertools import accumulate
 from typing import Callable, Dict, List, Optional, Sequence
 
 import torch
@@ -70,43 +71,60 @@ class Draft:
         self.twin = engine.twin(quantized(engine.model, group, zeros))
         self.drafted = self.stood = 0
 
-    def propose(self, slots: Sequence[int], last: Sequence[int], k: int, sampling: SamplingParams, seeds, counters):
-        """``k`` tokens for each of ``slots``, whose last tokens ``last`` the cache does not hold yet: (drafts [sequences, k] int32, the probabilities
-        that they were drawn from [sequences, k, vocab], or None for the most likely ones), on the device. The sequences keep their lengths."""
+    def propose(self, slots: Sequence[int], last: Sequence[int], k: int, sampling: SamplingParams, seeds, counters, counts: Optional[Sequence[int]] = None):
+        """``k`` tokens for each of ``slots`` (with ``counts`` so many of them for each, at most ``k``), whose last tokens ``last`` the cache does not
+        hold yet: (drafts [sequences, k] int32, the probabilities that they were drawn from [sequences, k, vocab], or None for the most likely ones),
+        on the device; places beyond a sequence's count hold nothing. The sequences keep their lengths."""
         n, twin = len(slots), self.twin
         lengths = [twin.sequence_length(s) for s in slots]
-        steps = torch.empty(k, n, dtype=torch.int32, device=twin.device)
+        steps = torch.zeros(k, n, dtype=torch.int32, device=twin.device)
         q = None if sampling.greedy else torch.empty(k, n, twin.vocab_size, dtype=torch.float32, device=twin.device)
         try:
+            rows = []
             for i in range(k):
-                logits = twin.decode(slots, list(last) if i == 0 else None)
-                ids = twin.decode_token_buffer(n)
+                before, rows = rows, [r for r in range(n) if counts is None or counts[r] > i]
+                ids, at = twin.decode_token_buffer(len(rows)), [slots[r] for r in rows]
+                whole = len(rows) == n
+                some = None if whole else torch.tensor(rows, dtype=torch.long, device=twin.device)
+                if i and rows != before:
+                    ids.copy_(steps[i - 1][some])
+                logits = twin.decode(at, None if i else [last[r] for r in rows])
+                tokens = steps[i] if whole else torch.empty(len(rows), dtype=torch.int32, device=twin.device)
                 if sampling.greedy:
-                    ops.argmax(logits, steps[i], also=ids)
+                    ops.argmax(logits, tokens, also=ids)
                 else:
-                    ops.probabilities(q[i], logits, sampling.temperature, sampling.top_k, sampling.top_p)
-                    ops.sample(logits, steps[i], sampling.temperature, sampling.top_k, sampling.top_p, seeds, counters, also=ids)
+                    p = q[i] if whole else torch.empty_like(logits)
+                    ops.probabilities(p, logits, sampling.temperature, sampling.top_k, sampling.top_p)
+                    numbers = (seeds, counters) if whole else (seeds[some], counters[some])
+                    ops.sample(logits, tokens, sampling.temperature, sampling.top_k, sampling.top_p, *numbers, also=ids)
+                    if not whole:
+                        q[i].index_copy_(0, some, p)
+                        counters.index_copy_(0, some, numbers[1])
+                if not whole:
+                    steps[i].index_copy_(0, some, tokens)
         finally:
             for slot, length in zip(slots, lengths):
                 twin.truncate(slot, length)
         return steps.t().contiguous(), None if q is None else q.transpose(0, 1)
 
 
-def _test(engine, logits, drafts, q, sampling: SamplingParams, seeds, counters):
-    """(how many drafted tokens of each sequence stand, those with the token after them [sequences, k + 1]), on the device."""
+def _test(engine, logits, drafts, q, sampling: SamplingParams, seeds, counters, counts=None):
+    """(how many drafted tokens of each sequence stand, those with the token after them [sequences, k + 1]), on the device. ``counts``: how many
+    drafts each sequence has; ``logits`` has k + 1 rows of each all the same."""
     n, k = drafts.shape
+    counts = None if counts is None else torch.tensor(counts, dtype=torch.int32, device=engine.device)
     accepted = torch.empty(n, dtype=torch.int32, device=engine.device)
     tokens = torch.empty(n, k + 1, dtype=torch.int32, device=engine.device)
     if sampling.greedy:
         chosen = torch.empty(n * (k + 1), dtype=torch.int32, device=engine.device)
         ops.argmax(logits, chosen)
-        ops.match_drafts(accepted, tokens, chosen.view(n, k + 1), drafts)
+        ops.match_drafts(accepted, tokens, chosen.view(n, k + 1), drafts, counts)
         return accepted, tokens
     p = torch.empty_like(logits)
     ops.probabilities(p, logits, sampling.temperature, sampling.top_k, sampling.top_p)
     u = torch.empty(n, k + 1, dtype=torch.float32, device=engine.device)
     ops.uniforms(u, seeds, counters)
-    ops.verify_drafts(accepted, tokens, p.view(n, k + 1, -1), q, drafts, u)
+    ops.verify_drafts(accepted, tokens, p.view(n, k + 1, -1), q, drafts, u, counts)
     return accepted, tokens
 
 
@@ -151,7 +169,9 @@ def decode_batch_drafted(engine, draft: Draft, sampling: SamplingParams, seed: i
             live = [live[row] for row in rows]
         at = [slots[r] for r in live]
         lengths = [engine.sequence_length(s) for s in at]
-        k = min(draft.tokens, max(max_new_tokens - len(results[r]) for r in live) - 1, engine.max_context - max(lengths) - 1)
+        # A run of c drafts and the token after them ends within a sequence's own budget (and pages, which are set aside for that) and the context.
+        counts = [max(0, min(draft.tokens, max_new_tokens - len(results[r]) - 1, engine.max_context - length - 1)) for r, length in zip(live, lengths)]
+        k = max(counts)
         tokens = [last[r] for r in live]
         if k < 1:                                            # one token is left to make: a step of its own
             logits = engine.decode(at, tokens)
@@ -162,13 +182,17 @@ def decode_batch_drafted(engine, draft: Draft, sampling: SamplingParams, seed: i
                 ops.sample(logits, first, sampling.temperature, sampling.top_k, sampling.top_p, seeds, counters)
             fresh = [[t] for t in first.tolist()]
             continue
-        drafts, q = draft.propose(at, tokens, k, sampling, draft_seeds, draft_counters)
-        runs = [[t] + d for t, d in zip(tokens, drafts.tolist())]
-        logits = engine.step(list(zip(at, runs)), [list(range(k + 1))] * len(at), few=True)
-        accepted, kept = _test(engine, logits, drafts, q, sampling, seeds, counters)
+        ragged = min(counts) < k
+        drafts, q = draft.propose(at, tokens, k, sampling, draft_seeds, draft_counters, counts if ragged else None)
+        runs = [[t] + d[:c] for t, d, c in zip(tokens, drafts.tolist(), counts)]
+        logits = engine.step(list(zip(at, runs)), [list(range(c + 1)) for c in counts], few=True)
+        if ragged:                                           # k + 1 rows a sequence: its last one again where it has fewer
+            ends = list(accumulate(c + 1 for c in counts))
+            logits = logits[torch.tensor([end - 1 - max(c - i, 0) for end, c in zip(ends, counts) for i in range(k + 1)], dtype=torch.long, device=device)]
+        accepted, kept = _test(engine, logits, drafts, q, sampling, seeds, counters, counts if ragged else None)
         accepted, kept = accepted.tolist(), kept.tolist()
         for slot, length, a in zip(at, lengths, accepted):
             engine.truncate(slot, length + 1 + a)
-        draft.drafted += k * len(at)
+        draft.drafted += sum(counts)
         draft.stood += sum(accepted)
         fresh = [row[:a + 1] for row, a in zip(kept, accepted)]
