@@ -994,7 +994,7 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
     ones in its low half, the odd ones in its high half, four bits each in ascending order), ``scales`` [in / group, out] of x's type for groups of
     32, 64 or 128 k, ``zeros`` [in / group, out] uint8, or 8 for all. 32-bit sums, rounded once; with ``EPI_F32_OUT`` y is float32 and the sums
     are not rounded. Made for steps of few tokens; any number is taken. ``quantize4`` makes the codes. ``workspace``: ``linear4_workspace`` bytes
-    (uint8); without it one kept per stream."""
+    (uint8); without it one kept per stream (a captured call: one of its graph's own)."""
     dtype = x.dtype
     # One expression while all is well (a draft's step makes hundreds of these calls); what is wrong is looked for afterwards.
     try:
@@ -1052,8 +1052,15 @@ def quantize4(codes, scales, w, zeros=None):
 _few_ws = {}
 
 
-def _workspace(kind: str, nbytes: int, device, stream: int, zeroed: bool = False) -> torch.Tensor:
-    """At least ``nbytes`` of the kind's work space for ``stream`` (calls on one stream follow one another), grown on demand."""
+def _workspace(kind: str, nbytes: int, device, stream: int, zeroed: int = 0) -> torch.Tensor:
+    """At least ``nbytes`` of the kind's work space, the last ``zeroed`` bytes zero when a call first gets them: for calls on ``stream``, which follow
+    one another, one that is kept and grown on demand. A call that is being captured gets one of its graph's own memory, and its fill is captured with
+    it: the graph is replayed whenever and wherever the program likes, so nothing else may use it, and it lasts as long as the graph."""
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        if zeroed:
+            ws[nbytes - zeroed:].zero_()
+        return ws
     key = (kind, device, stream)
     ws = _few_ws.get(key)
     if ws is None or ws.numel() < nbytes:
@@ -1083,7 +1090,7 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
     cu_seqlens[b] to cu_seqlens[b + 1] of q [n, nq, head_dim] (at most ``max_new`` of them, or none) are the last of the kv_lens[b] positions of the
     sequence in slot seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out [n, nq * head_dim]. bfloat16 (the
     32-bit path's sums do not depend on how a step is cut: ``attention_plain``). The work is shared out by the sequences' lengths on the device.
-    ``workspace``: ``attention_few_workspace`` bytes (uint8); without it one kept per stream."""
+    ``workspace``: ``attention_few_workspace`` bytes (uint8); without it one kept per stream (a captured call: one of its graph's own)."""
     seqs, n = kv_lens.numel(), q.shape[0]
     fits = out.dtype is _BF16 and q.dtype is _BF16 and k_cache.dtype is _BF16 and v_cache.dtype is _BF16 and out.is_cuda and q.is_cuda and \
         k_cache.is_cuda and v_cache.is_cuda and out.is_contiguous() and q.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous() and \
@@ -1164,15 +1171,15 @@ def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None):
     if seqs == 0:
         return
     stream = _stream()
-    # The tickets (zero before and after every call), then the stretches' sums.
-    head = (4 * seqs + 15) // 16 * 16
+    # The stretches' sums, then the tickets, which are zero before and after every call.
+    tickets = (4 * seqs + 15) // 16 * 16
     need = _verify_bytes.get(seqs)
     if need is None:
-        need = _verify_bytes[seqs] = head + int(lib().ti_verify_drafts_workspace(seqs))
-    # The place of the sums depends on the number of sequences: a work space is kept for each.
-    ws = _workspace(("verify", seqs), need, p.device, stream, zeroed=True).data_ptr()
+        need = _verify_bytes[seqs] = int(lib().ti_verify_drafts_workspace(seqs)) + tickets
+    # The place of the tickets depends on the number of sequences: a work space is kept for each.
+    ws = _workspace(("verify", seqs), need, p.device, stream, zeroed=tickets).data_ptr()
     rc = lib().ti_verify_drafts(accepted.data_ptr(), tokens.data_ptr(), p.data_ptr(), p.stride(0), p.stride(1), *q_args, drafts.data_ptr(),
-                                uniforms.data_ptr(), None if counts is None else counts.data_ptr(), seqs, k, vocab, ws + head, ws, stream)
+                                uniforms.data_ptr(), None if counts is None else counts.data_ptr(), seqs, k, vocab, ws, ws + need - tickets, stream)
     if rc:
         check(rc, "verify_drafts")
 
