@@ -1145,16 +1145,30 @@ def _refuse_run(what, accepted, tokens, drafts, counts, **others):
     raise KernelError(f"{what}: " + ", ".join(f"{name} {tuple(t.shape)} {t.dtype}" for name, t in said.items() if t is not None) + " do not fit")
 
 
-_verify_bytes = {}
+_verify_need = {}
 
 
-def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None):
+def verify_drafts_workspace(seqs: int) -> int:
+    """Bytes of work space that ``verify_drafts`` needs."""
+    need = _verify_need.get(seqs)
+    if need is None:
+        need = _verify_need[seqs] = int(lib().ti_verify_drafts_workspace(seqs)) + _tickets(seqs)
+    return need
+
+
+def _tickets(seqs: int) -> int:
+    return (4 * seqs + 15) // 16 * 16
+
+
+def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None, workspace=None):
     """Which drafted tokens stand: ``drafts`` [seqs, k] int32, drawn from the draft's probabilities ``q`` [seqs, k, vocab] (None: certain ones, as a
     greedy draft's), against the model's ``p`` [seqs, k + 1, vocab], with ``uniforms`` [seqs, k + 1] in [0, 1). Draft i stands while
     uniforms[i] * q[i, d] < p[i, d]; accepted[seq] is how many do, and tokens [seqs, k + 1] gets them, the token after them (by the last uniform
     number, in ascending order of ids, from max(p - q, 0) at the first refusal, from p after the last draft where all stand; in 2^-40 fixed
     point) and then -1. ``counts`` [seqs] int32: how many of a sequence's drafts there are (the rest of its row is not read). float32; p and q may
-    have any strides but for a dense last dimension. A row of p without weight gives the token -1."""
+    have any strides but for a dense last dimension. A row of p without weight gives the token -1. ``workspace``: ``verify_drafts_workspace`` bytes
+    (uint8) that are zero before the first call (each leaves them fit for the next, of as many sequences or fewer); without it one kept per stream
+    (a captured call: one of its graph's own)."""
     q_args = (None, 0, 0)
     try:
         (seqs, k), vocab = drafts.shape, p.shape[-1]
@@ -1171,15 +1185,17 @@ def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None):
     if seqs == 0:
         return
     stream = _stream()
-    # The stretches' sums, then the tickets, which are zero before and after every call.
-    tickets = (4 * seqs + 15) // 16 * 16
-    need = _verify_bytes.get(seqs)
-    if need is None:
-        need = _verify_bytes[seqs] = int(lib().ti_verify_drafts_workspace(seqs)) + tickets
-    # The place of the tickets depends on the number of sequences: a work space is kept for each.
-    ws = _workspace(("verify", seqs), need, p.device, stream, zeroed=tickets).data_ptr()
+    need, tickets = verify_drafts_workspace(seqs), _tickets(seqs)
+    if workspace is None:
+        workspace = _workspace("verify_drafts", need, p.device, stream, zeroed=tickets)
+    elif workspace.dtype is not _U8 or not workspace.is_cuda or not workspace.is_contiguous() or workspace.numel() < need or workspace.data_ptr() % 16:
+        raise KernelError(f"verify_drafts: work space of {workspace.numel()} {workspace.dtype} at {workspace.data_ptr():#x} on {workspace.device}; "
+                          f"{need} bytes needed, 16-byte aligned")
+    # The stretches' sums from the beginning, the tickets, which are zero before and after every call, up to the end: wherever the
+    # calls are of fewer sequences, no sums lie where another call's tickets do.
+    ws, end = workspace.data_ptr(), workspace.numel() // 16 * 16
     rc = lib().ti_verify_drafts(accepted.data_ptr(), tokens.data_ptr(), p.data_ptr(), p.stride(0), p.stride(1), *q_args, drafts.data_ptr(),
-                                uniforms.data_ptr(), None if counts is None else counts.data_ptr(), seqs, k, vocab, ws, ws + need - tickets, stream)
+                                uniforms.data_ptr(), None if counts is None else counts.data_ptr(), seqs, k, vocab, ws, ws + end - tickets, stream)
     if rc:
         check(rc, "verify_drafts")
 
