@@ -6,6 +6,7 @@ nothing and can be captured in a CUDA graph.
 """
 from __future__ import annotations
 
+import threading
 from typing import Optional
 
 import torch
@@ -994,7 +995,7 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
     ones in its low half, the odd ones in its high half, four bits each in ascending order), ``scales`` [in / group, out] of x's type for groups of
     32, 64 or 128 k, ``zeros`` [in / group, out] uint8, or 8 for all. 32-bit sums, rounded once; with ``EPI_F32_OUT`` y is float32 and the sums
     are not rounded. Made for steps of few tokens; any number is taken. ``quantize4`` makes the codes. ``workspace``: ``linear4_workspace`` bytes
-    (uint8); without it one kept per stream (a captured call: one of its graph's own)."""
+    (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
     dtype = x.dtype
     # One expression while all is well (a draft's step makes hundreds of these calls); what is wrong is looked for afterwards.
     try:
@@ -1049,23 +1050,28 @@ def quantize4(codes, scales, w, zeros=None):
                              out, k, k // groups, _stream()), "quantize4")
 
 
-_few_ws = {}
+_kept = threading.local()            # .spaces: the work spaces of the thread
 
 
 def _workspace(kind: str, nbytes: int, device, stream: int, zeroed: int = 0) -> torch.Tensor:
-    """At least ``nbytes`` of the kind's work space, the last ``zeroed`` bytes zero when a call first gets them: for calls on ``stream``, which follow
-    one another, one that is kept and grown on demand. A call that is being captured gets one of its graph's own memory, and its fill is captured with
+    """At least ``nbytes`` of the kind's work space, the last ``zeroed`` bytes zero when a call first gets them: for a thread's calls on ``stream``, which
+    follow one another, one that is kept and grown on demand (two threads' calls on one stream may alternate kernel by kernel, so each thread has its
+    own). A call that is being captured gets one of its graph's own memory, and its fill is captured with
     it: the graph is replayed whenever and wherever the program likes, so nothing else may use it, and it lasts as long as the graph."""
     if torch.cuda.is_current_stream_capturing():
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         if zeroed:
             ws[nbytes - zeroed:].zero_()
         return ws
+    try:
+        spaces = _kept.spaces
+    except AttributeError:
+        spaces = _kept.spaces = {}
     key = (kind, device, stream)
-    ws = _few_ws.get(key)
+    ws = spaces.get(key)
     if ws is None or ws.numel() < nbytes:
         make = torch.zeros if zeroed else torch.empty
-        ws = _few_ws[key] = make(max(nbytes, 4096), dtype=torch.uint8, device=device)
+        ws = spaces[key] = make(max(nbytes, 4096), dtype=torch.uint8, device=device)
     return ws
 
 
@@ -1090,7 +1096,7 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
     cu_seqlens[b] to cu_seqlens[b + 1] of q [n, nq, head_dim] (at most ``max_new`` of them, or none) are the last of the kv_lens[b] positions of the
     sequence in slot seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out [n, nq * head_dim]. bfloat16 (the
     32-bit path's sums do not depend on how a step is cut: ``attention_plain``). The work is shared out by the sequences' lengths on the device.
-    ``workspace``: ``attention_few_workspace`` bytes (uint8); without it one kept per stream (a captured call: one of its graph's own)."""
+    ``workspace``: ``attention_few_workspace`` bytes (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
     seqs, n = kv_lens.numel(), q.shape[0]
     fits = out.dtype is _BF16 and q.dtype is _BF16 and k_cache.dtype is _BF16 and v_cache.dtype is _BF16 and out.is_cuda and q.is_cuda and \
         k_cache.is_cuda and v_cache.is_cuda and out.is_contiguous() and q.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous() and \
@@ -1167,8 +1173,8 @@ def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None, workspa
     number, in ascending order of ids, from max(p - q, 0) at the first refusal, from p after the last draft where all stand; in 2^-40 fixed
     point) and then -1. ``counts`` [seqs] int32: how many of a sequence's drafts there are (the rest of its row is not read). float32; p and q may
     have any strides but for a dense last dimension. A row of p without weight gives the token -1. ``workspace``: ``verify_drafts_workspace`` bytes
-    (uint8) that are zero before the first call (each leaves them fit for the next, of as many sequences or fewer); without it one kept per stream
-    (a captured call: one of its graph's own)."""
+    (uint8) that are zero before the first call (each leaves them fit for the next, of as many sequences or fewer); without it one kept per
+    thread and stream (a captured call: one of its graph's own)."""
     q_args = (None, 0, 0)
     try:
         (seqs, k), vocab = drafts.shape, p.shape[-1]
