@@ -23,6 +23,18 @@ int ti_pdl_enabled = 1;
 // Switch programmatic dependent launch on or off for every later launch (default on).
 extern "C" void ti_set_pdl(int enabled) { ti_pdl_enabled = enabled ? 1 : 0; }
 
+// The word that kernels with bounded waits report to: zero from the library's loading on. It belongs to the library, not to an allocator, so a
+// program whose first such call is captured in a graph neither allocates nor clears it there.
+static __device__ int status_cell;
+extern "C" void* ti_status_word() {
+    void* at = nullptr;
+    if (cudaGetSymbolAddress(&at, status_cell) != cudaSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    return at;
+}
+
 // Streaming multiprocessors of the current device, read once; 148 (a B200) where no device answers, so
 // that the host-side plans can be computed and tested without one.
 extern "C" int ti_sm_count() {

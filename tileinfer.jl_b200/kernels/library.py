@@ -135,6 +135,8 @@ def lib():
         fn = getattr(handle, name)
         fn.restype, fn.argtypes = c_longlong, args
         setattr(wrapped, name, fn)
+    handle.ti_status_word.restype, handle.ti_status_word.argtypes = c_void_p, []
+    wrapped.ti_status_word = handle.ti_status_word
     wrapped.handle = handle
     for name, args in _SIGNATURES.items():
         fn = getattr(handle, name)

@@ -42,8 +42,18 @@ def status_word() -> torch.Tensor:
     """Device word that kernels with bounded waits write a code to when a wait runs out."""
     global _status
     if _status is None:
-        _status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        torch.cuda.current_stream()                          # sets CUDA up
+        _status = torch.as_tensor(_LibraryWord(lib().ti_status_word()), device="cuda")
     return _status
+
+
+class _LibraryWord:
+    """One 32-bit integer of the library's own memory, as torch takes it."""
+
+    def __init__(self, address):
+        if not address:
+            raise KernelError("the kernel library has no status word on this device")
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "strides": None, "version": 2}
 
 
 def check_status() -> None:
