@@ -22,14 +22,16 @@
 #define PB_BEST 512                  // tokens that reach the bound, of a block and of the row (both lists lie where the bins do)
 
 // exp((l - max) / T) = 2^((l - max) log2(e) / T), the factor as the sum of two 32-bit numbers: the rounding of the product alone, not of the factor as
-// well. What lies below 2^-126 becomes 0; a masked logit's difference, -inf or NaN, is held to a finite one. (expf with its range reduction took
-// 18 instructions of a token where this takes five, and instructions bounded the kernel.)
+// well. What lies below 2^-126 becomes 0; a difference beyond that, and a masked logit's, -inf or NaN, is held to one whose number is 0 and whose
+// products with both parts of the factor are finite at every temperature. (expf with its range reduction took 18 instructions of a token where this
+// takes five, and instructions bounded the kernel.)
 struct Temper {
     float inv;                                               // 1 / T, for the sampler's weights
     float factor, rest;                                      // log2(e) / T
+    float least;                                             // factor x least = -130
 };
 __device__ __forceinline__ float tempered(float l, float maxl, const Temper& t) {
-    const float d = fmaxf(l - maxl, -3e38f);
+    const float d = fmaxf(l - maxl, t.least);
     float e;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(d, t.factor, d * t.rest)));
     return e;
@@ -408,8 +410,11 @@ extern "C" int ti_probabilities(float* out, long long ldo, const float* logits, 
     TI_REQUIRE(temperature > 0.f, "probabilities: temperature must be > 0");
     TI_REQUIRE(top_k >= 0, "probabilities: top_k must be >= 0");
     TI_REQUIRE(top_p > 0.f && top_p <= 1.f, "probabilities: top_p must be in (0, 1]");
-    const double factor = 1.4426950408889634 / (double)temperature;
-    const Temper temper{1.0f / temperature, (float)factor, (float)(factor - (double)(float)factor)};
+    // The factor from 2^-118 on (a temperature of 5e35: beyond it, differences up to 1e28 are none to 32 bits), so that `least` is a number, and up to the
+    // largest of 32 bits (a temperature of 4e-39: beyond it, no two logits that differ by 1e-36 are near each other).
+    double factor = 1.4426950408889634 / (double)temperature;
+    factor = factor < 0x1p-118 ? 0x1p-118 : factor > 0x1.fffffep127 ? 0x1.fffffep127 : factor;
+    const Temper temper{1.0f / temperature, (float)factor, (float)(factor - (double)(float)factor), (float)(-130.0 / factor)};
     // As few blocks a row as can hold it; more while the rows leave SMs idle and a share stays above 2,048.
     int share = 1;
     while (share < 8 && ((vocab + share - 1) / share > PB_HELD || (n_rows * share * 2 <= ti_sm_count() && vocab / share > 4096))) share *= 2;

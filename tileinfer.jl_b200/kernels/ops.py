@@ -1136,7 +1136,7 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
 
 def probabilities(out, logits, temperature, top_k=0, top_p=1.0):
     """out [rows, vocab] = what ``sample`` draws from with these settings: exp((l - max) / temperature) over the ``top_k`` best (ties to the smaller
-    id; 0: all), then over the smallest best-first prefix whose mass reaches ``top_p``, divided by its sum; 0 elsewhere. A logit of -inf or NaN has
+    id, -0 behind +0; 0: all), then over the smallest best-first prefix whose mass reaches ``top_p``, divided by its sum; 0 elsewhere. A logit of -inf or NaN has
     probability 0. float32; rows of both may be strided."""
     _need(logits, "logits", torch.float32, contiguous=False); _need(out, "out", torch.float32, contiguous=False)
     if logits.dim() != 2 or out.shape != logits.shape or (logits.numel() and (logits.stride(1) != 1 or out.stride(1) != 1)):
