@@ -1,0 +1,38 @@
+"""Tensors that the drafting operators refuse for where they lie, with an error and nothing launched."""
+import pytest
+import torch
+
+from test_attention_few_gpu import make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from tileinfer_b200.kernels import ops
+    return ops
+
+
+def attention_args(nq=4, nkv=2, dim=64):
+    d = {key: t.cuda() for key, t in make([(2, 70)], nq, nkv, dim).items()}
+    return dict(out=torch.zeros(2, nq * dim, dtype=torch.bfloat16, device="cuda"), q=d["q"], k_cache=d["k"], v_cache=d["v"], block_table=d["table"],
+                seq_slots=d["seq_slots"], cu_seqlens=d["cu"], kv_lens=d["lens"], scale=0.1, nq=nq, nkv=nkv, head_dim=dim, page_size=64, max_new=2)
+
+
+def shifted(t, by):
+    """The same values in a contiguous view that begins ``by`` elements further on."""
+    held = torch.zeros(t.numel() + by, dtype=t.dtype, device="cuda")
+    held[by:].copy_(t.reshape(-1))
+    return held[by:].view(t.shape)
+
+
+def test_attention_queries_and_outputs_at_odd_places(ops):
+    args = attention_args()
+    ops.attention_few(**args)
+    want = args["out"].clone()
+    for name in ("q", "out"):
+        with pytest.raises(ops.KernelError, match="4-byte aligned"):
+            ops.attention_few(**{**args, name: shifted(args[name], 1)})
+    out = shifted(torch.zeros_like(want), 2)
+    ops.attention_few(**{**args, "q": shifted(args["q"], 2), "out": out})
+    assert torch.equal(out, want)

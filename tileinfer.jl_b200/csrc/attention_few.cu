@@ -522,6 +522,7 @@ extern "C" int ti_attention_few(void* out, const void* q, const void* k_cache, c
         return 2;
     }
     TI_REQUIRE(status != nullptr && aligned16(k_cache) && aligned16(v_cache), "attention_few: pages must be 16-byte aligned");
+    TI_REQUIRE(((uintptr_t)q | (uintptr_t)out) % 4 == 0, "attention_few: queries and outputs must be 4-byte aligned (two elements are moved at a time)");
     if ((long long)pages * nkv * AF_PAGE > 0x7fffffffLL) {
         ti_fail("attention_few: a pool of %d pages of %d heads has more than 2^31 rows", pages, nkv);
         return 2;
