@@ -36,3 +36,21 @@ def test_attention_queries_and_outputs_at_odd_places(ops):
     out = shifted(torch.zeros_like(want), 2)
     ops.attention_few(**{**args, "q": shifted(args["q"], 2), "out": out})
     assert torch.equal(out, want)
+
+
+def linear_args(n=20, out=1024, k=4096):
+    codes = torch.zeros(out, k // 8, dtype=torch.int32, device="cuda")
+    return dict(y=torch.zeros(n, out, dtype=torch.bfloat16, device="cuda"), x=torch.ones(n, k, dtype=torch.bfloat16, device="cuda"), codes=codes,
+                scales=torch.ones(k // 128, out, dtype=torch.bfloat16, device="cuda"))
+
+
+def test_linear4_work_spaces(ops):
+    args, need = linear_args(), ops.linear4_workspace(20, 1024, 4096)
+    held = torch.empty(2 * need, dtype=torch.uint8, device="cuda")
+    ops.linear4(**args, workspace=held[:need])
+    want = args["y"].clone()
+    ops.linear4(**args, workspace=held[16:])
+    assert torch.equal(args["y"], want)
+    for ws in (held[1:], held[4:], held[:need - 1], held.cpu()):
+        with pytest.raises(ops.KernelError, match="work space"):
+            ops.linear4(**args, workspace=ws)

@@ -25,3 +25,12 @@ def test_attention_few_queries_and_outputs(change):
 @pytest.mark.parametrize("change", [dict(k=AT + 8), dict(v=AT + 2), dict(ws=AT + 4)])
 def test_attention_few_pages_and_work_space(change):
     assert "aligned" in refused(attention_few(**change)) or "work space" in refused(attention_few(**change))
+
+
+@pytest.mark.parametrize("n,out,k", [(20, 4096, 4096), (8, 2048, 9216)])
+@pytest.mark.parametrize("shift", [1, 4, 8])
+def test_linear4_work_space(n, out, k, shift):
+    lib = library.lib()
+    assert lib.ti_linear4_parts(n, out, k) > 0                # such a product takes one
+    rc = lib.ti_linear4(AT, out, AT, k, AT, AT, None, n, out, k, 128, 0, 0.0, 0.0, 0.0, 0.0, 1, AT + shift, AT, None)
+    assert "work space must be 16-byte aligned" in refused(rc)

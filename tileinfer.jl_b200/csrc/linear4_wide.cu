@@ -322,6 +322,7 @@ extern "C" long long ti_linear4_parts(int n, int out, int K) {
 int linear4_wide(void* y, long long ldy, const void* x, long long ldx, const void* codes, const void* scales, const void* zeros, int n, int out, int K,
                  int group, int epilogue, XieluParams act, void* parts, int* status, cudaStream_t stream) {
     TI_REQUIRE(parts != nullptr && status != nullptr, "linear4: work space missing");
+    TI_REQUIRE(aligned16(parts), "linear4: the work space must be 16-byte aligned");
     const int N = tokens_at_once(n);
     CUtensorMap map_codes, map_x;
     {   // The codes as [out, K / 4] numbers of 16 bits, moved as they are.
