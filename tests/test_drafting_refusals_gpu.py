@@ -54,3 +54,15 @@ def test_linear4_work_spaces(ops):
     for ws in (held[1:], held[4:], held[:need - 1], held.cpu()):
         with pytest.raises(ops.KernelError, match="work space"):
             ops.linear4(**args, workspace=ws)
+
+
+@pytest.mark.parametrize("what", ["attention_few", "linear4"])
+def test_work_spaces_that_are_none(ops, what):
+    """On the host, of another type, with holes, or one byte seen many times: refused before anything is launched."""
+    args = attention_args() if what == "attention_few" else linear_args()
+    need = ops.attention_few_workspace(1, 2, 4, 2, 64) if what == "attention_few" else ops.linear4_workspace(20, 1024, 4096)
+    held = torch.empty(2 * need, dtype=torch.uint8, device="cuda")
+    getattr(ops, what)(**args, workspace=held)
+    for ws in (held.cpu(), held[:1].expand(2 * need), held[::2], held[:need // 4 * 4].view(torch.int32), held[:need - 1], held[8:]):
+        with pytest.raises(ops.KernelError, match="work space"):
+            getattr(ops, what)(**args, workspace=ws)

@@ -1032,8 +1032,8 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
     if need:
         if workspace is None:
             workspace = _workspace("linear4", need, x.device, stream)
-        elif workspace.numel() < need or not workspace.is_cuda:
-            raise KernelError(f"linear4: work space of {workspace.numel()} bytes, {need} needed")
+        else:
+            _need_workspace(workspace, need, "linear4")
         parts, status = workspace.data_ptr(), status_word().data_ptr()
     rc = lib().ti_linear4(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(),
                           None if zeros is None else zeros.data_ptr(), n, out, k, group, epilogue, *act, code, parts, status, stream)
@@ -1085,6 +1085,13 @@ def _workspace(kind: str, nbytes: int, device, stream: int, zeroed: int = 0) -> 
     return ws
 
 
+def _need_workspace(ws: torch.Tensor, need: int, what: str) -> None:
+    """A work space that the caller brings."""
+    if not (ws.is_cuda and ws.dtype is _U8 and ws.is_contiguous() and ws.numel() >= need and ws.data_ptr() % 16 == 0):
+        raise KernelError(f"{what}: work space of {tuple(ws.shape)} {ws.dtype} with strides {ws.stride()} at {ws.data_ptr():#x} on {ws.device}; {need} bytes "
+                          "(uint8) in one piece on the device are needed, 16-byte aligned")
+
+
 FEW_HEAD_DIMS, FEW_PAGE = (16, 32, 48, 64, 80, 96, 112, 128, 256), 64        # what attention_few takes
 
 
@@ -1125,8 +1132,11 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
     if n == 0 or seqs == 0:
         return
     stream = _stream()
+    need = attention_few_workspace(seqs, max_new, nq, nkv, head_dim)
     if workspace is None:
-        workspace = _workspace("attention_few", attention_few_workspace(seqs, max_new, nq, nkv, head_dim), q.device, stream)
+        workspace = _workspace("attention_few", need, q.device, stream)
+    else:
+        _need_workspace(workspace, need, "attention_few")
     rc = lib().ti_attention_few(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
                                 seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), workspace.data_ptr(), workspace.numel(),
                                 status_word().data_ptr(), scale, seqs, nq, nkv, head_dim, page_size, max_new, k_cache.shape[0], window or 0, stream)
@@ -1204,9 +1214,8 @@ def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None, workspa
     need, tickets = verify_drafts_workspace(seqs), _tickets(seqs)
     if workspace is None:
         workspace = _workspace("verify_drafts", need, p.device, stream, zeroed=tickets)
-    elif workspace.dtype is not _U8 or not workspace.is_cuda or not workspace.is_contiguous() or workspace.numel() < need or workspace.data_ptr() % 16:
-        raise KernelError(f"verify_drafts: work space of {workspace.numel()} {workspace.dtype} at {workspace.data_ptr():#x} on {workspace.device}; "
-                          f"{need} bytes needed, 16-byte aligned")
+    else:
+        _need_workspace(workspace, need, "verify_drafts")
     # The stretches' sums from the beginning, the tickets, which are zero before and after every call, up to the end: wherever the
     # calls are of fewer sequences, no sums lie where another call's tickets do.
     ws, end = workspace.data_ptr(), workspace.numel() // 16 * 16
