@@ -66,3 +66,13 @@ def test_work_spaces_that_are_none(ops, what):
     for ws in (held.cpu(), held[:1].expand(2 * need), held[::2], held[:need // 4 * 4].view(torch.int32), held[:need - 1], held[8:]):
         with pytest.raises(ops.KernelError, match="work space"):
             getattr(ops, what)(**args, workspace=ws)
+
+
+def test_attention_caches_of_other_dimensions(ops):
+    """A cache is [pages, heads, 64, head size]: with one dimension more, its first is not the number of pages (those beyond it read as zeros)."""
+    args = attention_args()
+    k, v = args["k_cache"], args["v_cache"]
+    pages = k.shape[0]
+    for change in ((k[None], v[None]), (k.view(1, pages, 1, 2, 64, 64), v.view(1, pages, 1, 2, 64, 64)), (k[0], v[0])):
+        with pytest.raises(ops.KernelError, match="do not fit"):
+            ops.attention_few(**{**args, "k_cache": change[0], "v_cache": change[1]})

@@ -1109,18 +1109,20 @@ def attention_few_workspace(seqs: int, max_new: int, nq: int, nkv: int, head_dim
 
 def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, kv_lens, scale, nq, nkv, head_dim, page_size, max_new, window=0,
                   workspace=None) -> None:
-    """Attention of a few new tokens of every sequence over its pages, which hold the new tokens' keys and values already: the tokens
-    cu_seqlens[b] to cu_seqlens[b + 1] of q [n, nq, head_dim] (at most ``max_new`` of them, or none) are the last of the kv_lens[b] positions of the
-    sequence in slot seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out [n, nq * head_dim]. bfloat16 (the
-    32-bit path's sums do not depend on how a step is cut: ``attention_plain``). The work is shared out by the sequences' lengths on the device.
-    ``workspace``: ``attention_few_workspace`` bytes (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
+    """Attention of a few new tokens of every sequence over its pages (k_cache and v_cache [pages, nkv, page_size, head_dim]), which hold the new
+    tokens' keys and values already: the tokens cu_seqlens[b] to cu_seqlens[b + 1] of q [n, nq, head_dim] (at most ``max_new`` of them, or none) are the
+    last of the kv_lens[b] positions of the sequence in slot seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out
+    [n, nq * head_dim]. bfloat16 (the 32-bit path's sums do not depend on how a step is cut: ``attention_plain``). The work is shared out by the
+    sequences' lengths on the device. ``workspace``: ``attention_few_workspace`` bytes (uint8); without it one kept per thread and stream (a captured
+    call: one of its graph's own)."""
     seqs, n = kv_lens.numel(), q.shape[0]
     fits = out.dtype is _BF16 and q.dtype is _BF16 and k_cache.dtype is _BF16 and v_cache.dtype is _BF16 and out.is_cuda and q.is_cuda and \
         k_cache.is_cuda and v_cache.is_cuda and out.is_contiguous() and q.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous() and \
         block_table.dtype is _I32 and seq_slots.dtype is _I32 and cu_seqlens.dtype is _I32 and kv_lens.dtype is _I32 and block_table.is_cuda and \
         seq_slots.is_cuda and cu_seqlens.is_cuda and kv_lens.is_cuda and seq_slots.is_contiguous() and cu_seqlens.is_contiguous() and \
         kv_lens.is_contiguous() and nkv > 0 and nq > 0 and nq % nkv == 0 and head_dim > 0 and max_new >= 0 and window >= 0 and \
-        q.numel() == n * nq * head_dim == out.numel() and k_cache.shape == v_cache.shape and k_cache.shape[-3:] == (nkv, page_size, head_dim) and \
+        q.numel() == n * nq * head_dim == out.numel() and k_cache.shape == v_cache.shape and k_cache.dim() == 4 and \
+        k_cache.shape[1:] == (nkv, page_size, head_dim) and \
         cu_seqlens.numel() == seqs + 1 and seq_slots.numel() == seqs and block_table.dim() == 2 and (not block_table.numel() or block_table.stride(1) == 1)
     if not fits:
         for t, name in ((out, "out"), (q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache")):
