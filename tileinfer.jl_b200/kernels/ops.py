@@ -1004,10 +1004,9 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
     """y [n, out] = x [n, in] Wᵀ for W[o, k] = (code - zero) * scale: ``codes`` [out, in / 8] int32 hold eight consecutive k a word (the even
     ones in its low half, the odd ones in its high half, four bits each in ascending order), ``scales`` [in / group, out] of x's type for groups of
     32, 64 or 128 k, ``zeros`` [in / group, out] uint8, or 8 for all. 32-bit sums, rounded once; with ``EPI_F32_OUT`` y is float32 and the sums
-    are not rounded. Made for steps of few tokens; any number is taken. ``quantize4`` makes the codes. Codes, scales and zeros are read while the kernel
-    right ahead may still run: they come from ``quantize4``, copies or torch's operations, not from another of this library's kernels right
-    ahead. ``workspace``: ``linear4_workspace`` bytes
-    (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
+    are not rounded. Made for steps of few tokens; any number is taken. ``quantize4`` makes the codes. Codes, scales and zeros are read while kernels
+    ahead may still run: they come from ``quantize4``, copies or torch's operations, not from other kernels of this library. ``workspace``:
+    ``linear4_workspace`` bytes (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
     dtype = x.dtype
     # One expression while all is well (a draft's step makes hundreds of these calls); what is wrong is looked for afterwards.
     try:
@@ -1115,9 +1114,9 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
     tokens' keys and values already: the tokens cu_seqlens[b] to cu_seqlens[b + 1] of q [n, nq, head_dim] (at most ``max_new`` of them, or none) are the
     last of the kv_lens[b] positions of the sequence in slot seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out
     [n, nq * head_dim]. bfloat16 (the 32-bit path's sums do not depend on how a step is cut: ``attention_plain``). The work is shared out by the
-    sequences' lengths on the device. Lengths, ranges, slots, table, and the pages before those of the new tokens are read while the kernel right ahead
-    may still run: they come from copies, torch's operations or earlier steps, and of this library's kernels the one right ahead may have written q and
-    the new tokens' keys and values alone. ``workspace``: ``attention_few_workspace`` bytes (uint8); without it one kept per thread and stream (a captured
+    sequences' lengths on the device. Lengths, ranges, slots, table, and the pages before those of the new tokens are read while kernels ahead may
+    still run: they come from copies, torch's operations or earlier steps; what this library's kernels ahead write is q and the new tokens' keys
+    and values alone. ``workspace``: ``attention_few_workspace`` bytes (uint8); without it one kept per thread and stream (a captured
     call: one of its graph's own)."""
     seqs, n = kv_lens.numel(), q.shape[0]
     fits = out.dtype is _BF16 and q.dtype is _BF16 and k_cache.dtype is _BF16 and v_cache.dtype is _BF16 and out.is_cuda and q.is_cuda and \
