@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(AF_THREADS, FewSmem<D>::BLOCKS) attention_few_
             }
             if (whole) {
                 const int row = at.slab * M + r, i = row / group;
-                out[((size_t)(first_token + i) * nq + (size_t)at.kvh * group + (row - i * group)) * D + d] = __float2bfloat16_rn(sum > 0.f ? acc / sum : 0.f);
+                out[((size_t)(first_token + i) * nq + (size_t)at.kvh * group + (row - i * group)) * D + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
             } else {
                 ws_o[(slot * M + r) * D + d] = acc;
                 if (d == 0) { ws_ml[(slot * M + r) * 2] = mm; ws_ml[(slot * M + r) * 2 + 1] = sum; }
@@ -456,7 +456,8 @@ __global__ void __launch_bounds__(32 * AF_JOIN_WARPS) attention_few_join_kernel(
                 acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
             }
         }
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        if (sum == 0.f) { acc = make_float4(0.f, 0.f, 0.f, 0.f); sum = 1.f; }            // nothing was visible; a NaN sum stays one
+        const float inv = 1.f / sum;
         if (on) {
             reinterpret_cast<__nv_bfloat162*>(dst + d)[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
             reinterpret_cast<__nv_bfloat162*>(dst + d)[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
