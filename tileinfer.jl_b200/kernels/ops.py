@@ -1031,11 +1031,8 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
     parts = status = None
     need = linear4_workspace(n, out, k) if code == BF16 else 0
     if need:
-        if workspace is None:
-            workspace = _workspace("linear4", need, x.device, stream)
-        else:
-            _need_workspace(workspace, need, "linear4")
-        parts, status = workspace.data_ptr(), status_word().data_ptr()
+        held = _workspace("linear4", need, x.device, stream) if workspace is None else _need_workspace(workspace, need, "linear4")
+        parts, status = held[0], status_word().data_ptr()
     rc = lib().ti_linear4(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(),
                           None if zeros is None else zeros.data_ptr(), n, out, k, group, epilogue, *act, code, parts, status, stream)
     if rc:
@@ -1062,35 +1059,36 @@ def quantize4(codes, scales, w, zeros=None):
 
 
 _kept = threading.local()            # .spaces: the work spaces of the thread
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
-def _workspace(kind: str, nbytes: int, device, stream: int, zeroed: int = 0) -> torch.Tensor:
-    """At least ``nbytes`` of the kind's work space, the last ``zeroed`` bytes zero when a call first gets them: for a thread's calls on ``stream``, which
-    follow one another, one that is kept and grown on demand (two threads' calls on one stream may alternate kernel by kernel, so each thread has its
-    own). A call that is being captured gets one of its graph's own memory, and its fill is captured with
-    it: the graph is replayed whenever and wherever the program likes, so nothing else may use it, and it lasts as long as the graph."""
-    if torch.cuda.is_current_stream_capturing():
+def _workspace(kind: str, nbytes: int, device, stream: int, zeroed: int = 0):
+    """(address, bytes, tensor) of at least ``nbytes`` of the kind's work space, the last ``zeroed`` bytes zero when a call first gets them: for a
+    thread's calls on ``stream``, which follow one another, one that is kept and grown on demand (two threads' calls on one stream may alternate kernel
+    by kernel, so each thread has its own). A call that is being captured gets one of its graph's own memory, and its fill is captured with it: the
+    graph is replayed whenever and wherever the program likes, so nothing else may use it, and it lasts as long as the graph."""
+    if stream and _capturing():                              # CUDA's default stream (0) cannot be captured: a test less for most calls
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         if zeroed:
             ws[nbytes - zeroed:].zero_()
-        return ws
+        return ws.data_ptr(), nbytes, ws
     try:
-        spaces = _kept.spaces
+        held = _kept.spaces.get((kind, stream, device))
     except AttributeError:
-        spaces = _kept.spaces = {}
-    key = (kind, device, stream)
-    ws = spaces.get(key)
-    if ws is None or ws.numel() < nbytes:
-        make = torch.zeros if zeroed else torch.empty
-        ws = spaces[key] = make(max(nbytes, 4096), dtype=torch.uint8, device=device)
-    return ws
+        _kept.spaces, held = {}, None
+    if held is None or held[1] < nbytes:
+        nbytes = max(nbytes, 4096)
+        ws = (torch.zeros if zeroed else torch.empty)(nbytes, dtype=torch.uint8, device=device)
+        held = _kept.spaces[kind, stream, device] = ws.data_ptr(), nbytes, ws
+    return held
 
 
-def _need_workspace(ws: torch.Tensor, need: int, what: str) -> None:
-    """A work space that the caller brings."""
+def _need_workspace(ws: torch.Tensor, need: int, what: str):
+    """(address, bytes, tensor) of a work space that the caller brings."""
     if not (ws.is_cuda and ws.dtype is _U8 and ws.is_contiguous() and ws.numel() >= need and ws.data_ptr() % 16 == 0):
         raise KernelError(f"{what}: work space of {tuple(ws.shape)} {ws.dtype} with strides {ws.stride()} at {ws.data_ptr():#x} on {ws.device}; {need} bytes "
                           "(uint8) in one piece on the device are needed, 16-byte aligned")
+    return ws.data_ptr(), ws.numel(), ws
 
 
 FEW_HEAD_DIMS, FEW_PAGE = (16, 32, 48, 64, 80, 96, 112, 128, 256), 64        # what attention_few takes
@@ -1138,12 +1136,9 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
         return
     stream = _stream()
     need = attention_few_workspace(seqs, max_new, nq, nkv, head_dim)
-    if workspace is None:
-        workspace = _workspace("attention_few", need, q.device, stream)
-    else:
-        _need_workspace(workspace, need, "attention_few")
+    held = _workspace("attention_few", need, q.device, stream) if workspace is None else _need_workspace(workspace, need, "attention_few")
     rc = lib().ti_attention_few(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                                seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                                seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), held[0], held[1],
                                 status_word().data_ptr(), scale, seqs, nq, nkv, head_dim, page_size, max_new, k_cache.shape[0], window or 0, stream)
     if rc:
         check(rc, "attention_few")
@@ -1179,16 +1174,18 @@ def _refuse_run(what, accepted, tokens, drafts, counts, **others):
 _verify_need = {}
 
 
+def _verify_sizes(seqs: int):
+    """(bytes of work space that a test of so many sequences' drafts needs, those of its tickets)."""
+    sizes = _verify_need.get(seqs)
+    if sizes is None:
+        tickets = (4 * seqs + 15) // 16 * 16
+        sizes = _verify_need[seqs] = int(lib().ti_verify_drafts_workspace(seqs)) + tickets, tickets
+    return sizes
+
+
 def verify_drafts_workspace(seqs: int) -> int:
     """Bytes of work space that ``verify_drafts`` needs."""
-    need = _verify_need.get(seqs)
-    if need is None:
-        need = _verify_need[seqs] = int(lib().ti_verify_drafts_workspace(seqs)) + _tickets(seqs)
-    return need
-
-
-def _tickets(seqs: int) -> int:
-    return (4 * seqs + 15) // 16 * 16
+    return _verify_sizes(seqs)[0]
 
 
 def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None, workspace=None):
@@ -1216,16 +1213,12 @@ def verify_drafts(accepted, tokens, p, q, drafts, uniforms, counts=None, workspa
     if seqs == 0:
         return
     stream = _stream()
-    need, tickets = verify_drafts_workspace(seqs), _tickets(seqs)
-    if workspace is None:
-        workspace = _workspace("verify_drafts", need, p.device, stream, zeroed=tickets)
-    else:
-        _need_workspace(workspace, need, "verify_drafts")
+    need, tickets = _verify_sizes(seqs)
+    ws, size, _held = _workspace("verify_drafts", need, p.device, stream, tickets) if workspace is None else _need_workspace(workspace, need, "verify_drafts")
     # The stretches' sums from the beginning, the tickets, which are zero before and after every call, up to the end: wherever the
     # calls are of fewer sequences, no sums lie where another call's tickets do.
-    ws, end = workspace.data_ptr(), workspace.numel() // 16 * 16
     rc = lib().ti_verify_drafts(accepted.data_ptr(), tokens.data_ptr(), p.data_ptr(), p.stride(0), p.stride(1), *q_args, drafts.data_ptr(),
-                                uniforms.data_ptr(), None if counts is None else counts.data_ptr(), seqs, k, vocab, ws, ws + end - tickets, stream)
+                                uniforms.data_ptr(), None if counts is None else counts.data_ptr(), seqs, k, vocab, ws, ws + size // 16 * 16 - tickets, stream)
     if rc:
         check(rc, "verify_drafts")
 
