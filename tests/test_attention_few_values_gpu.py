@@ -49,3 +49,18 @@ def test_they_reach_the_rows_that_see_them(ops, dim, nq, nkv, where, what, key):
 def test_in_a_runs_last_key_or_query(ops, dim, nq, nkv, where, what):
     """Every sequence's last position, which its last token alone sees."""
     check(ops, spoiled(where, what, 10 ** 6, nq, nkv, dim), nq, nkv, dim)
+
+
+@pytest.mark.parametrize("dim,nq,nkv", [(16, 4, 2), (64, 4, 2), (80, 8, 1), (96, 12, 2), (256, 4, 2), (128, 32, 2), (128, 64, 2), (32, 60, 2)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("window", [0, 1, 2, 70])
+def test_a_value_that_some_tokens_of_a_run_do_not_see(ops, dim, nq, nkv, what, window):
+    """A drafted token's own value, which the tokens before it do not see; with a window the first values, which the later tokens do not see any more."""
+    runs = ((3, 700), (2, 90), (1, 5000), (3, 65), (3, 3))
+    check(ops, spoiled("v", what, 10 ** 6, nq, nkv, dim, runs), nq, nkv, dim, window)
+    c = spoiled("v", what, 10 ** 6, nq, nkv, dim, runs)
+    for b, (new, length) in enumerate(runs):
+        for at in (length - 2, length - window - 1):          # the middle of a run; the last that its last token but one sees, not its last
+            if at >= 0:
+                c["v"][int(c["table"][int(c["seq_slots"][b]), at // 64]), 1 % nkv, at % 64, 3] = what
+    check(ops, c, nq, nkv, dim, window)

@@ -11,7 +11,8 @@
 //
 // Four warps share a tile out as MT groups of 16 rows x 4 / MT groups of keys. Scores, the running maximum and sum, and the output stand in
 // 32-bit; P is rounded to bfloat16 as the operand of P V alone (its sum is not), O once. A tile's keys and values beyond the sequence's end or
-// before the first visible key may hold anything: their scores are replaced and their values zeroed.
+// before the first visible key may hold anything: their scores are replaced and their values zeroed. An infinite or NaN value of a key that some
+// rows see and others do not (a drafted token's own) reaches the rows that see it alone.
 //
 // 5 tokens after 65,531 (32 / 8 heads of 128, 268 MB) 51.6 us, 5.2 TB/s; 64 x 4 tokens after 1,024 59 us, 4.6 TB/s with the joins of two or three parts an
 // item; 8 x 8 tokens after up to 32,768 (64 / 8 heads: slabs of 64 rows) 126 us, 1.48 of the bytes' time: the softmax's instructions beside the MMAs.
@@ -50,6 +51,10 @@ template <int D> struct FewSmem {
 template <int D> __device__ __forceinline__ int few_at(int row, int c) {
     if (FewSmem<D>::TMA) return (c >> 3) * (AF_PAGE * 64) + row * 64 + (((c & 7) ^ (row & 7)) << 3);
     return (row * (D / 8) + swz<D>(row, c)) * 8;
+}
+// Two bfloat16 numbers with 0 in the place of an infinity or NaN.
+__device__ __forceinline__ unsigned finite_pair(unsigned pair) {
+    return ((pair & 0x7F80u) == 0x7F80u ? 0u : pair & 0xFFFFu) | ((pair & 0x7F800000u) == 0x7F800000u ? 0u : pair & 0xFFFF0000u);
 }
 // Below 2^-126: 0.
 __device__ __forceinline__ float power2(float x) {
@@ -224,6 +229,7 @@ __global__ void __launch_bounds__(AF_THREADS, FewSmem<D>::BLOCKS) attention_few_
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
+        bool odd = false;
         int tile = s.t0 + at.tile;
         for (; u < seg_end; ++u, ++tile) {
             if (SM::TMA) ok = tc::mbar_wait(smem_u32(s_full + stage), phase, status, 28);
@@ -243,6 +249,26 @@ __global__ void __launch_bounds__(AF_THREADS, FewSmem<D>::BLOCKS) attention_few_
                 if (SM::TMA) tc::fence_async_smem();
                 __syncthreads();
             }
+            // A tile at the run's or the window's edge holds keys that some rows see and others do not. 0 x infinity and 0 x NaN are NaN, so a warp takes such
+            // values out of its share of the tile and adds them at the segment's end, to the rows that see them. (Warps of other rows take out the same.)
+            const bool edge = key_base + AF_PAGE > s.L - s.T + 1 || (window > 0 && key_base < s.L - window);
+            if (edge && s.T > 1) {
+                const int share = key_base + wk * MT * 16;
+                bool found = false;
+                auto take_out = [&](int from, int to) {      // keys from `from` up to `to`, as far as they lie in the share
+                    const int first = max(from - share, 0), count = (min(to - share, MT * 16) - first) * CPR;
+                    for (int c = lane; c < count; c += 32) {
+                        uint4* at16 = reinterpret_cast<uint4*>(vt + few_at<D>(wk * MT * 16 + first + c / CPR, c % CPR));
+                        const uint4 v = *at16, f = make_uint4(finite_pair(v.x), finite_pair(v.y), finite_pair(v.z), finite_pair(v.w));
+                        if ((v.x ^ f.x) | (v.y ^ f.y) | (v.z ^ f.z) | (v.w ^ f.w)) { *at16 = f; found = true; }
+                    }
+                };
+                take_out(s.L - s.T + 1, s.L);
+                if (window > 0) take_out(s.first, s.L - window);
+                if (SM::TMA && found) tc::fence_async_smem();
+                odd |= __any_sync(0xffffffffu, found);
+                __syncwarp();
+            }
             float sc[2 * MT][4];
 #pragma unroll
             for (int i = 0; i < 2 * MT; ++i)
@@ -259,11 +285,10 @@ __global__ void __launch_bounds__(AF_THREADS, FewSmem<D>::BLOCKS) attention_few_
                     mma16816(sc[2 * nb], qf[ks], kb[0], kb[1]);
                     mma16816(sc[2 * nb + 1], qf[ks], kb[2], kb[3]);
                 }
-            // Maxima of the unscaled scores (the scale, which is positive, is taken with the exponent); a tile at the run's or the window's edge has
-            // its scores replaced first.
+            // Maxima of the unscaled scores (the scale, which is positive, is taken with the exponent); a tile at an edge has its scores replaced first.
             float mx0 = -INFINITY, mx1 = -INFINITY;
-            if (key_base + AF_PAGE > s.L - s.T + 1 || (window > 0 && key_base < s.L - window)) {
-                const int key0 = key_base + wk * MT * 16 + 2 * t;
+            const int key0 = key_base + wk * MT * 16 + 2 * t;
+            if (edge) {
 #pragma unroll
                 for (int i = 0; i < 2 * MT; ++i)
 #pragma unroll
@@ -319,6 +344,25 @@ __global__ void __launch_bounds__(AF_THREADS, FewSmem<D>::BLOCKS) attention_few_
             if (u + 1 < seg_end) issue();
         }
         if (!ok) break;
+        if (s.T > 1 && __syncthreads_or(odd)) {              // what was taken out (by any warp): infinite or NaN whatever its weight
+            auto put_back = [&](int from, int to) {
+                for (int key = max(from, (s.t0 + at.tile) * AF_PAGE); key < min(to, tile * AF_PAGE); ++key) {
+                    if ((key % AF_PAGE) / (MT * 16) != wk) continue;
+                    const int page = __ldcg(block_table + (size_t)s_slot[at.b] * table_stride + key / AF_PAGE);
+                    const bf16* value = v_cache + (((size_t)page * nkv + at.kvh) * AF_PAGE + key % AF_PAGE) * D + 2 * t;
+                    const bool s0 = key <= pos[0] && key >= low[0], s1 = key <= pos[1] && key >= low[1];
+#pragma unroll
+                    for (int c = 0; c < NT; ++c) {
+                        const unsigned v = __ldcg(reinterpret_cast<const unsigned*>(value + 8 * c)), e = v ^ finite_pair(v);         // 0 for what stayed
+                        const float e0 = __uint_as_float(e << 16), e1 = __uint_as_float(e & 0xFFFF0000u);
+                        if (s0) { o[c][0] += e0; o[c][1] += e1; }
+                        if (s1) { o[c][2] += e0; o[c][3] += e1; }
+                    }
+                }
+            };
+            put_back(s.L - s.T + 1, s.L);
+            if (window > 0) put_back(s.first, min(s.L - window, s.L - s.T + 1));
+        }
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
 
