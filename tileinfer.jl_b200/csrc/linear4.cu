@@ -357,8 +357,9 @@ extern "C" int ti_linear4(void* y, long long ldy, const void* x, long long ldx, 
                   x_wide, epilogue, act);
         return ti_check_launch("linear4");
     }
-    // Rows of x that TMA does not take go eight tokens at a time, too.
-    if (ti_linear4_shared(n, out, K) && aligned16(x) && ldx % 8 == 0)
+    if (n == 1) ldx = K;                                     // a single row's pitch means nothing
+    // Rows of x that TMA does not take (unaligned ones, ones that overlap) go eight tokens at a time, too.
+    if (ti_linear4_shared(n, out, K) && aligned16(x) && ldx % 8 == 0 && ldx >= K)
         return linear4_wide(y, ldy, x, ldx, codes, scales, zeros, n, out, K, group, epilogue, act, parts, status, stream);
     TI_REQUIRE((n + 7) / 8 <= 65535, "linear4: %d tokens in one launch", n);
     const bool y32 = epilogue == L4_EPI_F32_OUT;
