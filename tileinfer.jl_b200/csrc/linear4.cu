@@ -1,9 +1,10 @@
 // Products with weights of 4 bits for steps of few tokens (a draft's): y[n, out] = x[n, in] · W[out, in]ᵀ with
 //   W[o, k] = (code[o, k] - zero[k / group, o]) * scale[k / group, o],
 // codes 0 to 15 (eight consecutive k in a 32-bit word: the even ones in its low half, the odd ones in its high half, four bits each in
-// ascending order), a scale of x's type per row and group of 32, 64 or 128 k, and a zero per row and group (8 for all without a table).
+// ascending order), a scale of x's type per row and group of 32, 64 or 128 k, and a zero of 0 to 128 per row and group (8 for all without a table).
 //
-// Exactness: code - zero is a whole number of at most 15 and exact in bfloat16. A group's products x (code - zero) are summed in 32-bit,
+// Exactness: code - zero is a whole number from -128 to 15 and exact in bfloat16, and so is 128 + zero, by way of which it is made (beyond 128 it would
+// not be). A group's products x (code - zero) are summed in 32-bit,
 // the sum is multiplied by the group's scale in 32-bit, and the groups' sums are added in 32-bit; the result is rounded once. Nothing is
 // rounded to fewer bits before that (a weight (code - zero) * scale rounded to bfloat16 would cost as much again as the output's rounding).
 #include "linear4.cuh"

@@ -1003,7 +1003,7 @@ def linear4_workspace(n: int, out_features: int, in_features: int) -> int:
 def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0.0, 0.0), workspace=None):
     """y [n, out] = x [n, in] Wᵀ for W[o, k] = (code - zero) * scale: ``codes`` [out, in / 8] int32 hold eight consecutive k a word (the even
     ones in its low half, the odd ones in its high half, four bits each in ascending order), ``scales`` [in / group, out] of x's type for groups of
-    32, 64 or 128 k, ``zeros`` [in / group, out] uint8, or 8 for all. 32-bit sums, rounded once; with ``EPI_F32_OUT`` y is float32 and the sums
+    32, 64 or 128 k, ``zeros`` [in / group, out] uint8 of 0 to 128, or 8 for all. 32-bit sums, rounded once; with ``EPI_F32_OUT`` y is float32 and the sums
     are not rounded. Made for steps of few tokens; any number is taken. ``quantize4`` makes the codes. Codes, scales and zeros are read while kernels
     ahead may still run: they come from ``quantize4``, copies or torch's operations, not from other kernels of this library. ``workspace``:
     ``linear4_workspace`` bytes (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
