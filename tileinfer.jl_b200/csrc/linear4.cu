@@ -228,6 +228,13 @@ __global__ void __launch_bounds__(L4_WARPS * 32, 2) linear4_kernel(const unsigne
     }
 }
 
+// Blocks and passes over a block's rows, of the fours of rows that `out` makes.
+static void linear4_grid(int out, int& blocks, int& passes) {
+    const int fours = (out + 3) / 4, slots = 2 * ti_sm_count();
+    blocks = fours < slots ? fours : slots;
+    passes = (fours + blocks * (4 * L4_MT) - 1) / (blocks * (4 * L4_MT));
+}
+
 template <int GROUP>
 static int launch_linear4(const void* codes, const void* scales, const void* zeros, const void* x, long long ldx, void* y, long long ldy, int n,
                           int out, int K, int epilogue, XieluParams act, bool y32, cudaStream_t stream) {
@@ -241,9 +248,8 @@ static int launch_linear4(const void* codes, const void* scales, const void* zer
         if (e != cudaSuccess) return ti_fail("linear4: %s", cudaGetErrorString(e));
         configured = true;
     }
-    const int fours = (out + 3) / 4, slots = 2 * ti_sm_count();
-    const int blocks = fours < slots ? fours : slots;
-    const int passes = (fours + blocks * (4 * L4_MT) - 1) / (blocks * (4 * L4_MT));
+    int blocks, passes;
+    linear4_grid(out, blocks, passes);
     const bool x_wide = aligned16(x) && ldx % 8 == 0;
     const bool s_wide = out % 4 == 0 && (uintptr_t)scales % 4 == 0 && (uintptr_t)zeros % 4 == 0;
     ti_launch(linear4_kernel<GROUP>, dim3(blocks, (n + 7) / 8), dim3(L4_WARPS * 32), smem, stream, (const unsigned*)codes,
@@ -326,15 +332,36 @@ __global__ void __launch_bounds__(L4F_WARPS * 32) linear4_f32_kernel(const unsig
 }
 
 // Which of the two bfloat16 kernels: eight tokens at a time, each time over all codes, or up to 32 tokens through shared memory (linear4_wide.cu), whose
-// blocks take equal runs of units and need a second kernel to join shared tiles. Up to eight tokens the first reads a block's tokens once per
-// stretch of k, for few rows that is most of its work: it is left to short k. us, eights / shared memory: 1 token x 21,504 x 4,096 14.6 / 17.1,
-// x 6,144 x 4,096 7.4 / 8.3, x 12,856 x 8,000 18.5 / 20.3, x 65,536 x 2,048 24.1 / 22.8, x 131,072 x 4,096 84 / 70; x 1,024 x 8,192 9.2 / 7.7, x 200 x 11,904
-// 8.9 / 7.9; 16 tokens x 21,504 x 4,096 31 / 18.9, x 1,024 x 1,024 5.7 / 4.9, x 512 x 512 2.9 / 5.2; 32 tokens x 1,024 x 1,024 11.2 / 6.4, x 320 x 2,048
-// 6.1 / 6.9; 64 tokens x 512 x 512 11 / 6.5.
+// blocks take equal runs of units and need a second kernel to join shared tiles. The one that an estimate of its microseconds says is the faster. The
+// estimates are fitted to 738 measured shapes (1 to 64 tokens, 100 to 131,072 rows, 128 to 28,672 k); on those and 160 others, what is chosen takes 1.4 %
+// more than the better of the two on average, and more than a tenth more in one of twenty.
+//   Eights: the rounds of blocks, each with a start, a time per k and tile of 16 rows that a block takes one after the other, its tokens read once a
+//   pass (twice as dear where two blocks share an SM), an end per pass, and, where rows are no whole fours, scales by loads that every piece waits for.
+//   Shared memory: a start, the units an SM takes, wider stages from 17 tokens on, and for runs that cut items the join and its parts.
+// us, eights / shared memory: 1 token x 21,504 x 4,096 14.6 / 17.1, x 28,672 x 4,096 22.4 / 20.4, x 8,192 x 8,192 13.1 / 13.9, x 10,240 x 8,192 17.3 / 16.1,
+// x 12,856 x 8,000 18.2 / 19.8, x 131,072 x 4,096 83.6 / 68.1; 8 tokens x 1,024 x 6,144 10.2 / 6.7, x 4,096 x 4,096 6.7 / 7.7, x 4,096 x 8,192 12.1 / 9.9; 16 x
+// 1,024 x 512 5.5 / 4.4, x 512 x 512 2.7 / 4.3; 32 x 320 x 2,048 6.3 / 6.4, x 256 x 2,048 4.1 / 6.3; 48 x 1,024 x 256 13.7 / 4.7; 7 x 27,221 x 224 17.1 / 3.8.
 extern "C" int ti_linear4_shared(int n, int out, int K) {
-    const long long weights = (long long)out * K;
-    if (n <= 8) return weights >= 1LL << 27 || (weights >= 1LL << 21 && K >= 8192);
-    return (long long)((n + 7) / 8) * weights >= 1LL << 21;
+    if (n <= 0 || out <= 0 || K <= 0) return 0;
+    const int sms = ti_sm_count(), tokens = n <= 8 ? 8 : n <= 16 ? 16 : 32;
+    const long long steps = (K + L4_KC - 1) / L4_KC, row_tiles = (out + 255) / 256;
+    int blocks, passes;
+    linear4_grid(out, blocks, passes);
+    const long long resident = (long long)blocks * ((n + 7) / 8), rounds = (resident + 2 * sms - 1) / (2 * sms);
+    const long long share = ((out + 3) / 4 + (long long)passes * blocks - 1) / ((long long)passes * blocks);
+    const double tiles = (double)passes * ((share + 3) / 4), k = steps * L4_KC / 1000.0, dense = resident > sms ? 2 : 1;
+    const double eighths = (n < 8 ? n : 8) / 8.0;
+    double eights = 1.9 + 3.5 * (passes - 1) + k * (0.46 * tiles + passes * dense * (0.17 + 0.2 * eighths * eighths));
+    if (out % 4 != 0) eights += 0.6 * ((steps + L4_WARPS - 1) / L4_WARPS) * tiles;
+    eights *= rounds;
+
+    const long long units = row_tiles * ((n + tokens - 1) / tokens) * steps, runs = units < sms ? units : sms;
+    double shared = 2.4 + 1.45 * units / sms + (tokens == 32 ? 1.55 : 0.0);
+    if (units % runs != 0 || units / runs % steps != 0) {
+        const double parts = sms / (double)row_tiles;
+        shared += 1.4 + 0.095 * (steps < parts ? steps : parts);
+    }
+    return shared < eights;
 }
 
 // codes [out, K / 8] words, scales [K / group, out] of x's type, zeros [K / group, out] bytes or null; y [n, ldy] of x's type, or 32-bit sums
