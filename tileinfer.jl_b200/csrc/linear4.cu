@@ -355,9 +355,9 @@ extern "C" int ti_linear4_shared(int n, int out, int K) {
     if (out % 4 != 0) eights += 0.6 * ((steps + L4_WARPS - 1) / L4_WARPS) * tiles;
     eights *= rounds;
 
-    const long long units = row_tiles * ((n + tokens - 1) / tokens) * steps, runs = units < sms ? units : sms;
+    const long long units = row_tiles * ((n + tokens - 1) / tokens) * steps;
     double shared = 2.4 + 1.45 * units / sms + (tokens == 32 ? 1.55 : 0.0);
-    if (units % runs != 0 || units / runs % steps != 0) {
+    if (linear4_cuts_items(units, steps)) {
         const double parts = sms / (double)row_tiles;
         shared += 1.4 + 0.095 * (steps < parts ? steps : parts);
     }

@@ -34,6 +34,12 @@ inline bool linear4_epilogue_known(int e) {
     return e == L4_EPI_NONE || e == L4_EPI_XIELU || e == L4_EPI_F32_OUT || (e >= TI_EPI_GELU_ERF && e <= TI_EPI_LAST);
 }
 
+// Whether runs of equal length end inside of an item of `steps` units, whose parts a second kernel then joins.
+inline bool linear4_cuts_items(long long units, long long steps) {
+    const long long runs = units < ti_sm_count() ? units : ti_sm_count();
+    return units % runs != 0 || units / runs % steps != 0;
+}
+
 // linear4_wide.cu
 extern "C" int ti_linear4_shared(int n, int out, int K);
 int linear4_wide(void* y, long long ldy, const void* x, long long ldx, const void* codes, const void* scales, const void* zeros, int n, int out, int K,

@@ -304,7 +304,7 @@ template <int NT, int GROUP> int launch(const CUtensorMap& codes, const CUtensor
     const int blocks = (int)a.units < ti_sm_count() ? (int)a.units : ti_sm_count();
     ti_launch(linear4_wide_kernel<NT, GROUP>, dim3(blocks), dim3(S::THREADS), smem, stream, codes, x, a);
     if (int rc = ti_check_launch("linear4_wide")) return rc;
-    if (a.units % blocks == 0 && (a.units / blocks) % a.steps == 0) return 0;            // every run ends with an item: no parts
+    if (!linear4_cuts_items(a.units, a.steps)) return 0;     // every run ends with an item: no parts
     const int tiles = (a.out + ROWS - 1) / ROWS;
     const bool by_cuts = (long long)tiles * a.chunks > blocks - 1 || a.chunks > 65535;
     ti_launch(linear4_join_kernel, dim3(2 * (by_cuts ? blocks - 1 : tiles), ((a.n < 8 * NT ? a.n : 8 * NT) + JOIN_TOKENS - 1) / JOIN_TOKENS, by_cuts ? 1 : a.chunks),
@@ -317,6 +317,13 @@ template <int NT, int GROUP> int launch(const CUtensorMap& codes, const CUtensor
 // Bytes of the work space for parts: 0 where the product takes none.
 extern "C" long long ti_linear4_parts(int n, int out, int K) {
     return ti_linear4_shared(n, out, K) ? 2LL * ti_sm_count() * tokens_at_once(n) * ROWS * 4 : 0;
+}
+
+// Kernels of a product whose rows TMA takes: two where it goes through shared memory and leaves parts to join.
+extern "C" int ti_linear4_kernels(int n, int out, int K) {
+    if (!ti_linear4_shared(n, out, K)) return 1;
+    const long long steps = (K + KC - 1) / KC, N = tokens_at_once(n);
+    return linear4_cuts_items((long long)((out + ROWS - 1) / ROWS) * ((n + N - 1) / N) * steps, steps) ? 2 : 1;
 }
 
 int linear4_wide(void* y, long long ldy, const void* x, long long ldx, const void* codes, const void* scales, const void* zeros, int n, int out, int K,

@@ -135,6 +135,8 @@ def lib():
         fn = getattr(handle, name)
         fn.restype, fn.argtypes = c_longlong, args
         setattr(wrapped, name, fn)
+    handle.ti_linear4_kernels.restype, handle.ti_linear4_kernels.argtypes = c_int, [_I] * 3
+    wrapped.ti_linear4_kernels = handle.ti_linear4_kernels
     handle.ti_status_word.restype, handle.ti_status_word.argtypes = c_void_p, []
     wrapped.ti_status_word = handle.ti_status_word
     wrapped.handle = handle

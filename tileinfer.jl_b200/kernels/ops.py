@@ -992,12 +992,18 @@ LINEAR4_GROUPS = (32, 64, 128)
 _linear4_need = {}
 
 
+def _linear4_sizes(n: int, out_features: int, in_features: int):
+    """(bytes of work space, kernels) of a bfloat16 product whose rows go through shared memory where that is the faster."""
+    sizes = _linear4_need.get((n, out_features, in_features))
+    if sizes is None:
+        shape = n, out_features, in_features
+        sizes = _linear4_need[shape] = int(lib().ti_linear4_parts(*shape)), lib().ti_linear4_kernels(*shape)
+    return sizes
+
+
 def linear4_workspace(n: int, out_features: int, in_features: int) -> int:
     """Bytes of work space that ``linear4`` needs for n bfloat16 tokens (0: none)."""
-    need = _linear4_need.get((n, out_features, in_features))
-    if need is None:
-        need = _linear4_need[n, out_features, in_features] = int(lib().ti_linear4_parts(n, out_features, in_features))
-    return need
+    return _linear4_sizes(n, out_features, in_features)[0]
 
 
 def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0.0, 0.0), workspace=None):
@@ -1029,7 +1035,7 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
     code = dtype_code(dtype)
     stream = _stream()
     parts = status = None
-    need = linear4_workspace(n, out, k) if code == BF16 else 0
+    need, kernels = _linear4_sizes(n, out, k) if code == BF16 else (0, 1)
     if need:
         held = _workspace("linear4", need, x.device, stream) if workspace is None else _need_workspace(workspace, need, "linear4")
         parts, status = held[0], status_word().data_ptr()
@@ -1037,6 +1043,8 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
                           None if zeros is None else zeros.data_ptr(), n, out, k, group, epilogue, *act, code, parts, status, stream)
     if rc:
         check(rc, "linear4")
+    if kernels > 1 and x.data_ptr() % 16 == 0 and (n == 1 or (x.stride(0) % 8 == 0 and x.stride(0) >= k)):
+        _library.add_launches(1)                             # the join; rows that TMA does not take have none
 
 
 def quantize4(codes, scales, w, zeros=None):
@@ -1092,6 +1100,7 @@ def _need_workspace(ws: torch.Tensor, need: int, what: str):
 
 
 FEW_HEAD_DIMS, FEW_PAGE = (16, 32, 48, 64, 80, 96, 112, 128, 256), 64        # what attention_few takes
+FEW_MAX_SEQS = 512                                                            # sequences of its one launch (csrc/attention_few.cu: AF_MAX_SEQS)
 
 
 _attention_few_need = {}
@@ -1142,6 +1151,8 @@ def attention_few(out, q, k_cache, v_cache, block_table, seq_slots, cu_seqlens, 
                                 status_word().data_ptr(), scale, seqs, nq, nkv, head_dim, page_size, max_new, k_cache.shape[0], window or 0, stream)
     if rc:
         check(rc, "attention_few")
+    if seqs > FEW_MAX_SEQS:
+        _library.add_launches(2 * ((seqs - 1) // FEW_MAX_SEQS))
 
 
 def probabilities(out, logits, temperature, top_k=0, top_p=1.0):
