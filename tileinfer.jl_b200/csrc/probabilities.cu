@@ -65,7 +65,7 @@ __device__ __forceinline__ u64 pb_scan(u64 v, u64* scratch, u64& total) {
 
 template <int C>
 __global__ void __launch_bounds__(PB_THREADS, 3) probabilities_kernel(float* out, long long ldo, const float* logits, long long ld, int vocab, int per,
-                                                                   Temper temper, int top_k, float top_p, bool held, bool masses) {
+                                                                   Temper temper, int top_k, float top_p, bool held) {
     extern __shared__ __align__(16) unsigned char pb_smem[];
     __shared__ float scratch[33];
     __shared__ u64 scan[PB_WARPS];
@@ -398,7 +398,7 @@ static int launch_probabilities(float* out, long long ldo, const float* logits, 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ti_pdl_enabled ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, probabilities_kernel<C>, out, ldo, logits, ld, vocab, per, temper, top_k, top_p, held, masses);
+    cudaLaunchKernelEx(&cfg, probabilities_kernel<C>, out, ldo, logits, ld, vocab, per, temper, top_k, top_p, held);
     return ti_check_launch("probabilities");
 }
 
