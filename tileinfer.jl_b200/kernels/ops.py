@@ -1039,11 +1039,12 @@ def linear4(y, x, codes, scales, zeros=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0
     if need:
         held = _workspace("linear4", need, x.device, stream) if workspace is None else _need_workspace(workspace, need, "linear4")
         parts, status = held[0], status_word().data_ptr()
-    rc = lib().ti_linear4(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(),
+    at, pitch = x.data_ptr(), x.stride(0)
+    rc = lib().ti_linear4(y.data_ptr(), y.stride(0), at, pitch, codes.data_ptr(), scales.data_ptr(),
                           None if zeros is None else zeros.data_ptr(), n, out, k, group, epilogue, *act, code, parts, status, stream)
     if rc:
         check(rc, "linear4")
-    if kernels > 1 and x.data_ptr() % 16 == 0 and (n == 1 or (x.stride(0) % 8 == 0 and x.stride(0) >= k)):
+    if kernels > 1 and at % 16 == 0 and (n == 1 or (pitch % 8 == 0 and pitch >= k)):
         _library.add_launches(1)                             # the join; rows that TMA does not take have none
 
 
