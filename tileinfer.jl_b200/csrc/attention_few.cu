@@ -10,12 +10,13 @@
 // item that several blocks share are left in 32-bit (maximum, sum, unnormalised output) and joined by a second kernel in ascending order.
 //
 // Four warps share a tile out as MT groups of 16 rows x 4 / MT groups of keys. Scores, the running maximum and sum, and the output stand in
-// 32-bit; P is rounded to bfloat16 as the operand of P V alone (its sum is not), O once. A tile's keys and values beyond the sequence's end or
-// before the first visible key may hold anything: their scores are replaced and their values zeroed. An infinite or NaN value of a key that some
-// rows see and others do not (a drafted token's own) reaches the rows that see it alone.
+// 32-bit; P is rounded to bfloat16 as the operand of P V alone (its sum is not), O once: outputs are off by 2.1e-3 to 2.3e-3 of their size, where O's
+// own rounding makes 1.7e-3. A tile's keys and values beyond the sequence's end or before the first visible key may hold anything: their scores are
+// replaced and their values zeroed. An infinite or NaN value of a key that some rows see and others do not (a drafted token's own) reaches the rows
+// that see it alone.
 //
-// 5 tokens after 65,531 (32 / 8 heads of 128, 268 MB) 51.6 us, 5.2 TB/s; 64 x 4 tokens after 1,024 59 us, 4.6 TB/s with the joins of two or three parts an
-// item; 8 x 8 tokens after up to 32,768 (64 / 8 heads: slabs of 64 rows) 126 us, 1.48 of the bytes' time: the softmax's instructions beside the MMAs.
+// 5 tokens after 65,531 (32 / 8 heads of 128, 268 MB) 53.7 us, 5.0 TB/s; 64 x 4 tokens after 1,024 61 us, 4.4 TB/s with the joins of two or three parts an
+// item; 8 x 8 tokens after up to 32,768 (64 / 8 heads: slabs of 64 rows) 124 us, 1.44 of the bytes' time: the softmax's instructions beside the MMAs.
 #include "even_runs.cuh"
 #include "mma_util.cuh"
 #include "tcgen05.cuh"
