@@ -339,7 +339,10 @@ __global__ void __launch_bounds__(AF_THREADS, FewSmem<D>::BLOCKS) attention_few_
                     mma16816(o[c + 1], pf, vb[2], vb[3]);
                 }
             }
-            // The stage is filled again as soon as all have left it, before the next tile is waited for.
+            // The stage is filled again as soon as all have left it, before the next tile is waited for. A barrier alone does not keep the copies, which are
+            // another proxy's, behind reads that a warp has asked for and not yet used: without the fence a few of a hundred thousand items met the
+            // next but one tile's values.
+            if (SM::TMA) tc::fence_async_smem();
             ok = __syncthreads_and(ok);
             if (!ok) break;
             if (u + 1 < seg_end) issue();
