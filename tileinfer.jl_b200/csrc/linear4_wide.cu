@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(Shape<NT, GROUP>::THREADS, 1) linear4_wide_ker
             scales += S::S_ROW; zeros += S::Z_ROW;
             s_low += 2u * (unsigned)p.out; z_low += (unsigned)p.out;
         }
+        fence_async_smem();                                  // the stage's next copies are another proxy's than these reads
         __syncwarp();
         if (lane == 0) mbar_arrive(empty0 + 8 * stage);
         if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
