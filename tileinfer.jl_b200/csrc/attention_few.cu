@@ -15,7 +15,7 @@
 // replaced and their values zeroed. An infinite or NaN value of a key that some rows see and others do not (a drafted token's own) reaches the rows
 // that see it alone.
 //
-// 5 tokens after 65,531 (32 / 8 heads of 128, 268 MB) 53.7 us, 5.0 TB/s; 64 x 4 tokens after 1,024 61 us, 4.4 TB/s with the joins of two or three parts an
+// 5 tokens after 65,531 (32 / 8 heads of 128, 268 MB) 53.5 us, 5.0 TB/s; 64 x 4 tokens after 1,024 61 us, 4.4 TB/s with the joins of two or three parts an
 // item; 8 x 8 tokens after up to 32,768 (64 / 8 heads: slabs of 64 rows) 124 us, 1.44 of the bytes' time: the softmax's instructions beside the MMAs.
 #include "even_runs.cuh"
 #include "mma_util.cuh"
