@@ -135,6 +135,10 @@ def lib():
         fn = getattr(handle, name)
         fn.restype, fn.argtypes = c_longlong, args
         setattr(wrapped, name, fn)
+    for name, args in (("ti_linear8_workspace", [_I] * 4), ("ti_attention8_workspace", [_I] * 6)):
+        fn = getattr(handle, name)
+        fn.restype, fn.argtypes = c_longlong, args
+        setattr(wrapped, name, fn)
     handle.ti_linear4_kernels.restype, handle.ti_linear4_kernels.argtypes = c_int, [_I] * 3
     wrapped.ti_linear4_kernels = handle.ti_linear4_kernels
     handle.ti_status_word.restype, handle.ti_status_word.argtypes = c_void_p, []
@@ -282,4 +286,12 @@ _SIGNATURES.update({
     "ti_verify_drafts": [_P, _P, _P, _L, _L, _P, _L, _L, _P, _P, _P, _I, _I, _I, _P, _P, _P],
     "ti_match_drafts": [_P, _P, _P, _P, _P, _I, _I, _P],
     "ti_uniforms": [_P, _P, _P, _I, _I, _P],
+})
+
+# Serving in 8-bit floating point: codes of matrices, products with them, the cache's new rows, attention over it.
+_SIGNATURES.update({
+    "ti_quantize8": [_P, _P, _P, _L, _I, _I, _I, _I, _P],
+    "ti_linear8": [_P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _F, _F, _F, _F, _P, _L, _P, _P],
+    "ti_cache_write8": [_P, _P, _P, _P, _P, _L, _L, _P, _L, _L, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
+    "ti_attention8": [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _L, _P, _F, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
 })

@@ -16,7 +16,7 @@ from . import library as _library
 from .library import KernelError, check, lib
 
 F32, BF16 = 0, 1
-_F32, _I32, _U8, _BF16 = torch.float32, torch.int32, torch.uint8, torch.bfloat16
+_F32, _I32, _U8, _BF16, _E4M3 = torch.float32, torch.int32, torch.uint8, torch.bfloat16, torch.float8_e4m3fn
 EPI_NONE, EPI_XIELU, EPI_F32_OUT = 0, 1, 2
 EPI_GELU_ERF, EPI_GELU_TANH = 4, 5          # GELU of the rounded sum, exact or tanh form (3: raw partial sums, inside the library)
 EPI_RELU2 = 6                               # max(rounded sum, 0)^2
@@ -1256,3 +1256,160 @@ def uniforms(out, seeds, counters):
     if out.dim() != 2 or seeds.numel() != out.shape[0] or counters.numel() != out.shape[0]:
         raise KernelError(f"uniforms: out {tuple(out.shape)} for {seeds.numel()} seeds, {counters.numel()} counters")
     check(lib().ti_uniforms(out.data_ptr(), seeds.data_ptr(), counters.data_ptr(), out.shape[0], out.shape[1], _stream()), "uniforms")
+
+
+# ---------------------------------------------------------------- numbers of 8 bits: e4m3 codes with a scale per block
+BLOCK8 = 128                         # columns (and, of weights, rows) of a matrix that share a scale
+
+
+def _blocks8(n: int) -> int:
+    return -(-n // BLOCK8)
+
+
+def quantize8(codes, scales, x, rows: int = 1):
+    """codes [n, k] float8_e4m3fn and scales [ceil(k / 128), ceil(n / rows)] float32 of x [n, k] (float32 or bfloat16; its rows may be strided): a scale for every
+    128 columns of each row (``rows`` 1: a product's inputs) or of 128 rows (128: its weights). A block's scale is the smallest power of two s >= 2^-100
+    with |x| <= 448 s over its finite x, its codes are x / s rounded to nearest even; what is infinite or NaN has the code of NaN. k is a multiple of 16."""
+    _need(x, "x", contiguous=False); _need(codes, "codes", _E4M3); _need(scales, "scales", _F32)
+    if rows not in (1, BLOCK8):
+        raise KernelError(f"quantize8: blocks of 1 or {BLOCK8} rows, not {rows}")
+    if x.dim() != 2 or codes.shape != x.shape or x.shape[1] % 16 or tuple(scales.shape) != (_blocks8(x.shape[1]), -(-x.shape[0] // rows)) or \
+            (x.numel() and x.stride(1) != 1):
+        raise KernelError(f"quantize8: x {tuple(x.shape)} with strides {x.stride()}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)} do not fit (dense rows of "
+                          f"a multiple of 16 elements, scales [ceil(k / {BLOCK8}), ceil(n / {rows})])")
+    check(lib().ti_quantize8(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), x.stride(0), dtype_code(x.dtype), x.shape[0], x.shape[1], rows, _stream()),
+          "quantize8")
+
+
+_linear8_need = {}
+
+
+def linear8_workspace(n: int, out_features: int, in_features: int, given: bool = False) -> int:
+    """Bytes of work space that ``linear8`` needs for n tokens (``given``: that come as codes); 0: none."""
+    key = (n, out_features, in_features, given)
+    need = _linear8_need.get(key)
+    if need is None:
+        need = _linear8_need[key] = int(lib().ti_linear8_workspace(*key))
+    return need
+
+
+def linear8(y, x, codes, scales, x_scales=None, epilogue=EPI_NONE, act=(0.0, 0.0, 0.0, 0.0), workspace=None):
+    """y [n, out] = x [n, in] Wᵀ for W of e4m3 ``codes`` [out, in] with ``scales`` [ceil(in / 128), ceil(out / 128)] (``quantize8`` with ``rows`` 128; any
+    positive scales are taken). x is bfloat16 and quantised by row in groups of 128 on the way, as ``quantize8`` does it, or codes with ``x_scales``
+    [ceil(in / 128), n]. 32-bit sums of every group, scaled and added in 32-bit, rounded once to y's bfloat16; with ``EPI_F32_OUT`` y is float32 and the sums
+    are not rounded. ``in`` is a multiple of 16; rows of x and y may be strided. Codes and scales of the weights are read while kernels ahead may still run:
+    they come from ``quantize8`` before other work, copies or torch's operations. ``workspace``: ``linear8_workspace`` bytes (uint8); without it
+    one kept per thread and stream (a captured call: one of its graph's own)."""
+    try:
+        (n, k), (out, columns), given = x.shape, codes.shape, x_scales is not None
+        fits = x.is_cuda and y.is_cuda and codes.is_cuda and scales.is_cuda and codes.dtype is _E4M3 and scales.dtype is _F32 and columns == k and \
+            k % 16 == 0 and k > 0 and codes.is_contiguous() and scales.is_contiguous() and scales.shape == (_blocks8(k), _blocks8(out)) and \
+            y.shape == (n, out) and y.dtype is (_F32 if epilogue == EPI_F32_OUT else _BF16) and (x.stride(1) == 1 or not n) and \
+            (y.stride(1) == 1 or not n * out) and x.dtype is (_E4M3 if given else _BF16) and \
+            (not given or (x_scales.is_cuda and x_scales.dtype is _F32 and x_scales.shape == (_blocks8(k), n) and x_scales.is_contiguous()))
+    except ValueError:
+        raise KernelError("linear8: x, y and codes have two dimensions") from None
+    if not fits:
+        for t, name, want in ((x, "x", _BF16 if x_scales is None else _E4M3), (y, "y", None), (codes, "codes", _E4M3), (scales, "scales", _F32), (x_scales, "x_scales", _F32)):
+            if t is not None:
+                _need(t, name, want, contiguous=name not in ("x", "y"))
+        raise KernelError(f"linear8: x {tuple(x.shape)} {x.stride()}, x_scales {None if x_scales is None else tuple(x_scales.shape)}, codes {tuple(codes.shape)}, "
+                          f"scales {tuple(scales.shape)}, y {tuple(y.shape)} {y.stride()} of {y.dtype} do not fit (in a multiple of 16, scales for blocks of "
+                          f"{BLOCK8}, dense rows, y bfloat16 or float32 with EPI_F32_OUT)")
+    stream = _stream()
+    need = linear8_workspace(n, out, k, given)
+    ws, size = None, 0
+    if need:
+        ws, size, _held = _workspace("linear8", need, x.device, stream) if workspace is None else _need_workspace(workspace, need, "linear8")
+    rc = lib().ti_linear8(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), x_scales.data_ptr() if given else None, codes.data_ptr(), scales.data_ptr(), n, out, k,
+                          epilogue, *act, ws, size, status_word().data_ptr(), stream)
+    if rc:
+        check(rc, "linear8")
+
+
+def _paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, page_size) -> bool:
+    """What the two operators on an 8-bit cache ask of what they share."""
+    seqs = kv_lens.numel()
+    return k_cache.dtype is _E4M3 and v_cache.dtype is _E4M3 and k_cache.is_cuda and v_cache.is_cuda and k_cache.dim() == 4 and k_cache.shape == v_cache.shape and \
+        k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.shape[2] == page_size and k_scales.dtype is _F32 and v_scales.dtype is _F32 and \
+        k_scales.is_cuda and v_scales.is_cuda and k_scales.is_contiguous() and v_scales.is_contiguous() and k_scales.shape == k_cache.shape[:2] and \
+        v_scales.shape == k_cache.shape[:2] and block_table.dtype is _I32 and seq_slots.dtype is _I32 and cu_seqlens.dtype is _I32 and kv_lens.dtype is _I32 and \
+        block_table.is_cuda and seq_slots.is_cuda and cu_seqlens.is_cuda and kv_lens.is_cuda and seq_slots.is_contiguous() and cu_seqlens.is_contiguous() and \
+        kv_lens.is_contiguous() and cu_seqlens.numel() == seqs + 1 and seq_slots.numel() == seqs and block_table.dim() == 2 and \
+        (not block_table.numel() or block_table.stride(1) == 1)
+
+
+def _refuse_paged8(what, k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, said):
+    for t, name, want in ((k_cache, "k_cache", _E4M3), (v_cache, "v_cache", _E4M3), (k_scales, "k_scales", _F32), (v_scales, "v_scales", _F32),
+                          (block_table, "block_table", _I32), (seq_slots, "seq_slots", _I32), (cu_seqlens, "cu_seqlens", _I32), (kv_lens, "kv_lens", _I32)):
+        _need(t, name, want, contiguous=name != "block_table")
+    raise KernelError(f"{what}: {said}, pages {tuple(k_cache.shape)} and {tuple(v_cache.shape)}, scales {tuple(k_scales.shape)} and {tuple(v_scales.shape)}, "
+                      f"{kv_lens.numel()} sequences, table {tuple(block_table.shape)} do not fit (scales [pages, heads])")
+
+
+def cache_write8(k_cache, v_cache, k_scales, v_scales, k, v, block_table, seq_slots, cu_seqlens, kv_lens, max_new) -> None:
+    """The rows cu_seqlens[b] to cu_seqlens[b + 1] of k and v [n, nkv, head_dim] (bfloat16 or float32, any strides but for a dense last dimension) become the last of the
+    kv_lens[b] positions of the sequence in slot seq_slots[b], in its pages of k_cache and v_cache [pages, nkv, 64, head_dim] float8_e4m3fn. A page's head is
+    a block with a scale of its own for keys and for values (``k_scales``, ``v_scales`` [pages, nkv] float32): the smallest power of two s >= 2^-100
+    with |x| <= 448 s. In a page whose first new row is not its first position the scale never shrinks, and where it grows the codes before that row move
+    with it; a page that is new from its first position on begins afresh. What lies behind a sequence's last position stays as it was. ``max_new``: the most new
+    rows of a sequence (a sequence may have none). No two sequences may be given rows of one page. A sequence whose slot, page or length is none that
+    exists is left out. Infinite and NaN values get the code of NaN."""
+    said = f"k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}, {max_new} new rows"
+    if not (_paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, PAGE8) and k.is_cuda and v.is_cuda and
+            k.dtype in (_BF16, _F32) and v.dtype is k.dtype and k.dim() == 3 and k.shape == v.shape and k.shape[1:] == (k_cache.shape[1], k_cache.shape[3]) and
+            (not k.numel() or (k.stride(2) == 1 and v.stride(2) == 1)) and max_new >= 0):
+        _need(k, "k", contiguous=False); _need(v, "v", k.dtype, contiguous=False); dtype_code(k.dtype)
+        _refuse_paged8("cache_write8", k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, said)
+    pages, nkv, page, dim = k_cache.shape
+    if not k.numel() or not kv_lens.numel() or not block_table.numel():
+        return
+    rc = lib().ti_cache_write8(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), k.data_ptr(), k.stride(0), k.stride(1),
+                               v.data_ptr(), v.stride(0), v.stride(1), block_table.data_ptr(), block_table.stride(0), block_table.shape[0], seq_slots.data_ptr(),
+                               cu_seqlens.data_ptr(), kv_lens.data_ptr(), kv_lens.numel(), k.shape[0], nkv, dim, page, pages, max_new,
+                               BF16 if k.dtype is _BF16 else F32, _stream())
+    if rc:
+        check(rc, "cache_write8")
+
+
+PAGE8, HEAD8 = 64, 256               # positions of a page; heads are multiples of 16 up to this
+_attention8_need = {}
+
+
+def attention8_workspace(seqs: int, max_new: int, nq: int, nkv: int, head_dim: int, max_len: int) -> int:
+    """Bytes of work space that ``attention8`` needs for sequences of up to ``max_len`` positions."""
+    key = (seqs, max_new, nq, nkv, head_dim, max_len)
+    need = _attention8_need.get(key)
+    if need is None:
+        need = _attention8_need[key] = int(lib().ti_attention8_workspace(*key))
+    return need
+
+
+def attention8(out, q, k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, scale, nq, nkv, head_dim, page_size, max_new, window=0,
+               max_len=None, workspace=None) -> None:
+    """Attention of the new tokens of every sequence over its pages in 8 bits, which hold the new tokens' keys and values already (``cache_write8``): the tokens
+    cu_seqlens[b] to cu_seqlens[b + 1] of q [n, nq, head_dim] (at most ``max_new``, or none) are the last of the kv_lens[b] positions of the sequence in slot
+    seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out [n, nq * head_dim]; q and out bfloat16. A key stands for its code times
+    k_scales[page, head], a value for its code times v_scales[page, head] (positive, 2^-100 to 2^120). ``max_len``: no kv_lens is larger (None: as many as the
+    table's rows have pages for). What no token sees may hold any codes; a NaN code that some see reaches those alone. Lengths, ranges, slots, table, and the
+    pages before those of the new tokens are read while kernels ahead may still run: they come from copies, torch's operations or earlier steps. ``workspace``:
+    ``attention8_workspace`` bytes (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
+    seqs, n = kv_lens.numel(), q.shape[0]
+    if not (_paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, page_size) and out.is_cuda and q.is_cuda and
+            out.dtype is _BF16 and q.dtype is _BF16 and out.is_contiguous() and q.is_contiguous() and nkv > 0 and nq > 0 and nq % nkv == 0 and head_dim > 0 and
+            max_new >= 0 and window >= 0 and q.numel() == n * nq * head_dim == out.numel() and k_cache.shape[1:] == (nkv, page_size, head_dim) and
+            (max_len is None or max_len >= 0)):
+        _need(out, "out", _BF16); _need(q, "q", _BF16)
+        _refuse_paged8("attention8", k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens,
+                       f"q {tuple(q.shape)}, out {tuple(out.shape)}, {nq} / {nkv} heads of {head_dim} on pages of {page_size}, {max_new} new tokens, window {window}")
+    if n == 0 or seqs == 0 or max_new == 0:
+        return
+    stream, whole = _stream(), block_table.shape[1] * page_size
+    max_len = whole if max_len is None else min(max_len, whole)
+    need = attention8_workspace(seqs, max_new, nq, nkv, head_dim, max_len)
+    ws, size, _held = _workspace("attention8", need, q.device, stream) if workspace is None else _need_workspace(workspace, need, "attention8")
+    rc = lib().ti_attention8(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(),
+                             block_table.stride(0), seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), ws, size, status_word().data_ptr(), scale, seqs, n,
+                             nq, nkv, head_dim, page_size, max_new, max_len, k_cache.shape[0], window or 0, stream)
+    if rc:
+        check(rc, "attention8")
