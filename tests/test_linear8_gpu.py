@@ -60,6 +60,7 @@ def check(ops, n, out, k, given=False, f32=False, seed=0, any_scale=False):
     off = (y[:n].to(F64) - want).abs()
     assert bool((off <= bound).all()), float((off / bound.clamp_min(1e-30)).max())
     assert bool((y[n:] == 7).all())
+    ops.check_status()
 
 
 SIZES = [(1, 1, 16), (1, 128, 128), (1, 300, 2064), (5, 320, 96), (3, 129, 144), (8, 256, 4096), (9, 1000, 1040), (16, 2048, 512), (17, 513, 384), (32, 640, 272),
