@@ -5,6 +5,16 @@ extern "C" int ti_quantize8(void* codes, void* scales, const void* x, long long 
 
 static long long up16(long long bytes) { return (bytes + 15) / 16 * 16; }
 
+// Weight rows in the lanes, 64 tokens at once (linear8_mid.cu), or tokens in the lanes on SM pairs (linear8_many.cu): the shorter by estimates in microseconds. The
+// one takes half of one for every 128 x 64 x 128 that an SM gets, the other 0.75 for every step of 256 of k of a pair's tiles, rounds of which are whole.
+// Microseconds in turn: 64 tokens of 21,504 x 4,096 29 / 38, 256 81 / 41, 2,048 502 / 210; 128 of 4,096 x 21,504 40 / 72, 512 129 / 78; 256 of 4,096 x 4,096
+// 16.2 / 15.8.
+static bool takes_many(int n, int out, int K) {
+    const double groups = (K + 127) / 128, units = (double)((out + 127) / 128) * ((n + 63) / 64) * groups;
+    const long long tiles = (long long)((out + 127) / 128) * ((n + 255) / 256), pairs = ti_sm_count() / 2, rounds = (tiles + pairs - 1) / pairs;
+    return 3.0 + rounds * (1.0 + 0.75 * ((groups + 1) / 2)) < 5.0 + 0.5 * units / ti_sm_count();
+}
+
 // Tokens that come as bfloat16 are quantised by every block that needs them where they are few, else by a launch of its own ahead (1.5 us more): 21,504 x
 // 4,096 takes 20.9 us for one token, 23.0 for four, 26.9 for eight in one launch; 21.3 for eight whose codes are given.
 static bool quantized_ahead(int n, int out, int K) { return n > 4 || !linear8_takes_few(n, out, K); }
@@ -21,6 +31,7 @@ extern "C" int ti_linear8(void* y, long long ldy, const void* x, long long ldx, 
     TI_REQUIRE(n > 0 && out > 0 && K > 0 && K % 16 == 0, "linear8: %d tokens x %d x %d", n, out, K);
     TI_REQUIRE(linear4_epilogue_known(epilogue), "linear8: unknown epilogue %d", epilogue);
     TI_REQUIRE(aligned16(codes) && (x_scales == nullptr || (aligned16(x) && (n == 1 || ldx % 16 == 0))), "linear8: rows of codes must be 16-byte aligned");
+    TI_REQUIRE((uintptr_t)x % 2 == 0 && (uintptr_t)y % 2 == 0, "linear8: a misaligned address");
     TI_REQUIRE(status != nullptr, "linear8: status word missing");
     const long long need = ti_linear8_workspace(n, out, K, x_scales != nullptr);
     TI_REQUIRE(need == 0 || (ws != nullptr && aligned16(ws) && ws_bytes >= need), "linear8: work space of %lld bytes, %lld needed", ws_bytes, need);
@@ -31,5 +42,6 @@ extern "C" int ti_linear8(void* y, long long ldy, const void* x, long long ldx, 
         x = made; ldx = K; x_scales = made_scales;
     }
     const Linear8 a = {y, ldy, x, ldx, x_scales, (const unsigned char*)codes, scales, n, out, K, epilogue, XieluParams{alpha_p, alpha_n, beta, eps}, status};
-    return linear8_takes_few(n, out, K) ? linear8_few(a, stream) : linear8_mid(a, stream);
+    if (linear8_takes_few(n, out, K)) return linear8_few(a, stream);
+    return takes_many(n, out, K) ? linear8_many(a, stream) : linear8_mid(a, stream);
 }

@@ -25,6 +25,20 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, unsigned (&r)[16]) {
         : "r"(taddr) : "memory");
 }
 
+// One thread of a warp, the same one every time: code that only this guards stays uniform for the compiler, which keeps descriptors and counters in uniform
+// registers then (an issuing loop under `lane == 0` took four times the cycles a group).
+__device__ __forceinline__ bool elected() {
+    unsigned one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+// A whole warp's wait: one lane tests the barrier, the others follow it.
+__device__ __forceinline__ bool warp_wait(unsigned bar, unsigned parity, int* status, int code) {
+    bool ok = true;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, status, code);
+    return __all_sync(0xffffffffu, ok);
+}
+
 }  // namespace tc
 
 struct Linear8 {
@@ -84,3 +98,4 @@ inline void linear8_launch(void (*kernel)(KArgs...), dim3 grid, int threads, siz
 bool linear8_takes_few(int n, int out, int K);
 int linear8_few(const Linear8& a, cudaStream_t stream);
 int linear8_mid(const Linear8& a, cudaStream_t stream);
+int linear8_many(const Linear8& a, cudaStream_t stream);

@@ -91,10 +91,19 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
 
     // The tokens' codes and factors: eight lanes a token's group of codes, sixteen of bfloat16 numbers.
     if (GIVEN) {
-        for (int e = threadIdx.x; e < own * N * 8; e += THREADS) {
-            const int piece = e & 7, token = (e >> 3) % N, group = (e >> 3) / N, k = (lo + group) * KB + piece * 16;
-            const uint4 v = token < p.n && k < p.K ? __ldcg(reinterpret_cast<const uint4*>((const unsigned char*)p.x + (long long)token * p.ldx + k)) : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(smem + (group * N + token) * KB + ((piece ^ (token & 7)) << 4)) = v;
+        constexpr int BATCH = 6;
+        for (int e0 = threadIdx.x; e0 < own * N * 8; e0 += BATCH * THREADS) {
+            uint4 v[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int e = e0 + i * THREADS, token = (e >> 3) % N, k = (lo + (e >> 3) / N) * KB + (e & 7) * 16;
+                v[i] = e < own * N * 8 && token < p.n && k < p.K ? __ldcg(reinterpret_cast<const uint4*>((const unsigned char*)p.x + (long long)token * p.ldx + k)) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int e = e0 + i * THREADS, token = (e >> 3) % N;
+                if (e < own * N * 8) *reinterpret_cast<uint4*>(smem + (e >> 3) * KB + (((e & 7) ^ token) << 4)) = v[i];
+            }
         }
         for (int e = threadIdx.x; e < own * N; e += THREADS) factors[e] = e % N < p.n ? __ldcg(p.x_scales + (long long)(lo + e / N) * p.n + e % N) : 0.f;
     } else {

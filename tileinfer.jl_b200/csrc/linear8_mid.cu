@@ -16,7 +16,7 @@ using namespace tc;
 constexpr int ROWS = 128, KB = 128, W_BYTES = ROWS * KB, THREADS = 352, MAX_SPLIT = 8;
 
 template <int N> struct Shape {
-    static constexpr int ACCS = N <= 64 ? 4 : 2, COLS = ACCS * N, X_BYTES = N * KB, STAGE = W_BYTES + X_BYTES;
+    static constexpr int ACCS = 4, COLS = ACCS * N, X_BYTES = N * KB, STAGE = W_BYTES + X_BYTES;
     static constexpr int STAGES = 104 * 1024 / STAGE;        // two blocks an SM
     // Factors of a group's tokens: a place is written again when the group STAGES + ACCS before has been added (its accumulator was given to a
     // group whose stage has been read since).
@@ -91,24 +91,26 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_mid_kernel(const __grid_co
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ---------------------------------------------------------------- MMAs, one thread
+        // ---------------------------------------------------------------- MMAs: one thread of a warp that walks along
         int stage = 0, slot = 0;
         unsigned phase = 0, slot_phase = 0;
-        for (int g = lo; lane == 0 && g < hi; ++g) {
-            ok = mbar_wait(acce0 + 8 * slot, slot_phase ^ 1, p.status, 19) && mbar_wait(full0 + 8 * stage, phase, p.status, 20);
+        const unsigned long long first = smem_desc_sw128(smem_addr(tiles));
+        for (int g = lo; g < hi; ++g) {
+            ok = __all_sync(0xffffffffu, mbar_wait(acce0 + 8 * slot, slot_phase ^ 1, p.status, 19) && mbar_wait(full0 + 8 * stage, phase, p.status, 20));
             if (!ok) break;
             tc_fence_after();
-            const unsigned from = smem_addr(tiles + stage * S::STAGE);
-            const unsigned long long dw = smem_desc_sw128(from), dx = smem_desc_sw128(from + W_BYTES);
+            const unsigned long long dw = first + (unsigned)(stage * (S::STAGE >> 4)), dx = dw + (W_BYTES >> 4);
+            if (elected()) {
 #pragma unroll
-            for (int k = 0; k < KB / 32; ++k)                // 32 bytes further along the swizzled rows
-                umma_e4m3(tmem + slot * N, dw + 2 * k, dx + 2 * k, instr_desc_e4m3(N), k > 0);
-            umma_commit(empty0 + 8 * stage);
-            umma_commit(accf0 + 8 * slot);
+                for (int k = 0; k < KB / 32; ++k)            // 32 bytes further along the swizzled rows
+                    umma_e4m3(tmem + slot * N, dw + 2 * k, dx + 2 * k, instr_desc_e4m3(N), k > 0);
+                umma_commit(empty0 + 8 * stage);
+                umma_commit(accf0 + 8 * slot);
+            }
+            __syncwarp();
             if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
             if (++slot == S::ACCS) { slot = 0; slot_phase ^= 1; }
         }
-        __syncwarp();
     } else if (warp < 10) {
         // ---------------------------------------------------------------- the groups' sums, scaled and added: a thread a weight row, half of the tokens
         constexpr int H = N / 2;
@@ -120,7 +122,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_mid_kernel(const __grid_co
         unsigned slot_phase = 0, place_phase = 0;
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
         for (int g = lo; g < hi; ++g) {
-            ok = __all_sync(0xffffffffu, mbar_wait(fac0 + 8 * place, place_phase, p.status, 21) && mbar_wait(accf0 + 8 * slot, slot_phase, p.status, 22));
+            ok = warp_wait(fac0 + 8 * place, place_phase, p.status, 21) && warp_wait(accf0 + 8 * slot, slot_phase, p.status, 22);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -172,7 +174,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_mid_kernel(const __grid_co
 #pragma unroll
                 for (int i = 0; i < V; ++i) now[i] = f[j][i];
                 load(g0 + j + 2, f[j]);
-                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * stage, phase ^ 1, p.status, 23));
+                ok = warp_wait(empty0 + 8 * stage, phase ^ 1, p.status, 23);
                 if (!ok) break;
 #pragma unroll
                 for (int i = 0; i < V; ++i) s_factor[place][lane + 32 * i] = now[i];
@@ -235,10 +237,10 @@ template <int N> int launch(const Linear8& p, int split, cudaStream_t stream) {
 }  // namespace
 
 int linear8_mid(const Linear8& p, cudaStream_t stream) {
-    const int groups = (p.K + KB - 1) / KB, N = p.n <= 32 ? 32 : p.n <= 64 ? 64 : 128;
+    const int groups = (p.K + KB - 1) / KB, N = p.n <= 32 ? 32 : 64;
     const long long tiles = (long long)((p.out + ROWS - 1) / ROWS) * ((p.n + N - 1) / N);
     int split = 1;                                           // blocks of a cluster: powers of two, as in linear8_few.cu
     while (split < MAX_SPLIT && 2 * split <= groups && 2 * split * tiles <= 2 * ti_sm_count()) split *= 2;
     TI_REQUIRE((p.n + N - 1) / N <= 65535, "linear8: %d tokens are too many", p.n);
-    return N == 32 ? launch<32>(p, split, stream) : N == 64 ? launch<64>(p, split, stream) : launch<128>(p, split, stream);
+    return N == 32 ? launch<32>(p, split, stream) : launch<64>(p, split, stream);
 }

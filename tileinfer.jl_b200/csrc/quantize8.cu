@@ -64,7 +64,16 @@ template <typename T> int launch(unsigned char* codes, float* scales, const T* x
     if (rows == 1) {
         const dim3 grid((groups + Q_GROUPS - 1) / Q_GROUPS, (n + Q_ROWS - 1) / Q_ROWS);
         TI_REQUIRE(grid.y <= 65535, "quantize8: %d rows, each with scales of its own, are too many", n);
-        ti_launch(vec ? quantize8_rows_kernel<T, true> : quantize8_rows_kernel<T, false>, grid, dim3(256), 0, stream, codes, scales, x, ldx, n, k, groups);
+        auto* kernel = vec ? quantize8_rows_kernel<T, true> : quantize8_rows_kernel<T, false>;
+        static bool configured[2] = {};
+        if (!configured[vec]) {
+            // A product's blocks come up beside this kernel's and keep the split of the SMs that they find; without this those of 4,096 x 21,504 waited until the
+            // SMs were free (5 tokens 34 us instead of 21).
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+            if (e != cudaSuccess) return ti_fail("quantize8: %s", cudaGetErrorString(e));
+            configured[vec] = true;
+        }
+        ti_launch(kernel, grid, dim3(256), 0, stream, codes, scales, x, ldx, n, k, groups);
     } else {
         const int row_blocks = (n + E4M3_BLOCK - 1) / E4M3_BLOCK;
         TI_REQUIRE(row_blocks <= 65535, "quantize8: %d rows are too many", n);
