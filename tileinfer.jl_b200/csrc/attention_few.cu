@@ -17,27 +17,14 @@
 //
 // 5 tokens after 65,531 (32 / 8 heads of 128, 268 MB) 53.5 us, 5.0 TB/s; 64 x 4 tokens after 1,024 61 us, 4.4 TB/s with the joins of two or three parts an
 // item; 8 x 8 tokens after up to 32,768 (64 / 8 heads: slabs of 64 rows) 124 us, 1.44 of the bytes' time: the softmax's instructions beside the MMAs.
-#include "even_runs.cuh"
+#include "attention_parts.cuh"
 #include "mma_util.cuh"
 #include "tcgen05.cuh"
 #include "tensor_map.h"
 
-#define AF_PAGE 64
 #define AF_THREADS 128
 #define AF_MAX_SEQS 512                  // of one launch: their lengths, slots and units stand in shared memory
 
-struct FewShape {
-    int T, L, first, t0, tiles, slabs;                       // new tokens, length, first visible key, first tile, tiles, slabs of rows
-};
-__device__ __forceinline__ FewShape few_shape(int T, int L, int window, int group, int M) {
-    FewShape s;
-    s.T = T; s.L = L;
-    s.first = window > 0 ? max(0, L - T - window + 1) : 0;
-    s.t0 = s.first / AF_PAGE;
-    s.tiles = T > 0 && L > 0 ? (L + AF_PAGE - 1) / AF_PAGE - s.t0 : 0;
-    s.slabs = (T * group + M - 1) / M;
-    return s;
-}
 template <int D> struct FewSmem {
     // Two tiles in flight a block, and as many blocks an SM as the registers let in: 65,536 keys of one sequence, 5 tokens, 32 / 8 heads of 128, took
     // 67.4 us with three stages and 62.3 with two, which leave room for the joining kernel beside it; heads of 32 took 35 us in two blocks and 27.6 in
@@ -57,13 +44,6 @@ template <int D> __device__ __forceinline__ int few_at(int row, int c) {
 __device__ __forceinline__ unsigned finite_pair(unsigned pair) {
     return ((pair & 0x7F80u) == 0x7F80u ? 0u : pair & 0xFFFFu) | ((pair & 0x7F800000u) == 0x7F800000u ? 0u : pair & 0xFFFF0000u);
 }
-// Below 2^-126: 0.
-__device__ __forceinline__ float power2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 template <int D, int MT>
 __global__ void __launch_bounds__(AF_THREADS, FewSmem<D>::BLOCKS) attention_few_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                                      const __grid_constant__ CUtensorMap map_v, bf16* out, const bf16* q,
@@ -420,99 +400,6 @@ __global__ void __launch_bounds__(AF_THREADS, FewSmem<D>::BLOCKS) attention_few_
     if (!ok) tc::drain_after_timeout();                      // a wait ran out: let what is in flight land
 }
 
-// The parts of the rows that several blocks share, joined in ascending order: AF_JOIN_WARPS / WPR rows a block, WPR warps a row, four elements a lane,
-// every WPRth part a warp. Rows of items that one block did are done; rows without keys get zeros. What bounds it is one dependent load after another
-// with the kernel before gone: so where the parts lie is worked out before that kernel ends, and maxima, sums and outputs of eight parts are asked
-// for together.
-#define AF_JOIN_WARPS 4
-template <int WPR>
-__global__ void __launch_bounds__(32 * AF_JOIN_WARPS) attention_few_join_kernel(bf16* out, const int* cu, const int* kv_lens, const float* ws_o,
-                                                                                const float* ws_ml, int B, int nq, int nkv, int D, int M, int window,
-                                                                                int blocks) {
-    __shared__ unsigned s_sum[AF_JOIN_WARPS][2];
-    __shared__ float4 s_o[WPR > 1 ? WPR : 1][32];
-    __shared__ float2 s_ml[WPR];
-    const int b = blockIdx.z, kvh = blockIdx.y, group = nq / nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    unsigned before = 0, U = 0;
-    for (int c = threadIdx.x; c < B; c += 32 * AF_JOIN_WARPS) {
-        const FewShape s = few_shape(__ldcg(cu + c + 1) - __ldcg(cu + c), __ldcg(kv_lens + c), window, group, M);
-        U += s.tiles * s.slabs * nkv;
-        if (c < b) before += s.tiles * s.slabs * nkv;
-    }
-    U = __reduce_add_sync(0xffffffffu, U);
-    before = __reduce_add_sync(0xffffffffu, before);
-    if (lane == 0) { s_sum[warp][0] = before; s_sum[warp][1] = U; }
-    __syncthreads();
-    before = U = 0;
-#pragma unroll
-    for (int w = 0; w < AF_JOIN_WARPS; ++w) { before += s_sum[w][0]; U += s_sum[w][1]; }
-    const int first_token = __ldcg(cu + b), T = __ldcg(cu + b + 1) - first_token, row = blockIdx.x * (AF_JOIN_WARPS / WPR) + warp / WPR, mine = warp % WPR;
-    const FewShape s = few_shape(T, __ldcg(kv_lens + b), window, group, M);
-    const int i = row / group, slab = row / M, in = row - slab * M;
-    const Runs runs(U, max(min((unsigned)blocks, U), 1u));
-    const unsigned u0 = before + (unsigned)((kvh * s.slabs + slab) * s.tiles);
-    const bool empty = s.tiles == 0, real = row < T * group;
-    const unsigned c0 = real && !empty ? runs.owner(u0) : 0, c1 = real && !empty ? runs.owner(u0 + s.tiles - 1) : 0;
-    pdl_enter();
-    if (!real || (!empty && c0 == c1)) return;               // with WPR > 1 the block's one row: all leave
-    bf16* dst = out + ((size_t)(first_token + i) * nq + (size_t)kvh * group + (row - i * group)) * D;
-    const int parts = empty ? 0 : (int)(c1 - c0 + 1);
-    // A run that begins before the item holds its part in the second slot: the first part alone may.
-    const size_t first = empty ? 0 : (size_t)runs.slot(c0, u0) * M + in, others = (size_t)2 * c0 * M + in;
-    auto at = [&](int c) { return c == 0 ? first : others + (size_t)2 * c * M; };
-    const float2* ml = reinterpret_cast<const float2*>(ws_ml);
-    for (int d0 = 0; d0 < D; d0 += 128) {
-        const int d = d0 + 4 * lane;
-        const bool on = d < D;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f, mm = -INFINITY;
-        for (int p = mine; p < parts; p += 8 * WPR) {
-            float4 v[8];
-            const int pl = p + lane * WPR;
-            const float2 x = lane < 8 && pl < parts ? __ldcg(ml + at(pl)) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                v[k] = on && p + k * WPR < parts ? __ldcg(reinterpret_cast<const float4*>(ws_o + at(p + k * WPR) * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float top = fmaxf(mm, warp_max(x.x)), base = top == -INFINITY ? 0.f : top;
-            const float old = exp2f(mm - base), f = exp2f(x.x - base);
-            mm = top;
-            sum = sum * old + warp_sum(x.y * f);
-            acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float w = __shfl_sync(0xffffffffu, f, k);
-                acc.x = fmaf(v[k].x, w, acc.x); acc.y = fmaf(v[k].y, w, acc.y); acc.z = fmaf(v[k].z, w, acc.z); acc.w = fmaf(v[k].w, w, acc.w);
-            }
-        }
-        if (WPR > 1) {
-            if (d0 > 0) __syncthreads();
-            s_o[mine][lane] = acc;
-            if (lane == 0) s_ml[mine] = make_float2(mm, sum);
-            __syncthreads();
-            if (mine > 0) continue;
-            mm = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < WPR; ++w) mm = fmaxf(mm, s_ml[w].x);
-            const float base = mm == -INFINITY ? 0.f : mm;
-            acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < WPR; ++w) {
-                const float f = exp2f(s_ml[w].x - base);
-                const float4 v = s_o[w][lane];
-                sum = fmaf(s_ml[w].y, f, sum);
-                acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
-            }
-        }
-        if (sum == 0.f) { acc = make_float4(0.f, 0.f, 0.f, 0.f); sum = 1.f; }            // nothing was visible; a NaN sum stays one
-        const float inv = 1.f / sum;
-        if (on) {
-            reinterpret_cast<__nv_bfloat162*>(dst + d)[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-            reinterpret_cast<__nv_bfloat162*>(dst + d)[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-        }
-    }
-}
-
 static int few_rows(int max_rows, int D) { return D > 128 || max_rows <= 16 ? 16 : max_rows <= 32 ? 32 : 64; }
 static int few_blocks(int D) { return (D <= 64 ? 3 : D <= 128 ? 2 : 1) * ti_sm_count(); }
 
@@ -546,11 +433,7 @@ static int launch_few(bf16* out, const bf16* q, const bf16* k, const bf16* v, co
     ti_launch(attention_few_kernel<D, MT>, dim3(G), dim3(AF_THREADS), FewSmem<D>::BYTES, stream, map_k, map_v, out, q, k, v, table, table_stride, seq_slots, cu,
               kv_lens, ws_o, ws_ml, status, scale * 1.4426950408889634f, B, nq, nkv, window);
     if (int rc = ti_check_launch("attention_few")) return rc;
-    const int rows = max_new * (nq / nkv);
-    // More than eight parts an item: four warps a row (59.9 us in place of 62.3 at 37 parts; at two parts 90 in place of 70).
-    const bool deep = 8LL * B * nkv * ((rows + M - 1) / M) < G;
-    ti_launch(deep ? attention_few_join_kernel<4> : attention_few_join_kernel<1>, dim3(deep ? rows : (rows + AF_JOIN_WARPS - 1) / AF_JOIN_WARPS, nkv, B),
-              dim3(32 * AF_JOIN_WARPS), 0, stream, out, cu, kv_lens, ws_o, ws_ml, B, nq, nkv, D, M, window, G);
+    join_parts(out, cu, kv_lens, ws_o, ws_ml, B, nq, nkv, D, M, max_new, window, G, stream);
     return ti_check_launch("attention_few_join");
 }
 

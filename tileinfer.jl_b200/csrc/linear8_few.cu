@@ -27,10 +27,6 @@ struct Args {
 __device__ __forceinline__ void copy16(unsigned dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0));
 }
-__device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ float4 cluster_read(const float* at, unsigned rank) {
     unsigned a;
     float4 v;
@@ -172,7 +168,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
                     for (int q = 0; q < 4; ++q) {
                         const unsigned f[4] = {e4m3_half2((unsigned short)lo_w[q]), e4m3_half2((unsigned short)hi_w[q]), e4m3_half2((unsigned short)(lo_w[q] >> 16)),
                                                e4m3_half2((unsigned short)(hi_w[q] >> 16))};
-                        mma_f16(part[h], f, e4m3_half2((unsigned short)xw[q]), e4m3_half2((unsigned short)(xw[q] >> 16)));
+                        mma16816_f16(part[h], f, e4m3_half2((unsigned short)xw[q]), e4m3_half2((unsigned short)(xw[q] >> 16)));
                     }
                 }
                 __syncwarp();

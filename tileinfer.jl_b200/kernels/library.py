@@ -99,7 +99,7 @@ _SIGNATURES = {
 }
 
 
-_KERNELS_PER_CALL = {"ti_attention_few": 2, "ti_memory_chunks": 3, "ti_ssm_chunks": 3, "ti_ssm_chunks_tc": 3}
+_KERNELS_PER_CALL = {"ti_attention_few": 2, "ti_attention8": 2, "ti_memory_chunks": 3, "ti_ssm_chunks": 3, "ti_ssm_chunks_tc": 3}
 
 
 def lib():

@@ -1325,6 +1325,8 @@ def linear8(y, x, codes, scales, x_scales=None, epilogue=EPI_NONE, act=(0.0, 0.0
                           epilogue, *act, ws, size, status_word().data_ptr(), stream)
     if rc:
         check(rc, "linear8")
+    if need and n:
+        _library.add_launches(1)                             # the tokens' codes are made by a launch of their own
 
 
 def _paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, page_size) -> bool:
@@ -1413,3 +1415,5 @@ def attention8(out, q, k_cache, v_cache, k_scales, v_scales, block_table, seq_sl
                              nq, nkv, head_dim, page_size, max_new, max_len, k_cache.shape[0], window or 0, stream)
     if rc:
         check(rc, "attention8")
+    if seqs > FEW_MAX_SEQS:
+        _library.add_launches(2 * ((seqs - 1) // FEW_MAX_SEQS))
