@@ -1102,6 +1102,7 @@ def _need_workspace(ws: torch.Tensor, need: int, what: str):
 
 FEW_HEAD_DIMS, FEW_PAGE = (16, 32, 48, 64, 80, 96, 112, 128, 256), 64        # what attention_few takes
 FEW_MAX_SEQS = 512                                                            # sequences of its one launch (csrc/attention_few.cu: AF_MAX_SEQS)
+ATTENTION8_MAX_SEQS = 256                                                     # of attention8 (csrc/attention8.cu: A8_MAX_SEQS)
 
 
 _attention_few_need = {}
@@ -1415,5 +1416,5 @@ def attention8(out, q, k_cache, v_cache, k_scales, v_scales, block_table, seq_sl
                              nq, nkv, head_dim, page_size, max_new, max_len, k_cache.shape[0], window or 0, stream)
     if rc:
         check(rc, "attention8")
-    if seqs > FEW_MAX_SEQS:
-        _library.add_launches(2 * ((seqs - 1) // FEW_MAX_SEQS))
+    if seqs > ATTENTION8_MAX_SEQS:
+        _library.add_launches(2 * ((seqs - 1) // ATTENTION8_MAX_SEQS))
