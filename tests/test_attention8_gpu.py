@@ -77,9 +77,11 @@ def call(ops, c, nq, nkv, dim, max_new, window=0, scale=None, **kw):
     return out[:-1].cpu()
 
 
-def check(ops, runs, nq, nkv, dim, window=0, seed=0, long=False, max_len=None, any_scale=False, **kw):
+def check(ops, runs, nq, nkv, dim, window=0, seed=0, max_len=None, any_scale=False, **kw):
     c = make(runs, nq, nkv, dim, seed, any_scale=any_scale)
-    got = call(ops, c, nq, nkv, dim, max([t for t, _ in runs] + [1]), window, max_len=max_len, **kw)
+    new = max([t for t, _ in runs] + [1])
+    got = call(ops, c, nq, nkv, dim, new, window, max_len=max_len, **kw)
+    long = bool(ops.lib().ti_attention8_widens(len(runs), new, nq, nkv, dim, max_len or PAGE * c["table"].shape[1]))
     want, bound = reference(c, dim ** -0.5, window, 8 if long else 11)
     assert bool(torch.isfinite(got).all())
     off = (got.to(F64) - want).abs()
@@ -133,13 +135,13 @@ def test_one_long_sequence(ops, nq, nkv, dim):
 @pytest.mark.parametrize("window", [0, 130])
 def test_prompts(ops, nq, nkv, dim, window):
     for runs in ([(500, 500)], [(700, 1000), (33, 40), (0, 90), (1, 300), (128, 128)], [(64, 64), (200, 711)]):
-        check(ops, runs, nq, nkv, dim, window, seed=dim, long=True, any_scale=False)
-        check(ops, runs, nq, nkv, dim, window, seed=dim, long=True, max_len=1000)
+        check(ops, runs, nq, nkv, dim, window, seed=dim, any_scale=False)
+        check(ops, runs, nq, nkv, dim, window, seed=dim, max_len=1000)
 
 
 def test_a_long_prompt_in_two_calls(ops):
-    check(ops, [(2048, 4096)], 8, 2, 128, long=True)
-    check(ops, [(1500, 1500), (3, 4000)], 8, 2, 64, long=True)
+    check(ops, [(2048, 4096)], 8, 2, 128)
+    check(ops, [(1500, 1500), (3, 4000)], 8, 2, 64)
 
 
 @pytest.mark.parametrize("spread", [0, 10, 60])

@@ -17,17 +17,18 @@ _BACKENDS = {"fast": "fast", "plain": "plain"}
 
 
 def load_model(model_dir: str, dtype: str = "bfloat16", backend: str = "fast", max_context: int = 4096,
-               max_tokens: Optional[int] = None, max_seqs: int = 8, **kw) -> Engine:
+               max_tokens: Optional[int] = None, max_seqs: int = 8, cache: str = "model", weights: str = "model", **kw) -> Engine:
     """Load the model folder ``model_dir`` (config.json + safetensors) onto the GPU.
 
     ``dtype``: "bfloat16" or "float32" (the true 32-bit path). ``backend``: "fast" (tensor-core and
     bandwidth kernels) or "plain" (the simple reference kernels), like the reference's tile/ref.
     ``max_context`` is the longest sequence in tokens (it sizes the rotary tables); ``max_tokens`` the
-    most tokens all live sequences hold together (default: ``max_seqs × max_context``)."""
+    most tokens all live sequences hold together (default: ``max_seqs × max_context``). ``cache``, ``weights``: "e4m3" holds keys and
+    values, or the matrices, in 8 bits (bfloat16 models of plain attention and feed-forward layers; see ``Engine``)."""
     if backend not in _BACKENDS:
         raise ValueError("backend expects fast or plain")
     return Engine.load(model_dir, dtype=dtype, kernels=_BACKENDS[backend], max_context=max_context,
-                       max_tokens=max_tokens or max_seqs * max_context, max_seqs=max_seqs, **kw)
+                       max_tokens=max_tokens or max_seqs * max_context, max_seqs=max_seqs, cache=cache, weights=weights, **kw)
 
 
 def generation_defaults(model_dir: str, engine: Engine):

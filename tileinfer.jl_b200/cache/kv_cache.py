@@ -204,6 +204,26 @@ class PagedGroup:
         return self.pools_per_layer * len(self.layers) * r.kv_heads * r.head_dim * self.k.element_size()
 
 
+@register_cache_kind("paged_kv8")
+class PagedGroup8(PagedGroup):
+    """Pages of keys and values as e4m3 codes with a scale for each page's head (``ops.cache_write8``): a layer's view carries the two tables of scales
+    [pages, kv_heads] as ``extra``. Books, windows and block tables are the paged group's. A page that is handed out again keeps its old scales until its first
+    position is written, which sets them anew."""
+
+    def _pools(self, shape, dtype, device):
+        if shape[3] != 64:
+            raise ValueError(f"a cache in 8 bits has pages of 64 positions, not {shape[3]}")
+        self.scales = torch.ones((2,) + shape[:3], dtype=torch.float32, device=device)
+        return tuple(torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
+
+    def views(self):
+        return [dataclasses.replace(view, extra=(self.scales[0, j], self.scales[1, j])) for j, view in enumerate(super().views())]
+
+    def bytes_per_position(self) -> int:
+        """Codes, rounded up by a page's scales."""
+        return super().bytes_per_position() + -(-2 * len(self.layers) * self.request.kv_heads * 4 // self.page_size)
+
+
 @register_cache_kind("paged_latent")
 class PagedLatentGroup(PagedGroup):
     """Pages that hold ONE vector per position and layer (``head_dim`` elements, ``kv_heads`` = 1): a latent from which

@@ -67,11 +67,13 @@ OPTIONS: Dict[str, Option] = {o.name: o for o in (
     Option("seed", int, None, "random seed (default: drawn at random)"),
     Option("backend", ("fast", "plain"), "fast", "tensor-core kernels or the plain reference kernels"),
     Option("dtype", ("bfloat16", "float32"), "bfloat16", "element type of weights, activations and cache"),
+    Option("cache", ("model", "e4m3"), "model", "keys and values in the element type or in 8 bits"),
+    Option("weights", ("model", "e4m3"), "model", "matrices in the element type or in 8 bits"),
     Option("max-seqs", int, 8, "sequences per batch at most"),
     Option("draft", int, 0, "tokens to draft a step with the model's matrices in 4 bits, for the model to test (0: none)"),
     Option("stop-ids", token_ids, None, "stop tokens instead of the configuration's EOS ids (\"\" for none)"),
 )}
-GENERATION = ("max-tokens", "max-context", "temperature", "top-k", "top-p", "seed", "backend", "dtype", "max-seqs", "draft", "stop-ids")
+GENERATION = ("max-tokens", "max-context", "temperature", "top-k", "top-p", "seed", "backend", "dtype", "cache", "weights", "max-seqs", "draft", "stop-ids")
 
 
 @dataclass(frozen=True)
@@ -136,7 +138,7 @@ def load_for_generation(model_dir: str, values):
     from .api import generation_defaults, load_model
     from .sampling import SamplingParams
     engine = load_model(model_dir, dtype=values["dtype"], backend=values["backend"], max_seqs=values["max-seqs"],
-                        max_context=values["max-context"])
+                        max_context=values["max-context"], cache=values["cache"], weights=values["weights"])
     defaults, stop = generation_defaults(model_dir, engine)
     pick = lambda name, fallback: fallback if values[name] is None else values[name]
     sampling = SamplingParams(temperature=pick("temperature", defaults.temperature), top_k=pick("top-k", defaults.top_k),

@@ -27,6 +27,8 @@
 #include "linear8.cuh"
 #include "mma_util.cuh"
 
+#include <cmath>
+
 namespace {
 
 constexpr int A8_THREADS = 160, A8_MAX_SEQS = 256;           // four warps that compute, one that asks; sequences of one launch
@@ -546,9 +548,31 @@ template <int DP, bool EXACT> int launch_rows(const Call& c, int eights) {
 
 }  // namespace
 
-// Bytes of the work space: two slots of rows a block.
+int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
+                 int table_stride, const int* seq_slots, const int* cu, const int* kv_lens, int B, int nkv, int D, int pages, int per_seq, int window, cudaStream_t stream);
+extern "C" int ti_attention_prefill_tc(void* out, const void* q, const void* k_cache, const void* v_cache, int n_pages, const int* block_table, int table_stride,
+                                       const int* seq_slots, const int* cu_seqlens, const int* kv_lens, int n_seqs, int n_tokens, int total_blocks, float scale, int nq,
+                                       int nkv, int D, int page_size, int window, int* status, cudaStream_t stream);
+// Whether a step goes through pages widened to bfloat16 and the prompts' kernel on the fifth-generation tensor cores: the shorter by estimates in microseconds, for
+// sequences of max_len positions. Slabs: 4.8 ns for a slab's tile of heads of 128, 57 ns for its other work. Widened: a walk along the longest sequence
+// (19 ns a position), rounds of the SMs, the widened bytes. Microseconds in turn, 32 / 8 heads of 128: one sequence, 64 new of 8,192 62 / 170, 128 of 1,024 30 / 32,
+// 256 of 4,096 122 / 94, 2,048 of 4,096 1,212 / 139; four sequences, 32 of 512 25 / 25, 128 of 128 45 / 17.
+extern "C" int ti_attention8_widens(int B, int max_new, int nq, int nkv, int D, int max_len) {
+    if (B <= 0 || nkv <= 0 || nq % nkv != 0 || (D != 64 && D != 128) || nq / nkv > 128 || B > 65535 || max_new * (long long)(nq / nkv) <= 24) return 0;
+    const double group = nq / nkv, heads = (double)B * nkv, items = heads * ceil(max_new * group / 24), size = D / 128.0;
+    const double slabs = 5 + (0.0048 * items * (max_len / 64.0) + 0.057 * items) * size;
+    const double waves = heads * ceil(max_new * group / 256) / ti_sm_count(), walk = waves * (max_len - 0.5 * max_new);
+    return 11 + 0.0193 * (walk > max_len ? walk : max_len) + 2 * waves + heads * max_len * D * 6 / 5e6 < slabs;
+}
+static long long up16(long long bytes) { return (bytes + 15) / 16 * 16; }
+
+// Bytes of the work space: two slots of rows a block, or the widened pages with their table.
 extern "C" long long ti_attention8_workspace(int B, int max_new, int nq, int nkv, int D, int max_len) {
     if (B <= 0 || max_new <= 0 || nq <= 0 || nkv <= 0 || D <= 0) return 0;
+    if (ti_attention8_widens(B, max_new, nq, nkv, D, max_len)) {
+        const long long pages = (long long)B * ((max_len + AF_PAGE - 1) / AF_PAGE);
+        return pages * nkv * AF_PAGE * D * 4 + up16(4 * pages) + up16(4LL * B);
+    }
     const int eights = slab_eights(max_new * (long long)(nq / nkv), D);
     return 2LL * sm_blocks(eights, D) * ti_sm_count() * 8 * eights * (D + 2) * 4;
 }
@@ -579,6 +603,18 @@ extern "C" int ti_attention8(void* out, const void* q, const void* k, const void
     TI_REQUIRE(((uintptr_t)q | (uintptr_t)out) % 4 == 0, "attention8: queries and outputs must be 4-byte aligned (two elements are moved at a time)");
     const long long need = ti_attention8_workspace(B, max_new, nq, nkv, D, max_len);
     TI_REQUIRE(ws != nullptr && aligned16(ws) && ws_bytes >= need, "attention8: work space of %lld bytes, %lld needed", ws_bytes, need);
+    if (ti_attention8_widens(B, max_new, nq, nkv, D, max_len)) {
+        const int per_seq = (max_len + AF_PAGE - 1) / AF_PAGE;
+        const long long all = (long long)B * per_seq, pool = all * nkv * AF_PAGE * D;
+        TI_REQUIRE(all * nkv * AF_PAGE <= 0x7fffffffLL, "attention8: %d sequences of up to %d positions are too many for one step", B, max_len);
+        TI_REQUIRE(((uintptr_t)q | (uintptr_t)out) % 16 == 0, "attention8: queries and outputs of long runs must be 16-byte aligned");
+        bf16 *k16 = (bf16*)ws, *v16 = k16 + pool;
+        int *table16 = (int*)(v16 + pool), *slots16 = (int*)((unsigned char*)table16 + up16(4 * all));
+        if (int rc = cache_widen8(k16, v16, table16, slots16, k, v, k_scales, v_scales, table, table_stride, seq_slots, cu, kv_lens, B, nkv, D, pages, per_seq, window, stream)) return rc;
+        // As many blocks as the runs can need: those beyond leave at once.
+        const int tokens = 2 * (128 / (nq / nkv)), blocks = n / tokens + (B < n ? B : n);
+        return ti_attention_prefill_tc(out, q, k16, v16, (int)all, table16, per_seq, slots16, cu, kv_lens, B, n, blocks, scale, nq, nkv, D, page_size, window, status, stream);
+    }
     Call c;
     c.max_new = max_new;
     c.stream = stream;

@@ -7,6 +7,9 @@
 // 2^-6 of the scale. One block of threads writes a page's head, keys or values, which keeps its new rows in registers between their maximum and their codes.
 //
 // Bound by launch and three dependent reads (lengths, the page, its rows and old scale); a prompt by its bytes.
+//
+// Widening, for kernels that read bfloat16: the pages that a step's tokens see become pages of bfloat16 in a pool of their own, page j of sequence b at
+// b x (pages a sequence) + j, with its block table. A code times a power of two is exact in bfloat16. Positions that nobody sees become zeros.
 #include "e4m3.cuh"
 
 namespace {
@@ -69,6 +72,45 @@ __global__ void __launch_bounds__(THREADS) cache_write8_kernel(unsigned char* k_
     if (threadIdx.x == 0) *scale = after;
 }
 
+// blockIdx: page, head, sequence.
+__global__ void __launch_bounds__(THREADS) cache_widen8_kernel(bf16* k_out, bf16* v_out, int* table_out, int* slots_out, const unsigned char* k, const unsigned char* v,
+                                                               const float* k_scales, const float* v_scales, const int* table, int table_stride, const int* seq_slots,
+                                                               const int* cu, const int* kv_lens, int nkv, int D, int pages, int per_seq, int window) {
+    const int j = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    pdl_enter();
+    const int T_new = __ldcg(cu + b + 1) - __ldcg(cu + b), L = __ldcg(kv_lens + b), slot = __ldcg(seq_slots + b);
+    if (kvh == 0 && threadIdx.x == 0) {
+        table_out[(size_t)b * per_seq + j] = b * per_seq + j;
+        if (j == 0) slots_out[b] = b;
+    }
+    const int first = window > 0 ? max(0, L - T_new - window + 1) : 0;
+    if (T_new <= 0 || j * PAGE >= L || j < first / PAGE / 2 * 2) return;              // the readers walk the pages in pairs
+    const int page = j < table_stride && (j + 1) * PAGE > first ? __ldcg(table + (size_t)slot * table_stride + j) : -1;
+    const bool there = page >= 0 && page < pages;
+    const size_t from = ((size_t)page * nkv + kvh) * PAGE * D, to = (((size_t)b * per_seq + j) * nkv + kvh) * PAGE * D;
+    const float sk = there ? __ldcg(k_scales + (size_t)page * nkv + kvh) : 0.f, sv = there ? __ldcg(v_scales + (size_t)page * nkv + kvh) : 0.f;
+    const int pieces = PAGE * D / 16;
+    for (int e = threadIdx.x; e < 2 * pieces; e += THREADS) {
+        const bool is_v = e >= pieces;
+        const int piece = is_v ? e - pieces : e, key = j * PAGE + piece * 16 / D;
+        const float s = is_v ? sv : sk;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (there && key >= first && key < L) w = __ldcg(reinterpret_cast<const uint4*>((is_v ? v : k) + from) + piece);
+        const unsigned c[4] = {w.x, w.y, w.z, w.w};
+        unsigned o[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 lo = e4m3_float2((unsigned short)c[i]), hi = e4m3_float2((unsigned short)(c[i] >> 16));
+            const __nv_bfloat162 x = __floats2bfloat162_rn(lo.x * s, lo.y * s), y = __floats2bfloat162_rn(hi.x * s, hi.y * s);
+            o[2 * i] = *reinterpret_cast<const unsigned*>(&x);
+            o[2 * i + 1] = *reinterpret_cast<const unsigned*>(&y);
+        }
+        uint4* dst = reinterpret_cast<uint4*>((is_v ? v_out : k_out) + to) + 2 * piece;
+        dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+}
+
 }  // namespace
 
 // k and v: [n, nkv, D] rows of `dtype` with the given pitches of tokens and heads (in elements); pools [pages, nkv, 64, D] and scales [pages, nkv]; the page of
@@ -93,4 +135,12 @@ extern "C" int ti_cache_write8(void* k_codes, void* v_codes, float* k_scales, fl
                                        stream, (unsigned char*)k_codes, (unsigned char*)v_codes, k_scales, v_scales, kr, vr, table, table_stride, slots,
                                        seq_slots, cu, kv_lens, n, nkv, D, pages, (int)touched));
     return ti_check_launch("cache_write8");
+}
+
+// For attention8.cu: pools k_out, v_out [B * per_seq, nkv, 64, D] bfloat16, table_out [B, per_seq], slots_out [B].
+int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
+                 int table_stride, const int* seq_slots, const int* cu, const int* kv_lens, int B, int nkv, int D, int pages, int per_seq, int window, cudaStream_t stream) {
+    ti_launch(cache_widen8_kernel, dim3(per_seq, nkv, B), dim3(THREADS), 0, stream, (bf16*)k_out, (bf16*)v_out, table_out, slots_out, (const unsigned char*)k,
+              (const unsigned char*)v, k_scales, v_scales, table, table_stride, seq_slots, cu, kv_lens, nkv, D, pages, per_seq, window);
+    return ti_check_launch("cache_widen8");
 }

@@ -30,6 +30,11 @@ def quantized(model, group: int = 128, zeros: bool = False):
         if layer.mixer.kind not in MIXERS or (layer.feed_forward is not None and layer.feed_forward.kind not in FEED_FORWARDS):
             raise ValueError(f"a copy in 4 bits is made of layers of {', '.join(MIXERS)} and {', '.join(FEED_FORWARDS)}, not of {layer.mixer.kind} and "
                              f"{layer.feed_forward.kind if layer.feed_forward is not None else 'none'}")
+    return with_matrices(model, lambda linear: Linear4(linear, group, zeros))
+
+
+def with_matrices(model, make: Callable):
+    """A copy of ``model`` that shares everything with it but its products, each of which is ``make(product)``."""
     made: Dict[int, object] = {}
 
     def view(obj):
@@ -37,7 +42,7 @@ def quantized(model, group: int = 128, zeros: bool = False):
             return type(obj)(view(v) for v in obj)
         if isinstance(obj, Linear):
             if id(obj) not in made:
-                made[id(obj)] = Linear4(obj, group, zeros)
+                made[id(obj)] = make(obj)
             return made[id(obj)]
         if isinstance(obj, Part) and not isinstance(obj, PositionEncoding):
             if id(obj) not in made:

@@ -23,9 +23,10 @@ import torch
 
 from ..cache import Cache, DEFAULT_PAGE_SIZE
 from ..config import load_config, resolve_architecture
-from ..parts import Runtime
+from ..parts import Linear8, Runtime
 from ..weights import load_tensors, random_tensors
 from .model import DecoderModel, ignorable_tensors, tensor_declarations
+from ..kernels import ops
 from ..kernels.host import nvtx_range
 from .step import StepPlanner
 
@@ -44,16 +45,27 @@ class Engine:
     def __init__(self, config, tensors: Dict[str, torch.Tensor], dtype="bfloat16", device="cuda",
                  max_tokens: int = 4096, max_seqs: int = 8, max_context: Optional[int] = None,
                  page_size: int = DEFAULT_PAGE_SIZE, max_step_tokens: int = 8192, kernels: str = "fast",
-                 graphs: bool = True, model_factory=None):
+                 graphs: bool = True, model_factory=None, cache: str = "model", weights: str = "model"):
+        """``cache``: "model" (keys and values in the element type) or "e4m3" (8 bits, a scale for each page of 64 positions and KV head). ``weights``: "model"
+        or "e4m3" (the matrices of products and head in 8 bits, a scale for each 128 x 128, their inputs quantised on the way). Both take models of plain
+        attention and feed-forward layers in bfloat16."""
+        for name, value in (("cache", cache), ("weights", weights)):
+            if value not in ("model", "e4m3"):
+                raise ValueError(f"{name} expects model or e4m3, not {value}")
         self.device = require_cuda(device)
         self.config = config
         self.dtype = _DTYPES[dtype]
-        self.rt = Runtime(self.dtype, self.device, kernels)
         self.spec = config.model_spec()
+        if "e4m3" in (cache, weights):
+            self._check8(kernels, page_size)
+        self.rt = Runtime(self.dtype, self.device, kernels, cache8=cache == "e4m3")
         max_context = int(min(max_context or self.spec.max_positions, self.spec.max_positions))
         self.max_context = max_context
         factory = model_factory or DecoderModel
         self.model = factory(self.spec, tensors, self.rt, max_context)
+        if weights == "e4m3":
+            from .drafting import with_matrices
+            self.model = with_matrices(self.model, Linear8)
         self.cache = Cache(self.model.cache_requests(), self.dtype, self.device, max_tokens=max_tokens,
                            max_seqs=max_seqs, page_size=page_size, max_seq_len=max_context,
                            share=self.model.cache_shares(), max_step_tokens=int(max_step_tokens))
@@ -61,6 +73,16 @@ class Engine:
         self.use_graphs = graphs
         self.vocab_size = self.spec.vocab_size
         self._start_planning()
+
+    def _check8(self, kernels: str, page_size: int) -> None:
+        from .drafting import FEED_FORWARDS, MIXERS
+        if self.dtype != torch.bfloat16 or kernels != "fast" or page_size != DEFAULT_PAGE_SIZE:
+            raise ValueError(f"8 bits go with bfloat16, the fast kernels and pages of {DEFAULT_PAGE_SIZE}")
+        for layer in self.spec.layers:
+            mixer, ff = layer.mixer, layer.feed_forward
+            if mixer.kind not in MIXERS or (ff is not None and ff.kind not in FEED_FORWARDS) or mixer.head_dim % 16 or mixer.head_dim > ops.HEAD8:
+                raise ValueError(f"8 bits go with layers of {', '.join(MIXERS)} (heads of a multiple of 16 up to {ops.HEAD8}) and {', '.join(FEED_FORWARDS)}, not of "
+                                 f"{mixer.kind} (heads of {getattr(mixer, 'head_dim', None)}) and {ff.kind if ff is not None else 'none'}")
 
     def _start_planning(self) -> None:
         """A planner for this engine's steps, and no graphs yet."""

@@ -56,13 +56,13 @@ class Attention(Mixer):
     def cache_request(self):
         if self.spec.kv_source is not None:
             return None
-        return CacheRequest("paged_kv", kv_heads=self.spec.num_kv_heads, head_dim=self.spec.head_dim,
+        return CacheRequest("paged_kv8" if self.rt.cache8 else "paged_kv", kv_heads=self.spec.num_kv_heads, head_dim=self.spec.head_dim,
                             window=self.spec.window)
 
     def decode_plan(self, group):
         """The fast decode kernel reads the keys of a step's sequences in B x splits work slots; how they are
         shared out among sequences of unequal lengths is a table in the step's metadata."""
-        if not (self.rt.fast and self.rt.dtype == torch.bfloat16) or self.spec.kv_source is not None:
+        if not (self.rt.fast and self.rt.dtype == torch.bfloat16) or self.spec.kv_source is not None or self.rt.cache8:
             return None
         from ..kernels import fast
         return fast.SplitKvPlan(self.spec.num_kv_heads, group.page_size, group.num_pages * group.page_size)
@@ -77,12 +77,15 @@ class Attention(Mixer):
         qkv = self.qkv.forward(h, qkv, allow_partials=n <= 256)
         q = rt.buffer("attention.q", (n, nq, D))
         meta = step.group(cache.group_index)
-        ops.attention_inputs(qkv, q, cache.k, cache.v, self.q_norm, self.k_norm, s.qk_norm_eps,
-                             self.rotation, step.positions, meta.slot_mapping, nq, nkv, D,
-                             cache.page_size, write_kv=own_kv)
         attn = rt.buffer("attention.out", (n, nq * D))
-        done = False
-        if rt.fast:
+        done = cache.kind == "paged_kv8"
+        if done:
+            self._attend8(qkv, q, attn, step, meta, cache, own_kv)
+        else:
+            ops.attention_inputs(qkv, q, cache.k, cache.v, self.q_norm, self.k_norm, s.qk_norm_eps,
+                                 self.rotation, step.positions, meta.slot_mapping, nq, nkv, D,
+                                 cache.page_size, write_kv=own_kv)
+        if rt.fast and not done:
             from ..kernels import fast
             done = fast.attention(attn, q, cache, meta, step, s)
         if not done:
@@ -90,3 +93,19 @@ class Attention(Mixer):
                                 s.scale, nq, nkv, D, cache.page_size, window=s.window or 0)
         proj = rt.buffer("mixer.delta", (n, s.hidden_size))
         return self.o.forward(attn, proj, allow_partials=True)
+
+    def _attend8(self, qkv, q, attn, step, meta, cache, own_kv):
+        """Keys and values in 8 bits: the new rows in bfloat16 first (each a page of one position), then their codes, then attention over the pages."""
+        s, rt = self.spec, self.rt
+        n, nq, nkv, D = q.shape[0], s.num_heads, s.num_kv_heads, s.head_dim
+        k_scales, v_scales = cache.extra
+        k, v = (rt.buffer(name, (n, nkv, D)) for name in ("attention.k8", "attention.v8")) if own_kv else (None, None)
+        ops.attention_inputs(qkv, q, k, v, self.q_norm, self.k_norm, s.qk_norm_eps, self.rotation, step.positions, rt.counting(n), nq, nkv, D, 1, write_kv=own_kv)
+        where = meta.block_table, step.seq_slots, step.cu_seqlens, step.kv_lens
+        if own_kv:
+            ops.cache_write8(cache.k, cache.v, k_scales, v_scales, k, v, *where, step.max_q_len)
+        # A captured step is replayed at any length.
+        longest = meta.block_table.shape[1] * cache.page_size if step.is_decode else step.max_kv_len
+        need = ops.attention8_workspace(step.n_seqs, step.max_q_len, nq, nkv, D, longest)
+        ops.attention8(attn, q, cache.k, cache.v, k_scales, v_scales, *where, s.scale, nq, nkv, D, cache.page_size, step.max_q_len, window=s.window or 0, max_len=longest,
+                       workspace=rt.buffer("attention.parts8", (need,), torch.uint8))

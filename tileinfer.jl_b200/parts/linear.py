@@ -50,6 +50,8 @@ class Linear4(Linear):
         fit = next((g for g in sorted(ops.LINEAR4_GROUPS, reverse=True) if g <= group and other.in_features % g == 0), None)
         if fit is None:
             raise ValueError(f"{other.name}: {other.in_features} inputs do not divide into groups of {', '.join(map(str, ops.LINEAR4_GROUPS))} up to {group}")
+        if getattr(other, "weight", None) is None:
+            raise ValueError(f"{other.name}: codes are made from the matrix itself, which is held in 8 bits here")
         self.rt, self.name, self.partials_name = other.rt, other.name, other.partials_name
         self.out_features, self.in_features, w = other.out_features, other.in_features, other.weight
         groups = self.in_features // fit
@@ -69,3 +71,29 @@ class Linear4(Linear):
     def _workspace(self, n: int):
         need = ops.linear4_workspace(n, self.out_features, self.in_features) if self.rt.dtype == torch.bfloat16 else 0
         return self.rt.buffer("linear4.parts", (need,), torch.uint8) if need else None
+
+
+class Linear8(Linear):
+    """The same product with a matrix of e4m3 codes, made from another's, with a scale for every 128 x 128 of them; the inputs are quantised on the way, by row in
+    groups of 128. bfloat16 models only. Nothing of the other is kept; there is no ``weight``."""
+
+    def __init__(self, other: Linear):
+        if getattr(other, "weight", None) is None or other.weight.dtype != torch.bfloat16 or other.in_features % 16:
+            raise ValueError(f"{other.name}: codes of 8 bits are made from bfloat16 matrices of a multiple of 16 inputs, not {other.in_features}")
+        self.rt, self.name, self.partials_name = other.rt, other.name, other.partials_name
+        self.out_features, self.in_features, w = other.out_features, other.in_features, other.weight
+        self.codes = torch.empty(self.out_features, self.in_features, dtype=torch.uint8, device=w.device).view(torch.float8_e4m3fn)
+        self.scales = torch.empty(-(-self.in_features // ops.BLOCK8), -(-self.out_features // ops.BLOCK8), dtype=torch.float32, device=w.device)
+        ops.quantize8(self.codes, self.scales, w, ops.BLOCK8)
+
+    def forward(self, x: torch.Tensor, out: torch.Tensor, epilogue: int = ops.EPI_NONE, act=(0.0, 0.0, 0.0, 0.0), allow_partials: bool = False):
+        ops.linear8(out, x, self.codes, self.scales, None, epilogue, act, self._workspace(x.shape[0]))
+        return out
+
+    def forward_f32(self, x: torch.Tensor, out: torch.Tensor):
+        ops.linear8(out, x, self.codes, self.scales, None, ops.EPI_F32_OUT, workspace=self._workspace(x.shape[0]))
+        return out
+
+    def _workspace(self, n: int):
+        need = ops.linear8_workspace(n, self.out_features, self.in_features)
+        return self.rt.buffer("linear8.inputs", (need,), torch.uint8) if need else None

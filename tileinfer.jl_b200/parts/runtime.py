@@ -12,7 +12,7 @@ import torch
 
 
 class Runtime:
-    def __init__(self, dtype: torch.dtype, device: str = "cuda", kernels: str = "fast"):
+    def __init__(self, dtype: torch.dtype, device: str = "cuda", kernels: str = "fast", cache8: bool = False):
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"the model runs in float32 or bfloat16, not {dtype}")
         if kernels not in ("fast", "plain"):
@@ -21,6 +21,7 @@ class Runtime:
         self.device = torch.device(device)
         # "plain": only the simple CUDA-core kernels, also in bfloat16. The 32-bit path always uses them.
         self.kernels = "plain" if dtype == torch.float32 else kernels
+        self.cache8 = cache8                             # keys and values in 8 bits (the parts that ask for them see to it)
         self._buffers: Dict[str, torch.Tensor] = {}
         self._views: Dict[tuple, torch.Tensor] = {}     # (name, shape, dtype) -> the view handed out last time
         # Counts (re)allocations of scratch buffers: a captured CUDA graph holds the addresses of the
@@ -53,6 +54,16 @@ class Runtime:
             self._views.clear()
         view = self._views[key] = buf[:count].view(*shape)
         return view
+
+    def counting(self, n: int) -> torch.Tensor:
+        """0 to n - 1, int32 on the device."""
+        held = getattr(self, "_counting", None)
+        if held is None or held.numel() < n:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the numbers 0 to n - 1 would be made during graph capture")
+            held = self._counting = torch.arange(max(n, 1024), dtype=torch.int32, device=self.device)
+            self.generation += 1                         # a captured graph holds the old one's address
+        return held[:n]
 
     def ones1(self) -> torch.Tensor:
         """[1.0] float32 on the device (the blend of a stream that has one copy)."""
