@@ -2,11 +2,87 @@
 //
 //   scales[g, i] = the smallest power of two s with |x| <= 448 s over the block;  codes = rn(x / s).
 //
-// Bound by reading x and writing the codes once (3 bytes an element of bfloat16): a block's elements stay in registers between its maximum and its codes.
+// Bound by reading x and writing the codes once (3 bytes an element of bfloat16): a block's elements stay in registers between its maximum and its codes, as they
+// were read. Instructions would be the bound otherwise, so sizes are compared as integers (two of bfloat16 at once) and what is not finite, which they show,
+// is dealt with only where it is.
 // Scales lie [k / 128, rows]: a block of threads makes sixteen rows' next to one another.
 #include "e4m3.cuh"
 
 namespace {
+
+// Eight elements as they lie in memory; bits of sizes grow with the sizes.
+template <typename T> struct Eight;
+template <> struct Eight<bf16> {
+    unsigned w[4];
+    template <bool VEC> __device__ __forceinline__ void load(const bf16* p) {
+        if (VEC) {
+            const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p));
+            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+        } else {
+            const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __ldcg(h + 2 * i) | (unsigned)__ldcg(h + 2 * i + 1) << 16;
+        }
+    }
+    __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0; }
+    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16); }
+    // The largest size of two lanes of 16 bits, and then of one number.
+    __device__ __forceinline__ unsigned sizes(unsigned m) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        return m;
+    }
+    static __device__ __forceinline__ unsigned size(unsigned m) { return max(m << 16, m & 0xFFFF0000u); }
+};
+template <> struct Eight<float> {
+    unsigned w[8];
+    template <bool VEC> __device__ __forceinline__ void load(const float* p) {
+        const unsigned* u = reinterpret_cast<const unsigned*>(p);
+        if (VEC) {
+            const uint4 a = __ldcg(reinterpret_cast<const uint4*>(u)), b = __ldcg(reinterpret_cast<const uint4*>(u + 4));
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __ldcg(u + i);
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(w[i]); }
+    __device__ __forceinline__ unsigned sizes(unsigned m) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+        return m;
+    }
+    static __device__ __forceinline__ unsigned size(unsigned m) { return m; }
+};
+// The largest finite size of N eights, and whether all are finite.
+template <typename T, int N> __device__ __forceinline__ float largest(const Eight<T> (&e)[N], bool& finite) {
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) m = e[j].sizes(m);
+    float f = __uint_as_float(Eight<T>::size(m));
+    finite = f < INFINITY;
+    if (!finite) {
+        f = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f = fmaxf(f, finite_size(e[j][i]));
+    }
+    return f;
+}
+template <typename T> __device__ __forceinline__ uint2 codes_of(const Eight<T>& e, float inverse, bool finite) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = e[i];
+    if (!finite) return codes8(v, inverse);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= inverse;
+    return make_uint2(e4m3_pair(v[0], v[1]) | (unsigned)e4m3_pair(v[2], v[3]) << 16, e4m3_pair(v[4], v[5]) | (unsigned)e4m3_pair(v[6], v[7]) << 16);
+}
 
 // Rows on their own: sixteen lanes a row's group, four groups of sixteen rows a block of 256 threads.
 constexpr int Q_ROWS = 16, Q_GROUPS = 4;
@@ -14,22 +90,23 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize8_rows_kernel(unsigned char* codes, float* scales, const T* x, long long ldx, int n, int k, int groups) {
     const int row = blockIdx.y * Q_ROWS + (threadIdx.x >> 4), part = threadIdx.x & 15, g0 = blockIdx.x * Q_GROUPS;
     pdl_enter();
-    float v[Q_GROUPS][8];
+    Eight<T> v[Q_GROUPS];
 #pragma unroll
     for (int g = 0; g < Q_GROUPS; ++g) {
         const int col = (g0 + g) * E4M3_BLOCK + part * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[g][i] = 0.f;
-        if (row < n && col < k) load8<T, VEC>(v[g], x + (long long)row * ldx + col);
+        v[g].clear();
+        if (row < n && col < k) v[g].template load<VEC>(x + (long long)row * ldx + col);
     }
 #pragma unroll
     for (int g = 0; g < Q_GROUPS; ++g) {
         const int col = (g0 + g) * E4M3_BLOCK + part * 8;
-        float m = largest8(v[g]);
+        bool finite;
+        const Eight<T> one[1] = {v[g]};
+        float m = largest(one, finite);
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const int power = e4m3_scale_power(m);
-        if (row < n && col < k) *reinterpret_cast<uint2*>(codes + (long long)row * k + col) = codes8(v[g], power_of_two(-power));
+        if (row < n && col < k) *reinterpret_cast<uint2*>(codes + (long long)row * k + col) = codes_of(v[g], power_of_two(-power), finite);
         if (row < n && part == 0 && g0 + g < groups) scales[(long long)(g0 + g) * n + row] = power_of_two(power);
     }
 }
@@ -40,21 +117,19 @@ __global__ void __launch_bounds__(256) quantize8_blocks_kernel(unsigned char* co
     __shared__ float scratch[33];
     const int g = blockIdx.x, row0 = blockIdx.y * E4M3_BLOCK + (threadIdx.x >> 4), col = g * E4M3_BLOCK + (threadIdx.x & 15) * 8;
     pdl_enter();
-    float v[8][8];
-    float m = 0.f;
+    Eight<T> v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
-        if (row0 + 16 * j < n && col < k) load8<T, VEC>(v[j], x + (long long)(row0 + 16 * j) * ldx + col);
+        v[j].clear();
+        if (row0 + 16 * j < n && col < k) v[j].template load<VEC>(x + (long long)(row0 + 16 * j) * ldx + col);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, largest8(v[j]));
+    bool finite;
+    const float m = largest(v, finite);
     const int power = e4m3_scale_power(block_max(m, scratch));
     const float inverse = power_of_two(-power);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-        if (row0 + 16 * j < n && col < k) *reinterpret_cast<uint2*>(codes + (long long)(row0 + 16 * j) * k + col) = codes8(v[j], inverse);
+        if (row0 + 16 * j < n && col < k) *reinterpret_cast<uint2*>(codes + (long long)(row0 + 16 * j) * k + col) = codes_of(v[j], inverse, finite);
     if (threadIdx.x == 0) scales[(long long)g * row_blocks + blockIdx.y] = power_of_two(power);
 }
 

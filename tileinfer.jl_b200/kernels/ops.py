@@ -1263,23 +1263,20 @@ def uniforms(out, seeds, counters):
 BLOCK8 = 128                         # columns (and, of weights, rows) of a matrix that share a scale
 
 
-def _blocks8(n: int) -> int:
-    return -(-n // BLOCK8)
-
-
 def quantize8(codes, scales, x, rows: int = 1):
     """codes [n, k] float8_e4m3fn and scales [ceil(k / 128), ceil(n / rows)] float32 of x [n, k] (float32 or bfloat16; its rows may be strided): a scale for every
     128 columns of each row (``rows`` 1: a product's inputs) or of 128 rows (128: its weights). A block's scale is the smallest power of two s >= 2^-100
     with |x| <= 448 s over its finite x, its codes are x / s rounded to nearest even; what is infinite or NaN has the code of NaN. k is a multiple of 16."""
-    _need(x, "x", contiguous=False); _need(codes, "codes", _E4M3); _need(scales, "scales", _F32)
-    if rows not in (1, BLOCK8):
-        raise KernelError(f"quantize8: blocks of 1 or {BLOCK8} rows, not {rows}")
-    if x.dim() != 2 or codes.shape != x.shape or x.shape[1] % 16 or tuple(scales.shape) != (_blocks8(x.shape[1]), -(-x.shape[0] // rows)) or \
-            (x.numel() and x.stride(1) != 1):
-        raise KernelError(f"quantize8: x {tuple(x.shape)} with strides {x.stride()}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)} do not fit (dense rows of "
-                          f"a multiple of 16 elements, scales [ceil(k / {BLOCK8}), ceil(n / {rows})])")
-    check(lib().ti_quantize8(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), x.stride(0), dtype_code(x.dtype), x.shape[0], x.shape[1], rows, _stream()),
-          "quantize8")
+    shape, dtype = x.shape, x.dtype
+    if not (x.is_cuda and codes.is_cuda and scales.is_cuda and codes.dtype is _E4M3 and scales.dtype is _F32 and (dtype is _BF16 or dtype is _F32) and
+            codes.is_contiguous() and scales.is_contiguous() and (rows == 1 or rows == BLOCK8) and len(shape) == 2 and codes.shape == shape and shape[1] % 16 == 0 and
+            scales.shape == (-(-shape[1] // BLOCK8), -(-shape[0] // rows)) and (x.stride(1) == 1 or not x.numel())):
+        _need(x, "x", contiguous=False); _need(codes, "codes", _E4M3); _need(scales, "scales", _F32); dtype_code(dtype)
+        raise KernelError(f"quantize8: x {tuple(x.shape)} with strides {x.stride()}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)} do not fit blocks of {rows} "
+                          f"rows (1 or {BLOCK8}; dense rows of a multiple of 16 elements, scales [ceil(k / {BLOCK8}), ceil(n / rows)])")
+    rc = lib().ti_quantize8(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), x.stride(0), BF16 if dtype is _BF16 else F32, shape[0], shape[1], rows, _stream())
+    if rc:
+        check(rc, "quantize8")
 
 
 _linear8_need = {}
@@ -1304,10 +1301,10 @@ def linear8(y, x, codes, scales, x_scales=None, epilogue=EPI_NONE, act=(0.0, 0.0
     try:
         (n, k), (out, columns), given = x.shape, codes.shape, x_scales is not None
         fits = x.is_cuda and y.is_cuda and codes.is_cuda and scales.is_cuda and codes.dtype is _E4M3 and scales.dtype is _F32 and columns == k and \
-            k % 16 == 0 and k > 0 and codes.is_contiguous() and scales.is_contiguous() and scales.shape == (_blocks8(k), _blocks8(out)) and \
+            k % 16 == 0 and k > 0 and codes.is_contiguous() and scales.is_contiguous() and scales.shape == (-(-k // BLOCK8), -(-out // BLOCK8)) and \
             y.shape == (n, out) and y.dtype is (_F32 if epilogue == EPI_F32_OUT else _BF16) and (x.stride(1) == 1 or not n) and \
             (y.stride(1) == 1 or not n * out) and x.dtype is (_E4M3 if given else _BF16) and \
-            (not given or (x_scales.is_cuda and x_scales.dtype is _F32 and x_scales.shape == (_blocks8(k), n) and x_scales.is_contiguous()))
+            (not given or (x_scales.is_cuda and x_scales.dtype is _F32 and x_scales.shape == (-(-k // BLOCK8), n) and x_scales.is_contiguous()))
     except ValueError:
         raise KernelError("linear8: x, y and codes have two dimensions") from None
     if not fits:
@@ -1330,16 +1327,16 @@ def linear8(y, x, codes, scales, x_scales=None, epilogue=EPI_NONE, act=(0.0, 0.0
         _library.add_launches(1)                             # the tokens' codes are made by a launch of their own
 
 
-def _paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, page_size) -> bool:
+def _paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, page_size, seqs) -> bool:
     """What the two operators on an 8-bit cache ask of what they share."""
-    seqs = kv_lens.numel()
-    return k_cache.dtype is _E4M3 and v_cache.dtype is _E4M3 and k_cache.is_cuda and v_cache.is_cuda and k_cache.dim() == 4 and k_cache.shape == v_cache.shape and \
-        k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.shape[2] == page_size and k_scales.dtype is _F32 and v_scales.dtype is _F32 and \
-        k_scales.is_cuda and v_scales.is_cuda and k_scales.is_contiguous() and v_scales.is_contiguous() and k_scales.shape == k_cache.shape[:2] and \
-        v_scales.shape == k_cache.shape[:2] and block_table.dtype is _I32 and seq_slots.dtype is _I32 and cu_seqlens.dtype is _I32 and kv_lens.dtype is _I32 and \
+    shape = k_cache.shape
+    return k_cache.dtype is _E4M3 and v_cache.dtype is _E4M3 and k_cache.is_cuda and v_cache.is_cuda and len(shape) == 4 and shape == v_cache.shape and \
+        shape[2] == page_size and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scales.dtype is _F32 and v_scales.dtype is _F32 and \
+        k_scales.is_cuda and v_scales.is_cuda and k_scales.is_contiguous() and v_scales.is_contiguous() and k_scales.shape == shape[:2] == v_scales.shape and \
+        block_table.dtype is _I32 and seq_slots.dtype is _I32 and cu_seqlens.dtype is _I32 and kv_lens.dtype is _I32 and \
         block_table.is_cuda and seq_slots.is_cuda and cu_seqlens.is_cuda and kv_lens.is_cuda and seq_slots.is_contiguous() and cu_seqlens.is_contiguous() and \
         kv_lens.is_contiguous() and cu_seqlens.numel() == seqs + 1 and seq_slots.numel() == seqs and block_table.dim() == 2 and \
-        (not block_table.numel() or block_table.stride(1) == 1)
+        (block_table.stride(1) == 1 or not block_table.numel())
 
 
 def _refuse_paged8(what, k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, said):
@@ -1358,19 +1355,20 @@ def cache_write8(k_cache, v_cache, k_scales, v_scales, k, v, block_table, seq_sl
     with it; a page that is new from its first position on begins afresh. What lies behind a sequence's last position stays as it was. ``max_new``: the most new
     rows of a sequence (a sequence may have none). No two sequences may be given rows of one page. A sequence whose slot, page or length is none that
     exists is left out. Infinite and NaN values get the code of NaN."""
-    said = f"k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}, {max_new} new rows"
-    if not (_paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, PAGE8) and k.is_cuda and v.is_cuda and
-            k.dtype in (_BF16, _F32) and v.dtype is k.dtype and k.dim() == 3 and k.shape == v.shape and k.shape[1:] == (k_cache.shape[1], k_cache.shape[3]) and
-            (not k.numel() or (k.stride(2) == 1 and v.stride(2) == 1)) and max_new >= 0):
-        _need(k, "k", contiguous=False); _need(v, "v", k.dtype, contiguous=False); dtype_code(k.dtype)
-        _refuse_paged8("cache_write8", k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, said)
-    pages, nkv, page, dim = k_cache.shape
-    if not k.numel() or not kv_lens.numel() or not block_table.numel():
+    seqs, dtype, shape = kv_lens.numel(), k.dtype, k.shape
+    if not (_paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, PAGE8, seqs) and k.is_cuda and v.is_cuda and
+            (dtype is _BF16 or dtype is _F32) and v.dtype is dtype and len(shape) == 3 and shape == v.shape and shape[1] == k_cache.shape[1] and
+            shape[2] == k_cache.shape[3] and ((k.stride(2) == 1 and v.stride(2) == 1) or not k.numel()) and max_new >= 0):
+        _need(k, "k", contiguous=False); _need(v, "v", dtype, contiguous=False); dtype_code(dtype)
+        _refuse_paged8("cache_write8", k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens,
+                       f"k {tuple(k.shape)} {k.dtype} {k.stride()}, v {tuple(v.shape)} {v.dtype} {v.stride()}, {max_new} new rows")
+    if not (seqs and shape[0]) or not block_table.numel():
         return
-    rc = lib().ti_cache_write8(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), k.data_ptr(), k.stride(0), k.stride(1),
-                               v.data_ptr(), v.stride(0), v.stride(1), block_table.data_ptr(), block_table.stride(0), block_table.shape[0], seq_slots.data_ptr(),
-                               cu_seqlens.data_ptr(), kv_lens.data_ptr(), kv_lens.numel(), k.shape[0], nkv, dim, page, pages, max_new,
-                               BF16 if k.dtype is _BF16 else F32, _stream())
+    k_token, k_head, _ = k.stride()
+    v_token, v_head, _ = v.stride()
+    rc = lib().ti_cache_write8(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), k.data_ptr(), k_token, k_head, v.data_ptr(), v_token,
+                               v_head, block_table.data_ptr(), block_table.stride(0), block_table.shape[0], seq_slots.data_ptr(), cu_seqlens.data_ptr(),
+                               kv_lens.data_ptr(), seqs, shape[0], shape[1], shape[2], PAGE8, k_cache.shape[0], max_new, BF16 if dtype is _BF16 else F32, _stream())
     if rc:
         check(rc, "cache_write8")
 
@@ -1394,13 +1392,15 @@ def attention8(out, q, k_cache, v_cache, k_scales, v_scales, block_table, seq_sl
     cu_seqlens[b] to cu_seqlens[b + 1] of q [n, nq, head_dim] (at most ``max_new``, or none) are the last of the kv_lens[b] positions of the sequence in slot
     seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out [n, nq * head_dim]; q and out bfloat16. A key stands for its code times
     k_scales[page, head], a value for its code times v_scales[page, head] (positive, 2^-100 to 2^120). ``max_len``: no kv_lens is larger (None: as many as the
-    table's rows have pages for). What no token sees may hold any codes; a NaN code that some see reaches those alone. Lengths, ranges, slots, table, and the
-    pages before those of the new tokens are read while kernels ahead may still run: they come from copies, torch's operations or earlier steps. ``workspace``:
-    ``attention8_workspace`` bytes (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
+    table's rows have pages for). What no token sees may hold any codes; a NaN code that some see reaches those alone. Long
+    runs go through pages widened to bfloat16: codes times scales that are no powers of two are rounded to it, and a NaN value that some rows of a run see may
+    reach others of the run; their q and out must be 16-byte aligned (others' 4-byte). Lengths, ranges, slots, table, and the pages before those of the new tokens
+    are read while kernels ahead may still run: they come from copies, torch's operations or earlier steps. ``workspace``: ``attention8_workspace`` bytes (uint8);
+    without it one kept per thread and stream (a captured call: one of its graph's own)."""
     seqs, n = kv_lens.numel(), q.shape[0]
-    if not (_paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, page_size) and out.is_cuda and q.is_cuda and
+    if not (_paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, page_size, seqs) and out.is_cuda and q.is_cuda and
             out.dtype is _BF16 and q.dtype is _BF16 and out.is_contiguous() and q.is_contiguous() and nkv > 0 and nq > 0 and nq % nkv == 0 and head_dim > 0 and
-            max_new >= 0 and window >= 0 and q.numel() == n * nq * head_dim == out.numel() and k_cache.shape[1:] == (nkv, page_size, head_dim) and
+            max_new >= 0 and window >= 0 and q.numel() == n * nq * head_dim == out.numel() and k_cache.shape[1] == nkv and k_cache.shape[3] == head_dim and
             (max_len is None or max_len >= 0)):
         _need(out, "out", _BF16); _need(q, "q", _BF16)
         _refuse_paged8("attention8", k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens,
