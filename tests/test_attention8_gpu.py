@@ -166,6 +166,30 @@ def test_queries_of_any_size(ops, size):
     assert bool(((got.to(F64) - want).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("window", [0, 20])
+def test_zero_queries_over_zero_pages(ops, new, window):
+    """The smallest scale times the smallest factor of a row is no 32-bit number; keys that nobody sees stay out all the same."""
+    c = make([(new, 70), (new, 40)], 8, 2, 64, seed=3)
+    c["q"].zero_(), c["ks"].fill_(2.0 ** -100)
+    got = call(ops, c, 8, 2, 64, new, window)
+    want, bound = reference(c, 0.125, window, 11)
+    assert bool(((got.to(F64) - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("runs,widened", [([(200, 300), (300, 1500), (1, 64)], True), ([(1, 300), (2, 1500), (0, 900)], False)])
+def test_a_sequence_longer_than_was_said_stays_within_its_own(ops, runs, widened):
+    """``max_len`` says 512: what the sequence of 1,500 gets is not defined, the others' results are."""
+    new = max(t for t, _ in runs)
+    assert bool(ops.lib().ti_attention8_widens(3, new, 16, 2, 64, 512)) == widened
+    c = make(runs, 16, 2, 64, seed=5)
+    got = call(ops, c, 16, 2, 64, new, max_len=512)
+    want, bound = reference(c, 0.125, 0, 8)
+    right = ((got.to(F64) - want).abs() <= bound).all(-1)
+    first, end = int(c["cu"][1]), int(c["cu"][2])
+    assert bool(right[:first].all()) and bool(right[end:].all())
+
+
 def test_nan_codes_reach_the_rows_that_see_them_alone(ops):
     """A NaN value or key of a new token reaches that token and those after it; one before a window's first key nobody."""
     for dim in (64, 128, 48):

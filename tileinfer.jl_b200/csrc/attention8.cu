@@ -86,13 +86,14 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
     extern __shared__ __align__(128) unsigned char smem_dyn[];
     __shared__ unsigned s_units[A8_MAX_SEQS + 1], s_scan[A8_THREADS / 32];
     __shared__ int s_cu[A8_MAX_SEQS + 1], s_len[A8_MAX_SEQS], s_slot[A8_MAX_SEQS];
-    __shared__ float s_ml[4][M][2], s_row[M], s_scale[STAGES][4];                    // s_row: a row's factor of its scores; s_scale: sk, log2 sv, 1 / sv
+    __shared__ float s_ml[4][M][2], s_row[M];                                           // s_row: a row's factor of its scores
+    __shared__ float4 s_scale[64];                           // of the run's tiles in turn: sk, log2 sv, 1 / sv
     __shared__ __align__(8) unsigned long long bars[2 * STAGES];
     unsigned char* ring = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
     const int D = EXACT ? DP : a.D, tile_bytes = AF_PAGE * D, B = a.B, nkv = a.nkv, group = a.nq / nkv;
     const unsigned full0 = smem_u32(bars), empty0 = full0 + 8 * STAGES;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { tc::mbar_init(full0 + 8 * s, 1); tc::mbar_init(empty0 + 8 * s, 4); }
+        for (int s = 0; s < STAGES; ++s) { tc::mbar_init(full0 + 8 * s, 2); tc::mbar_init(empty0 + 8 * s, 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -155,44 +156,71 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
     };
 
     if (warp == 4) {
-        // ---------------------------------------------------------------- copies: lane 0, with a tile's page asked for one tile ahead
-        bool ok = true, waited = false;
-        unsigned u = lo, phase = 0;
-        int stage = 0;
-        Place at{};
-        const int* pages = nullptr;
-        int page = 0;
-        auto enter = [&] {
-            at = locate(u);
-            pages = a.table + (size_t)s_slot[at.b] * a.table_stride + at.s.t0;
-            page = __ldcg(pages + at.tile);
+        // ---------------------------------------------------------------- copies: lane 0 asks; the lanes look up the pages of 32 tiles at once, and of the next 32
+        // meanwhile, and hand the tiles' scales over, which need not be there when a tile is asked for
+        struct Ahead {
+            int block;                                       // the tile's page and head, -1 beyond the pool
+            bool fresh, scaled;                              // with new keys; its scales are here
+            float sk, sv;
         };
-        if (lane == 0 && u < hi) enter();
-        while (lane == 0 && u < hi) {
+        bool ok = true, waited = false, placed = false;      // placed: all scales that are here have been handed over
+        unsigned phase = 0;
+        int stage = 0, pending = 0;                          // tiles asked for and not yet handed over
+        auto look = [&](unsigned u) {
+            Ahead x = {-1, false, true, 1.f, 1.f};
+            if (u >= hi) return x;
+            const Place p = locate(u);
+            const int tile = p.s.t0 + p.tile, page = __ldcg(a.table + (size_t)s_slot[p.b] * a.table_stride + tile);
             // Tiles with new keys were written by the kernel before this one; the others stand since earlier steps.
-            if (!waited && (at.s.t0 + at.tile + 1) * AF_PAGE > at.s.L - at.s.T) { pdl_wait(); waited = true; }
-            const bool there = page >= 0 && page < a.pages;  // a page that does not exist reads as zeros
-            const int block = there ? page * nkv + at.kvh : -1;
-            const float sk = there ? __ldcg(a.k_scales + block) : 1.f, sv = there ? __ldcg(a.v_scales + block) : 1.f;
-            const bool last = at.tile + 1 == at.s.tiles;
-            const int next_page = last ? 0 : __ldcg(pages + at.tile + 1);
-            ok = tc::mbar_wait(empty0 + 8 * stage, phase ^ 1, a.status, 29);
-            if (!ok) break;
-            const unsigned bar = full0 + 8 * stage, to = smem_u32(ring) + stage * 2 * tile_bytes;
-            s_scale[stage][0] = sk;
-            s_scale[stage][1] = __log2f(sv);
-            s_scale[stage][2] = 1.f / sv;
-            tc::mbar_expect_tx(bar, 2 * tile_bytes);
-            tc::tma_load_2d(to, &map_k, 0, block * (D / 2), bar);
-            tc::tma_load_2d(to + tile_bytes, &map_v, 0, block * (D / 2), bar);
-            if (++stage == STAGES) { stage = 0; phase ^= 1; }
-            ++u;
-            if (last) {
-                if (u < hi) enter();
-            } else {
-                ++at.tile;
-                page = next_page;
+            x.fresh = (tile + 1) * AF_PAGE > p.s.L - p.s.T;
+            if (page >= 0 && page < a.pages) { x.block = page * nkv + p.kvh; x.scaled = false; }                     // a page that does not exist reads as zeros
+            return x;
+        };
+        auto scales = [&](Ahead& x) {
+            if (x.scaled || (x.fresh && !waited)) return;
+            x.sk = __ldcg(a.k_scales + x.block);
+            x.sv = __ldcg(a.v_scales + x.block);
+            x.scaled = true;
+        };
+        auto place = [&](const Ahead& x, unsigned u0) {
+            if (x.scaled) s_scale[(u0 - lo + lane) % 64] = make_float4(x.sk, __log2f(x.sv), 1.f / x.sv, 0.f);
+            __syncwarp();
+            for (; pending > 0; --pending)
+                if (lane == 0) tc::mbar_arrive(full0 + 8 * (stage < pending ? stage - pending + STAGES : stage - pending));
+            placed = true;
+        };
+        Ahead now = look(lo + lane), then;
+        for (unsigned u0 = lo; ok && u0 < hi; u0 += 32) {
+            scales(now);
+            if (u0 != lo) place(now, u0);
+            then = look(u0 + 32 + lane);
+            for (int i = 0; i < 32 && u0 + i < hi; ++i) {
+                if (i == 8) scales(then);
+                if (!waited && __shfl_sync(0xffffffffu, now.fresh, i)) {
+                    pdl_wait();
+                    waited = true;
+                    placed = false;
+                    scales(now);
+                }
+                if (pending == STAGES) place(now, u0);
+                const int block = __shfl_sync(0xffffffffu, now.block, i);
+                if (lane == 0) {
+                    ok = tc::mbar_wait(empty0 + 8 * stage, phase ^ 1, a.status, 29);
+                    if (ok) {
+                        const unsigned bar = full0 + 8 * stage, to = smem_u32(ring) + stage * 2 * tile_bytes;
+                        tc::mbar_expect_tx(bar, 2 * tile_bytes);
+                        tc::tma_load_2d(to, &map_k, 0, block * (D / 2), bar);
+                        tc::tma_load_2d(to + tile_bytes, &map_v, 0, block * (D / 2), bar);
+                        if (placed) tc::mbar_arrive(bar);
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
+                if (!placed) ++pending;
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
+            if (pending > 0) place(now, u0);
+            now = then;
         }
         if (!ok) tc::drain_after_timeout();                  // a wait ran out: let what is in flight land
         __syncwarp();
@@ -300,7 +328,8 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
             if (!ok) continue;
             const unsigned char* kt = ring + stage * 2 * tile_bytes;
             const unsigned char* vt = kt + tile_bytes;
-            const float sk = s_scale[stage][0], lv = s_scale[stage][1], inv = s_scale[stage][2];
+            const float4 scales = s_scale[(u - lo) % 64];
+            const float sk = scales.x, lv = scales.y, inv = scales.z;
             const int key_base = tile * AF_PAGE + share;
             float sc[NQ][4];
 #pragma unroll
@@ -349,7 +378,7 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
             for (int n = 0; n < NQ; ++n)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    sc[n][j] = fmaf(sc[n][j], rf[n][j & 1] * sk, lv);
+                    sc[n][j] = fmaf(sc[n][j], fmaxf(rf[n][j & 1] * sk, 1.1754944e-38f), lv);           // off zero: a score of -inf stays one
                     above |= sc[n][j] > m[n][j & 1] + SLACK;
                 }
             if (__any_sync(0xffffffffu, above)) {
@@ -548,7 +577,7 @@ template <int DP, bool EXACT> int launch_rows(const Call& c, int eights) {
 
 }  // namespace
 
-int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
+int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, int* lens_out, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
                  int table_stride, const int* seq_slots, const int* cu, const int* kv_lens, int B, int nkv, int D, int pages, int per_seq, int window, cudaStream_t stream);
 extern "C" int ti_attention_prefill_tc(void* out, const void* q, const void* k_cache, const void* v_cache, int n_pages, const int* block_table, int table_stride,
                                        const int* seq_slots, const int* cu_seqlens, const int* kv_lens, int n_seqs, int n_tokens, int total_blocks, float scale, int nq,
@@ -571,7 +600,7 @@ extern "C" long long ti_attention8_workspace(int B, int max_new, int nq, int nkv
     if (B <= 0 || max_new <= 0 || nq <= 0 || nkv <= 0 || D <= 0) return 0;
     if (ti_attention8_widens(B, max_new, nq, nkv, D, max_len)) {
         const long long pages = (long long)B * ((max_len + AF_PAGE - 1) / AF_PAGE);
-        return pages * nkv * AF_PAGE * D * 4 + up16(4 * pages) + up16(4LL * B);
+        return pages * nkv * AF_PAGE * D * 4 + up16(4 * pages) + 2 * up16(4LL * B);
     }
     const int eights = slab_eights(max_new * (long long)(nq / nkv), D);
     return 2LL * sm_blocks(eights, D) * ti_sm_count() * 8 * eights * (D + 2) * 4;
@@ -609,11 +638,11 @@ extern "C" int ti_attention8(void* out, const void* q, const void* k, const void
         TI_REQUIRE(all * nkv * AF_PAGE <= 0x7fffffffLL, "attention8: %d sequences of up to %d positions are too many for one step", B, max_len);
         TI_REQUIRE(((uintptr_t)q | (uintptr_t)out) % 16 == 0, "attention8: queries and outputs of long runs must be 16-byte aligned");
         bf16 *k16 = (bf16*)ws, *v16 = k16 + pool;
-        int *table16 = (int*)(v16 + pool), *slots16 = (int*)((unsigned char*)table16 + up16(4 * all));
-        if (int rc = cache_widen8(k16, v16, table16, slots16, k, v, k_scales, v_scales, table, table_stride, seq_slots, cu, kv_lens, B, nkv, D, pages, per_seq, window, stream)) return rc;
+        int *table16 = (int*)(v16 + pool), *slots16 = table16 + up16(4 * all) / 4, *lens16 = slots16 + up16(4LL * B) / 4;
+        if (int rc = cache_widen8(k16, v16, table16, slots16, lens16, k, v, k_scales, v_scales, table, table_stride, seq_slots, cu, kv_lens, B, nkv, D, pages, per_seq, window, stream)) return rc;
         // As many blocks as the runs can need: those beyond leave at once.
         const int tokens = 2 * (128 / (nq / nkv)), blocks = n / tokens + (B < n ? B : n);
-        return ti_attention_prefill_tc(out, q, k16, v16, (int)all, table16, per_seq, slots16, cu, kv_lens, B, n, blocks, scale, nq, nkv, D, page_size, window, status, stream);
+        return ti_attention_prefill_tc(out, q, k16, v16, (int)all, table16, per_seq, slots16, cu, lens16, B, n, blocks, scale, nq, nkv, D, page_size, window, status, stream);
     }
     Call c;
     c.max_new = max_new;

@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(THREADS) cache_write8_kernel(unsigned char* k_
 }
 
 // blockIdx: page, head, sequence.
-__global__ void __launch_bounds__(THREADS) cache_widen8_kernel(bf16* k_out, bf16* v_out, int* table_out, int* slots_out, const unsigned char* k, const unsigned char* v,
+__global__ void __launch_bounds__(THREADS) cache_widen8_kernel(bf16* k_out, bf16* v_out, int* table_out, int* slots_out, int* lens_out, const unsigned char* k, const unsigned char* v,
                                                                const float* k_scales, const float* v_scales, const int* table, int table_stride, const int* seq_slots,
                                                                const int* cu, const int* kv_lens, int nkv, int D, int pages, int per_seq, int window) {
     const int j = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(THREADS) cache_widen8_kernel(bf16* k_out, bf16
     const int T_new = __ldcg(cu + b + 1) - __ldcg(cu + b), L = __ldcg(kv_lens + b), slot = __ldcg(seq_slots + b);
     if (kvh == 0 && threadIdx.x == 0) {
         table_out[(size_t)b * per_seq + j] = b * per_seq + j;
-        if (j == 0) slots_out[b] = b;
+        if (j == 0) { slots_out[b] = b; lens_out[b] = min(L, per_seq * PAGE); }             // readers stay within the table, whatever they were given
     }
     const int first = window > 0 ? max(0, L - T_new - window + 1) : 0;
     if (T_new <= 0 || j * PAGE >= L || j < first / PAGE / 2 * 2) return;              // the readers walk the pages in pairs
@@ -137,10 +137,10 @@ extern "C" int ti_cache_write8(void* k_codes, void* v_codes, float* k_scales, fl
     return ti_check_launch("cache_write8");
 }
 
-// For attention8.cu: pools k_out, v_out [B * per_seq, nkv, 64, D] bfloat16, table_out [B, per_seq], slots_out [B].
-int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
+// For attention8.cu: pools k_out, v_out [B * per_seq, nkv, 64, D] bfloat16, table_out [B, per_seq], slots_out [B], lens_out [B].
+int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, int* lens_out, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
                  int table_stride, const int* seq_slots, const int* cu, const int* kv_lens, int B, int nkv, int D, int pages, int per_seq, int window, cudaStream_t stream) {
-    ti_launch(cache_widen8_kernel, dim3(per_seq, nkv, B), dim3(THREADS), 0, stream, (bf16*)k_out, (bf16*)v_out, table_out, slots_out, (const unsigned char*)k,
+    ti_launch(cache_widen8_kernel, dim3(per_seq, nkv, B), dim3(THREADS), 0, stream, (bf16*)k_out, (bf16*)v_out, table_out, slots_out, lens_out, (const unsigned char*)k,
               (const unsigned char*)v, k_scales, v_scales, table, table_stride, seq_slots, cu, kv_lens, nkv, D, pages, per_seq, window);
     return ti_check_launch("cache_widen8");
 }
