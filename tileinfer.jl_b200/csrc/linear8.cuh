@@ -25,12 +25,31 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, unsigned (&r)[16]) {
         : "r"(taddr) : "memory");
 }
 
-// One thread of a warp, the same one every time: code that only this guards stays uniform for the compiler, which keeps descriptors and counters in uniform
-// registers then (an issuing loop under `lane == 0` took four times the cycles a group).
+// One thread of a warp, the same one every time: what only this guards stays uniform for the compiler.
 __device__ __forceinline__ bool elected() {
     unsigned one;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
     return one != 0;
+}
+// Whether a barrier's phase is over, asked by the lanes with `asks`. Beside MMAs that read shared memory the answer takes some 300 cycles, a ready one too, so loops
+// ask for their next step before they issue this one's work.
+__device__ __forceinline__ bool mbar_test(unsigned bar, unsigned parity, bool asks) {
+    unsigned done;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %3, 0;\n\t"
+        "mov.u32 %0, 1;\n\t"
+        "@q mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@q selp.u32 %0, 1, 0, p;\n\t}"
+        : "=&r"(done) : "r"(bar), "r"(parity), "r"((unsigned)asks) : "memory");
+    return done != 0;
+}
+// The wait that such an answer belongs to, for the whole warp.
+__device__ __forceinline__ bool warp_wait_after(bool ready, unsigned bar, unsigned parity, bool asks, int* status, int code) {
+    if (__all_sync(0xffffffffu, ready)) return true;
+    bool ok = true;
+    if (asks) ok = mbar_wait(bar, parity, status, code);
+    return __all_sync(0xffffffffu, ok);
 }
 // A whole warp's wait: one lane tests the barrier, the others follow it.
 __device__ __forceinline__ bool warp_wait(unsigned bar, unsigned parity, int* status, int code) {

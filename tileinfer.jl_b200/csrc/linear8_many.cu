@@ -17,15 +17,17 @@
 namespace {
 using namespace tc;
 
-constexpr int BM = 128, BN = 128, KB = 128, STEP = 2, SLOTS = 2, HALF = BN / 2, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
-constexpr int A_BYTES = BM * KB, B_BYTES = BN / 2 * KB, STAGE = STEP * (A_BYTES + B_BYTES);
-constexpr int OUT_COLS = 32, OUT = 32 * OUT_COLS * 4;        // a warp's results on their way out
-constexpr int STAGES = 4, BYTES = STAGES * STAGE + EPI_WARPS * OUT + 1024;
-static_assert(BYTES <= 227 * 1024, "shared memory");
+constexpr int BM = 128, BN = 128, KB = 128, HALF = BN / 2, EPI_WARPS = 8, THREADS = 96 + 32 * EPI_WARPS;
+constexpr int A_BYTES = BM * KB, B_BYTES = BN / 2 * KB, STAGE = A_BYTES + B_BYTES;
+constexpr int STAGES = 8, SLOTS = 4;                         // of operands; of sums
+constexpr int AHEAD = STAGES - SLOTS;                        // groups whose factors are brought before their products are there
+constexpr int OUT_COLS = 16, OUT = 32 * OUT_COLS * 4;        // a warp's results on their way out
+constexpr int BYTES = STAGES * STAGE + EPI_WARPS * OUT + 1024;
+static_assert(BYTES + STAGES * BM * 4 <= 226 * 1024 && SLOTS * BN <= 512, "shared and tensor memory");
 
 struct Args {
     Linear8 p;
-    int groups, steps, row_blocks, token_tiles, tiles;              // row_blocks: of 128 weight rows, as scales have them
+    int groups, row_blocks, token_tiles, tiles;              // row_blocks: of 128 weight rows, as scales have them
 };
 
 __device__ __forceinline__ unsigned cluster_rank() {
@@ -70,17 +72,18 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     unsigned char* tiles = smem_dyn + ((1024u - (smem_addr(smem_dyn) & 1023u)) & 1023u);
     __shared__ __align__(8) unsigned long long bars[2 * STAGES + SLOTS];
     __shared__ unsigned s_tmem;
-    // done: a stage has been read and its sums are complete.
+    __shared__ float s_factor[STAGES][BM];
+    // done: a stage has been read, its sums are complete and their factors there.
     const unsigned full0 = smem_addr(bars), done0 = full0 + 8 * STAGES, free0 = done0 + 8 * STAGES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(done0 + 8 * s, 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(done0 + 8 * s, 2); }
         for (int s = 0; s < SLOTS; ++s) mbar_init(free0 + 8 * s, 2 * EPI_WARPS);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(SLOTS * STEP * BN) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(SLOTS * BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -96,19 +99,21 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         // ---------------------------------------------------------------- copies, in both blocks, one thread
         int stage = 0;
         unsigned phase = 0;
+        bool ready = true;                                   // every stage is free at first
         for (int tile = pair; lane == 0 && ok && tile < a.tiles; tile += pairs) {
             const int token = tile % a.token_tiles * (2 * BM) + rank * BM, row = tile / a.token_tiles * BN + rank * (BN / 2);
-            for (int step = 0; step < a.steps; ++step) {
-                ok = mbar_wait(done0 + 8 * stage, phase ^ 1, p.status, 24);
+            for (int g = 0; g < a.groups; ++g) {
+                if (!ready) ok = mbar_wait(done0 + 8 * stage, phase ^ 1, p.status, 24);
                 if (!ok) break;
+                const int next = stage + 1 == STAGES ? 0 : stage + 1;
+                const unsigned next_phase = next == 0 ? phase ^ 1 : phase;
+                ready = mbar_test(done0 + 8 * next, next_phase ^ 1, true);
                 if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2 * STAGE);
                 const unsigned bar = in_block0(full0 + 8 * stage), to = smem_addr(tiles + stage * STAGE);
-#pragma unroll
-                for (int i = 0; i < STEP; ++i) {             // beyond the last group: zeros
-                    load_pair(to + i * A_BYTES, &map_x, (step * STEP + i) * (KB / 2), token, bar);
-                    load_pair(to + STEP * A_BYTES + i * B_BYTES, &map_w, (step * STEP + i) * (KB / 2), row, bar);
-                }
-                if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                load_pair(to, &map_x, g * (KB / 2), token, bar);
+                load_pair(to + A_BYTES, &map_w, g * (KB / 2), row, bar);
+                stage = next;
+                phase = next_phase;
             }
         }
         __syncwarp();
@@ -118,74 +123,109 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             int stage = 0, slot = 0;
             unsigned phase = 0, slot_phase = 0;
             const unsigned long long first = smem_desc_sw128(smem_addr(tiles));
+            // One lane asks for the operands, another for the accumulator.
+            const bool asks = lane < 2;
+            bool ready = false;
             for (int tile = pair; ok && tile < a.tiles; tile += pairs)
-                for (int step = 0; step < a.steps; ++step) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(free0 + 8 * slot, slot_phase ^ 1, p.status, 25) && mbar_wait(full0 + 8 * stage, phase, p.status, 26));
+                for (int g = 0; g < a.groups; ++g) {
+                    ok = warp_wait_after(ready, lane ? free0 + 8 * slot : full0 + 8 * stage, lane ? slot_phase ^ 1 : phase, asks, p.status, 25);
                     if (!ok) break;
                     tc_fence_after();
-                    const unsigned long long dx = first + (unsigned)(stage * (STAGE >> 4)), dw = dx + (STEP * A_BYTES >> 4);
-                    const unsigned to = tmem + slot * (STEP * BN);
-                    if (elected()) {
-#pragma unroll
-                        for (int i = 0; i < STEP; ++i)
-#pragma unroll
-                            for (int k = 0; k < KB / 32; ++k) mma_pair(to + i * BN, dx + i * (A_BYTES >> 4) + 2 * k, dw + i * (B_BYTES >> 4) + 2 * k, IDESC, k > 0);
-                        commit_pair(done0 + 8 * stage);
-                    }
-                    __syncwarp();
+                    const unsigned long long dx = first + (unsigned)(stage * (STAGE >> 4)), dw = dx + (A_BYTES >> 4);
+                    const unsigned to = tmem + slot * BN, done = done0 + 8 * stage;
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                     if (++slot == SLOTS) { slot = 0; slot_phase ^= 1; }
+                    ready = mbar_test(lane ? free0 + 8 * slot : full0 + 8 * stage, lane ? slot_phase ^ 1 : phase, asks);
+                    if (elected()) {
+#pragma unroll
+                        for (int k = 0; k < KB / 32; ++k) mma_pair(to, dx + 2 * k, dw + 2 * k, IDESC, k > 0);
+                        commit_pair(done);
+                    }
+                    __syncwarp();
                 }
+        }
+    } else if (warp == 2) {
+        // ---------------------------------------------------------------- the factors sx sw of the block's tokens, LOADS groups ahead in registers (multiplied when
+        // they are wanted: a product at once would wait for its loads, 1,600 cycles a group in all), then AHEAD in shared memory: a place is written again
+        // when the products AHEAD groups before are there, whose accumulator had been read before
+        constexpr int LOADS = 4, V = BM / 32;
+        int next_tile = pair, next_g = 0, at[V];
+        float sx[LOADS][V], sw[LOADS];
+        const float *from = nullptr, *from_w = nullptr;
+        auto ask = [&](float (&x)[V], float& w) {
+            if (next_tile >= a.tiles) return;
+            if (next_g == 0) {
+                const int token0 = next_tile % a.token_tiles * (2 * BM) + rank * BM + lane;
+#pragma unroll
+                for (int i = 0; i < V; ++i) at[i] = min(token0 + 32 * i, p.n - 1);
+                from = p.x_scales;
+                from_w = p.scales + next_tile / a.token_tiles;
+            }
+            w = __ldg(from_w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = __ldcg(from + at[i]);
+            from += p.n;
+            from_w += a.row_blocks;
+            if (++next_g == a.groups) { next_g = 0; next_tile += pairs; }
+        };
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) ask(sx[j], sw[j]);
+        const long long all = (long long)((a.tiles - pair + pairs - 1) / pairs) * a.groups;
+        int place = 0, behind = STAGES - AHEAD;
+        unsigned phase = 1;
+        bool ready = true;
+        for (long long s0 = 0; ok && s0 < all; s0 += LOADS) {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                if (s0 + j >= all) break;
+                ok = warp_wait_after(ready, done0 + 8 * behind, phase, lane == 0, p.status, 30);
+                if (!ok) break;
+                if (++behind == STAGES) { behind = 0; phase ^= 1; }
+                ready = mbar_test(done0 + 8 * behind, phase, lane == 0);
+#pragma unroll
+                for (int i = 0; i < V; ++i) s_factor[place][lane + 32 * i] = sx[j][i] * sw[j];
+                ask(sx[j], sw[j]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(done0 + 8 * place);
+                if (++place == STAGES) place = 0;
+            }
         }
     } else {
         // ---------------------------------------------------------------- sums: a thread a token, 64 weight rows
-        const int half = (warp - 2) >> 2, quarter = warp & 3;
+        const int half = (warp - 3) >> 2, quarter = warp & 3;
         const unsigned columns = tmem + ((unsigned)(quarter * 32) << 16) + half * HALF, release0 = in_block0(free0);
-        float* out = reinterpret_cast<float*>(tiles + STAGES * STAGE) + (warp - 2) * (OUT / 4);
+        float* out = reinterpret_cast<float*>(tiles + STAGES * STAGE) + (warp - 3) * (OUT / 4);
         const bool y32 = p.epilogue == L4_EPI_F32_OUT, quads = linear8_quads(p);
         // 32 bytes at a time straight from the registers.
         const bool direct = (p.epilogue == L4_EPI_NONE && ((uintptr_t)p.y & 31) == 0 && p.ldy % 16 == 0) || (y32 && ((uintptr_t)p.y & 31) == 0 && p.ldy % 8 == 0);
         int slot = 0, stage = 0;
         unsigned phase = 0;
+        bool ready = false;
         for (int tile = pair; ok && tile < a.tiles; tile += pairs) {
             const int token0 = tile % a.token_tiles * (2 * BM) + rank * BM + quarter * 32, token = min(token0 + lane, p.n - 1);
-            const int block = tile / a.token_tiles, row0 = block * BN + half * HALF;
-            const float *sx = p.x_scales + token, *sw = p.scales + block;
+            const int row0 = tile / a.token_tiles * BN + half * HALF;
             f32x2 acc[HALF / 2];
 #pragma unroll
             for (int c = 0; c < HALF / 2; ++c) acc[c] = 0ull;
-            // Factors of the next two steps' groups.
-            float f[2 * STEP];
-            auto factor = [&](int g) { return g < a.groups ? __ldcg(sx + (long long)g * p.n) * __ldg(sw + (long long)g * a.row_blocks) : 0.f; };
+            for (int g = 0; g < a.groups; ++g) {
+                ok = warp_wait_after(ready, done0 + 8 * stage, phase, lane == 0, p.status, 27);
+                if (!ok) break;
+                tc_fence_after();
+                unsigned r[2][32];
+                tmem_ld32(columns + slot * BN, r[0]);
+                tmem_ld32(columns + slot * BN + 32, r[1]);
+                const float f = s_factor[stage][quarter * 32 + lane];
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_block0(release0 + 8 * slot);
+                if (++slot == SLOTS) slot = 0;
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                ready = mbar_test(done0 + 8 * stage, phase, lane == 0);
+                const f32x2 ff = pack2(f, f);
 #pragma unroll
-            for (int i = 0; i < 2 * STEP; ++i) f[i] = factor(i);
-            for (int step0 = 0; ok && step0 < a.steps; step0 += 2) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if (step0 + j >= a.steps) break;
-                    ok = warp_wait(done0 + 8 * stage, phase, p.status, 27);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int i = 0; i < STEP; ++i) {
-                        unsigned r[2][32];
-                        tmem_ld32(columns + (slot * STEP + i) * BN, r[0]);
-                        tmem_ld32(columns + (slot * STEP + i) * BN + 32, r[1]);
-                        tmem_ld_wait();
-                        if (i == STEP - 1) {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) arrive_block0(release0 + 8 * slot);
-                        }
-                        const f32x2 ff = pack2(f[j * STEP + i], f[j * STEP + i]);
-                        f[j * STEP + i] = factor((step0 + j + 2) * STEP + i);
-#pragma unroll
-                        for (int c = 0; c < HALF / 2; ++c)
-                            acc[c] = fma2(pack2(__uint_as_float(r[c / 16][2 * c % 32]), __uint_as_float(r[c / 16][2 * c % 32 + 1])), ff, acc[c]);
-                    }
-                    slot ^= 1;
-                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
-                }
+                for (int c = 0; c < HALF / 2; ++c)
+                    acc[c] = fma2(pack2(__uint_as_float(r[c / 16][2 * c % 32]), __uint_as_float(r[c / 16][2 * c % 32 + 1])), ff, acc[c]);
             }
             if (!ok) break;
             if (direct && row0 + HALF <= p.out) {
@@ -213,7 +253,7 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 }
                 continue;
             }
-            // Others through shared memory, 32 columns at a time: [token][16-byte piece turned by the token], then eight lanes a token.
+            // Others through shared memory, 16 columns at a time: [token][16-byte piece turned by the token], then four lanes a token.
 #pragma unroll
             for (int c0 = 0; c0 < HALF; c0 += OUT_COLS) {
                 __syncwarp();
@@ -222,13 +262,13 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                     float4 v;
                     unpack2(acc[c0 / 2 + 2 * j], v.x, v.y);
                     unpack2(acc[c0 / 2 + 2 * j + 1], v.z, v.w);
-                    *reinterpret_cast<float4*>(out + lane * OUT_COLS + ((j ^ (lane & 7)) << 2)) = v;
+                    *reinterpret_cast<float4*>(out + lane * OUT_COLS + ((j ^ ((lane >> 1) & 3)) << 2)) = v;
                 }
                 __syncwarp();
-                const int o = row0 + c0 + (lane & 7) * 4;
+                const int o = row0 + c0 + (lane & 3) * 4;
 #pragma unroll 2
-                for (int t = lane >> 3; t < min(32, p.n - token0); t += 4)
-                    linear8_store(p, token0 + t, o, *reinterpret_cast<const float4*>(out + t * OUT_COLS + (((lane & 7) ^ (t & 7)) << 2)), quads, y32);
+                for (int t = lane >> 2; t < min(32, p.n - token0); t += 8)
+                    linear8_store(p, token0 + t, o, *reinterpret_cast<const float4*>(out + t * OUT_COLS + (((lane & 3) ^ ((t >> 1) & 3)) << 2)), quads, y32);
             }
         }
     }
@@ -237,7 +277,7 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     cluster_sync();                                          // neither block leaves while the other may still touch it
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(SLOTS * STEP * BN) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(SLOTS * BN) : "memory");
     }
 }
 
@@ -253,7 +293,6 @@ int linear8_many(const Linear8& p, cudaStream_t stream) {
     Args a;
     a.p = p;
     a.groups = (p.K + KB - 1) / KB;
-    a.steps = (a.groups + STEP - 1) / STEP;
     a.row_blocks = (p.out + E4M3_BLOCK - 1) / E4M3_BLOCK;
     a.token_tiles = (p.n + 2 * BM - 1) / (2 * BM);
     const long long tiles = (long long)a.token_tiles * ((p.out + BN - 1) / BN);

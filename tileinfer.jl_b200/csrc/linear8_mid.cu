@@ -150,34 +150,30 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_mid_kernel(const __grid_co
 #pragma unroll
         for (int c = 0; c < H; ++c) sums[(first + c) * ROWS] = acc[c];
     } else {
-        // ---------------------------------------------------------------- the factors, two groups ahead
+        // ---------------------------------------------------------------- the factors, LOADS groups ahead, multiplied when they are wanted (a product at once would
+        // wait for its loads)
         pdl_enter();
-        constexpr int V = N / 32;
+        constexpr int V = N / 32, LOADS = 4;
         int stage = 0, place = 0;
         unsigned phase = 0;
-        float f[2][V];
-        auto load = [&](int g, float (&to)[V]) {
-            const float sw = g < hi ? __ldg(p.scales + (long long)g * a.row_tiles + tile) : 0.f;
+        float sx[LOADS][V], sw[LOADS];
+        auto ask = [&](int g, float (&x)[V], float& w) {
+            if (g >= hi) return;
+            w = __ldg(p.scales + (long long)g * a.row_tiles + tile);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int t = token0 + lane + 32 * i;
-                to[i] = g < hi && t < p.n ? __ldcg(p.x_scales + (long long)g * p.n + t) * sw : 0.f;
-            }
+            for (int i = 0; i < V; ++i) x[i] = __ldcg(p.x_scales + (long long)g * p.n + min(token0 + lane + 32 * i, p.n - 1));
         };
-        load(lo, f[0]);
-        load(lo + 1, f[1]);
-        for (int g0 = lo; ok && g0 < hi; g0 += 2) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < LOADS; ++j) ask(lo + j, sx[j], sw[j]);
+        for (int g0 = lo; ok && g0 < hi; g0 += LOADS) {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
                 if (g0 + j >= hi) break;
-                float now[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) now[i] = f[j][i];
-                load(g0 + j + 2, f[j]);
                 ok = warp_wait(empty0 + 8 * stage, phase ^ 1, p.status, 23);
                 if (!ok) break;
 #pragma unroll
-                for (int i = 0; i < V; ++i) s_factor[place][lane + 32 * i] = now[i];
+                for (int i = 0; i < V; ++i) s_factor[place][lane + 32 * i] = sx[j][i] * sw[j];
+                ask(g0 + j + LOADS, sx[j], sw[j]);
                 __syncwarp();
                 // The group's MMAs wait for this too: were they ahead, the stage could be emptied again before the wait above has seen it emptied once.
                 if (lane == 0) { mbar_arrive(full0 + 8 * stage); mbar_arrive(fac0 + 8 * place); }
