@@ -6,13 +6,12 @@ extern "C" int ti_quantize8(void* codes, void* scales, const void* x, long long 
 static long long up16(long long bytes) { return (bytes + 15) / 16 * 16; }
 
 // Weight rows in the lanes, 64 tokens at once (linear8_mid.cu), or tokens in the lanes on SM pairs (linear8_many.cu): the shorter by estimates in microseconds. The
-// one takes half of one for every 128 x 64 x 128 that an SM gets, the other 0.75 for every step of 256 of k of a pair's tiles, rounds of which are whole.
-// Microseconds in turn: 64 tokens of 21,504 x 4,096 29 / 38, 256 81 / 41, 2,048 502 / 210; 128 of 4,096 x 21,504 40 / 72, 512 129 / 78; 256 of 4,096 x 4,096
-// 16.2 / 15.8.
+// one takes half of one for every 128 x 64 x 128 that an SM gets, the other 0.65 for every step of 256 of k of a pair's tiles, rounds of which are whole.
+// Microseconds in turn: 64 tokens of 21,504 x 4,096 26 / 38, 256 78 / 39; 128 of 4,096 x 21,504 36 / 57, 256 70 / 57; 256 of 4,096 x 4,096 16 / 15.5.
 static bool takes_many(int n, int out, int K) {
     const double groups = (K + 127) / 128, units = (double)((out + 127) / 128) * ((n + 63) / 64) * groups;
     const long long tiles = (long long)((out + 127) / 128) * ((n + 255) / 256), pairs = ti_sm_count() / 2, rounds = (tiles + pairs - 1) / pairs;
-    return 3.0 + rounds * (1.0 + 0.75 * ((groups + 1) / 2)) < 5.0 + 0.5 * units / ti_sm_count();
+    return 3.0 + rounds * (1.0 + 0.65 * ((groups + 1) / 2)) < 5.0 + 0.5 * units / ti_sm_count();
 }
 
 // Tokens that come as bfloat16 are quantised by every block that needs them where they are few, else by a launch of its own ahead (1.5 us more): 21,504 x

@@ -6,8 +6,11 @@
 // receives its 128 tokens' sums. A step is two groups of 128 of k (48 KB a block); a group's sums stand in an accumulator of their own, and eight warps (two a
 // quarter of the lanes, 64 columns each) add them, times sx sw, to 32-bit sums in registers: a thread has a token, so that sx sw is one number a group.
 //
-// The tensor cores need 512 cycles a step. What it takes is the issuing warp's own instructions: two waits, eight MMAs and one commit, which frees the stage and
-// gives the accumulators over at once. With a step of one group and two commits, 256 tokens of 4,096 x 21,504 took 109 us.
+// Bound by the hand-overs: the tensor cores need 512 cycles a step and are busy for half of the time. A step takes the issuing warp about 800 cycles (its waits, eight
+// MMAs, one commit, which frees the stage and gives the sums over at once), the adding warps about 1,000. What took the longest was found by reading the clock in every
+// warp: a factor multiplied as soon as it was asked for (the adding warps waited for its loads; now a warp of its own brings factors), and waits for barriers that
+// were over long since, 300 cycles each beside the MMAs (now asked one step ahead). 256 tokens of 4,096 x 21,504 69.6 -> 57.1 us, 2,048 of 21,504 x 4,096
+// 225 -> 198 us, 1,820 TFLOP/s (at cold clocks; both sides on the same machine). Tiles of 256 x 256 took the same time for the same work, sixteen adding warps 7 % more.
 //
 // Block 0 of the pair issues the MMAs; its `full` barriers count the bytes of both blocks' loads; commits arrive on both blocks' barriers; the partner's
 // warps arrive on block 0's accumulator barriers. All waits are bounded.
@@ -18,16 +21,16 @@ namespace {
 using namespace tc;
 
 constexpr int BM = 128, BN = 128, KB = 128, HALF = BN / 2, EPI_WARPS = 8, THREADS = 96 + 32 * EPI_WARPS;
-constexpr int A_BYTES = BM * KB, B_BYTES = BN / 2 * KB, STAGE = A_BYTES + B_BYTES;
-constexpr int STAGES = 8, SLOTS = 4;                         // of operands; of sums
-constexpr int AHEAD = STAGES - SLOTS;                        // groups whose factors are brought before their products are there
+constexpr int A_BYTES = BM * KB, B_BYTES = BN / 2 * KB, STEP = 2, STAGE = STEP * (A_BYTES + B_BYTES);
+constexpr int STAGES = 4, SLOTS = 2;                         // of operands; of sums: a step's
+constexpr int AHEAD = STAGES - SLOTS;                        // steps whose factors are brought before their products are there
 constexpr int OUT_COLS = 16, OUT = 32 * OUT_COLS * 4;        // a warp's results on their way out
 constexpr int BYTES = STAGES * STAGE + EPI_WARPS * OUT + 1024;
-static_assert(BYTES + STAGES * BM * 4 <= 226 * 1024 && SLOTS * BN <= 512, "shared and tensor memory");
+static_assert(BYTES + STAGES * STEP * BM * 4 <= 226 * 1024 && SLOTS * STEP * BN <= 512, "shared and tensor memory");
 
 struct Args {
     Linear8 p;
-    int groups, row_blocks, token_tiles, tiles;              // row_blocks: of 128 weight rows, as scales have them
+    int groups, steps, row_blocks, token_tiles, tiles;              // row_blocks: of 128 weight rows, as scales have them
 };
 
 __device__ __forceinline__ unsigned cluster_rank() {
@@ -72,7 +75,7 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     unsigned char* tiles = smem_dyn + ((1024u - (smem_addr(smem_dyn) & 1023u)) & 1023u);
     __shared__ __align__(8) unsigned long long bars[2 * STAGES + SLOTS];
     __shared__ unsigned s_tmem;
-    __shared__ float s_factor[STAGES][BM];
+    __shared__ float s_factor[STAGES][STEP][BM];
     // done: a stage has been read, its sums are complete and their factors there.
     const unsigned full0 = smem_addr(bars), done0 = full0 + 8 * STAGES, free0 = done0 + 8 * STAGES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -83,7 +86,7 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(SLOTS * BN) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(SLOTS * STEP * BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -102,7 +105,7 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         bool ready = true;                                   // every stage is free at first
         for (int tile = pair; lane == 0 && ok && tile < a.tiles; tile += pairs) {
             const int token = tile % a.token_tiles * (2 * BM) + rank * BM, row = tile / a.token_tiles * BN + rank * (BN / 2);
-            for (int g = 0; g < a.groups; ++g) {
+            for (int step = 0; step < a.steps; ++step) {
                 if (!ready) ok = mbar_wait(done0 + 8 * stage, phase ^ 1, p.status, 24);
                 if (!ok) break;
                 const int next = stage + 1 == STAGES ? 0 : stage + 1;
@@ -110,8 +113,11 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 ready = mbar_test(done0 + 8 * next, next_phase ^ 1, true);
                 if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2 * STAGE);
                 const unsigned bar = in_block0(full0 + 8 * stage), to = smem_addr(tiles + stage * STAGE);
-                load_pair(to, &map_x, g * (KB / 2), token, bar);
-                load_pair(to + A_BYTES, &map_w, g * (KB / 2), row, bar);
+#pragma unroll
+                for (int i = 0; i < STEP; ++i) {             // beyond the last group: zeros
+                    load_pair(to + i * A_BYTES, &map_x, (step * STEP + i) * (KB / 2), token, bar);
+                    load_pair(to + STEP * A_BYTES + i * B_BYTES, &map_w, (step * STEP + i) * (KB / 2), row, bar);
+                }
                 stage = next;
                 phase = next_phase;
             }
@@ -127,50 +133,57 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             const bool asks = lane < 2;
             bool ready = false;
             for (int tile = pair; ok && tile < a.tiles; tile += pairs)
-                for (int g = 0; g < a.groups; ++g) {
+                for (int step = 0; step < a.steps; ++step) {
                     ok = warp_wait_after(ready, lane ? free0 + 8 * slot : full0 + 8 * stage, lane ? slot_phase ^ 1 : phase, asks, p.status, 25);
                     if (!ok) break;
                     tc_fence_after();
-                    const unsigned long long dx = first + (unsigned)(stage * (STAGE >> 4)), dw = dx + (A_BYTES >> 4);
-                    const unsigned to = tmem + slot * BN, done = done0 + 8 * stage;
+                    const unsigned long long dx = first + (unsigned)(stage * (STAGE >> 4)), dw = dx + (STEP * A_BYTES >> 4);
+                    const unsigned to = tmem + slot * (STEP * BN), done = done0 + 8 * stage;
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                     if (++slot == SLOTS) { slot = 0; slot_phase ^= 1; }
                     ready = mbar_test(lane ? free0 + 8 * slot : full0 + 8 * stage, lane ? slot_phase ^ 1 : phase, asks);
                     if (elected()) {
 #pragma unroll
-                        for (int k = 0; k < KB / 32; ++k) mma_pair(to, dx + 2 * k, dw + 2 * k, IDESC, k > 0);
+                        for (int i = 0; i < STEP; ++i)
+#pragma unroll
+                            for (int k = 0; k < KB / 32; ++k) mma_pair(to + i * BN, dx + i * (A_BYTES >> 4) + 2 * k, dw + i * (B_BYTES >> 4) + 2 * k, IDESC, k > 0);
                         commit_pair(done);
                     }
                     __syncwarp();
                 }
         }
     } else if (warp == 2) {
-        // ---------------------------------------------------------------- the factors sx sw of the block's tokens, LOADS groups ahead in registers (multiplied when
-        // they are wanted: a product at once would wait for its loads, 1,600 cycles a group in all), then AHEAD in shared memory: a place is written again
-        // when the products AHEAD groups before are there, whose accumulator had been read before
-        constexpr int LOADS = 4, V = BM / 32;
-        int next_tile = pair, next_g = 0, at[V];
-        float sx[LOADS][V], sw[LOADS];
+        // ---------------------------------------------------------------- the factors sx sw of the block's tokens, LOADS steps ahead in registers (multiplied when they
+        // are wanted: a product at once would wait for its loads), then AHEAD in shared memory: a place is written again when the products AHEAD steps before are
+        // there, for which the sums of STAGES steps before had to have been read
+        constexpr int LOADS = 2, V = BM / 32;
+        int next_tile = pair, next_step = 0, at[V];
+        float sx[LOADS][STEP][V], sw[LOADS][STEP];
         const float *from = nullptr, *from_w = nullptr;
-        auto ask = [&](float (&x)[V], float& w) {
+        auto ask = [&](float (&x)[STEP][V], float (&w)[STEP]) {
             if (next_tile >= a.tiles) return;
-            if (next_g == 0) {
+            if (next_step == 0) {
                 const int token0 = next_tile % a.token_tiles * (2 * BM) + rank * BM + lane;
 #pragma unroll
                 for (int i = 0; i < V; ++i) at[i] = min(token0 + 32 * i, p.n - 1);
                 from = p.x_scales;
                 from_w = p.scales + next_tile / a.token_tiles;
             }
-            w = __ldg(from_w);
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[i] = __ldcg(from + at[i]);
-            from += p.n;
-            from_w += a.row_blocks;
-            if (++next_g == a.groups) { next_g = 0; next_tile += pairs; }
+            for (int j = 0; j < STEP; ++j) {
+                const bool there = next_step * STEP + j < a.groups;              // products beyond the last group are zeros
+                w[j] = there ? __ldg(from_w) : 0.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[j][i] = there ? __ldcg(from + at[i]) : 0.f;
+                if (!there) continue;
+                from += p.n;
+                from_w += a.row_blocks;
+            }
+            if (++next_step == a.steps) { next_step = 0; next_tile += pairs; }
         };
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) ask(sx[j], sw[j]);
-        const long long all = (long long)((a.tiles - pair + pairs - 1) / pairs) * a.groups;
+        const long long all = (long long)((a.tiles - pair + pairs - 1) / pairs) * a.steps;
         int place = 0, behind = STAGES - AHEAD;
         unsigned phase = 1;
         bool ready = true;
@@ -183,7 +196,9 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 if (++behind == STAGES) { behind = 0; phase ^= 1; }
                 ready = mbar_test(done0 + 8 * behind, phase, lane == 0);
 #pragma unroll
-                for (int i = 0; i < V; ++i) s_factor[place][lane + 32 * i] = sx[j][i] * sw[j];
+                for (int h = 0; h < STEP; ++h)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) s_factor[place][h][lane + 32 * i] = sx[j][h][i] * sw[j][h];
                 ask(sx[j], sw[j]);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(done0 + 8 * place);
@@ -207,25 +222,30 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             f32x2 acc[HALF / 2];
 #pragma unroll
             for (int c = 0; c < HALF / 2; ++c) acc[c] = 0ull;
-            for (int g = 0; g < a.groups; ++g) {
+            for (int step = 0; step < a.steps; ++step) {
                 ok = warp_wait_after(ready, done0 + 8 * stage, phase, lane == 0, p.status, 27);
                 if (!ok) break;
                 tc_fence_after();
-                unsigned r[2][32];
-                tmem_ld32(columns + slot * BN, r[0]);
-                tmem_ld32(columns + slot * BN + 32, r[1]);
-                const float f = s_factor[stage][quarter * 32 + lane];
-                tmem_ld_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) arrive_block0(release0 + 8 * slot);
-                if (++slot == SLOTS) slot = 0;
-                if (++stage == STAGES) { stage = 0; phase ^= 1; }
-                ready = mbar_test(done0 + 8 * stage, phase, lane == 0);
-                const f32x2 ff = pack2(f, f);
 #pragma unroll
-                for (int c = 0; c < HALF / 2; ++c)
-                    acc[c] = fma2(pack2(__uint_as_float(r[c / 16][2 * c % 32]), __uint_as_float(r[c / 16][2 * c % 32 + 1])), ff, acc[c]);
+                for (int i = 0; i < STEP; ++i) {
+                    unsigned r[2][32];
+                    tmem_ld32(columns + (slot * STEP + i) * BN, r[0]);
+                    tmem_ld32(columns + (slot * STEP + i) * BN + 32, r[1]);
+                    float f = s_factor[stage][i][quarter * 32 + lane];
+                    tmem_ld_wait();
+                    if (i == STEP - 1) {
+                        tc_fence_before();
+                        f = __shfl_sync(0xffffffffu, f, lane);               // every lane's factor has been read, too, when lane 0 gives step and factors back
+                        if (lane == 0) arrive_block0(release0 + 8 * slot);
+                        if (++slot == SLOTS) slot = 0;
+                        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                        ready = mbar_test(done0 + 8 * stage, phase, lane == 0);
+                    }
+                    const f32x2 ff = pack2(f, f);
+#pragma unroll
+                    for (int c = 0; c < HALF / 2; ++c)
+                        acc[c] = fma2(pack2(__uint_as_float(r[c / 16][2 * c % 32]), __uint_as_float(r[c / 16][2 * c % 32 + 1])), ff, acc[c]);
+                }
             }
             if (!ok) break;
             if (direct && row0 + HALF <= p.out) {
@@ -277,7 +297,7 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     cluster_sync();                                          // neither block leaves while the other may still touch it
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(SLOTS * BN) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(SLOTS * STEP * BN) : "memory");
     }
 }
 
@@ -293,6 +313,7 @@ int linear8_many(const Linear8& p, cudaStream_t stream) {
     Args a;
     a.p = p;
     a.groups = (p.K + KB - 1) / KB;
+    a.steps = (a.groups + STEP - 1) / STEP;
     a.row_blocks = (p.out + E4M3_BLOCK - 1) / E4M3_BLOCK;
     a.token_tiles = (p.n + 2 * BM - 1) / (2 * BM);
     const long long tiles = (long long)a.token_tiles * ((p.out + BN - 1) / BN);

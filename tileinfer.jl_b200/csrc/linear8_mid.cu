@@ -1,4 +1,4 @@
-// Products of e4m3 codes for some tens to a few hundred tokens: the weight rows in the lanes of tcgen05.mma.
+// Products of e4m3 codes for nine to some hundred tokens: the weight rows in the lanes of tcgen05.mma.
 //
 //   y[t, o] = sum_g sx[g, t] sw[g, o / 128] sum_{k in g} cx[t, k] cw[o, k]
 //
@@ -6,6 +6,10 @@
 // tensor memory, from where eight warps (two a quarter of the lanes, half of the columns each) add it, times sx sw, to 32-bit sums in registers. The blocks that
 // share 128 rows stand in one cluster, each with its stretch of k; their sums meet in the cluster's shared memory and are added in rank order: one
 // launch, no work space for parts.
+//
+// Bound by reading the weights, 16 KB of them a group: 16 tokens of 21,504 x 4,096 take 22.9 us with their quantisation, 64 take 26.0 (88 MB, 13.5 us at the rate of a
+// copy; 18 us of it the weights' own stream, the rest launches, the fill and the cluster's sums). Four groups' factors are on their way at once: multiplied as they
+// came, they cost a group the latency of its loads (26.1 and 28.2 us).
 //
 // Warp 0 asks for weights and tokens (TMA), warp 1 issues the MMAs, warps 2 to 9 add, warp 10 brings the factors sx sw. All waits are bounded.
 #include "linear8.cuh"
