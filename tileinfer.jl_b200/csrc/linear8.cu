@@ -14,9 +14,9 @@ static bool takes_many(int n, int out, int K) {
     return 3.0 + rounds * (1.0 + 0.65 * ((groups + 1) / 2)) < 5.0 + 0.5 * units / ti_sm_count();
 }
 
-// Tokens that come as bfloat16 are quantised by every block that needs them where they are few, else by a launch of its own ahead (1.5 us more): 21,504 x
-// 4,096 takes 20.9 us for one token, 23.0 for four, 26.9 for eight in one launch; 21.3 for eight whose codes are given.
-static bool quantized_ahead(int n, int out, int K) { return n > 4 || !linear8_takes_few(n, out, K); }
+// Tokens that come as bfloat16 are quantised by every block that needs them where they are few, else by a launch of its own ahead. Microseconds ahead / in the
+// blocks: eight tokens of 1,024 x 1,024 5.2 / 4.0, 4,096 x 4,096 9.0 / 7.8, 14,336 x 4,096 16.0 / 16.3, 21,504 x 4,096 22.9 / 26.9; four of that 24.5 / 23.2.
+static bool quantized_ahead(int n, int out, int K) { return !linear8_takes_few(n, out, K) || (n > 4 && (long long)out * K > 48000000); }
 
 // Bytes of the work space: the tokens' codes and scales, where they are made ahead.
 extern "C" long long ti_linear8_workspace(int n, int out, int K, int given) {
