@@ -41,8 +41,9 @@ def test_linear8_work_space(n):
     """Nothing for tokens that come as codes, or that are few; else what their codes and scales take."""
     need = library.lib().ti_linear8_workspace
     assert need(n, 4096, 4096, 1) == 0
-    assert need(n, 4096, 4096, 0) == (0 if n <= 4 else n * 4096 + n * 32 * 4)
-    assert need(n, 4096, 400, 0) == (0 if n <= 4 else -(-n * 400 // 16) * 16 + -(-n * 16 // 16) * 16)
+    assert need(n, 4096, 4096, 0) == (0 if n <= 8 else n * 4096 + n * 32 * 4)
+    assert need(n, 4096, 400, 0) == (0 if n <= 8 else -(-n * 400 // 16) * 16 + -(-n * 16 // 16) * 16)
+    assert need(n, 21504, 4096, 0) == (0 if n <= 4 else n * 4096 + n * 32 * 4)
 
 
 def write(k_codes=AT, v_codes=AT, k=AT, v=AT, page_size=64, dim=128, max_new=1, seqs=4, dtype=1, pages=100):
@@ -54,3 +55,22 @@ def write(k_codes=AT, v_codes=AT, k=AT, v=AT, page_size=64, dim=128, max_new=1, 
                                               (dict(max_new=2 ** 31 - 1, seqs=2 ** 20), "too many", 1), (dict(dtype=7), "element type", 1), (dict(pages=0), "sequences", 1)])
 def test_cache_write8(change, word, code):
     refused(write(**change), word, code=code)
+
+
+def attention(out=AT, q=AT, k=AT, v=AT, ws=AT, ws_bytes=1 << 40, status=AT, scale=0.1, seqs=4, n=4, nq=8, nkv=2, dim=64, page_size=64, max_new=1, max_len=1000, pages=100,
+              window=0, table_stride=16):
+    return library.lib().ti_attention8(out, q, k, v, AT, AT, AT, table_stride, AT, AT, AT, ws, ws_bytes, status, scale, seqs, n, nq, nkv, dim, page_size, max_new, max_len, pages,
+                                       window, None)
+
+
+@pytest.mark.parametrize("change,word,code", [(dict(k=AT + 8), "16-byte", 1), (dict(v=AT + 8), "16-byte", 1), (dict(q=AT + 2), "4-byte", 1), (dict(out=AT + 2), "4-byte", 1),
+                                              (dict(ws=None), "work space", 1), (dict(ws=AT + 8), "work space", 1), (dict(status=None), "16-byte", 1), (dict(scale=0.0), "scale", 1),
+                                              (dict(scale=-1.0), "scale", 1), (dict(seqs=-1), "sequences", 1), (dict(window=-1), "sequences", 1), (dict(pages=0), "sequences", 1),
+                                              (dict(page_size=32), "pages of 64", 2), (dict(dim=24), "multiple of 16", 2), (dict(dim=272), "multiple of 16", 2),
+                                              (dict(nq=9), "heads", 2), (dict(pages=2 ** 26, nkv=2), "2^31 rows", 2), (dict(table_stride=2 ** 30, seqs=8), "2^31 tiles", 2)])
+def test_attention8(change, word, code):
+    refused(attention(**change), word, code=code)
+
+
+def test_attention8_without_work():
+    assert attention(seqs=0) == 0 and attention(n=0) == 0 and attention(max_new=0) == 0
