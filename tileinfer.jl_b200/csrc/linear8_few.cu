@@ -10,6 +10,9 @@
 // operands are permuted alike, so that a lane's 32 consecutive codes of a row are its share of eight MMAs. The tokens' codes of the block's stretch
 // of k lie in shared memory, made from bfloat16 (or copied, where they are given) while the first weights are coming. A row's 16-byte pieces are turned by the
 // row (the token), so that the reads of a warp meet all banks.
+//
+// Bound by reading the weights: one token of 21,504 x 4,096 takes 20.9 us (88 MB, 4.2 TB/s: about 5 us are launch, the first reads and the cluster's sums), of
+// 131,072 x 4,096 90.5 (5.9 TB/s). A copy reads 6.5 TB/s.
 #include "linear8.cuh"
 #include "mma_util.cuh"
 

