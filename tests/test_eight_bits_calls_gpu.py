@@ -1,0 +1,156 @@
+"""The 8-bit operators as programs call them: together, from several threads, counted, with tables and lengths that are wrong."""
+import threading
+
+import pytest
+import torch
+
+from numbers8 import E4M3, F64, PAGE
+from test_attention8_gpu import make, reference
+from test_drafting_launches_gpu import kernels
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from tileinfer_b200.kernels import ops
+    return ops
+
+
+def product(ops, n, out, k, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    w, x = torch.randn(out, k, generator=g).bfloat16().cuda(), torch.randn(n, k, generator=g).bfloat16().cuda()
+    codes, scales = torch.empty(out, k, dtype=torch.uint8, device="cuda").view(E4M3), torch.empty(-(-k // 128), -(-out // 128), device="cuda")
+    ops.quantize8(codes, scales, w, 128)
+    y = torch.empty(n, out, dtype=torch.bfloat16, device="cuda")
+    return lambda: ops.linear8(y, x, codes, scales), y
+
+
+def attention(ops, runs, nq=8, nkv=2, dim=64, seed=0, **kw):
+    c = make(runs, nq, nkv, dim, seed=seed)
+    d = {key: t.cuda() for key, t in c.items()}
+    out = torch.empty(c["q"].shape[0], nq * dim, dtype=torch.bfloat16, device="cuda")
+    new = max(t for t, _ in runs)
+    return lambda: ops.attention8(out, d["q"], d["k"], d["v"], d["ks"], d["vs"], d["table"], d["seq_slots"], d["cu"], d["lens"], dim ** -0.5, nq, nkv, dim, PAGE, new, **kw), out
+
+
+CASES = {"few": lambda ops, s: product(ops, 3 + s, 640, 512, s), "mid": lambda ops, s: product(ops, 10 + s, 640, 512, s), "many": lambda ops, s: product(ops, 700 + s, 4096, 512, s),
+         "short": lambda ops, s: attention(ops, [(1, 900 + s), (2, 5000), (1, 64)], seed=s), "long": lambda ops, s: attention(ops, [(400 + s, 900), (300, 300)], 16, seed=s)}
+
+
+@pytest.mark.parametrize("kind", CASES)
+def test_two_threads_on_one_stream(ops, kind):
+    cases = [CASES[kind](ops, seed) for seed in (1, 2, 3)]
+    want = []
+    for call, out in cases:
+        call()
+        want.append(out.clone())
+    wrong, start = [], threading.Barrier(len(cases))
+
+    def work(i):
+        call, out = cases[i]
+        start.wait()
+        for _ in range(20):
+            seen = []
+            for _ in range(10):
+                call()
+                seen.append(out.clone())
+            wrong.extend(i for got in seen if not torch.equal(got, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == []
+
+
+@pytest.mark.parametrize("n", [1, 4, 5, 8, 9, 64, 300, 2000])
+@pytest.mark.parametrize("out,k", [(256, 512), (14336, 4096)])
+def test_launches_of_products(ops, n, out, k):
+    found, counted = kernels(product(ops, n, out, k)[0])
+    assert found == counted and found in (1, 2)
+
+
+@pytest.mark.parametrize("runs,nq", [([(1, 70)], 8), ([(1, 70)] * 256, 8), ([(1, 70)] * 257, 8), ([(2, 70)] * 1100, 8), ([(500, 700)], 16), ([(70, 70)] * 300, 16), ([(0, 70), (3, 3)], 8)])
+def test_launches_of_attention(ops, runs, nq):
+    found, counted = kernels(attention(ops, runs, nq)[0])
+    assert found == counted
+
+
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 500), (128, 500)])
+def test_launches_of_the_others(ops, rows, n):
+    x = torch.zeros(n, 256, device="cuda")
+    codes, scales = torch.empty(n, 256, dtype=torch.uint8, device="cuda").view(E4M3), torch.empty(2, -(-n // rows), device="cuda")
+    found, counted = kernels(lambda: ops.quantize8(codes, scales, x, rows))
+    assert found == counted == 1
+    c = make([(3, 100), (1, 5)], 4, 2, 64)
+    d = {key: t.cuda() for key, t in c.items()}
+    new = torch.zeros(4, 2, 64, dtype=torch.bfloat16, device="cuda")
+    found, counted = kernels(lambda: ops.cache_write8(d["k"], d["v"], d["ks"], d["vs"], new, new, d["table"], d["seq_slots"], d["cu"], d["lens"], 3))
+    assert found == counted == 1
+
+
+@pytest.mark.parametrize("runs,nq,longest", [([(1, 500), (2, 700), (1, 300)], 8, None), ([(200, 500), (300, 700), (100, 300)], 16, 700)])
+@pytest.mark.parametrize("bad", [-1, 2 ** 31 - 1, 10 ** 6])
+def test_pages_that_do_not_exist(ops, runs, nq, longest, bad):
+    """A sequence whose table names none gets something; nothing else is read or written, and the others get what they should."""
+    dim, nkv, new = 64, 2, max(t for t, _ in runs)
+    c = make(runs, nq, nkv, dim, seed=11)
+    want, bound = reference(c, dim ** -0.5, 0, 8)
+    c["table"][c["seq_slots"][1], 3] = bad
+    c["table"][c["seq_slots"][1], 9] = bad
+    d = {key: t.cuda() for key, t in c.items()}
+    out = torch.full((c["q"].shape[0] + 1, nq * dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.attention8(out[:-1], d["q"], d["k"], d["v"], d["ks"], d["vs"], d["table"], d["seq_slots"], d["cu"], d["lens"], dim ** -0.5, nq, nkv, dim, PAGE, new, max_len=longest)
+    off = (out[:-1].cpu().to(F64) - want).abs()
+    first, end = int(c["cu"][1]), int(c["cu"][2])
+    right = (off <= bound).all(-1)
+    assert bool(right[:first].all()) and bool(right[end:].all()) and bool((out[-1] == 7).all())
+    ops.check_status()
+
+
+@pytest.mark.parametrize("new", [1, 4, 200])
+def test_writing_and_reading_in_turn_on_another_stream(ops, new):
+    """Rows go into the cache and are read in the same step, step after step, without a wait of the host; then the same steps captured."""
+    nq, nkv, dim, steps = 8, 2, 64, 6
+    seqs, longest = 3, 64 + new * steps
+    pages = -(-longest // PAGE)
+    g = torch.Generator().manual_seed(new)
+    table = torch.randperm(seqs * pages, generator=g).to(torch.int32).view(seqs, pages).cuda()
+    slots, cu = torch.arange(seqs, dtype=torch.int32).cuda(), (torch.arange(seqs + 1) * new).to(torch.int32).cuda()
+    lens = [torch.tensor([new * (i + 1)] * seqs, dtype=torch.int32).cuda() for i in range(steps)]
+    k, v = (torch.randn(steps, seqs * new, nkv, dim, generator=g).bfloat16().cuda() for _ in range(2))
+    q = torch.randn(steps, seqs * new, nq, dim, generator=g).bfloat16().cuda()
+
+    def run(pools, out):
+        kc, vc, ks, vs = pools
+        for i in range(steps):
+            ops.cache_write8(kc, vc, ks, vs, k[i], v[i], table, slots, cu, lens[i], new)
+            ops.attention8(out[i], q[i], kc, vc, ks, vs, table, slots, cu, lens[i], dim ** -0.5, nq, nkv, dim, PAGE, new)
+
+    def fresh():
+        kc, vc = (torch.full((seqs * pages, nkv, PAGE, dim), 0x7F, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+        return kc, vc, torch.full((seqs * pages, nkv), 3.0, device="cuda"), torch.full((seqs * pages, nkv), 3.0, device="cuda")
+
+    results = []
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        pools, out = fresh(), torch.empty(steps, seqs * new, nq * dim, dtype=torch.bfloat16, device="cuda")
+        run(pools, out)
+        results.append(out)
+        again, out = fresh(), torch.empty_like(out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            run(again, out)
+        for _ in range(2):                                    # the second time over its own pages: each is written from its first position on
+            graph.replay()
+        results.append(out)
+    torch.cuda.synchronize()
+    assert torch.equal(results[0], results[1])
+    # The last step against the definition, over the codes that stand now.
+    c = dict(q=q[-1].cpu(), k=pools[0].cpu(), v=pools[1].cpu(), ks=pools[2].cpu(), vs=pools[3].cpu(), table=table.cpu(), seq_slots=slots.cpu(), cu=cu.cpu(), lens=lens[-1].cpu())
+    want, bound = reference(c, dim ** -0.5, 0, 8)
+    off = (results[0][-1].cpu().to(F64) - want).abs()
+    assert bool((off <= bound).all())

@@ -1287,6 +1287,8 @@ def linear8_workspace(n: int, out_features: int, in_features: int, given: bool =
     key = (n, out_features, in_features, given)
     need = _linear8_need.get(key)
     if need is None:
+        if len(_linear8_need) >= 4096:
+            _linear8_need.clear()
         need = _linear8_need[key] = int(lib().ti_linear8_workspace(*key))
     return need
 
@@ -1382,6 +1384,8 @@ def attention8_workspace(seqs: int, max_new: int, nq: int, nkv: int, head_dim: i
     key = (seqs, max_new, nq, nkv, head_dim, max_len)
     need = _attention8_need.get(key)
     if need is None:
+        if len(_attention8_need) >= 4096:                    # every length of a served sequence is a key
+            _attention8_need.clear()
         need = _attention8_need[key] = int(lib().ti_attention8_workspace(*key))
     return need
 
