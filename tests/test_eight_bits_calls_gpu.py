@@ -154,3 +154,61 @@ def test_writing_and_reading_in_turn_on_another_stream(ops, new):
     want, bound = reference(c, dim ** -0.5, 0, 8)
     off = (results[0][-1].cpu().to(F64) - want).abs()
     assert bool((off <= bound).all())
+
+
+@pytest.mark.parametrize("n", [1, 8, 20, 300])
+def test_products_beyond_32_bits(ops, n):
+    """More than 2^31 codes: first and last rows against 64 bits."""
+    out, k = 140000, 16384
+    codes = torch.randint(0, 120, (out, k), dtype=torch.uint8, device="cuda").view(E4M3)
+    scales = torch.exp2(torch.randint(-9, -6, (k // 128, -(-out // 128)), device="cuda").float())
+    x, y = torch.randn(n, k, device="cuda").bfloat16(), torch.empty(n, out, dtype=torch.bfloat16, device="cuda")
+    made, x_scales = torch.empty(n, k, dtype=torch.uint8, device="cuda").view(E4M3), torch.empty(k // 128, n, device="cuda")
+    ops.quantize8(made, x_scales, x, 1)
+    ops.linear8(y, x, codes, scales)
+    wide = made.float().double() * x_scales.t().double().repeat_interleave(128, 1)
+    for rows in (slice(0, 64), slice(out - 64, out)):
+        w = codes[rows].float().double() * scales.t()[torch.arange(out, device="cuda")[rows] // 128].double().repeat_interleave(128, 1)
+        want = wide @ w.t()
+        # a 32-bit sum of 16,384 products, off by at most 2^-23 a step of their sizes, and one rounding to bfloat16
+        bound = wide.abs() @ w.abs().t() * 16384 * 2.0 ** -23 + want.abs() * 2.0 ** -8
+        assert bool(((y[:, rows].double() - want).abs() <= bound).all())
+
+
+def test_quantising_beyond_32_bits(ops):
+    n, k = 70000, 32768
+    x = torch.empty(n, k, dtype=torch.bfloat16, device="cuda").normal_()
+    codes = torch.empty(n, k, dtype=torch.uint8, device="cuda").view(E4M3)
+    for rows in (1, 128):
+        scales = torch.empty(k // 128, -(-n // rows), device="cuda")
+        ops.quantize8(codes, scales, x, rows)
+        few, some = torch.empty(112, k, dtype=torch.uint8, device="cuda").view(E4M3), torch.empty(k // 128, -(-112 // rows), device="cuda")
+        ops.quantize8(few, some, x[-112:], rows)              # 70,000 = 546 x 128 + 112
+        assert torch.equal(codes[-112:].view(torch.uint8), few.view(torch.uint8)) and torch.equal(scales[:, -some.shape[1]:], some)
+
+
+def test_a_cache_beyond_32_bits(ops):
+    """Pools of more than 2^32 bytes: a sequence whose pages are the first and the last ones."""
+    nq, nkv, dim, length = 16, 8, 128, 200
+    pages = 2 ** 32 // (nkv * PAGE * dim) + 50
+    pools = [torch.zeros(pages, nkv, PAGE, dim, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2)]
+    scales = [torch.ones(pages, nkv, device="cuda") for _ in range(2)]
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(length, nkv, dim, generator=g).bfloat16() for _ in range(2))
+    q = torch.randn(length, nq, dim, generator=g).bfloat16()
+    small = [torch.zeros(4, nkv, PAGE, dim, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2)], [torch.ones(4, nkv, device="cuda") for _ in range(2)]
+    outs = []
+    for (kc, vc), (ks, vs), order in ((pools, scales, [pages - 1, 0, pages - 2, 1]), (*small, [0, 1, 2, 3])):
+        table, slots = torch.tensor([order], dtype=torch.int32).cuda(), torch.zeros(1, dtype=torch.int32).cuda()
+        for new in (1, length):
+            cu, lens = torch.tensor([0, new], dtype=torch.int32).cuda(), torch.tensor([length], dtype=torch.int32).cuda()
+            out = torch.empty(new, nq * dim, dtype=torch.bfloat16, device="cuda")
+            if new == length:
+                ops.cache_write8(kc, vc, ks, vs, k.cuda(), v.cuda(), table, slots, cu, lens, new)
+            ops.attention8(out, q[-new:].cuda(), kc, vc, ks, vs, table, slots, cu, lens, dim ** -0.5, nq, nkv, dim, PAGE, new)
+            outs.append(out.cpu())
+        cu = torch.tensor([0, 1], dtype=torch.int32).cuda()
+        out = torch.empty(1, nq * dim, dtype=torch.bfloat16, device="cuda")
+        ops.attention8(out, q[-1:].cuda(), kc, vc, ks, vs, table, slots, cu, lens, dim ** -0.5, nq, nkv, dim, PAGE, 1)
+        outs.append(out.cpu())
+    assert bool(outs[1].abs().max() > 0) and all(torch.equal(a, b) for a, b in zip(outs[:3], outs[3:]))
