@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
     const unsigned char* ring = smem_dyn + warp * (AHEAD * UNIT);
     const unsigned ring_to = smem_u32(ring) + (lane >> 3) * KB;
     const unsigned char* rows[4];                            // a lane copies the same piece of every fourth row
+    float scale[AHEAD];                                      // of the groups on their way: a product with one asked for in its own group waits for the read
     auto enter = [&] {
 #pragma unroll
         for (int i = 0; i < 4; ++i) rows[i] = p.codes + (size_t)min(next_tile * ROWS + warp * 16 + 4 * i + (lane >> 3), p.out - 1) * p.K + (lane & 7) * 16;
@@ -72,10 +73,12 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
         if (next_tile < a.row_tiles) {
             const int k = next_group * KB;
             const bool there = k + (lane & 7) * 16 < p.K;
-            if (next_group < hi)
+            if (next_group < hi) {
+                scale[place] = __ldg(p.scales + (long long)next_group * a.row_tiles + next_tile);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     copy16(ring_to + place * UNIT + 4 * i * KB + (((lane & 7) ^ ((4 * i + (lane >> 3)) & 7)) << 4), there ? rows[i] + k : p.codes, there);
+            }
             if (++next_group == end) {
                 next_group = lo;
                 next_tile += stride;
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
                 __syncwarp();
                 const unsigned char* w = ring + i * UNIT + g * KB;
                 const unsigned char* x = x_row + (group - lo) * (N * KB);
-                const float sw = __ldg(p.scales + (long long)group * a.row_tiles + tile);
+                const float sw = scale[i];
                 float part[2][4] = {};                       // of the even and the odd pieces: two chains of MMAs
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
