@@ -3,7 +3,7 @@
 //   y[t, o] = sum_g sx[g, t] sw[g, o / 128] sum_{k in g} cx[t, k] cw[o, k]
 //
 // Both operands' codes are widened to 16 bits in registers, which is exact (one instruction for two), and multiplied by mma.sync with 32-bit sums. A block of
-// eight warps takes 128 rows, sixteen a warp, and then further ones; where there are fewer rows than that keeps the device busy, the blocks of a cluster
+// up to eight warps takes sixteen rows a warp, and then further ones; where there are fewer rows than that keeps the device busy, the blocks of a cluster
 // take a stretch of k each, and their sums meet in the cluster's shared memory, added in rank order: one launch, no work space. A warp copies its rows' groups
 // (2 KB) to shared memory of its own, AHEAD of them in flight, and waits for no other warp. (With the codes kept in registers until they are used, a group took
 // as long as its reads from memory do: a warp has six counters for what it waits for, and the reads ahead shared them with everything else.) The k of both
@@ -11,18 +11,18 @@
 // of k lie in shared memory, made from bfloat16 (or copied, where they are given) while the first weights are coming. A row's 16-byte pieces are turned by the
 // row (the token), so that the reads of a warp meet all banks.
 //
-// Bound by reading the weights: one token of 21,504 x 4,096 takes 20.9 us (88 MB, 4.2 TB/s: about 5 us are launch, the first reads and the cluster's sums), of
-// 131,072 x 4,096 90.5 (5.9 TB/s). A copy reads 6.5 TB/s.
+// Bound by reading the weights: one token of 21,504 x 4,096 takes 18.1 us (88 MB, 4.9 TB/s; launch, first reads and the last blocks are some 5 us), of
+// 4,096 x 21,504 17.6, of 131,072 x 4,096 87 (6.2 TB/s). A copy reads 6.5 TB/s.
 #include "linear8.cuh"
 #include "mma_util.cuh"
 
 namespace {
 
-constexpr int N = 8, ROWS = 128, KB = 128, THREADS = 256, AHEAD = 4, UNIT = 16 * KB, RING = 8 * AHEAD * UNIT, MAX_SPLIT = 8, MAX_SMEM = 113 * 1024;  // two blocks an SM
+constexpr int N = 8, KB = 128, WARPS = 8, AHEAD = 4, UNIT = 16 * KB, MAX_SPLIT = 8, MAX_SMEM = 113 * 1024;         // WARPS: of a block at most; two blocks an SM
 
 struct Args {
     Linear8 p;
-    int groups, row_tiles, split;
+    int groups, row_tiles, row_blocks, split;                // row_blocks: of 128 rows, as scales have them
     bool vec;                                                // bfloat16 tokens in 16-byte pieces
 };
 
@@ -41,14 +41,15 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
-// Bytes of shared memory: the warps' rings, codes [groups][N][128], factors [groups][N], sums [N][128].
-int few_bytes(int groups) { return RING + groups * N * (KB + 4) + N * ROWS * 4; }
+// Bytes of shared memory: the warps' rings, codes [groups][N][128], factors [groups][N], sums [N][rows].
+int few_bytes(int groups, int warps) { return warps * AHEAD * UNIT + groups * N * (KB + 4) + N * 16 * warps * 4; }
 
 template <bool GIVEN>
-__global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * WARPS, 2) linear8_few_kernel(const Args a) {
     const Linear8& p = a.p;
     extern __shared__ __align__(128) unsigned char smem_dyn[];
-    unsigned char* smem = smem_dyn + RING;
+    const int threads = blockDim.x, ROWS = threads / 2;      // sixteen rows a warp
+    unsigned char* smem = smem_dyn + threads / 32 * (AHEAD * UNIT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % a.split, stride = gridDim.x / a.split;
     const int lo = (int)((long long)a.groups * rank / a.split), hi = (int)((long long)a.groups * (rank + 1) / a.split), own = hi - lo;
@@ -64,7 +65,9 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
     const unsigned ring_to = smem_u32(ring) + (lane >> 3) * KB;
     const unsigned char* rows[4];                            // a lane copies the same piece of every fourth row
     float scale[AHEAD];                                      // of the groups on their way: a product with one asked for in its own group waits for the read
+    int next_block = 0;
     auto enter = [&] {
+        next_block = min(next_tile * ROWS + warp * 16, p.out - 1) / E4M3_BLOCK;
 #pragma unroll
         for (int i = 0; i < 4; ++i) rows[i] = p.codes + (size_t)min(next_tile * ROWS + warp * 16 + 4 * i + (lane >> 3), p.out - 1) * p.K + (lane & 7) * 16;
     };
@@ -74,7 +77,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
             const int k = next_group * KB;
             const bool there = k + (lane & 7) * 16 < p.K;
             if (next_group < hi) {
-                scale[place] = __ldg(p.scales + (long long)next_group * a.row_tiles + next_tile);
+                scale[place] = __ldg(p.scales + (long long)next_group * a.row_blocks + next_block);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     copy16(ring_to + place * UNIT + 4 * i * KB + (((lane & 7) ^ ((4 * i + (lane >> 3)) & 7)) << 4), there ? rows[i] + k : p.codes, there);
@@ -94,29 +97,29 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
     // The tokens' codes and factors: eight lanes a token's group of codes, sixteen of bfloat16 numbers.
     if (GIVEN) {
         constexpr int BATCH = 6;
-        for (int e0 = threadIdx.x; e0 < own * N * 8; e0 += BATCH * THREADS) {
+        for (int e0 = threadIdx.x; e0 < own * N * 8; e0 += BATCH * threads) {
             uint4 v[BATCH];
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                const int e = e0 + i * THREADS, token = (e >> 3) % N, k = (lo + (e >> 3) / N) * KB + (e & 7) * 16;
+                const int e = e0 + i * threads, token = (e >> 3) % N, k = (lo + (e >> 3) / N) * KB + (e & 7) * 16;
                 v[i] = e < own * N * 8 && token < p.n && k < p.K ? __ldcg(reinterpret_cast<const uint4*>((const unsigned char*)p.x + (long long)token * p.ldx + k)) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                const int e = e0 + i * THREADS, token = (e >> 3) % N;
+                const int e = e0 + i * threads, token = (e >> 3) % N;
                 if (e < own * N * 8) *reinterpret_cast<uint4*>(smem + (e >> 3) * KB + (((e & 7) ^ token) << 4)) = v[i];
             }
         }
-        for (int e = threadIdx.x; e < own * N; e += THREADS) factors[e] = e % N < p.n ? __ldcg(p.x_scales + (long long)(lo + e / N) * p.n + e % N) : 0.f;
+        for (int e = threadIdx.x; e < own * N; e += threads) factors[e] = e % N < p.n ? __ldcg(p.x_scales + (long long)(lo + e / N) * p.n + e % N) : 0.f;
     } else {
         constexpr int BATCH = 4;
         const int piece = lane & 15, total = own * p.n;
-        for (int first = 2 * warp; first < total; first += BATCH * (THREADS / 16)) {         // the same for a warp's two halves: they exchange maxima
+        for (int first = 2 * warp; first < total; first += BATCH * (threads / 16)) {         // the same for a warp's two halves: they exchange maxima
             const int e0 = first + (lane >> 4);
             uint4 v[BATCH];
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                const int e = e0 + i * (THREADS / 16), token = e / own, k = (lo + e - token * own) * KB + piece * 8;
+                const int e = e0 + i * (threads / 16), token = e / own, k = (lo + e - token * own) * KB + piece * 8;
                 v[i] = make_uint4(0, 0, 0, 0);
                 if (e < total && k < p.K) {
                     const bf16* from = (const bf16*)p.x + (long long)token * p.ldx + k;
@@ -130,7 +133,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
             }
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                const int e = e0 + i * (THREADS / 16), token = e / own, group = e - token * own;
+                const int e = e0 + i * (threads / 16), token = e / own, group = e - token * own;
                 Vec16<bf16> x;
                 x.unpack(v[i]);
                 float m = largest8(x.v);
@@ -197,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
             continue;
         }
         cluster_sync();                                      // one tile a cluster
-        for (int e = rank * THREADS + threadIdx.x; e < p.n * (ROWS / 4); e += a.split * THREADS) {
+        for (int e = rank * threads + threadIdx.x; e < p.n * (ROWS / 4); e += a.split * threads) {
             float4 v[MAX_SPLIT];
 #pragma unroll
             for (int r = 0; r < MAX_SPLIT; ++r) v[r] = r < a.split ? cluster_read(sums + 4 * e, r) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -210,14 +213,15 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_few_kernel(const Args a) {
     }
 }
 
-template <bool GIVEN> int launch(const Linear8& p, int split, cudaStream_t stream) {
+template <bool GIVEN> int launch(const Linear8& p, int warps, int split, cudaStream_t stream) {
     Args a;
     a.p = p;
     a.groups = (p.K + KB - 1) / KB;
-    a.row_tiles = (p.out + ROWS - 1) / ROWS;
+    a.row_tiles = (p.out + 16 * warps - 1) / (16 * warps);
+    a.row_blocks = (p.out + E4M3_BLOCK - 1) / E4M3_BLOCK;
     a.split = split;
     a.vec = aligned16(p.x) && (p.n == 1 || p.ldx % 8 == 0);
-    const int bytes = few_bytes((a.groups + split - 1) / split);
+    const int bytes = few_bytes((a.groups + split - 1) / split, warps);
     static bool configured = false;
     if (!configured) {
         cudaError_t e = cudaFuncSetAttribute(linear8_few_kernel<GIVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
@@ -226,22 +230,39 @@ template <bool GIVEN> int launch(const Linear8& p, int split, cudaStream_t strea
     }
     // Clusters take one tile each; single blocks go on to further ones, so that a block's tokens are made once.
     const int slots = 2 * ti_sm_count(), blocks = split > 1 || a.row_tiles < slots ? a.row_tiles * split : slots;
-    linear8_launch(linear8_few_kernel<GIVEN>, dim3(blocks), THREADS, bytes, split, stream, a);
+    linear8_launch(linear8_few_kernel<GIVEN>, dim3(blocks), 32 * warps, bytes, split, stream, a);
     return ti_check_launch("linear8_few");
+}
+
+// Blocks of the cluster that shares a product's rows; 0 where the tokens' codes do not fit. As many as two blocks an SM have room for: 4,096 x 4,096 takes
+// 6.5 us with 8, 7.4 with 4, 10.2 with 2. Powers of two: clusters of 6 do not fill the device (6,144 x 4,096 8.2 us with 4, 13.0 with 6).
+int few_split(int out, int K, int warps) {
+    const int groups = (K + KB - 1) / KB, tiles = (out + 16 * warps - 1) / (16 * warps);
+    int split = 1;
+    while (split < MAX_SPLIT && 2 * split <= groups && (2LL * split * tiles <= 2 * ti_sm_count() || few_bytes((groups + split - 1) / split, warps) > MAX_SMEM)) split *= 2;
+    return few_bytes((groups + split - 1) / split, warps) > MAX_SMEM ? 0 : split;
+}
+// Groups of sixteen rows that the busiest SM reads.
+long long few_load(int out, int K, int warps) {
+    const int groups = (K + KB - 1) / KB, split = few_split(out, K, warps);
+    const long long blocks = (long long)((out + 16 * warps - 1) / (16 * warps)) * split, sms = ti_sm_count();
+    return split == 0 ? 1LL << 62 : (blocks + sms - 1) / sms * warps * ((groups + split - 1) / split);
+}
+// Warps of a block: eight, or the most that leave the busiest SM at least a fifth less to read (168 blocks of 128 rows leave 20 of 148 SMs two). Microseconds for
+// one and eight tokens with 8, 7, 6, 5: 21,504 x 4,096 19.9 / 22.5, 19.7 / 22.7, 18.1 / 21.2, 18.3 / 21.8 (6 is taken); 6,144 x 4,096 7.7 / 9.0, 7.5 / 9.7, 7.2 / 9.4 (6),
+// 9.7 / 14.1; 4,096 x 21,504 17.6 / 20.5 (8), 26.1 / 29.6, 22.1 / 25.8, 23.2 / 25.3.
+int few_warps(int out, int K) {
+    int w = WARPS;
+    while (--w >= 4)
+        if (few_load(out, K, w) * 5 <= few_load(out, K, WARPS) * 4) return w;
+    return WARPS;
 }
 
 }  // namespace
 
-// Blocks of the cluster that shares a product's rows; 0 where the tokens' codes do not fit. As many as two blocks an SM have room for: 4,096 x 4,096 takes
-// 6.5 us with 8, 7.4 with 4, 10.2 with 2. Powers of two: clusters of 6 do not fill the device (6,144 x 4,096 8.2 us with 4, 13.0 with 6).
-static int few_split(int out, int K) {
-    const int groups = (K + KB - 1) / KB, tiles = (out + ROWS - 1) / ROWS;
-    int split = 1;
-    while (split < MAX_SPLIT && 2 * split <= groups && (2LL * split * tiles <= 2 * ti_sm_count() || few_bytes((groups + split - 1) / split) > MAX_SMEM)) split *= 2;
-    return few_bytes((groups + split - 1) / split) > MAX_SMEM ? 0 : split;
-}
-bool linear8_takes_few(int n, int out, int K) { return n <= N && few_split(out, K) > 0; }
+bool linear8_takes_few(int n, int out, int K) { return n <= N && few_split(out, K, few_warps(out, K)) > 0; }
 
 int linear8_few(const Linear8& p, cudaStream_t stream) {
-    return p.x_scales != nullptr ? launch<true>(p, few_split(p.out, p.K), stream) : launch<false>(p, few_split(p.out, p.K), stream);
+    const int warps = few_warps(p.out, p.K), split = few_split(p.out, p.K, warps);
+    return p.x_scales != nullptr ? launch<true>(p, warps, split, stream) : launch<false>(p, warps, split, stream);
 }
