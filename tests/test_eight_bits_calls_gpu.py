@@ -212,3 +212,22 @@ def test_a_cache_beyond_32_bits(ops):
         ops.attention8(out, q[-1:].cuda(), kc, vc, ks, vs, table, slots, cu, lens, dim ** -0.5, nq, nkv, dim, PAGE, 1)
         outs.append(out.cpu())
     assert bool(outs[1].abs().max() > 0) and all(torch.equal(a, b) for a, b in zip(outs[:3], outs[3:]))
+
+
+def test_long_runs_in_turns(ops):
+    """Pages are widened for as many sequences at once as half a gigabyte holds: six with room for 32,768 positions each come in two turns."""
+    nq, nkv, dim, longest = 32, 8, 128, 32768
+    runs = [(100, 200), (0, 50), (7, 7), (100, 1000), (64, 640), (33, 90)]
+    c = make(runs, nq, nkv, dim, seed=21)
+    want, bound = reference(c, dim ** -0.5, 0, 8)
+    c["table"] = torch.cat([c["table"], torch.full((c["table"].shape[0], longest // PAGE - c["table"].shape[1]), -1, dtype=torch.int32)], 1)
+    d = {key: t.cuda() for key, t in c.items()}
+    out = torch.full((c["q"].shape[0] + 1, nq * dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    assert ops.lib().ti_attention8_widens(6, 100, nq, nkv, dim, longest) == 1
+    assert ops.attention8_workspace(6, 100, nq, nkv, dim, longest) <= 2 ** 29 + 2 ** 20
+    found, counted = kernels(lambda: ops.attention8(out[:-1], d["q"], d["k"], d["v"], d["ks"], d["vs"], d["table"], d["seq_slots"], d["cu"], d["lens"], dim ** -0.5, nq, nkv, dim,
+                                                    PAGE, 100))
+    torch.cuda.synchronize()
+    assert found == counted == 4
+    assert bool(((out[:-1].cpu().to(F64) - want).abs() <= bound).all()) and bool((out[-1] == 7).all())
+    ops.check_status()

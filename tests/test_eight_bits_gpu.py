@@ -135,3 +135,18 @@ def test_loading(ti, tmp_path):
     assert len(ti.generate(model, [5, 17, 3], max_new_tokens=9, stop_ids=[])) == 9
     with pytest.raises(ValueError, match="bfloat16"):
         ti.load_model(str(tmp_path / "m"), dtype="float32", cache="e4m3")
+
+
+def test_matrices_go_as_their_codes_are_made(ti):
+    """Making an engine with 8-bit matrices takes little more memory than the matrices it begins with, and holds half of them."""
+    raw = {**helpers.TINY_B, "hidden_size": 1024, "num_attention_heads": 16, "num_key_value_heads": 4, "head_dim": 64, "intermediate_size": 4096, "vocab_size": 512,
+           "num_hidden_layers": 8}
+    _, plain = make(ti, raw)
+    whole = plain.model.weight_bytes()
+    del plain
+    torch.cuda.empty_cache()
+    base = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    _, eng = make(ti, raw, weights="e4m3")
+    assert eng.model.weight_bytes() < 0.52 * whole
+    assert torch.cuda.max_memory_allocated() - base < 1.3 * whole

@@ -607,14 +607,25 @@ extern "C" int ti_attention8_widens(int B, int max_new, int nq, int nkv, int D, 
     const double waves = heads * ceil(max_new * group / 256) / ti_sm_count(), walk = waves * (max_len - 0.5 * max_new);
     return 11 + 0.0193 * (walk > max_len ? walk : max_len) + 2 * waves + heads * max_len * D * 6 / 5e6 < slabs;
 }
+// Sequences whose pages are widened at once: as many as half a gigabyte holds, one at least.
+static int widened_at_once(int B, int nkv, int D, int max_len) {
+    const long long one = ((long long)max_len + AF_PAGE - 1) / AF_PAGE * nkv * AF_PAGE * D * 4, fit = one > 0 ? (1LL << 29) / one : B;
+    return (int)(fit < 1 ? 1 : fit < B ? fit : B);
+}
+// Kernels of one call.
+extern "C" int ti_attention8_launches(int B, int max_new, int nq, int nkv, int D, int max_len) {
+    if (B <= 0 || max_new <= 0) return 0;
+    const int turn = ti_attention8_widens(B, max_new, nq, nkv, D, max_len) ? widened_at_once(B, nkv, D, max_len) : A8_MAX_SEQS;
+    return 2 * ((B - 1) / turn + 1);
+}
 static long long up16(long long bytes) { return (bytes + 15) / 16 * 16; }
 
 // Bytes of the work space: two slots of rows a block, or the widened pages with their table.
 extern "C" long long ti_attention8_workspace(int B, int max_new, int nq, int nkv, int D, int max_len) {
     if (B <= 0 || max_new <= 0 || nq <= 0 || nkv <= 0 || D <= 0) return 0;
     if (ti_attention8_widens(B, max_new, nq, nkv, D, max_len)) {
-        const long long pages = (long long)B * ((max_len + AF_PAGE - 1) / AF_PAGE);
-        return pages * nkv * AF_PAGE * D * 4 + up16(4 * pages) + 2 * up16(4LL * B);
+        const long long turn = widened_at_once(B, nkv, D, max_len), pages = turn * ((max_len + AF_PAGE - 1) / AF_PAGE);
+        return pages * nkv * AF_PAGE * D * 4 + up16(4 * pages) + 2 * up16(4 * turn);
     }
     const int eights = slab_eights(max_new * (long long)(nq / nkv), D);
     return 2LL * sm_blocks(eights, D) * ti_sm_count() * 8 * eights * (D + 2) * 4;
@@ -647,16 +658,23 @@ extern "C" int ti_attention8(void* out, const void* q, const void* k, const void
     const long long need = ti_attention8_workspace(B, max_new, nq, nkv, D, max_len);
     TI_REQUIRE(ws != nullptr && aligned16(ws) && ws_bytes >= need, "attention8: work space of %lld bytes, %lld needed", ws_bytes, need);
     if (ti_attention8_widens(B, max_new, nq, nkv, D, max_len)) {
-        const int per_seq = (max_len + AF_PAGE - 1) / AF_PAGE;
-        const long long all = (long long)B * per_seq, pool = all * nkv * AF_PAGE * D;
-        TI_REQUIRE(all * nkv * AF_PAGE <= 0x7fffffffLL, "attention8: %d sequences of up to %d positions are too many for one step", B, max_len);
+        const int per_seq = (max_len + AF_PAGE - 1) / AF_PAGE, turn = widened_at_once(B, nkv, D, max_len);
+        const long long all = (long long)turn * per_seq, pool = all * nkv * AF_PAGE * D;
+        TI_REQUIRE(all * nkv * AF_PAGE <= 0x7fffffffLL, "attention8: %d positions of %d heads are too many for a long run", max_len, nkv);
         TI_REQUIRE(((uintptr_t)q | (uintptr_t)out) % 16 == 0, "attention8: queries and outputs of long runs must be 16-byte aligned");
         bf16 *k16 = (bf16*)ws, *v16 = k16 + pool;
-        int *table16 = (int*)(v16 + pool), *slots16 = table16 + up16(4 * all) / 4, *lens16 = slots16 + up16(4LL * B) / 4;
-        if (int rc = cache_widen8(k16, v16, table16, slots16, lens16, k, v, k_scales, v_scales, table, table_stride, seq_slots, cu, kv_lens, B, nkv, D, pages, per_seq, window, stream)) return rc;
-        // As many blocks as the runs can need: those beyond leave at once.
-        const int tokens = 2 * (128 / (nq / nkv)), blocks = n / tokens + (B < n ? B : n);
-        return ti_attention_prefill_tc(out, q, k16, v16, (int)all, table16, per_seq, slots16, cu, lens16, B, n, blocks, scale, nq, nkv, D, page_size, window, status, stream);
+        int *table16 = (int*)(v16 + pool), *slots16 = table16 + up16(4 * all) / 4, *lens16 = slots16 + up16(4LL * turn) / 4;
+        for (int b0 = 0; b0 < B; b0 += turn) {
+            const int these = B - b0 < turn ? B - b0 : turn;
+            if (int rc = cache_widen8(k16, v16, table16, slots16, lens16, k, v, k_scales, v_scales, table, table_stride, seq_slots + b0, cu + b0, kv_lens + b0, these, nkv, D, pages,
+                                      per_seq, window, stream)) return rc;
+            // As many blocks as the runs can need: those beyond leave at once.
+            const int tokens = 2 * (128 / (nq / nkv)), blocks = n / tokens + (these < n ? these : n);
+            const long long most = (long long)these * (((long long)max_new + tokens - 1) / tokens);
+            if (int rc = ti_attention_prefill_tc(out, q, k16, v16, (int)all, table16, per_seq, slots16, cu + b0, lens16, these, n, blocks < most ? blocks : (int)most, scale, nq, nkv,
+                                                 D, page_size, window, status, stream)) return rc;
+        }
+        return 0;
     }
     Call c;
     c.max_new = max_new;

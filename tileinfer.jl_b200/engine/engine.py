@@ -45,10 +45,11 @@ class Engine:
     def __init__(self, config, tensors: Dict[str, torch.Tensor], dtype="bfloat16", device="cuda",
                  max_tokens: int = 4096, max_seqs: int = 8, max_context: Optional[int] = None,
                  page_size: int = DEFAULT_PAGE_SIZE, max_step_tokens: int = 8192, kernels: str = "fast",
-                 graphs: bool = True, model_factory=None, cache: str = "model", weights: str = "model"):
+                 graphs: bool = True, model_factory=None, cache: str = "model", weights: str = "model", take_tensors: bool = False):
         """``cache``: "model" (keys and values in the element type) or "e4m3" (8 bits, a scale for each page of 64 positions and KV head). ``weights``: "model"
         or "e4m3" (the matrices of products and head in 8 bits, a scale for each 128 x 128, their inputs quantised on the way). Both take models of plain
-        attention and feed-forward layers in bfloat16."""
+        attention and feed-forward layers in bfloat16. ``take_tensors``: ``tensors`` is emptied once the model is made, so that matrices in the element type go
+        one by one as those in 8 bits are made from them."""
         for name, value in (("cache", cache), ("weights", weights)):
             if value not in ("model", "e4m3"):
                 raise ValueError(f"{name} expects model or e4m3, not {value}")
@@ -65,7 +66,14 @@ class Engine:
         self.model = factory(self.spec, tensors, self.rt, max_context)
         if weights == "e4m3":
             from .drafting import with_matrices
-            self.model = with_matrices(self.model, Linear8)
+            if take_tensors:
+                tensors.clear()
+
+            def in_codes(linear):
+                made = Linear8(linear)
+                linear.weight = None                     # the model around it is this engine's own and is given up
+                return made
+            self.model = with_matrices(self.model, in_codes)
         self.cache = Cache(self.model.cache_requests(), self.dtype, self.device, max_tokens=max_tokens,
                            max_seqs=max_seqs, page_size=page_size, max_seq_len=max_context,
                            share=self.model.cache_shares(), max_step_tokens=int(max_step_tokens))
@@ -114,14 +122,14 @@ class Engine:
         config = arch.config_class.from_dict(raw)
         spec = config.model_spec()
         tensors = load_tensors(model_dir, tensor_declarations(spec), ignorable_tensors(spec))
-        return cls(config, tensors, model_factory=arch.model_factory, **kw)
+        return cls(config, tensors, model_factory=arch.model_factory, take_tensors=True, **kw)
 
     @classmethod
     def random(cls, config, seed: int = 0, **kw) -> "Engine":
         """Random weights drawn on the device (nothing is written to disk)."""
         device = require_cuda(kw.get("device", "cuda"))
         tensors = random_tensors(tensor_declarations(config.model_spec()), seed, dtype=torch.bfloat16, device=str(device))
-        return cls(config, tensors, **kw)
+        return cls(config, tensors, take_tensors=True, **kw)
 
     def twin(self, model) -> "Engine":
         """An engine that runs ``model`` on THIS engine's sequences: the same cache, lengths and scratch buffers, with step metadata and graphs of

@@ -139,8 +139,9 @@ def lib():
         fn = getattr(handle, name)
         fn.restype, fn.argtypes = c_longlong, args
         setattr(wrapped, name, fn)
-    handle.ti_attention8_widens.restype, handle.ti_attention8_widens.argtypes = c_int, [_I] * 6
-    wrapped.ti_attention8_widens = handle.ti_attention8_widens
+    for name in ("ti_attention8_widens", "ti_attention8_launches"):
+        getattr(handle, name).restype, getattr(handle, name).argtypes = c_int, [_I] * 6
+        setattr(wrapped, name, getattr(handle, name))
     handle.ti_linear4_kernels.restype, handle.ti_linear4_kernels.argtypes = c_int, [_I] * 3
     wrapped.ti_linear4_kernels = handle.ti_linear4_kernels
     handle.ti_status_word.restype, handle.ti_status_word.argtypes = c_void_p, []

@@ -1420,5 +1420,5 @@ def attention8(out, q, k_cache, v_cache, k_scales, v_scales, block_table, seq_sl
                              nq, nkv, head_dim, page_size, max_new, max_len, k_cache.shape[0], window or 0, stream)
     if rc:
         check(rc, "attention8")
-    if seqs > ATTENTION8_MAX_SEQS and not lib().ti_attention8_widens(seqs, max_new, nq, nkv, head_dim, max_len):
-        _library.add_launches(2 * ((seqs - 1) // ATTENTION8_MAX_SEQS))
+    if seqs > 1 and (seqs > ATTENTION8_MAX_SEQS or max_new > 1):
+        _library.add_launches(lib().ti_attention8_launches(seqs, max_new, nq, nkv, head_dim, max_len) - 2)
