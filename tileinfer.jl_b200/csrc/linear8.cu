@@ -15,8 +15,8 @@ static bool takes_many(int n, int out, int K) {
 }
 
 // Tokens that come as bfloat16 are quantised by every block that needs them where they are few, else by a launch of its own ahead. Microseconds ahead / in the
-// blocks: eight tokens of 1,024 x 1,024 5.2 / 4.0, 4,096 x 4,096 9.0 / 7.8, 14,336 x 4,096 16.0 / 16.3, 21,504 x 4,096 22.9 / 26.9; four of that 24.5 / 23.2.
-static bool quantized_ahead(int n, int out, int K) { return !linear8_takes_few(n, out, K) || (n > 4 && (long long)out * K > 48000000); }
+// blocks: eight tokens of 1,024 x 1,024 4.9 / 3.8, 4,096 x 4,096 9.1 / 7.5, 14,336 x 4,096 16.1 / 16.3, 21,504 x 4,096 21.3 / 25.7; four of that 21.0 / 21.4.
+static bool quantized_ahead(int n, int out, int K) { return !linear8_takes_few(n, out, K) || (n > 4 && (long long)out * K > 70000000); }
 
 // Bytes of the work space: the tokens' codes and scales, where they are made ahead.
 extern "C" long long ti_linear8_workspace(int n, int out, int K, int given) {

@@ -6,11 +6,12 @@
 // receives its 128 tokens' sums. A step is two groups of 128 of k (48 KB a block); a group's sums stand in an accumulator of their own, and eight warps (two a
 // quarter of the lanes, 64 columns each) add them, times sx sw, to 32-bit sums in registers: a thread has a token, so that sx sw is one number a group.
 //
-// Bound by the hand-overs: the tensor cores need 512 cycles a step and are busy for half of the time. A step takes the issuing warp about 800 cycles (its waits, eight
-// MMAs, one commit, which frees the stage and gives the sums over at once), the adding warps about 1,000. What took the longest was found by reading the clock in every
-// warp: a factor multiplied as soon as it was asked for (the adding warps waited for its loads; now a warp of its own brings factors), and waits for barriers that
-// were over long since, 300 cycles each beside the MMAs (now asked one step ahead). 256 tokens of 4,096 x 21,504 69.6 -> 57.1 us, 2,048 of 21,504 x 4,096
-// 225 -> 198 us, 1,820 TFLOP/s (at cold clocks; both sides on the same machine). Tiles of 256 x 256 took the same time for the same work, sixteen adding warps 7 % more.
+// Bound by the hand-overs: the tensor cores need 256 cycles a group and are busy for half of the time. By the clock, read in every warp of a block with one group
+// a step, the issuing warp took 620 cycles a group (waits 100; the next step's question, four MMAs and a commit 350; its loop), the adding warps 650. What had
+// taken the longest: a factor multiplied as soon as it was asked for (the adding warps waited for its loads; now a warp of its own brings factors), and waits for
+// barriers that were over long since, 300 cycles each beside the MMAs (now asked one step ahead). A commit frees the stage and gives the sums over at once.
+// 256 tokens of 4,096 x 21,504 69.6 -> 55.0 us, 2,048 of 21,504 x 4,096 221 -> 198 us, 1,820 TFLOP/s. Tiles of 256 x 256 took the same time for the same work,
+// one group a step 59.3 us, sixteen adding warps 63.5.
 //
 // Block 0 of the pair issues the MMAs; its `full` barriers count the bytes of both blocks' loads; commits arrive on both blocks' barriers; the partner's
 // warps arrive on block 0's accumulator barriers. All waits are bounded.
