@@ -231,3 +231,18 @@ def test_long_runs_in_turns(ops):
     assert found == counted == 4
     assert bool(((out[:-1].cpu().to(F64) - want).abs() <= bound).all()) and bool((out[-1] == 7).all())
     ops.check_status()
+
+
+def test_lengths_beyond_the_table(ops):
+    """A length that the table's row has no pages for: what lies beyond reads as zeros, the others get what they should."""
+    runs, nq, nkv, dim = [(2, 300), (2, 500), (1, 70)], 8, 2, 64
+    c = make(runs, nq, nkv, dim, seed=2)
+    want, bound = reference(c, dim ** -0.5, 0, 11)
+    c["lens"][1] = 64 * (c["table"].shape[1] + 40)
+    c["table"] = c["table"][:int(c["seq_slots"].max()) + 1].contiguous()
+    d = {key: t.cuda() for key, t in c.items()}
+    out = torch.empty(c["q"].shape[0], nq * dim, dtype=torch.bfloat16, device="cuda")
+    ops.attention8(out, d["q"], d["k"], d["v"], d["ks"], d["vs"], d["table"], d["seq_slots"], d["cu"], d["lens"], dim ** -0.5, nq, nkv, dim, PAGE, 2)
+    right = ((out.cpu().to(F64) - want).abs() <= bound).all(-1)
+    assert bool(right[:2].all()) and bool(right[4:].all())
+    ops.check_status()

@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
             Ahead x = {-1, false, true, 1.f, 1.f};
             if (u >= hi) return x;
             const Place p = locate(u);
-            const int tile = p.s.t0 + p.tile, page = __ldcg(a.table + (size_t)s_slot[p.b] * a.table_stride + tile);
+            const int tile = p.s.t0 + p.tile, page = tile < a.table_stride ? __ldcg(a.table + (size_t)s_slot[p.b] * a.table_stride + tile) : -1;
             // Tiles with new keys were written by the kernel before this one; the others stand since earlier steps.
             x.fresh = (tile + 1) * AF_PAGE > p.s.L - p.s.T;
             if (page >= 0 && page < a.pages) { x.block = page * nkv + p.kvh; x.scaled = false; }                     // a page that does not exist reads as zeros
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
             auto put_back = [&](int from, int to) {
                 for (int key = max(from, (s.t0 + at.tile) * AF_PAGE); key < min(to, tile * AF_PAGE); ++key) {
                     if (key % AF_PAGE / 16 != warp) continue;
-                    const int page = __ldcg(a.table + (size_t)s_slot[at.b] * a.table_stride + key / AF_PAGE);
+                    const int page = key / AF_PAGE < a.table_stride ? __ldcg(a.table + (size_t)s_slot[at.b] * a.table_stride + key / AF_PAGE) : -1;
                     if (page < 0 || page >= a.pages) continue;
                     const unsigned char* value = a.v + (((size_t)page * nkv + at.kvh) * AF_PAGE + key % AF_PAGE) * D;
 #pragma unroll

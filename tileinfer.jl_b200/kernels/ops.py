@@ -1396,7 +1396,7 @@ def attention8(out, q, k_cache, v_cache, k_scales, v_scales, block_table, seq_sl
     cu_seqlens[b] to cu_seqlens[b + 1] of q [n, nq, head_dim] (at most ``max_new``, or none) are the last of the kv_lens[b] positions of the sequence in slot
     seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out [n, nq * head_dim]; q and out bfloat16. A key stands for its code times
     k_scales[page, head], a value for its code times v_scales[page, head] (positive, 2^-100 to 2^120). ``max_len``: no kv_lens is larger (None: as many as the
-    table's rows have pages for). What no token sees may hold any codes; a NaN code that some see reaches those alone. Long
+    table's rows have pages for). A page that does not exist reads as zeros. What no token sees may hold any codes; a NaN code that some see reaches those alone. Long
     runs go through pages widened to bfloat16: codes times scales that are no powers of two are rounded to it, and a NaN value that some rows of a run see may
     reach others of the run; their q and out must be 16-byte aligned (others' 4-byte). Lengths, ranges, slots, table, and the pages before those of the new tokens
     are read while kernels ahead may still run: they come from copies, torch's operations or earlier steps. ``workspace``: ``attention8_workspace`` bytes (uint8);
