@@ -291,3 +291,11 @@ def test_refusals(ops):
         with pytest.raises(ops.KernelError, match="multiple"):
             ops.attention8(torch.zeros(2, dim, dtype=torch.bfloat16, device="cuda"), c["q"], c["k"], c["v"], c["ks"], c["vs"], c["table"], c["seq_slots"], c["cu"],
                            c["lens"], 0.1, 1, 1, dim, 64, 2)
+
+
+@pytest.mark.parametrize("dim", [16, 32, 48, 80, 96, 112, 144, 208, 256])
+@pytest.mark.parametrize("window", [0, 300])
+def test_prompts_of_every_head_size(ops, dim, window):
+    """Sizes whose long runs go through widened pages, and sizes that no prompts' kernel takes."""
+    check(ops, [(900, 1000), (0, 70), (300, 300), (1, 64)], 16, 2, dim, window, seed=dim)
+    assert bool(ops.lib().ti_attention8_widens(4, 900, 16, 2, dim, 1088)) == (dim <= 128 or dim == 256)

@@ -596,16 +596,24 @@ int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, int* 
 extern "C" int ti_attention_prefill_tc(void* out, const void* q, const void* k_cache, const void* v_cache, int n_pages, const int* block_table, int table_stride,
                                        const int* seq_slots, const int* cu_seqlens, const int* kv_lens, int n_seqs, int n_tokens, int total_blocks, float scale, int nq,
                                        int nkv, int D, int page_size, int window, int* status, cudaStream_t stream);
-// Whether a step goes through pages widened to bfloat16 and the prompts' kernel on the fifth-generation tensor cores: the shorter by estimates in microseconds, for
-// sequences of max_len positions. Slabs: 4.8 ns for a slab's tile of heads of 128, 57 ns for its other work. Widened: a walk along the longest sequence
-// (19 ns a position), rounds of the SMs, the widened bytes. Microseconds in turn, 32 / 8 heads of 128: one sequence, 64 new of 8,192 62 / 170, 128 of 1,024 30 / 32,
-// 256 of 4,096 122 / 94, 2,048 of 4,096 1,212 / 139; four sequences, 32 of 512 25 / 25, 128 of 128 45 / 17.
+extern "C" int ti_attention_prefill(void* out, const void* q, const void* k_cache, const void* v_cache, const int* block_table, int table_stride, const int* seq_slots,
+                                    const int* cu_seqlens, const int* kv_lens, int n_seqs, int total_tiles, float scale, int nq, int nkv, int D, int page_size, int window,
+                                    cudaStream_t stream);
+// Whether a step goes through pages widened to bfloat16 and the prompts' kernels, for heads of 64 and 128 on the fifth-generation tensor cores (attention_prefill_tc.cu),
+// else with mma.sync (attention_prefill.cu): the shorter by estimates in microseconds, for sequences of max_len positions. Slabs: a slab's tile (heads of 128 4.8 ns;
+// of the sizes between 6.4, up to 64 3.8, of 256 9.5), 57 ns for a slab's other work. Widened: a walk along the longest sequence (19 ns a position; with mma.sync 15 and
+// 0.265 for each of the head's dimensions), rounds of the SMs, the widened bytes. Microseconds in turn, 32 / 8 heads of 128: one sequence, 64 new of 8,192 62 / 170,
+// 128 of 1,024 30 / 32, 256 of 4,096 122 / 94, 2,048 of 4,096 1,212 / 139; four sequences, 32 of 512 25 / 25, 128 of 128 45 / 17. Heads of 96: 68 / 321, 32 / 45,
+// 135 / 166, 1,316 / 504, 24 / 29, 43 / 15; of 256: 128 / 680, 55 / 96, 278 / 349, 3,394 / 1,057, 38 / 59, 86 / 31.
 extern "C" int ti_attention8_widens(int B, int max_new, int nq, int nkv, int D, int max_len) {
-    if (B <= 0 || nkv <= 0 || nq % nkv != 0 || (D != 64 && D != 128) || nq / nkv > 128 || B > 65535 || max_new * (long long)(nq / nkv) <= 24) return 0;
-    const double group = nq / nkv, heads = (double)B * nkv, items = heads * ceil(max_new * group / 24), size = D / 128.0;
-    const double slabs = 5 + (0.0048 * items * (max_len / 64.0) + 0.057 * items) * size;
-    const double waves = heads * ceil(max_new * group / 256) / ti_sm_count(), walk = waves * (max_len - 0.5 * max_new);
-    return 11 + 0.0193 * (walk > max_len ? walk : max_len) + 2 * waves + heads * max_len * D * 6 / 5e6 < slabs;
+    if (B <= 0 || nkv <= 0 || nq % nkv != 0 || (D != 256 && (D > 128 || D % 16 != 0)) || nq / nkv > 128 || B > 65535 || max_len <= 0 || max_new * (long long)(nq / nkv) <= 24)
+        return 0;
+    const bool fifth = D == 64 || D == 128;
+    const double rows = max_new * (double)(nq / nkv), heads = (double)B * nkv, items = heads * ceil(rows / (D > 128 ? 16 : 24)), bytes = heads * max_len * D * 6 / 5e6;
+    const double tile = fifth ? 4.8 * D / 128 : D < 64 ? 3.8 : D < 128 ? 6.4 : 9.5, size = fifth ? D / 128.0 : D < 64 ? 0.5 : 1.0;
+    const double slabs = 5 + 0.001 * tile * items * (max_len / 64.0) + 0.057 * items * size;
+    const double waves = heads * ceil(rows / (fifth ? 256 : 128)) / ti_sm_count(), walk = (fifth ? waves : ceil(waves)) * (max_len - 0.5 * max_new);
+    return 11 + (fifth ? 0.0193 : 0.015 + 0.000265 * D) * (walk > max_len ? walk : max_len) + 2 * waves + bytes < slabs;
 }
 // Sequences whose pages are widened at once: as many as half a gigabyte holds, one at least.
 static int widened_at_once(int B, int nkv, int D, int max_len) {
@@ -669,10 +677,13 @@ extern "C" int ti_attention8(void* out, const void* q, const void* k, const void
             if (int rc = cache_widen8(k16, v16, table16, slots16, lens16, k, v, k_scales, v_scales, table, table_stride, seq_slots + b0, cu + b0, kv_lens + b0, these, nkv, D, pages,
                                       per_seq, window, stream)) return rc;
             // As many blocks as the runs can need: those beyond leave at once.
-            const int tokens = 2 * (128 / (nq / nkv)), blocks = n / tokens + (these < n ? these : n);
+            const bool fifth = D == 64 || D == 128;          // generation of tensor cores
+            const int tokens = (fifth ? 2 : 1) * (128 / (nq / nkv)), blocks = n / tokens + (these < n ? these : n);
             const long long most = (long long)these * (((long long)max_new + tokens - 1) / tokens);
-            if (int rc = ti_attention_prefill_tc(out, q, k16, v16, (int)all, table16, per_seq, slots16, cu + b0, lens16, these, n, blocks < most ? blocks : (int)most, scale, nq, nkv,
-                                                 D, page_size, window, status, stream)) return rc;
+            const int grid = blocks < most ? blocks : (int)most;
+            if (int rc = fifth ? ti_attention_prefill_tc(out, q, k16, v16, (int)all, table16, per_seq, slots16, cu + b0, lens16, these, n, grid, scale, nq, nkv, D, page_size,
+                                                         window, status, stream)
+                               : ti_attention_prefill(out, q, k16, v16, table16, per_seq, slots16, cu + b0, lens16, these, grid, scale, nq, nkv, D, page_size, window, stream)) return rc;
         }
         return 0;
     }
