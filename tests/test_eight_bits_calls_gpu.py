@@ -246,3 +246,36 @@ def test_lengths_beyond_the_table(ops):
     right = ((out.cpu().to(F64) - want).abs() <= bound).all(-1)
     assert bool(right[:2].all()) and bool(right[4:].all())
     ops.check_status()
+
+
+@pytest.mark.parametrize("n", [4, 20, 33, 64, 1000])
+@pytest.mark.parametrize("name", ["EPI_NONE", "EPI_XIELU", "EPI_GELU_ERF", "EPI_GELU_TANH", "EPI_RELU2", "EPI_F32_OUT"])
+def test_launches_with_an_activation(ops, n, name):
+    """An activation that is a launch of its own is counted, and gives what it gives over strided rows, where it is none."""
+    out, k, epilogue = 1040, 512, getattr(ops, name)
+    g = torch.Generator().manual_seed(n)
+    w, x = torch.randn(out, k, generator=g).bfloat16().cuda(), torch.randn(n, k, generator=g).bfloat16().cuda()
+    codes, scales = torch.empty(out, k, dtype=torch.uint8, device="cuda").view(E4M3), torch.empty(4, -(-out // 128), device="cuda")
+    ops.quantize8(codes, scales, w, 128)
+    dtype = torch.float32 if name == "EPI_F32_OUT" else torch.bfloat16
+    dense, wide = torch.empty(n, out, dtype=dtype, device="cuda"), torch.full((n, out + 16), 7.0, dtype=dtype, device="cuda")
+    act = (0.8, 0.8, 0.5, -1e-6)
+    found, counted = kernels(lambda: ops.linear8(dense, x, codes, scales, None, epilogue, act))
+    assert found == counted
+    found, counted = kernels(lambda: ops.linear8(wide[:, :out], x, codes, scales, None, epilogue, act))
+    assert found == counted and torch.equal(dense, wide[:, :out]) and bool((wide[:, out:] == 7).all())
+
+
+@pytest.mark.parametrize("act", [(0.75, 0.875, 0.5, -1e-6), (0.8, 0.8, 0.5, -1e-6)])
+@pytest.mark.parametrize("n,out", [(33, 1040), (64, 333), (700, 4096), (1, 64)])
+def test_xielu_is_the_library_s_own(ops, n, out, act):
+    """Factors that are bfloat16 numbers, and others: the bits of the sums' own activation."""
+    g = torch.Generator().manual_seed(n)
+    w, x = torch.randn(out, 512, generator=g).bfloat16().cuda(), torch.randn(n, 512, generator=g).bfloat16().cuda()
+    codes, scales = torch.empty(out, 512, dtype=torch.uint8, device="cuda").view(E4M3), torch.empty(4, -(-out // 128), device="cuda")
+    ops.quantize8(codes, scales, w, 128)
+    plain, got, want = (torch.empty(n, out, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    ops.linear8(plain, x, codes, scales)
+    ops.linear8(got, x, codes, scales, None, ops.EPI_XIELU, act)
+    ops.xielu(want, plain, *act)
+    assert torch.equal(got, want)

@@ -211,7 +211,7 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         const int half = (warp - 3) >> 2, quarter = warp & 3;
         const unsigned columns = tmem + ((unsigned)(quarter * 32) << 16) + half * HALF, release0 = in_block0(free0);
         float* out = reinterpret_cast<float*>(tiles + STAGES * STAGE) + (warp - 3) * (OUT / 4);
-        const bool y32 = p.epilogue == L4_EPI_F32_OUT, quads = linear8_quads(p);
+        const bool y32 = p.epilogue == L4_EPI_F32_OUT, quads = linear8_quads(p), singles = !quads || (p.epilogue != L4_EPI_NONE && !y32);
         // 32 bytes at a time straight from the registers.
         const bool direct = (p.epilogue == L4_EPI_NONE && ((uintptr_t)p.y & 31) == 0 && p.ldy % 16 == 0) || (y32 && ((uintptr_t)p.y & 31) == 0 && p.ldy % 8 == 0);
         int slot = 0, stage = 0;
@@ -274,7 +274,8 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 }
                 continue;
             }
-            // Others through shared memory, 16 columns at a time: [token][16-byte piece turned by the token], then four lanes a token.
+            // Others through shared memory, 16 columns at a time: [token][16-byte piece turned by the token], then four lanes a token; sixteen where four
+            // neighbouring results cannot be written at once (1,914 tokens of 18,375 x 304: a lane's four one after another 165 us, next to one another 78).
 #pragma unroll
             for (int c0 = 0; c0 < HALF; c0 += OUT_COLS) {
                 __syncwarp();
@@ -286,6 +287,13 @@ linear8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                     *reinterpret_cast<float4*>(out + lane * OUT_COLS + ((j ^ ((lane >> 1) & 3)) << 2)) = v;
                 }
                 __syncwarp();
+                if (singles) {
+                    const int column = lane & 15, o = row0 + c0 + column;
+#pragma unroll 4
+                    for (int t = lane >> 4; t < min(32, p.n - token0); t += 2)
+                        if (o < p.out) store_result(p.y, p.ldy, token0 + t, o, out[t * OUT_COLS + (((column >> 2) ^ ((t >> 1) & 3)) << 2) + (column & 3)], p.epilogue, p.act, y32);
+                    continue;
+                }
                 const int o = row0 + c0 + (lane & 3) * 4;
 #pragma unroll 2
                 for (int t = lane >> 2; t < min(32, p.n - token0); t += 8)

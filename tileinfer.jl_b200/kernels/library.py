@@ -139,6 +139,8 @@ def lib():
         fn = getattr(handle, name)
         fn.restype, fn.argtypes = c_longlong, args
         setattr(wrapped, name, fn)
+    handle.ti_linear8_apart.restype, handle.ti_linear8_apart.argtypes = c_int, [_I, _I, _L, _I]
+    wrapped.ti_linear8_apart = handle.ti_linear8_apart
     for name in ("ti_attention8_widens", "ti_attention8_launches"):
         getattr(handle, name).restype, getattr(handle, name).argtypes = c_int, [_I] * 6
         setattr(wrapped, name, getattr(handle, name))

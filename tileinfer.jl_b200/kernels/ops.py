@@ -1327,6 +1327,8 @@ def linear8(y, x, codes, scales, x_scales=None, epilogue=EPI_NONE, act=(0.0, 0.0
         check(rc, "linear8")
     if need and n:
         _library.add_launches(1)                             # the tokens' codes are made by a launch of their own
+    if epilogue != EPI_NONE and lib().ti_linear8_apart(n, out, y.stride(0), epilogue):
+        _library.add_launches(1)                             # so is the activation
 
 
 def _paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, page_size, seqs) -> bool:
