@@ -37,12 +37,13 @@ __global__ void __launch_bounds__(256) quantize8_rows_kernel(unsigned char* code
     }
 }
 
-// Blocks of 128 x 128: 256 threads hold one, 64 elements each.
+// Blocks of 128 x 128: 256 threads hold one, 64 elements each. The products ask for weights before they wait for the kernel before them, so this one lets nothing
+// start beside it and every thread's stores reach all before it ends.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize8_blocks_kernel(unsigned char* codes, float* scales, const T* x, long long ldx, int n, int k, int row_blocks) {
     __shared__ float scratch[33];
     const int g = blockIdx.x, row0 = blockIdx.y * E4M3_BLOCK + (threadIdx.x >> 4), col = g * E4M3_BLOCK + (threadIdx.x & 15) * 8;
-    pdl_enter();
+    pdl_wait();
     Eight<T> v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -57,6 +58,7 @@ __global__ void __launch_bounds__(256) quantize8_blocks_kernel(unsigned char* co
     for (int j = 0; j < 8; ++j)
         if (row0 + 16 * j < n && col < k) *reinterpret_cast<uint2*>(codes + (long long)(row0 + 16 * j) * k + col) = codes_of(v[j], inverse, finite);
     if (threadIdx.x == 0) scales[(long long)g * row_blocks + blockIdx.y] = power_of_two(power);
+    __threadfence();
 }
 
 template <typename T> int launch(unsigned char* codes, float* scales, const T* x, long long ldx, int n, int k, int rows, cudaStream_t stream) {

@@ -1297,9 +1297,9 @@ def linear8(y, x, codes, scales, x_scales=None, epilogue=EPI_NONE, act=(0.0, 0.0
     """y [n, out] = x [n, in] Wᵀ for W of e4m3 ``codes`` [out, in] with ``scales`` [ceil(in / 128), ceil(out / 128)] (``quantize8`` with ``rows`` 128; any
     positive scales are taken). x is bfloat16 and quantised by row in groups of 128 on the way, as ``quantize8`` does it, or codes with ``x_scales``
     [ceil(in / 128), n]. 32-bit sums of every group, scaled and added in 32-bit, rounded once to y's bfloat16; with ``EPI_F32_OUT`` y is float32 and the sums
-    are not rounded. ``in`` is a multiple of 16; rows of x and y may be strided. Codes and scales of the weights are read while kernels ahead may still run:
-    they come from ``quantize8`` before other work, copies or torch's operations. ``workspace``: ``linear8_workspace`` bytes (uint8); without it
-    one kept per thread and stream (a captured call: one of its graph's own)."""
+    are not rounded. ``in`` is a multiple of 16; rows of x and y may be strided. Codes and scales of the weights are read while the kernel ahead may still run;
+    ``quantize8`` with ``rows`` 128, copies and torch's operations let nothing start beside them, so what they wrote is there. ``workspace``:
+    ``linear8_workspace`` bytes (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
     try:
         (n, k), (out, columns), given = x.shape, codes.shape, x_scales is not None
         fits = x.is_cuda and y.is_cuda and codes.is_cuda and scales.is_cuda and codes.dtype is _E4M3 and scales.dtype is _F32 and columns == k and \
