@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from numbers8 import E4M3
+from numbers8 import E4M3, PAGE
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,64 @@ def test_products_directly_after_their_weights(ops, n, given, out, k):
             graph.replay()
             stream.synchronize()
             assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(outs))
+
+
+@pytest.mark.parametrize("written", [1, 2, 64, 200, 1000])
+@pytest.mark.parametrize("attending", [1, 3])
+def test_attention_of_fewer_tokens_than_were_just_written(ops, written, attending):
+    """A run's keys and values go into the cache and its last tokens alone attend, right behind; two runs take one place in turn."""
+    nq, nkv, dim, seqs = 8, 4, 128, 6
+    attending = min(attending, written)
+    pages = -(-(written + 70) // PAGE)
+    g = torch.Generator().manual_seed(written)
+    table = torch.randperm(seqs * pages, generator=g).to(torch.int32).view(seqs, pages).cuda()
+    slots = torch.arange(seqs, dtype=torch.int32).cuda()
+    ranges = [(torch.arange(seqs + 1) * t).to(torch.int32).cuda() for t in (written, attending)]
+    lens = torch.full((seqs,), written + 70, dtype=torch.int32).cuda()
+    new = [[torch.randn(seqs * written, nkv, dim, generator=g).bfloat16().cuda() * size for _ in "kv"] for size in (1.0, 3.0)]
+    q = torch.randn(seqs * attending, nq, dim, generator=g).bfloat16().cuda()
+    k, v = (torch.zeros(seqs * pages, nkv, PAGE, dim, dtype=torch.uint8, device="cuda").view(E4M3) for _ in "kv")
+    ks, vs = (torch.ones(seqs * pages, nkv, device="cuda") for _ in "kv")
+
+    def write(i):
+        ops.cache_write8(k, v, ks, vs, *new[i % 2], table, slots, ranges[0], lens, written)
+
+    def attend(out):
+        ops.attention8(out, q, k, v, ks, vs, table, slots, ranges[1], lens, dim ** -0.5, nq, nkv, dim, PAGE, attending)
+
+    outs = [torch.zeros(seqs * attending, nq * dim, dtype=torch.bfloat16, device="cuda") for _ in range(8)]
+
+    def fresh():
+        for t in (k, v):
+            t.view(torch.uint8).zero_()
+        ks.fill_(1.0), vs.fill_(1.0)
+
+    def turns(wait=False):
+        for i, out in enumerate(outs):
+            write(i)
+            if wait:
+                torch.cuda.synchronize()
+            attend(out)
+            if wait:
+                torch.cuda.synchronize()
+
+    fresh()
+    turns(wait=True)
+    want = [out.clone() for out in outs]
+    assert not torch.equal(want[0], want[1])
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        fresh()
+        turns()
+        stream.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            fresh()
+            turns()
+        for _ in range(5):
+            graph.replay()
+            stream.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    ops.check_status()

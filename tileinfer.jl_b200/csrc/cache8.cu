@@ -6,8 +6,12 @@
 // below 2^-6 s'. What lies behind the last new position stays as it was. So the codes do not depend on how the rows before came in, but for those below
 // 2^-6 of the scale. One block of threads writes a page's head, keys or values, which keeps its new rows in registers between their maximum and their codes.
 //
+// Attention over the cache (attention8.cu) asks for pages before it waits for the kernel ahead, but for those that hold one of its own new tokens. With at most one
+// new row a sequence these are all that is written here, so it may come up beside this kernel; with more, the tokens that attend may be fewer than those that are
+// written, so nothing starts until all stores have reached all (eight runs of up to 1,024 rows 10.2 -> 10.7 us, five rows of 64 sequences 5.4 -> 5.7; five rows of eight with their attention 35.4 -> 37.0).
+//
 // Bound by launch and three dependent reads (lengths, the page, its rows and old scale), so that blocks are small enough to come up at once where they are many:
-// one token of 64 sequences takes 3.8 us, eight runs of up to 1,024 rows 10.4 (8 heads of 128; 7.3 MB, 1.1 us at the rate of a copy).
+// one token of 64 sequences takes 3.8 us, eight runs of up to 1,024 rows 10.7 (8 heads of 128; 7.3 MB, 1.1 us at the rate of a copy).
 //
 // Widening, for kernels that read bfloat16: the pages that a step's tokens see become pages of bfloat16 in a pool of their own, page j of sequence b at
 // b x (pages a sequence) + j, with its block table. A code times a power of two is exact in bfloat16. Positions that nobody sees become zeros.
@@ -26,10 +30,11 @@ struct Rows {
 template <typename T, bool VEC, int NT, int J>
 __global__ void __launch_bounds__(NT) cache_write8_kernel(unsigned char* k_codes, unsigned char* v_codes, float* k_scales, float* v_scales, Rows k, Rows v,
                                                                const int* table, int table_stride, int slots, const int* seq_slots, const int* cu,
-                                                               const int* kv_lens, int n, int nkv, int D, int pages, int touched) {
+                                                               const int* kv_lens, int n, int nkv, int D, int pages, int touched, bool beside) {
     __shared__ float scratch[33];
     const int b = blockIdx.x / touched, kvh = blockIdx.y >> 1, is_v = blockIdx.y & 1;
-    pdl_enter();
+    pdl_wait();
+    if (beside) pdl_launch_dependents();
     const int begin = __ldcg(cu + b), T_new = __ldcg(cu + b + 1) - begin, L = __ldcg(kv_lens + b), slot = __ldcg(seq_slots + b);
     const int start = L - T_new, logical = start / PAGE + blockIdx.x % touched, base = logical * PAGE;
     // What does not fit (a length below the run's, a slot or page that does not exist) is not written.
@@ -62,8 +67,7 @@ __global__ void __launch_bounds__(NT) cache_write8_kernel(unsigned char* k_codes
         const int e = threadIdx.x + j * NT;
         if (e < rows * per_row) *reinterpret_cast<uint2*>(codes + (size_t)first * D + (size_t)e * 8) = codes_of(x[j], inverse, finite);
     }
-    if (after == before) return;
-    if (first > 0) {
+    if (after != before && first > 0) {
         const float by = before / after;
         const auto moved = [by](unsigned w) {
             const float2 a = e4m3_float2((unsigned short)w), c = e4m3_float2((unsigned short)(w >> 16));
@@ -81,7 +85,8 @@ __global__ void __launch_bounds__(NT) cache_write8_kernel(unsigned char* k_codes
                 if (e0 + j * NT < first * D / 16) old[e0 + j * NT] = make_uint4(moved(w[j].x), moved(w[j].y), moved(w[j].z), moved(w[j].w));
         }
     }
-    if (threadIdx.x == 0) *scale = after;
+    if (threadIdx.x == 0 && after != before) *scale = after;
+    if (!beside) __threadfence();
 }
 
 // blockIdx: page, head, sequence.
@@ -150,7 +155,7 @@ extern "C" int ti_cache_write8(void* k_codes, void* v_codes, float* k_scales, fl
                                             D <= 128 ? (vec ? cache_write8_kernel<T, true, THREADS, 4> : cache_write8_kernel<T, false, THREADS, 4>) :
                                                        (vec ? cache_write8_kernel<T, true, THREADS, 8> : cache_write8_kernel<T, false, THREADS, 8>);
                       ti_launch(kernel, dim3((unsigned)(touched * B), 2 * nkv), dim3(few ? 64 : THREADS), 0, stream, (unsigned char*)k_codes, (unsigned char*)v_codes,
-                                k_scales, v_scales, kr, vr, table, table_stride, slots, seq_slots, cu, kv_lens, n, nkv, D, pages, (int)touched));
+                                k_scales, v_scales, kr, vr, table, table_stride, slots, seq_slots, cu, kv_lens, n, nkv, D, pages, (int)touched, max_new == 1));
     return ti_check_launch("cache_write8");
 }
 

@@ -4,7 +4,7 @@
 //
 // Bound by reading x and writing the codes once (3 bytes an element of bfloat16): a block's elements stay in registers between its maximum and its codes, as they
 // were read. Instructions would be the bound otherwise, so sizes are compared as integers (two of bfloat16 at once) and what is not finite, which they show,
-// is dealt with only where it is. 21,504 x 4,096 of bfloat16 in 128 x 128 blocks 39.9 us (6.6 TB/s), 2,048 x 4,096 by rows 6.6 us (3.8 TB/s: a launch and one wave).
+// is dealt with only where it is. 4,096 x 21,504 of bfloat16 in 128 x 128 blocks 43.7 us (6.0 TB/s; 40.2 while kernels behind started beside it), 2,048 x 4,096 by rows 6.6 us (3.8 TB/s: a launch and one wave).
 // Scales lie [k / 128, rows]: a block of threads makes sixteen rows' next to one another.
 #include "e4m3.cuh"
 

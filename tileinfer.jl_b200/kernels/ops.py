@@ -1401,8 +1401,8 @@ def attention8(out, q, k_cache, v_cache, k_scales, v_scales, block_table, seq_sl
     table's rows have pages for). A page that does not exist reads as zeros. What no token sees may hold any codes; a NaN code that some see reaches those alone. Long
     runs go through pages widened to bfloat16: codes times scales that are no powers of two are rounded to it, and a NaN value that some rows of a run see may
     reach others of the run; their q and out must be 16-byte aligned (others' 4-byte). Lengths, ranges, slots, table, and the pages before those of the new tokens
-    are read while kernels ahead may still run: they come from copies, torch's operations or earlier steps. ``workspace``: ``attention8_workspace`` bytes (uint8);
-    without it one kept per thread and stream (a captured call: one of its graph's own)."""
+    are read while the kernel ahead may still run: they come from ``cache_write8``, copies or torch's operations, beside which nothing starts that could miss
+    what they write. ``workspace``: ``attention8_workspace`` bytes (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
     seqs, n = kv_lens.numel(), q.shape[0]
     if not (_paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, page_size, seqs) and out.is_cuda and q.is_cuda and
             out.dtype is _BF16 and q.dtype is _BF16 and out.is_contiguous() and q.is_contiguous() and nkv > 0 and nq > 0 and nq % nkv == 0 and head_dim > 0 and
