@@ -435,15 +435,16 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
                     }
                 }
                 if (edge) {
-                    // Values that nobody sees may have any code, and 0 x NaN is NaN; NaN codes that some rows see are added at the segment's end.
+                    // Values that nobody sees may have any code, and 0 x NaN is NaN; NaN codes that some rows see and others do not are added at the segment's end.
+                    // Those that all rows see stay.
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int key = key_base + 8 * (e >> 1) + (e & 1 ? key_t1 : key_t0);
-                        const bool seen = key < s.L && key >= s.first;
+                        const bool seen = key < s.L && key >= s.first, some = key > s.L - s.T || (a.window > 0 && key < s.L - a.window);
 #pragma unroll
                         for (int j = 0; j < VB / 4; ++j) {
                             if (!seen) w[e][j] = 0;
-                            else if (s.T > 1) {
+                            else if (some) {
                                 const unsigned bad = nan_codes(w[e][j]);
                                 odd |= bad != 0;
                                 w[e][j] &= ~bad;
