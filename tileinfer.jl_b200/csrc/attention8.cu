@@ -20,9 +20,14 @@
 // lane's share of four MMAs is 16 consecutive bytes; so are the keys, so that a warp's reads meet all banks.
 //
 // With z_j = (the score in base 2) + log2 sv[p(j)] and m near the maximum of z so far, P = 2^(z - m + 7) are the weights of the values' codes, rounded to 16
-// bits (2^-11) as the MMA's operand, and the denominator is the 32-bit sum of P / sv. So neither pages of very unequal scales nor a scale of 2^-100 (a page of
-// zeros) cost anything but an addition to the exponent. m stays until a z is more than 8 above it (P <= 2^15), so that most tiles exchange no maxima.
-// Scores, sums and outputs stand in 32-bit.
+// bits (2^-11) as the MMA's operand, and the denominator is the 32-bit sum of P / sv. So pages of unequal scales (a page of zeros has 2^-100) cost an addition to the
+// exponent. m stays until a z is more than 8 above it (P <= 2^15), so that most tiles exchange no maxima. Scores, sums and outputs stand in 32-bit.
+//
+// The denominator holds for value scales from 2^-100 to 2^120. With s the score without log2 sv, its terms are 2^(s - m + 7) in units of 2^10: between 2^-123 and some 2^125
+// for the largest of a row. P / sv loses a term where P, below 2^-126, becomes zero: in a tile whose log2 sv is at most 90 below the largest so far, m <= max s + that
+// largest, so that a lost term is below 2^-43 of the row's largest one. In other tiles, which the asking warp marks, the terms are computed from s. Sums are brought to
+// another m in two steps of half the power, as the power alone may vanish where the sum times it does not. (Without these steps a page of zeros left the denominator beside
+// values of 10^13; with them 40 rows over up to 32,768 positions take 140.0 us in place of 137.6, one row as long as before.)
 //
 // Keys and values beyond the sequence's end or before the first visible key may hold any codes: their scores are replaced and their values' codes are
 // zero. A NaN code of a key that some rows see and others do not (a drafted token's own) reaches the rows that see it alone.
@@ -37,6 +42,8 @@ namespace {
 
 constexpr int A8_THREADS = 160, A8_MAX_SEQS = 256;           // four warps that compute, one that asks; sequences of one launch
 constexpr float P_POWER = 7.f, SLACK = 8.f;
+constexpr float SUM_UNIT = 0x1p-10f;                         // of denominators
+constexpr unsigned SCALES_APART = 90;                        // beyond so many powers of two a tile's denominator has exponentials of its own
 
 // DP: D rounded up to 64, 128 or 256. NQ: queries in eights.
 template <int DP, int NQ> struct Shape8 {
@@ -66,6 +73,11 @@ struct Args8 {
 __device__ __forceinline__ int tile_at(int i) { return (i & ~0x70) | ((i ^ (i >> 3)) & 0x70); }
 // 0xFF in the places of NaN codes.
 __device__ __forceinline__ unsigned nan_codes(unsigned w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
+// A sum times 2^x, x <= 0, also where 2^x alone is below 2^-126.
+__device__ __forceinline__ float scaled(float sum, float x) {
+    const float half = power2(0.5f * x);
+    return sum * half * half;
+}
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
     unsigned r;
@@ -91,7 +103,7 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
     __shared__ unsigned s_units[A8_MAX_SEQS + 1], s_scan[A8_THREADS / 32];
     __shared__ int s_cu[A8_MAX_SEQS + 1], s_len[A8_MAX_SEQS], s_slot[A8_MAX_SEQS];
     __shared__ float s_ml[4][M][2], s_row[M];                                           // s_row: a row's factor of its scores
-    __shared__ float4 s_scale[64];                           // of the run's tiles in turn: sk, log2 sv, 1 / sv
+    __shared__ float4 s_scale[64];                           // of the run's tiles in turn: sk, log2 sv, SUM_UNIT / sv, below zero where sv lies apart
     __shared__ __align__(8) unsigned long long bars[2 * STAGES];
     unsigned char* ring = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
     const int D = EXACT ? DP : a.D, tile_bytes = AF_PAGE * D, B = a.B, nkv = a.nkv, group = a.nq / nkv;
@@ -186,8 +198,21 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
             x.sv = __ldcg(a.v_scales + x.block);
             x.scaled = true;
         };
+        unsigned top = 0;                                    // the largest exponent of sv of the tiles before these 32
         auto place = [&](const Ahead& x, unsigned u0) {
-            if (x.scaled) s_scale[(u0 - lo + lane) % 64] = make_float4(x.sk, __log2f(x.sv), 1.f / x.sv, 0.f);
+            const unsigned e = __float_as_uint(x.sv) >> 23;
+            bool apart = false;
+            if (max(top, __reduce_max_sync(0xffffffffu, x.scaled ? e : 0u)) > __reduce_min_sync(0xffffffffu, x.scaled ? e : 255u) + SCALES_APART) {
+                unsigned largest = x.scaled ? max(e, top) : top;             // up to this tile: scales that are not here yet are those of later ones
+#pragma unroll 1
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned v = __shfl_up_sync(0xffffffffu, largest, o);
+                    if (lane >= o) largest = max(largest, v);
+                }
+                apart = e + SCALES_APART < largest;
+            }
+            const float inv = SUM_UNIT / x.sv;
+            if (x.scaled) s_scale[(u0 - lo + lane) % 64] = make_float4(x.sk, __log2f(x.sv), apart ? -inv : inv, 0.f);
             __syncwarp();
             for (; pending > 0; --pending)
                 if (lane == 0) tc::mbar_arrive(full0 + 8 * (stage < pending ? stage - pending + STAGES : stage - pending));
@@ -224,6 +249,7 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
                 if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
             if (pending > 0) place(now, u0);
+            top = max(top, __reduce_max_sync(0xffffffffu, __float_as_uint(now.sv) >> 23));
             now = then;
         }
         if (!ok) tc::drain_after_timeout();                  // a wait ran out: let what is in flight land
@@ -341,7 +367,8 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
             const unsigned char* kt = ring + stage * 2 * tile_bytes;
             const unsigned char* vt = kt + tile_bytes;
             const float4 scales = s_scale[(u - lo) % 64];
-            const float sk = scales.x, lv = scales.y, inv = scales.z;
+            const float sk = scales.x, lv = scales.y;
+            float inv = scales.z;
             const int key_base = tile * AF_PAGE + share;
             float sc[NQ][4];
 #pragma unroll
@@ -385,7 +412,7 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
                         if (key_base + 8 + key_g > pos || key_base + 8 + key_g < low) sc[n][2 + e] = -INFINITY;
                     }
             }
-            bool above = false;
+            bool above = inv < 0.f;                          // or a tile whose denominator is apart
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -401,12 +428,17 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
                         float top = fmaxf(m[n][e], fmaxf(sc[n][e], sc[n][2 + e]));
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                        const float by = power2(m[n][e] - (top == -INFINITY ? 0.f : top));
+                        const float down = m[n][e] - (top == -INFINITY ? 0.f : top), by = power2(down);
                         m[n][e] = top;
-                        l[n][e] *= by;
+                        l[n][e] = scaled(l[n][e], down);
 #pragma unroll
                         for (int i = 0; i < MT; ++i) { o[n][i][e] *= by; o[n][i][2 + e] *= by; }
+                        if (inv < 0.f) {                     // 2^(s - m + 7) is up to 2^115: ten powers more leave room at the other end
+                            const float base = (top == -INFINITY ? 0.f : top - P_POWER) + lv - 10.f;
+                            l[n][e] = fmaf(power2(sc[n][e] - base) + power2(sc[n][2 + e] - base), SUM_UNIT * 0x1p-10f, l[n][e]);
+                        }
                     }
+                inv = fmaxf(inv, 0.f);
             }
             unsigned pf[NQ][2];
 #pragma unroll
@@ -535,10 +567,11 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float f = power2(s_ml[k][r][0] - base);
+                sum += scaled(s_ml[k][r][1], s_ml[k][r][0] - base);
                 const float4 x = *reinterpret_cast<const float4*>(mg + (size_t)(k * M + r) * DP + 4 * piece_at(r, piece));
-                sum = fmaf(s_ml[k][r][1], f, sum);
                 acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
             }
+            acc.x *= SUM_UNIT; acc.y *= SUM_UNIT; acc.z *= SUM_UNIT; acc.w *= SUM_UNIT;
             if (whole) {
                 const int row = at.slab * M + r, i = row / group;
                 __nv_bfloat162* to = reinterpret_cast<__nv_bfloat162*>(a.out + ((size_t)(first_token + i) * a.nq + (size_t)at.kvh * group + (row - i * group)) * D + 4 * piece);

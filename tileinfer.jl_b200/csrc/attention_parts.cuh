@@ -27,6 +27,13 @@ __device__ __forceinline__ float power2(float x) {
     return y;
 }
 
+// sum + part 2^x, x <= 0 and f = 2^x: in two steps where f would have lost bits or be zero (scales of 8-bit pages that lie far apart).
+__device__ __forceinline__ float add_times(float sum, float part, float x, float f) {
+    if (x > -100.f) return fmaf(part, f, sum);
+    const float half = exp2f(0.5f * x);
+    return sum + part * half * half;
+}
+
 // The parts of the rows that several blocks share, joined in ascending order: AF_JOIN_WARPS / WPR rows a block, WPR warps a row, four elements a lane,
 // every WPRth part a warp. Rows of items that one block did are done; rows without keys get zeros. What bounds it is one dependent load after another
 // with the kernel before gone: so where the parts lie is worked out before that kernel ends, and maxima, sums and outputs of eight parts are asked
@@ -82,8 +89,8 @@ __global__ void __launch_bounds__(32 * AF_JOIN_WARPS) attention_few_join_kernel(
                 v[k] = on && p + k * WPR < parts ? __ldcg(reinterpret_cast<const float4*>(ws_o + at(p + k * WPR) * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
             const float top = fmaxf(mm, warp_max(x.x)), base = top == -INFINITY ? 0.f : top;
             const float old = exp2f(mm - base), f = exp2f(x.x - base);
+            sum = add_times(warp_sum(add_times(0.f, x.y, x.x - base, f)), sum, mm - base, old);
             mm = top;
-            sum = sum * old + warp_sum(x.y * f);
             acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -107,7 +114,7 @@ __global__ void __launch_bounds__(32 * AF_JOIN_WARPS) attention_few_join_kernel(
             for (int w = 0; w < WPR; ++w) {
                 const float f = exp2f(s_ml[w].x - base);
                 const float4 v = s_o[w][lane];
-                sum = fmaf(s_ml[w].y, f, sum);
+                sum = add_times(sum, s_ml[w].y, s_ml[w].x - base, f);
                 acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
             }
         }
