@@ -36,6 +36,7 @@
 #include "linear8.cuh"
 #include "mma_util.cuh"
 
+#include <climits>
 #include <cmath>
 
 namespace {
@@ -61,7 +62,8 @@ struct Args8 {
     const unsigned char* v;                                  // for NaN codes that were taken out
     const float *k_scales, *v_scales;
     const int* table;
-    int table_stride;
+    int table_stride, slots, columns;
+    FewLimits limits;
     const int *seq_slots, *cu, *kv_lens;
     float *ws_o, *ws_ml;
     int* status;
@@ -120,8 +122,9 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
         const int b = b0 + threadIdx.x;
         unsigned v = 0;
         if (b < B) {
-            const int at = __ldcg(a.cu + b), end = __ldcg(a.cu + b + 1), len = __ldcg(a.kv_lens + b);
-            s_slot[b] = __ldcg(a.seq_slots + b);
+            const int at = a.limits.row(__ldcg(a.cu + b)), end = a.limits.row(__ldcg(a.cu + b + 1)), len = a.limits.length(__ldcg(a.kv_lens + b));
+            const int slot = __ldcg(a.seq_slots + b);
+            s_slot[b] = slot < a.slots ? slot : -1;          // a slot that does not exist has no pages
             s_cu[b] = at;
             if (b == B - 1) s_cu[B] = end;
             s_len[b] = len;
@@ -186,7 +189,8 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
             Ahead x = {-1, false, true, 1.f, 1.f};
             if (u >= hi) return x;
             const Place p = locate(u);
-            const int tile = p.s.t0 + p.tile, page = tile < a.table_stride ? __ldcg(a.table + (size_t)s_slot[p.b] * a.table_stride + tile) : -1;
+            const int tile = p.s.t0 + p.tile, slot = s_slot[p.b];
+            const int page = slot >= 0 && tile < a.columns ? __ldcg(a.table + (size_t)slot * a.table_stride + tile) : -1;
             // Tiles with new keys were written by the kernel before this one; the others stand since earlier steps.
             x.fresh = (tile + 1) * AF_PAGE > p.s.L - p.s.T;
             if (page >= 0 && page < a.pages) { x.block = page * nkv + p.kvh; x.scaled = false; }                     // a page that does not exist reads as zeros
@@ -513,7 +517,7 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
             auto put_back = [&](int from, int to) {
                 for (int key = max(from, (s.t0 + at.tile) * AF_PAGE); key < min(to, tile * AF_PAGE); ++key) {
                     if (key % AF_PAGE / 16 != warp) continue;
-                    const int page = key / AF_PAGE < a.table_stride ? __ldcg(a.table + (size_t)s_slot[at.b] * a.table_stride + key / AF_PAGE) : -1;
+                    const int slot = s_slot[at.b], page = slot >= 0 && key / AF_PAGE < a.columns ? __ldcg(a.table + (size_t)slot * a.table_stride + key / AF_PAGE) : -1;
                     if (page < 0 || page >= a.pages) continue;
                     const unsigned char* value = a.v + (((size_t)page * nkv + at.kvh) * AF_PAGE + key % AF_PAGE) * D;
 #pragma unroll
@@ -613,7 +617,7 @@ template <int DP, int NQ, bool EXACT> int launch(const Call& c) {
     const int G = S::BLOCKS * ti_sm_count();
     ti_launch(attention8_kernel<DP, NQ, EXACT>, dim3(G), dim3(A8_THREADS), S::bytes(c.a.D), c.stream, c.k, c.v, c.a);
     if (int rc = ti_check_launch("attention8")) return rc;
-    join_parts(c.a.out, c.a.cu, c.a.kv_lens, c.a.ws_o, c.a.ws_ml, c.a.B, c.a.nq, c.a.nkv, c.a.D, S::M, c.max_new, c.a.window, G, c.stream);
+    join_parts(c.a.out, c.a.cu, c.a.kv_lens, c.a.ws_o, c.a.ws_ml, c.a.B, c.a.nq, c.a.nkv, c.a.D, S::M, c.max_new, c.a.window, G, c.a.limits, c.stream);
     return ti_check_launch("attention8_join");
 }
 template <int DP, bool EXACT> int launch_rows(const Call& c, int eights) {
@@ -625,8 +629,9 @@ template <int DP, bool EXACT> int launch_rows(const Call& c, int eights) {
 
 }  // namespace
 
-int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, int* lens_out, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
-                 int table_stride, const int* seq_slots, const int* cu, const int* kv_lens, int B, int nkv, int D, int pages, int per_seq, int window, cudaStream_t stream);
+int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, int* lens_out, int* cu_out, const void* k, const void* v, const float* k_scales, const float* v_scales,
+                 const int* table, int table_stride, int slots, int columns, const int* seq_slots, const int* cu, const int* kv_lens, int B, int n, int nkv, int D, int pages, int per_seq,
+                 int window, cudaStream_t stream);
 extern "C" int ti_attention_prefill_tc(void* out, const void* q, const void* k_cache, const void* v_cache, int n_pages, const int* block_table, int table_stride,
                                        const int* seq_slots, const int* cu_seqlens, const int* kv_lens, int n_seqs, int n_tokens, int total_blocks, float scale, int nq,
                                        int nkv, int D, int page_size, int window, int* status, cudaStream_t stream);
@@ -667,28 +672,29 @@ extern "C" long long ti_attention8_workspace(int B, int max_new, int nq, int nkv
     if (B <= 0 || max_new <= 0 || nq <= 0 || nkv <= 0 || D <= 0) return 0;
     if (ti_attention8_widens(B, max_new, nq, nkv, D, max_len)) {
         const long long turn = widened_at_once(B, nkv, D, max_len), pages = turn * ((max_len + AF_PAGE - 1) / AF_PAGE);
-        return pages * nkv * AF_PAGE * D * 4 + up16(4 * pages) + 2 * up16(4 * turn);
+        return pages * nkv * AF_PAGE * D * 4 + up16(4 * pages) + 2 * up16(4 * turn) + up16(4 * (turn + 1));
     }
     const int eights = slab_eights(max_new * (long long)(nq / nkv), D);
     return 2LL * sm_blocks(eights, D) * ti_sm_count() * 8 * eights * (D + 2) * 4;
 }
 
 // q [n, nq, D] and out [n, nq * D]; pools [pages, nkv, 64, D] with scales [pages, nkv]; the tokens of sequence b are cu[b] to cu[b + 1], at most max_new;
-// kv_lens[b] its length with them, at most max_len; its pages are row seq_slots[b] of table. `status`: the word of bounded waits. Returns 2 for sizes
-// outside what it takes.
-extern "C" int ti_attention8(void* out, const void* q, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
-                             int table_stride, const int* seq_slots, const int* cu, const int* kv_lens, void* ws, long long ws_bytes, int* status, float scale,
-                             int B, int n, int nq, int nkv, int D, int page_size, int max_new, int max_len, int pages, int window, cudaStream_t stream) {
+// kv_lens[b] its length with them, at most max_len; its pages are row seq_slots[b] of table (`slots` rows of `columns`, table_stride apart). Ranges beyond the n rows of q and out are cut to them, a
+// length beyond a row of the table to that, and a slot that does not exist has no pages. `status`: the word of bounded waits. Returns 2 for sizes outside what it takes.
+extern "C" int ti_attention8_table(void* out, const void* q, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
+                                   int table_stride, const int* seq_slots, const int* cu, const int* kv_lens, void* ws, long long ws_bytes, int* status, float scale,
+                                   int B, int n, int nq, int nkv, int D, int page_size, int max_new, int max_len, int pages, int window, int slots, int columns, cudaStream_t stream) {
     if (B == 0 || n == 0 || max_new == 0) return 0;
     TI_REQUIRE(B > 0 && n > 0 && max_new > 0 && nq > 0 && nkv > 0 && D > 0 && window >= 0 && pages > 0, "attention8: %d sequences, %d new tokens, %d / %d heads of %d", B,
                max_new, nq, nkv, D);
+    TI_REQUIRE(slots >= 0 && columns >= 0 && table_stride >= 0, "attention8: a table of %d x %d", slots, columns);
     TI_REQUIRE(scale > 0.f, "attention8: scale must be positive");
     const long long rows = max_new * (long long)(nq / nkv);
     const int eights = nkv > 0 && nq % nkv == 0 ? slab_eights(rows, D) : 1, M = 8 * eights;
     if (page_size != AF_PAGE || D > 256 || D % 16 != 0 || nq % nkv != 0 || nkv > 65535 ||
-        (rows + M - 1) / M * nkv * table_stride * (B < A8_MAX_SEQS ? B : A8_MAX_SEQS) >= 1LL << 31) {
+        (rows + M - 1) / M * nkv * columns * (B < A8_MAX_SEQS ? B : A8_MAX_SEQS) >= 1LL << 31) {
         ti_fail("attention8 takes pages of %d, heads of a multiple of 16 up to 256 and fewer than 2^31 tiles of %d keys; got pages of %d, %d sequences of up to %d pages, %d new "
-                "tokens, %d / %d heads of %d", AF_PAGE, AF_PAGE, page_size, B, table_stride, max_new, nq, nkv, D);
+                "tokens, %d / %d heads of %d", AF_PAGE, AF_PAGE, page_size, B, columns, max_new, nq, nkv, D);
         return 2;
     }
     if ((long long)pages * nkv * (D / 2) > 0x7fffffffLL) {
@@ -705,19 +711,19 @@ extern "C" int ti_attention8(void* out, const void* q, const void* k, const void
         TI_REQUIRE(all * nkv * AF_PAGE <= 0x7fffffffLL, "attention8: %d positions of %d heads are too many for a long run", max_len, nkv);
         TI_REQUIRE(((uintptr_t)q | (uintptr_t)out) % 16 == 0, "attention8: queries and outputs of long runs must be 16-byte aligned");
         bf16 *k16 = (bf16*)ws, *v16 = k16 + pool;
-        int *table16 = (int*)(v16 + pool), *slots16 = table16 + up16(4 * all) / 4, *lens16 = slots16 + up16(4LL * turn) / 4;
+        int *table16 = (int*)(v16 + pool), *slots16 = table16 + up16(4 * all) / 4, *lens16 = slots16 + up16(4LL * turn) / 4, *cu16 = lens16 + up16(4LL * turn) / 4;
         for (int b0 = 0; b0 < B; b0 += turn) {
             const int these = B - b0 < turn ? B - b0 : turn;
-            if (int rc = cache_widen8(k16, v16, table16, slots16, lens16, k, v, k_scales, v_scales, table, table_stride, seq_slots + b0, cu + b0, kv_lens + b0, these, nkv, D, pages,
-                                      per_seq, window, stream)) return rc;
+            if (int rc = cache_widen8(k16, v16, table16, slots16, lens16, cu16, k, v, k_scales, v_scales, table, table_stride, slots, columns, seq_slots + b0, cu + b0, kv_lens + b0, these, n, nkv,
+                                      D, pages, per_seq, window, stream)) return rc;
             // As many blocks as the runs can need: those beyond leave at once.
             const bool fifth = D == 64 || D == 128;          // generation of tensor cores
             const int tokens = (fifth ? 2 : 1) * (128 / (nq / nkv)), blocks = n / tokens + (these < n ? these : n);
             const long long most = (long long)these * (((long long)max_new + tokens - 1) / tokens);
             const int grid = blocks < most ? blocks : (int)most;
-            if (int rc = fifth ? ti_attention_prefill_tc(out, q, k16, v16, (int)all, table16, per_seq, slots16, cu + b0, lens16, these, n, grid, scale, nq, nkv, D, page_size,
+            if (int rc = fifth ? ti_attention_prefill_tc(out, q, k16, v16, (int)all, table16, per_seq, slots16, cu16, lens16, these, n, grid, scale, nq, nkv, D, page_size,
                                                          window, status, stream)
-                               : ti_attention_prefill(out, q, k16, v16, table16, per_seq, slots16, cu + b0, lens16, these, grid, scale, nq, nkv, D, page_size, window, stream)) return rc;
+                               : ti_attention_prefill(out, q, k16, v16, table16, per_seq, slots16, cu16, lens16, these, grid, scale, nq, nkv, D, page_size, window, stream)) return rc;
         }
         return 0;
     }
@@ -729,12 +735,20 @@ extern "C" int ti_attention8(void* out, const void* q, const void* k, const void
     const unsigned box[2] = {64, (unsigned)D / 2};
     if (int rc = ti_tensor_map_bf16(&c.k, k, 2, dims, strides, box, true)) return rc;
     if (int rc = ti_tensor_map_bf16(&c.v, v, 2, dims, strides, box, true)) return rc;
-    const long long slots = 2LL * sm_blocks(eights, D) * ti_sm_count();
+    const long long parts = 2LL * sm_blocks(eights, D) * ti_sm_count(), positions = (long long)columns * AF_PAGE;
+    const FewLimits limits = {n, positions < INT_MAX / 2 ? (int)positions : INT_MAX / 2};
     for (int b0 = 0; b0 < B; b0 += A8_MAX_SEQS) {            // the sequences in turns of as many as a launch takes
-        c.a = Args8{(bf16*)out, (const bf16*)q, (const unsigned char*)v, k_scales, v_scales, table, table_stride, seq_slots + b0, cu + b0, kv_lens + b0, (float*)ws,
-                    (float*)ws + slots * M * D, status, scale * 1.4426950408889634f, B - b0 < A8_MAX_SEQS ? B - b0 : A8_MAX_SEQS, nq, nkv, D, window, pages};
+        c.a = Args8{(bf16*)out, (const bf16*)q, (const unsigned char*)v, k_scales, v_scales, table, table_stride, slots, columns, limits, seq_slots + b0, cu + b0, kv_lens + b0, (float*)ws,
+                    (float*)ws + parts * M * D, status, scale * 1.4426950408889634f, B - b0 < A8_MAX_SEQS ? B - b0 : A8_MAX_SEQS, nq, nkv, D, window, pages};
         if (int rc = D == 64 ? launch_rows<64, true>(c, eights) : D == 128 ? launch_rows<128, true>(c, eights) : D == 256 ? launch_rows<256, true>(c, eights) :
                      D < 64 ? launch_rows<64, false>(c, eights) : D < 128 ? launch_rows<128, false>(c, eights) : launch_rows<256, false>(c, eights)) return rc;
     }
     return 0;
+}
+// The same where every slot exists and a row has as many columns as its pitch.
+extern "C" int ti_attention8(void* out, const void* q, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
+                             int table_stride, const int* seq_slots, const int* cu, const int* kv_lens, void* ws, long long ws_bytes, int* status, float scale,
+                             int B, int n, int nq, int nkv, int D, int page_size, int max_new, int max_len, int pages, int window, cudaStream_t stream) {
+    return ti_attention8_table(out, q, k, v, k_scales, v_scales, table, table_stride, seq_slots, cu, kv_lens, ws, ws_bytes, status, scale, B, n, nq, nkv, D, page_size, max_new,
+                               max_len, pages, window, INT_MAX, table_stride, stream);
 }

@@ -11,6 +11,12 @@ namespace {
 struct FewShape {
     int T, L, first, t0, tiles, slabs;                       // new tokens, length, first visible key, first tile, tiles, slabs of rows
 };
+// What is given for a batch may be wrong: ranges stay within the n rows that there are, lengths within the positions that a sequence's row of the table has pages for.
+struct FewLimits {
+    int rows, positions;
+    __device__ __forceinline__ int row(int at) const { return min(max(at, 0), rows); }
+    __device__ __forceinline__ int length(int len) const { return min(max(len, 0), positions); }
+};
 __device__ __forceinline__ FewShape few_shape(int T, int L, int window, int group, int M) {
     FewShape s;
     s.T = T; s.L = L;
@@ -42,14 +48,14 @@ __device__ __forceinline__ float add_times(float sum, float part, float x, float
 template <int WPR>
 __global__ void __launch_bounds__(32 * AF_JOIN_WARPS) attention_few_join_kernel(bf16* out, const int* cu, const int* kv_lens, const float* ws_o,
                                                                                 const float* ws_ml, int B, int nq, int nkv, int D, int M, int window,
-                                                                                int blocks) {
+                                                                                int blocks, FewLimits limits) {
     __shared__ unsigned s_sum[AF_JOIN_WARPS][2];
     __shared__ float4 s_o[WPR > 1 ? WPR : 1][32];
     __shared__ float2 s_ml[WPR];
     const int b = blockIdx.z, kvh = blockIdx.y, group = nq / nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned before = 0, U = 0;
     for (int c = threadIdx.x; c < B; c += 32 * AF_JOIN_WARPS) {
-        const FewShape s = few_shape(__ldcg(cu + c + 1) - __ldcg(cu + c), __ldcg(kv_lens + c), window, group, M);
+        const FewShape s = few_shape(limits.row(__ldcg(cu + c + 1)) - limits.row(__ldcg(cu + c)), limits.length(__ldcg(kv_lens + c)), window, group, M);
         U += s.tiles * s.slabs * nkv;
         if (c < b) before += s.tiles * s.slabs * nkv;
     }
@@ -60,8 +66,8 @@ __global__ void __launch_bounds__(32 * AF_JOIN_WARPS) attention_few_join_kernel(
     before = U = 0;
 #pragma unroll
     for (int w = 0; w < AF_JOIN_WARPS; ++w) { before += s_sum[w][0]; U += s_sum[w][1]; }
-    const int first_token = __ldcg(cu + b), T = __ldcg(cu + b + 1) - first_token, row = blockIdx.x * (AF_JOIN_WARPS / WPR) + warp / WPR, mine = warp % WPR;
-    const FewShape s = few_shape(T, __ldcg(kv_lens + b), window, group, M);
+    const int first_token = limits.row(__ldcg(cu + b)), T = limits.row(__ldcg(cu + b + 1)) - first_token, row = blockIdx.x * (AF_JOIN_WARPS / WPR) + warp / WPR, mine = warp % WPR;
+    const FewShape s = few_shape(T, limits.length(__ldcg(kv_lens + b)), window, group, M);
     const int i = row / group, slab = row / M, in = row - slab * M;
     const Runs runs(U, max(min((unsigned)blocks, U), 1u));
     const unsigned u0 = before + (unsigned)((kvh * s.slabs + slab) * s.tiles);
@@ -130,12 +136,12 @@ __global__ void __launch_bounds__(32 * AF_JOIN_WARPS) attention_few_join_kernel(
 
 // Joins what `blocks` blocks have left of the rows of slabs of M.
 inline void join_parts(bf16* out, const int* cu, const int* kv_lens, const float* ws_o, const float* ws_ml, int B, int nq, int nkv, int D, int M, int max_new,
-                       int window, int blocks, cudaStream_t stream) {
+                       int window, int blocks, FewLimits limits, cudaStream_t stream) {
     const int rows = max_new * (nq / nkv);
     // More than eight parts an item: four warps a row (59.9 us in place of 62.3 at 37 parts; at two parts 90 in place of 70).
     const bool deep = 8LL * B * nkv * ((rows + M - 1) / M) < blocks;
     ti_launch(deep ? attention_few_join_kernel<4> : attention_few_join_kernel<1>, dim3(deep ? rows : (rows + AF_JOIN_WARPS - 1) / AF_JOIN_WARPS, nkv, B),
-              dim3(32 * AF_JOIN_WARPS), 0, stream, out, cu, kv_lens, ws_o, ws_ml, B, nq, nkv, D, M, window, blocks);
+              dim3(32 * AF_JOIN_WARPS), 0, stream, out, cu, kv_lens, ws_o, ws_ml, B, nq, nkv, D, M, window, blocks, limits);
 }
 
 }  // namespace

@@ -29,7 +29,7 @@ struct Rows {
 // blockIdx.x: sequence x page from the one with its first new position; blockIdx.y: head, keys or values. NT threads, J eights of new rows each.
 template <typename T, bool VEC, int NT, int J>
 __global__ void __launch_bounds__(NT) cache_write8_kernel(unsigned char* k_codes, unsigned char* v_codes, float* k_scales, float* v_scales, Rows k, Rows v,
-                                                               const int* table, int table_stride, int slots, const int* seq_slots, const int* cu,
+                                                               const int* table, int table_stride, int slots, int columns, const int* seq_slots, const int* cu,
                                                                const int* kv_lens, int n, int nkv, int D, int pages, int touched, bool beside) {
     __shared__ float scratch[33];
     const int b = blockIdx.x / touched, kvh = blockIdx.y >> 1, is_v = blockIdx.y & 1;
@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(NT) cache_write8_kernel(unsigned char* k_codes
     const int begin = __ldcg(cu + b), T_new = __ldcg(cu + b + 1) - begin, L = __ldcg(kv_lens + b), slot = __ldcg(seq_slots + b);
     const int start = L - T_new, logical = start / PAGE + blockIdx.x % touched, base = logical * PAGE;
     // What does not fit (a length below the run's, a slot or page that does not exist) is not written.
-    if (T_new <= 0 || start < 0 || base >= L || begin < 0 || begin + T_new > n || slot < 0 || slot >= slots || logical >= table_stride) return;
+    if (T_new <= 0 || start < 0 || base >= L || begin < 0 || begin + T_new > n || slot < 0 || slot >= slots || logical >= columns) return;
     const int page = __ldcg(table + (size_t)slot * table_stride + logical);
     if (page < 0 || page >= pages) return;
     const int first = max(start - base, 0), rows = min(L - base, PAGE) - first;
@@ -90,19 +90,27 @@ __global__ void __launch_bounds__(NT) cache_write8_kernel(unsigned char* k_codes
 }
 
 // blockIdx: page, head, sequence.
-__global__ void __launch_bounds__(THREADS) cache_widen8_kernel(bf16* k_out, bf16* v_out, int* table_out, int* slots_out, int* lens_out, const unsigned char* k, const unsigned char* v,
-                                                               const float* k_scales, const float* v_scales, const int* table, int table_stride, const int* seq_slots,
-                                                               const int* cu, const int* kv_lens, int nkv, int D, int pages, int per_seq, int window) {
+__global__ void __launch_bounds__(THREADS) cache_widen8_kernel(bf16* k_out, bf16* v_out, int* table_out, int* slots_out, int* lens_out, int* cu_out, const unsigned char* k, const unsigned char* v,
+                                                               const float* k_scales, const float* v_scales, const int* table, int table_stride, int slots,
+                                                               int columns, const int* seq_slots, const int* cu, const int* kv_lens, int n, int nkv, int D, int pages,
+                                                               int per_seq, int window) {
     const int j = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     pdl_enter();
-    const int T_new = __ldcg(cu + b + 1) - __ldcg(cu + b), L = __ldcg(kv_lens + b), slot = __ldcg(seq_slots + b);
+    // Readers stay within the table and the n rows of queries, whatever they were given.
+    const int begin = min(max(__ldcg(cu + b), 0), n), end = min(max(__ldcg(cu + b + 1), 0), n), T_new = end - begin;
+    const int L = min(max(__ldcg(kv_lens + b), 0), per_seq * PAGE), slot = __ldcg(seq_slots + b);
     if (kvh == 0 && threadIdx.x == 0) {
         table_out[(size_t)b * per_seq + j] = b * per_seq + j;
-        if (j == 0) { slots_out[b] = b; lens_out[b] = min(L, per_seq * PAGE); }             // readers stay within the table, whatever they were given
+        if (j == 0) {
+            slots_out[b] = b;
+            lens_out[b] = L;
+            cu_out[b] = begin;
+            if (b == gridDim.z - 1) cu_out[b + 1] = end;
+        }
     }
     const int first = window > 0 ? max(0, L - T_new - window + 1) : 0;
     if (T_new <= 0 || j * PAGE >= L || j < first / PAGE / 2 * 2) return;              // the readers walk the pages in pairs
-    const int page = j < table_stride && (j + 1) * PAGE > first ? __ldcg(table + (size_t)slot * table_stride + j) : -1;
+    const int page = slot >= 0 && slot < slots && j < columns && (j + 1) * PAGE > first ? __ldcg(table + (size_t)slot * table_stride + j) : -1;
     const bool there = page >= 0 && page < pages;
     const size_t from = ((size_t)page * nkv + kvh) * PAGE * D, to = (((size_t)b * per_seq + j) * nkv + kvh) * PAGE * D;
     const float sk = there ? __ldcg(k_scales + (size_t)page * nkv + kvh) : 0.f, sv = there ? __ldcg(v_scales + (size_t)page * nkv + kvh) : 0.f;
@@ -131,12 +139,12 @@ __global__ void __launch_bounds__(THREADS) cache_widen8_kernel(bf16* k_out, bf16
 }  // namespace
 
 // k and v: [n, nkv, D] rows of `dtype` with the given pitches of tokens and heads (in elements); pools [pages, nkv, 64, D] and scales [pages, nkv]; the page of
-// sequence b's positions from 64 i on is table[seq_slots[b], i] ([slots, table_stride]). max_new: the most new positions of a sequence.
-extern "C" int ti_cache_write8(void* k_codes, void* v_codes, float* k_scales, float* v_scales, const void* k, long long k_token, long long k_head, const void* v,
-                               long long v_token, long long v_head, const int* table, int table_stride, int slots, const int* seq_slots, const int* cu,
-                               const int* kv_lens, int B, int n, int nkv, int D, int page_size, int pages, int max_new, int dtype, cudaStream_t stream) {
+// sequence b's positions from 64 i on is table[seq_slots[b], i] ([slots, columns], rows table_stride apart). max_new: the most new positions of a sequence.
+extern "C" int ti_cache_write8_table(void* k_codes, void* v_codes, float* k_scales, float* v_scales, const void* k, long long k_token, long long k_head, const void* v,
+                                     long long v_token, long long v_head, const int* table, int table_stride, int slots, const int* seq_slots, const int* cu,
+                                     const int* kv_lens, int B, int n, int nkv, int D, int page_size, int pages, int max_new, int dtype, int columns, cudaStream_t stream) {
     if (B == 0 || n == 0 || max_new == 0) return 0;
-    TI_REQUIRE(B > 0 && n > 0 && max_new > 0 && nkv > 0 && pages > 0 && slots > 0 && table_stride > 0, "cache_write8: %d sequences, %d tokens", B, n);
+    TI_REQUIRE(B > 0 && n > 0 && max_new > 0 && nkv > 0 && pages > 0 && slots > 0 && columns > 0 && table_stride >= 0, "cache_write8: %d sequences, %d tokens", B, n);
     if (page_size != PAGE || D <= 0 || D > 256 || D % 16 != 0 || nkv > 32767) {
         ti_fail("cache_write8 takes pages of %d and heads of a multiple of 16 up to 256; got pages of %d, %d heads of %d", PAGE, page_size, nkv, D);
         return 2;
@@ -155,14 +163,23 @@ extern "C" int ti_cache_write8(void* k_codes, void* v_codes, float* k_scales, fl
                                             D <= 128 ? (vec ? cache_write8_kernel<T, true, THREADS, 4> : cache_write8_kernel<T, false, THREADS, 4>) :
                                                        (vec ? cache_write8_kernel<T, true, THREADS, 8> : cache_write8_kernel<T, false, THREADS, 8>);
                       ti_launch(kernel, dim3((unsigned)(touched * B), 2 * nkv), dim3(few ? 64 : THREADS), 0, stream, (unsigned char*)k_codes, (unsigned char*)v_codes,
-                                k_scales, v_scales, kr, vr, table, table_stride, slots, seq_slots, cu, kv_lens, n, nkv, D, pages, (int)touched, max_new == 1));
+                                k_scales, v_scales, kr, vr, table, table_stride, slots, columns, seq_slots, cu, kv_lens, n, nkv, D, pages, (int)touched, max_new == 1));
     return ti_check_launch("cache_write8");
 }
 
-// For attention8.cu: pools k_out, v_out [B * per_seq, nkv, 64, D] bfloat16, table_out [B, per_seq], slots_out [B], lens_out [B].
-int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, int* lens_out, const void* k, const void* v, const float* k_scales, const float* v_scales, const int* table,
-                 int table_stride, const int* seq_slots, const int* cu, const int* kv_lens, int B, int nkv, int D, int pages, int per_seq, int window, cudaStream_t stream) {
-    ti_launch(cache_widen8_kernel, dim3(per_seq, nkv, B), dim3(THREADS), 0, stream, (bf16*)k_out, (bf16*)v_out, table_out, slots_out, lens_out, (const unsigned char*)k,
-              (const unsigned char*)v, k_scales, v_scales, table, table_stride, seq_slots, cu, kv_lens, nkv, D, pages, per_seq, window);
+// The same where a row of the table has as many columns as its pitch.
+extern "C" int ti_cache_write8(void* k_codes, void* v_codes, float* k_scales, float* v_scales, const void* k, long long k_token, long long k_head, const void* v,
+                               long long v_token, long long v_head, const int* table, int table_stride, int slots, const int* seq_slots, const int* cu,
+                               const int* kv_lens, int B, int n, int nkv, int D, int page_size, int pages, int max_new, int dtype, cudaStream_t stream) {
+    return ti_cache_write8_table(k_codes, v_codes, k_scales, v_scales, k, k_token, k_head, v, v_token, v_head, table, table_stride, slots, seq_slots, cu, kv_lens, B, n, nkv, D,
+                                 page_size, pages, max_new, dtype, table_stride, stream);
+}
+
+// For attention8.cu: pools k_out, v_out [B * per_seq, nkv, 64, D] bfloat16, table_out [B, per_seq], slots_out [B], lens_out [B], cu_out [B + 1].
+int cache_widen8(void* k_out, void* v_out, int* table_out, int* slots_out, int* lens_out, int* cu_out, const void* k, const void* v, const float* k_scales, const float* v_scales,
+                 const int* table, int table_stride, int slots, int columns, const int* seq_slots, const int* cu, const int* kv_lens, int B, int n, int nkv, int D, int pages, int per_seq,
+                 int window, cudaStream_t stream) {
+    ti_launch(cache_widen8_kernel, dim3(per_seq, nkv, B), dim3(THREADS), 0, stream, (bf16*)k_out, (bf16*)v_out, table_out, slots_out, lens_out, cu_out, (const unsigned char*)k,
+              (const unsigned char*)v, k_scales, v_scales, table, table_stride, slots, columns, seq_slots, cu, kv_lens, n, nkv, D, pages, per_seq, window);
     return ti_check_launch("cache_widen8");
 }

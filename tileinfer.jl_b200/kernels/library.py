@@ -99,7 +99,7 @@ _SIGNATURES = {
 }
 
 
-_KERNELS_PER_CALL = {"ti_attention_few": 2, "ti_attention8": 2, "ti_memory_chunks": 3, "ti_ssm_chunks": 3, "ti_ssm_chunks_tc": 3}
+_KERNELS_PER_CALL = {"ti_attention_few": 2, "ti_attention8": 2, "ti_attention8_table": 2, "ti_memory_chunks": 3, "ti_ssm_chunks": 3, "ti_ssm_chunks_tc": 3}
 
 
 def lib():
@@ -300,3 +300,6 @@ _SIGNATURES.update({
     "ti_cache_write8": [_P, _P, _P, _P, _P, _L, _L, _P, _L, _L, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "ti_attention8": [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _L, _P, _F, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
 })
+# ... with the numbers of the table's columns, and of its rows and columns, before the stream
+_SIGNATURES["ti_cache_write8_table"] = _SIGNATURES["ti_cache_write8"][:-1] + [_I, _P]
+_SIGNATURES["ti_attention8_table"] = _SIGNATURES["ti_attention8"][:-1] + [_I, _I, _P]

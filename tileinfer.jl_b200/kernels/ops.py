@@ -1370,9 +1370,10 @@ def cache_write8(k_cache, v_cache, k_scales, v_scales, k, v, block_table, seq_sl
         return
     k_token, k_head, _ = k.stride()
     v_token, v_head, _ = v.stride()
-    rc = lib().ti_cache_write8(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), k.data_ptr(), k_token, k_head, v.data_ptr(), v_token,
-                               v_head, block_table.data_ptr(), block_table.stride(0), block_table.shape[0], seq_slots.data_ptr(), cu_seqlens.data_ptr(),
-                               kv_lens.data_ptr(), seqs, shape[0], shape[1], shape[2], PAGE8, k_cache.shape[0], max_new, BF16 if dtype is _BF16 else F32, _stream())
+    rc = lib().ti_cache_write8_table(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), k.data_ptr(), k_token, k_head, v.data_ptr(), v_token,
+                                     v_head, block_table.data_ptr(), block_table.stride(0), block_table.shape[0], seq_slots.data_ptr(), cu_seqlens.data_ptr(),
+                                     kv_lens.data_ptr(), seqs, shape[0], shape[1], shape[2], PAGE8, k_cache.shape[0], max_new, BF16 if dtype is _BF16 else F32,
+                                     block_table.shape[1], _stream())
     if rc:
         check(rc, "cache_write8")
 
@@ -1398,11 +1399,16 @@ def attention8(out, q, k_cache, v_cache, k_scales, v_scales, block_table, seq_sl
     cu_seqlens[b] to cu_seqlens[b + 1] of q [n, nq, head_dim] (at most ``max_new``, or none) are the last of the kv_lens[b] positions of the sequence in slot
     seq_slots[b], and see those up to themselves, with ``window`` > 0 the last so many. out [n, nq * head_dim]; q and out bfloat16. A key stands for its code times
     k_scales[page, head], a value for its code times v_scales[page, head] (positive, 2^-100 to 2^120). ``max_len``: no kv_lens is larger (None: as many as the
-    table's rows have pages for). A page that does not exist reads as zeros. What no token sees may hold any codes; a NaN code that some see reaches those alone. Long
-    runs go through pages widened to bfloat16: codes times scales that are no powers of two are rounded to it, and a NaN value that some rows of a run see may
-    reach others of the run; their q and out must be 16-byte aligned (others' 4-byte). Lengths, ranges, slots, table, and the pages before those of the new tokens
-    are read while the kernel ahead may still run: they come from ``cache_write8``, copies or torch's operations, beside which nothing starts that could miss
-    what they write. ``workspace``: ``attention8_workspace`` bytes (uint8); without it one kept per thread and stream (a captured call: one of its graph's own)."""
+    table's rows have pages for; a longer one counts as that).
+
+    A page that does not exist, or whose slot does not, reads as zeros; of ranges beyond the n rows nothing is read or written; a sequence shorter than its new
+    tokens gets results that mean nothing. What no token sees may hold any codes; a NaN code that some see reaches those alone. Long runs go through pages widened
+    to bfloat16: codes times scales that are no powers of two are rounded to it, and a NaN value that some rows of a run see may reach others of the run; their q
+    and out must be 16-byte aligned (others' 4-byte).
+
+    Lengths, ranges, slots, table, and the pages before those of the new tokens are read while the kernel ahead may still run: they come from ``cache_write8``,
+    copies or torch's operations, beside which nothing starts that could miss what they write. ``workspace``: ``attention8_workspace`` bytes (uint8); without it one
+    kept per thread and stream (a captured call: one of its graph's own)."""
     seqs, n = kv_lens.numel(), q.shape[0]
     if not (_paged8_fits(k_cache, v_cache, k_scales, v_scales, block_table, seq_slots, cu_seqlens, kv_lens, page_size, seqs) and out.is_cuda and q.is_cuda and
             out.dtype is _BF16 and q.dtype is _BF16 and out.is_contiguous() and q.is_contiguous() and nkv > 0 and nq > 0 and nq % nkv == 0 and head_dim > 0 and
@@ -1417,9 +1423,9 @@ def attention8(out, q, k_cache, v_cache, k_scales, v_scales, block_table, seq_sl
     max_len = whole if max_len is None else min(max_len, whole)
     need = attention8_workspace(seqs, max_new, nq, nkv, head_dim, max_len)
     ws, size, _held = _workspace("attention8", need, q.device, stream) if workspace is None else _need_workspace(workspace, need, "attention8")
-    rc = lib().ti_attention8(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(),
-                             block_table.stride(0), seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), ws, size, status_word().data_ptr(), scale, seqs, n,
-                             nq, nkv, head_dim, page_size, max_new, max_len, k_cache.shape[0], window or 0, stream)
+    rc = lib().ti_attention8_table(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(),
+                                   block_table.stride(0), seq_slots.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), ws, size, status_word().data_ptr(), scale, seqs, n,
+                                   nq, nkv, head_dim, page_size, max_new, max_len, k_cache.shape[0], window or 0, *block_table.shape, stream)
     if rc:
         check(rc, "attention8")
     if seqs > 1 and (seqs > ATTENTION8_MAX_SEQS or max_new > 1):
