@@ -242,16 +242,19 @@ int few_split(int out, int K, int warps) {
     while (split < MAX_SPLIT && 2 * split <= groups && (2LL * split * tiles <= 2 * ti_sm_count() || few_bytes((groups + split - 1) / split, warps) > MAX_SMEM)) split *= 2;
     return few_bytes((groups + split - 1) / split, warps) > MAX_SMEM ? 0 : split;
 }
-// Groups of sixteen rows that the busiest SM reads.
+// Groups of sixteen rows that the busiest SM reads, where the tokens' codes fit.
 long long few_load(int out, int K, int warps) {
     const int groups = (K + KB - 1) / KB, split = few_split(out, K, warps);
     const long long blocks = (long long)((out + 16 * warps - 1) / (16 * warps)) * split, sms = ti_sm_count();
-    return split == 0 ? 1LL << 62 : (blocks + sms - 1) / sms * warps * ((groups + split - 1) / split);
+    return (blocks + sms - 1) / sms * warps * ((groups + split - 1) / split);
 }
 // Warps of a block: eight, or the most that leave the busiest SM at least a fifth less to read (168 blocks of 128 rows leave 20 of 148 SMs two). Microseconds for
 // one and eight tokens with 8, 7, 6, 5: 21,504 x 4,096 19.9 / 22.5, 19.7 / 22.7, 18.1 / 21.2, 18.3 / 21.8 (6 is taken); 6,144 x 4,096 7.7 / 9.0, 7.5 / 9.7, 7.2 / 9.4 (6),
 // 9.7 / 14.1; 4,096 x 21,504 17.6 / 20.5 (8), 26.1 / 29.6, 22.1 / 25.8, 23.2 / 25.3.
+// Rows of more than 44,032 columns, whose tokens' codes fit beside four to seven warps alone, are linear8_mid.cu's: one and eight tokens of 4,096 x 50,000 53.0 / 63.9 here,
+// 40.3 / 42.1 there; 4,096 x 72,000 66.2 / 74.4, 52.5 / 53.6; 512 x 50,000 20.1 / 29.8, 25.3 / 25.9.
 int few_warps(int out, int K) {
+    if (few_split(out, K, WARPS) == 0) return WARPS;
     int w = WARPS;
     while (--w >= 4)
         if (few_load(out, K, w) * 5 <= few_load(out, K, WARPS) * 4) return w;
