@@ -16,6 +16,8 @@ from ..kernels import ops
 from .base import CacheRequest, Mixer, register_mixer
 from .linear import Linear
 
+PARTS8 = 8 << 20             # what attention over the 8-bit cache needs at most where it widens no pages (two parts a block of up to 24 rows of 128)
+
 
 @register_mixer("attention")
 class Attention(Mixer):
@@ -107,5 +109,10 @@ class Attention(Mixer):
         # A captured step is replayed at any length.
         longest = meta.block_table.shape[1] * cache.page_size if step.is_decode else step.max_kv_len
         need = ops.attention8_workspace(step.n_seqs, step.max_q_len, nq, nkv, D, longest)
+        # Widened pages of long runs grow with the sequences: in a scratch buffer every longer one would drop the captured steps, and stay.
+        if step.is_decode or need <= PARTS8:
+            space = rt.buffer("attention.parts8", (max(need, PARTS8),), torch.uint8)
+        else:
+            space = torch.empty(need, dtype=torch.uint8, device=q.device)
         ops.attention8(attn, q, cache.k, cache.v, k_scales, v_scales, *where, s.scale, nq, nkv, D, cache.page_size, step.max_q_len, window=s.window or 0, max_len=longest,
-                       workspace=rt.buffer("attention.parts8", (need,), torch.uint8))
+                       workspace=space)
