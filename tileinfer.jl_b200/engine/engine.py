@@ -48,7 +48,8 @@ class Engine:
                  graphs: bool = True, model_factory=None, cache: str = "model", weights: str = "model", take_tensors: bool = False):
         """``cache``: "model" (keys and values in the element type) or "e4m3" (8 bits, a scale for each page of 64 positions and KV head). ``weights``: "model"
         or "e4m3" (the matrices of products and head in 8 bits, a scale for each 128 x 128, their inputs quantised on the way). Both take models of plain
-        attention and feed-forward layers in bfloat16. ``take_tensors``: ``tensors`` is emptied once the model is made, so that matrices in the element type go
+        attention and feed-forward layers in bfloat16; the cache pages of 64 positions and heads of a multiple of 16 up to 256, the matrices multiples of 16
+        inputs. ``take_tensors``: ``tensors`` is emptied once the model is made, so that matrices in the element type go
         one by one as those in 8 bits are made from them."""
         for name, value in (("cache", cache), ("weights", weights)):
             if value not in ("model", "e4m3"):
@@ -58,7 +59,7 @@ class Engine:
         self.dtype = _DTYPES[dtype]
         self.spec = config.model_spec()
         if "e4m3" in (cache, weights):
-            self._check8(kernels, page_size)
+            self._check8(kernels, page_size, cache == "e4m3", weights == "e4m3")
         self.rt = Runtime(self.dtype, self.device, kernels, cache8=cache == "e4m3")
         max_context = int(min(max_context or self.spec.max_positions, self.spec.max_positions))
         self.max_context = max_context
@@ -82,15 +83,22 @@ class Engine:
         self.vocab_size = self.spec.vocab_size
         self._start_planning()
 
-    def _check8(self, kernels: str, page_size: int) -> None:
+    def _check8(self, kernels: str, page_size: int, cache: bool = True, weights: bool = False) -> None:
+        """Before anything is loaded: ``cache``, ``weights``: which of the two are to be held in 8 bits."""
         from .drafting import FEED_FORWARDS, MIXERS
-        if self.dtype != torch.bfloat16 or kernels != "fast" or page_size != DEFAULT_PAGE_SIZE:
-            raise ValueError(f"8 bits go with bfloat16, the fast kernels and pages of {DEFAULT_PAGE_SIZE}")
+        pages = f" and pages of {DEFAULT_PAGE_SIZE}"
+        if self.dtype != torch.bfloat16 or kernels != "fast" or (cache and page_size != DEFAULT_PAGE_SIZE):
+            raise ValueError(f"8 bits go with bfloat16{', the fast kernels' + pages if cache else ' and the fast kernels'}")
         for layer in self.spec.layers:
             mixer, ff = layer.mixer, layer.feed_forward
-            if mixer.kind not in MIXERS or (ff is not None and ff.kind not in FEED_FORWARDS) or mixer.head_dim % 16 or mixer.head_dim > ops.HEAD8:
-                raise ValueError(f"8 bits go with layers of {', '.join(MIXERS)} (heads of a multiple of 16 up to {ops.HEAD8}) and {', '.join(FEED_FORWARDS)}, not of "
-                                 f"{mixer.kind} (heads of {getattr(mixer, 'head_dim', None)}) and {ff.kind if ff is not None else 'none'}")
+            dim = getattr(mixer, "head_dim", None)
+            if mixer.kind not in MIXERS or (ff is not None and ff.kind not in FEED_FORWARDS) or (cache and (dim % 16 or dim > ops.HEAD8)):
+                heads = f" (heads of a multiple of 16 up to {ops.HEAD8})" if cache else ""
+                raise ValueError(f"8 bits go with layers of {', '.join(MIXERS)}{heads} and {', '.join(FEED_FORWARDS)}, not of {mixer.kind} (heads of {dim}) and "
+                                 f"{ff.kind if ff is not None else 'none'}")
+            inputs = (mixer.hidden_size, mixer.num_heads * dim) + ((ff.intermediate_size,) if ff is not None else ())
+            if weights and any(n % 16 for n in inputs):
+                raise ValueError(f"matrices in 8 bits have a multiple of 16 inputs, not {next(n for n in inputs if n % 16)}")
 
     def _start_planning(self) -> None:
         """A planner for this engine's steps, and no graphs yet."""
