@@ -6,6 +6,10 @@ model runs the drafted tokens through one step of its own, which writes their ke
 place. The longest run of drafted tokens that stands is kept, with one token more: at temperature 0 a drafted token stands while it is the model's
 own choice, else by the test of ``ops.verify_drafts``, so that every token is distributed as one sampled from the model (not the same token as
 without a draft: the uniform numbers are used up in another order). Sequences that cannot be cut back (recurrent states, windows) take no draft.
+
+Over a cache in 8 bits the model is the one that the cache makes of it, and drafts leave a trace there: a page's scale does not shrink while rows are added to it, so the draft's
+own rows and those that are cut back may raise it. What of the page's kept rows lies below 2^-6 of the larger scale is then rounded to steps of 2^-9 of it: off by
+at most 2^-10 of a scale whose largest value is 224 to 448. Without a draft those rows keep the bits below.
 """
 from __future__ import annotations
 

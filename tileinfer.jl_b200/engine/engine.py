@@ -49,7 +49,9 @@ class Engine:
         """``cache``: "model" (keys and values in the element type) or "e4m3" (8 bits, a scale for each page of 64 positions and KV head). ``weights``: "model"
         or "e4m3" (the matrices of products and head in 8 bits, a scale for each 128 x 128, their inputs quantised on the way). Both take models of plain
         attention and feed-forward layers in bfloat16; the cache pages of 64 positions and heads of a multiple of 16 up to 256, the matrices multiples of 16
-        inputs. ``take_tensors``: ``tensors`` is emptied once the model is made, so that matrices in the element type go
+        inputs. The cache in 8 bits is for its memory, and pays in time where a step reads much of it (a 16-layer model of 8B sizes, bfloat16 / 8-bit cache: 64
+        sequences of 1,023 positions 3.00 / 2.78 ms, one of 32,768 1.92 / 1.82; one of 1,023 1.52 / 1.54, as its rows are written by a launch of their own);
+        matrices in 8 bits pay in every step of few tokens. ``take_tensors``: ``tensors`` is emptied once the model is made, so that matrices in the element type go
         one by one as those in 8 bits are made from them."""
         for name, value in (("cache", cache), ("weights", weights)):
             if value not in ("model", "e4m3"):
@@ -164,7 +166,8 @@ class Engine:
         """Forget the positions of a sequence after its first ``length``: the next step continues from
         there (the reference rolls a sequence back the same way, src/kv/block_manager.jl:74-81, to drop a
         token that went through the model but is not kept). Pages beyond the new length go back to the
-        pool; nothing is cleared, the next tokens overwrite what was there. Layers with a per-sequence
+        pool; nothing is cleared, the next tokens overwrite what was there (a page of an 8-bit cache keeps the scale that the forgotten rows gave it until it is
+        written from its first position). Layers with a per-sequence
         state, or a window whose pages were already given back, cannot roll back and raise."""
         self.cache.truncate(slot, length)
 
