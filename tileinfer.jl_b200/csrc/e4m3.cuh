@@ -4,18 +4,11 @@
 #pragma once
 #include "common.cuh"
 
-#include <cstring>
-
 #define E4M3_BLOCK 128                   // columns (and, of weights, rows) that share a scale in a matrix
 
 // The scale of blocks whose largest finite |x| is `largest` >= 0: 448 = 1.75 x 2^8.
-__host__ __device__ __forceinline__ int e4m3_scale_power(float largest) {
-#ifdef __CUDA_ARCH__
+__device__ __forceinline__ int e4m3_scale_power(float largest) {
     const unsigned bits = __float_as_uint(largest);
-#else
-    unsigned bits;
-    memcpy(&bits, &largest, 4);
-#endif
     const int power = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
     return power < -100 ? -100 : power;
 }
@@ -25,13 +18,14 @@ __device__ __forceinline__ float finite_size(float x) {
     const float a = fabsf(x);
     return a < INFINITY ? a : 0.f;
 }
-// Four codes, the first in the lowest byte. `inverse` is 1 / scale, exact.
+// Two codes, the first in the lower byte.
 __device__ __forceinline__ unsigned e4m3_pair(float lo, float hi) {
     unsigned short c;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
     return c;
 }
 __device__ __forceinline__ float or_nan(float x) { return fabsf(x) < INFINITY ? x : __uint_as_float(0x7FFFFFFFu); }
+// Four codes, the first in the lowest byte. `inverse` is 1 / scale, exact.
 __device__ __forceinline__ unsigned e4m3_codes(float a, float b, float c, float d, float inverse) {
     return e4m3_pair(or_nan(a * inverse), or_nan(b * inverse)) | e4m3_pair(or_nan(c * inverse), or_nan(d * inverse)) << 16;
 }
@@ -47,19 +41,7 @@ __device__ __forceinline__ float2 e4m3_float2(unsigned short pair) {
     asm("{.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;}" : "=f"(f.x), "=f"(f.y) : "r"(h));
     return f;
 }
-// Eight elements as 32-bit numbers; VEC: they lie in 16-byte pieces.
-template <typename T, bool VEC> __device__ __forceinline__ void load8(float (&v)[8], const T* p) {
-    if (VEC) {
-        Vec16<T> a, b;
-        a.load_cg(p);
-        if (Vec16<T>::N == 4) b.load_cg(p + 4);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < Vec16<T>::N ? a.v[i % Vec16<T>::N] : b.v[i % Vec16<T>::N];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(__ldcg(p + i));
-    }
-}
+// Eight elements as 32-bit numbers: the largest size and the codes.
 __device__ __forceinline__ float largest8(const float (&v)[8]) {
     float m = 0.f;
 #pragma unroll

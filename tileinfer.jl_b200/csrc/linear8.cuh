@@ -95,6 +95,19 @@ __device__ __forceinline__ void linear8_store(const Linear8& p, int t, int o, fl
     }
 }
 
+// Four sums at this place of the cluster's block `rank`, and a barrier of the cluster's blocks around such reads.
+__device__ __forceinline__ float4 rank_sums(const float* at, unsigned rank) {
+    unsigned a;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(at)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_meets() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
 // A launch in clusters of `cluster` blocks, as a programmatic dependent of the kernel before.
 template <typename... KArgs, typename... Args>
 inline void linear8_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, Args... args) {

@@ -30,17 +30,6 @@ struct Args {
 __device__ __forceinline__ void copy16(unsigned dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0));
 }
-__device__ __forceinline__ float4 cluster_read(const float* at, unsigned rank) {
-    unsigned a;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(at)), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
 // Bytes of shared memory: the warps' rings, codes [groups][N][128], factors [groups][N], sums [N][rows].
 int few_bytes(int groups, int warps) { return warps * AHEAD * UNIT + groups * N * (KB + 4) + N * 16 * warps * 4; }
 
@@ -199,17 +188,17 @@ __global__ void __launch_bounds__(32 * WARPS, 2) linear8_few_kernel(const Args a
             __syncwarp();
             continue;
         }
-        cluster_sync();                                      // one tile a cluster
+        cluster_meets();                                     // one tile a cluster
         for (int e = rank * threads + threadIdx.x; e < p.n * (ROWS / 4); e += a.split * threads) {
             float4 v[MAX_SPLIT];
 #pragma unroll
-            for (int r = 0; r < MAX_SPLIT; ++r) v[r] = r < a.split ? cluster_read(sums + 4 * e, r) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int r = 0; r < MAX_SPLIT; ++r) v[r] = r < a.split ? rank_sums(sums + 4 * e, r) : make_float4(0.f, 0.f, 0.f, 0.f);
             float4 s = v[0];
 #pragma unroll
             for (int r = 1; r < MAX_SPLIT; ++r) { s.x += v[r].x; s.y += v[r].y; s.z += v[r].z; s.w += v[r].w; }
             linear8_store(p, e / (ROWS / 4), tile * ROWS + e % (ROWS / 4) * 4, s, quads, y32);
         }
-        cluster_sync();                                      // the others may still read this block's sums
+        cluster_meets();                                     // the others may still read this block's sums
     }
 }
 

@@ -33,18 +33,6 @@ struct Args {
     int groups, row_tiles, split;
 };
 
-__device__ __forceinline__ float4 cluster_read(const float* at, unsigned rank) {
-    unsigned a;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(at)), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
-
 template <int N>
 __global__ void __launch_bounds__(THREADS, 2) linear8_mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Args a) {
     typedef Shape<N> S;
@@ -188,7 +176,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_mid_kernel(const __grid_co
     }
     pdl_wait();                                              // y may still be read by the kernel before
     if (__syncthreads_or(!ok)) drain_after_timeout();        // a wait ran out: let what is in flight land
-    if (a.split > 1) cluster_sync();
+    if (a.split > 1) cluster_meets();
     // Four rows of a token at a time; all ranks' sums are asked for together.
     const float* sums = reinterpret_cast<const float*>(tiles);
     const bool y32 = p.epilogue == L4_EPI_F32_OUT, whole = linear8_quads(p);
@@ -198,7 +186,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_mid_kernel(const __grid_co
         else {
             float4 v[MAX_SPLIT];
 #pragma unroll
-            for (int r = 0; r < MAX_SPLIT; ++r) v[r] = r < a.split ? cluster_read(sums + 4 * e, r) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int r = 0; r < MAX_SPLIT; ++r) v[r] = r < a.split ? rank_sums(sums + 4 * e, r) : make_float4(0.f, 0.f, 0.f, 0.f);
             s = v[0];
 #pragma unroll
             for (int r = 1; r < MAX_SPLIT; ++r) { s.x += v[r].x; s.y += v[r].y; s.z += v[r].z; s.w += v[r].w; }
@@ -206,7 +194,7 @@ __global__ void __launch_bounds__(THREADS, 2) linear8_mid_kernel(const __grid_co
         linear8_store(p, token0 + e / (ROWS / 4), tile * ROWS + e % (ROWS / 4) * 4, s, whole, y32);
     }
     tc_fence_before();
-    if (a.split > 1) cluster_sync(); else __syncthreads();   // the others may still read this block's sums
+    if (a.split > 1) cluster_meets(); else __syncthreads();  // the others may still read this block's sums
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, S::COLS);
