@@ -153,3 +153,20 @@ def test_writing_through_tables_of_any_pitch(ops, written):
     part = wide.cuda()[:, 2:2 + columns]
     dense = table.cuda()
     assert torch.equal(run(part, slots), run(dense, slots))
+
+
+def test_runs_longer_than_was_said(ops):
+    """``max_new`` says one: what a sequence of 60,000 new tokens gets is not defined, and its work is not counted beyond 32 bits; the others' results are right."""
+    nkv, dim, columns, many = 64, 16, 10000, 60000
+    c = make([(1, 300), (1, 70)], nkv, nkv, dim, seed=6)
+    want, bound = reference(c, dim ** -0.5, 0, 8)
+    table = torch.full((c["table"].shape[0], columns), -1, dtype=torch.int32)
+    table[:, :c["table"].shape[1]] = c["table"]
+    slots = torch.tensor([int(c["seq_slots"][0]), int(c["seq_slots"][1]), int(c["seq_slots"][1])], dtype=torch.int32)
+    q = torch.cat([c["q"], torch.zeros(many, nkv, dim, dtype=torch.bfloat16)]).cuda()
+    cu, lens = torch.tensor([0, 1, 2, 2 + many], dtype=torch.int32), torch.tensor([300, 70, columns * PAGE], dtype=torch.int32)
+    out = torch.full((2 + many + 10, nkv * dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.attention8(out[:2 + many], q, *(c[key].cuda() for key in ("k", "v", "ks", "vs")), table.cuda(), slots.cuda(), cu.cuda(), lens.cuda(), dim ** -0.5, nkv, nkv, dim, PAGE, 1)
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert bool(((out[:2].cpu().to(F64) - want).abs() <= bound).all()) and bool((out[-10:] == 7).all())

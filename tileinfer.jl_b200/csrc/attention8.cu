@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
             s_cu[b] = at;
             if (b == B - 1) s_cu[B] = end;
             s_len[b] = len;
-            const FewShape s = few_shape(end - at, len, a.window, group, M);
+            const FewShape s = few_shape(a.limits.run(end - at), len, a.window, group, M);
             v = (unsigned)(s.tiles * s.slabs * nkv);
         }
         const unsigned own = v;
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(A8_THREADS, Shape8<DP, NQ>::BLOCKS) attention8
             if (s_units[mid] <= u) x = mid; else z = mid;
         }
         p.b = x;
-        p.s = few_shape(s_cu[x + 1] - s_cu[x], s_len[x], a.window, group, M);
+        p.s = few_shape(a.limits.run(s_cu[x + 1] - s_cu[x]), s_len[x], a.window, group, M);
         const int v = (int)(u - s_units[x]), item = v / p.s.tiles;
         p.tile = v - item * p.s.tiles;
         p.kvh = item / p.s.slabs;
@@ -736,7 +736,7 @@ extern "C" int ti_attention8_table(void* out, const void* q, const void* k, cons
     if (int rc = ti_tensor_map_bf16(&c.k, k, 2, dims, strides, box, true)) return rc;
     if (int rc = ti_tensor_map_bf16(&c.v, v, 2, dims, strides, box, true)) return rc;
     const long long parts = 2LL * sm_blocks(eights, D) * ti_sm_count(), positions = (long long)columns * AF_PAGE;
-    const FewLimits limits = {n, positions < INT_MAX / 2 ? (int)positions : INT_MAX / 2};
+    const FewLimits limits = {n, max_new, positions < INT_MAX / 2 ? (int)positions : INT_MAX / 2};
     for (int b0 = 0; b0 < B; b0 += A8_MAX_SEQS) {            // the sequences in turns of as many as a launch takes
         c.a = Args8{(bf16*)out, (const bf16*)q, (const unsigned char*)v, k_scales, v_scales, table, table_stride, slots, columns, limits, seq_slots + b0, cu + b0, kv_lens + b0, (float*)ws,
                     (float*)ws + parts * M * D, status, scale * 1.4426950408889634f, B - b0 < A8_MAX_SEQS ? B - b0 : A8_MAX_SEQS, nq, nkv, D, window, pages};

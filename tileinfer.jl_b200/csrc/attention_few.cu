@@ -433,7 +433,7 @@ static int launch_few(bf16* out, const bf16* q, const bf16* k, const bf16* v, co
     ti_launch(attention_few_kernel<D, MT>, dim3(G), dim3(AF_THREADS), FewSmem<D>::BYTES, stream, map_k, map_v, out, q, k, v, table, table_stride, seq_slots, cu,
               kv_lens, ws_o, ws_ml, status, scale * 1.4426950408889634f, B, nq, nkv, window);
     if (int rc = ti_check_launch("attention_few")) return rc;
-    join_parts(out, cu, kv_lens, ws_o, ws_ml, B, nq, nkv, D, M, max_new, window, G, FewLimits{INT_MAX, INT_MAX}, stream);
+    join_parts(out, cu, kv_lens, ws_o, ws_ml, B, nq, nkv, D, M, max_new, window, G, FewLimits{INT_MAX, INT_MAX, INT_MAX}, stream);
     return ti_check_launch("attention_few_join");
 }
 

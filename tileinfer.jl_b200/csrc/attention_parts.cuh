@@ -11,9 +11,11 @@ namespace {
 struct FewShape {
     int T, L, first, t0, tiles, slabs;                       // new tokens, length, first visible key, first tile, tiles, slabs of rows
 };
-// What is given for a batch may be wrong: ranges stay within the n rows that there are, lengths within the positions that a sequence's row of the table has pages for.
+// What is given for a batch may be wrong: ranges stay within the rows that there are, runs within the most new tokens that were said (the units' number was checked with them),
+// lengths within the positions that a sequence's row of the table has pages for.
 struct FewLimits {
-    int rows, positions;
+    int rows, most_new, positions;
+    __device__ __forceinline__ int run(int T) const { return min(T, most_new); }
     __device__ __forceinline__ int row(int at) const { return min(max(at, 0), rows); }
     __device__ __forceinline__ int length(int len) const { return min(max(len, 0), positions); }
 };
@@ -55,7 +57,7 @@ __global__ void __launch_bounds__(32 * AF_JOIN_WARPS) attention_few_join_kernel(
     const int b = blockIdx.z, kvh = blockIdx.y, group = nq / nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned before = 0, U = 0;
     for (int c = threadIdx.x; c < B; c += 32 * AF_JOIN_WARPS) {
-        const FewShape s = few_shape(limits.row(__ldcg(cu + c + 1)) - limits.row(__ldcg(cu + c)), limits.length(__ldcg(kv_lens + c)), window, group, M);
+        const FewShape s = few_shape(limits.run(limits.row(__ldcg(cu + c + 1)) - limits.row(__ldcg(cu + c))), limits.length(__ldcg(kv_lens + c)), window, group, M);
         U += s.tiles * s.slabs * nkv;
         if (c < b) before += s.tiles * s.slabs * nkv;
     }
@@ -66,7 +68,7 @@ __global__ void __launch_bounds__(32 * AF_JOIN_WARPS) attention_few_join_kernel(
     before = U = 0;
 #pragma unroll
     for (int w = 0; w < AF_JOIN_WARPS; ++w) { before += s_sum[w][0]; U += s_sum[w][1]; }
-    const int first_token = limits.row(__ldcg(cu + b)), T = limits.row(__ldcg(cu + b + 1)) - first_token, row = blockIdx.x * (AF_JOIN_WARPS / WPR) + warp / WPR, mine = warp % WPR;
+    const int first_token = limits.row(__ldcg(cu + b)), T = limits.run(limits.row(__ldcg(cu + b + 1)) - first_token), row = blockIdx.x * (AF_JOIN_WARPS / WPR) + warp / WPR, mine = warp % WPR;
     const FewShape s = few_shape(T, limits.length(__ldcg(kv_lens + b)), window, group, M);
     const int i = row / group, slab = row / M, in = row - slab * M;
     const Runs runs(U, max(min((unsigned)blocks, U), 1u));
