@@ -8,9 +8,9 @@
 // length (attention_parts.cuh). A page's head is one tile, 64 x D consecutive bytes of keys and as many of values, which come as two TMA copies of
 // rows of 128 swizzled bytes, whatever D is. A warp asks for them and brings the scales; four others take 16 keys of a tile each, on their own.
 //
-// Measured, heads of 128: one row over 65,536 positions 31.7 us (134 MB, 20.5 at the rate of a copy; 131,072 more positions take 40.7 us more, 6.6 TB/s, so that 11 us
-// are launches, the first look-ups and reads, and the join); 64 sequences of 1,024 37.0 us (3.7 TB/s: the same, and 2,000 cycles a tile in each of three blocks an SM);
-// 40 rows over 8 of up to 32,768 137.5 us (2.0 TB/s): a tile's chain of MMAs, exponentials and MMAs with two warps a scheduler, and codes widened twice, for two slabs.
+// Measured, heads of 128: one row over 65,536 positions 31.4 us (134 MB, 20.5 at the rate of a copy; 131,072 more positions take 40.7 us more, 6.6 TB/s, so that 11 us
+// are launches, the first look-ups and reads, and the join); 64 sequences of 1,024 35.9 us (3.8 TB/s: the same, and 2,000 cycles a tile in each of three blocks an SM);
+// 40 rows over 8 of up to 32,768 139.8 us (2.0 TB/s): a tile's chain of MMAs, exponentials and MMAs with two warps a scheduler, and codes widened twice, for two slabs.
 //
 // Keys and values are the MMAs' rows, the queries their columns, eight at a time: S^T = K Q^T, O^T = V^T P^T, so that a code is widened once whatever the
 // number of queries, and eight or fewer cost eight. P^T's fragments are S^T's, turned by movmatrix.

@@ -11,7 +11,7 @@
 // written, so nothing starts until all stores have reached all (eight runs of up to 1,024 rows 10.2 -> 10.7 us, five rows of 64 sequences 5.4 -> 5.7; five rows of eight with their attention 35.4 -> 37.0).
 //
 // Bound by launch and three dependent reads (lengths, the page, its rows and old scale), so that blocks are small enough to come up at once where they are many:
-// one token of 64 sequences takes 3.8 us, eight runs of up to 1,024 rows 10.7 (8 heads of 128; 7.3 MB, 1.1 us at the rate of a copy).
+// one token of 64 sequences takes 3.6 us, eight runs of up to 1,024 rows 10.7 (8 heads of 128; 7.3 MB, 1.1 us at the rate of a copy).
 //
 // Widening, for kernels that read bfloat16: the pages that a step's tokens see become pages of bfloat16 in a pool of their own, page j of sequence b at
 // b x (pages a sequence) + j, with its block table. A code times a power of two is exact in bfloat16. Positions that nobody sees become zeros.

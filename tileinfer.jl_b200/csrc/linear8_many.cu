@@ -10,7 +10,7 @@
 // a step, the issuing warp took 620 cycles a group (waits 100; the next step's question, four MMAs and a commit 350; its loop), the adding warps 650. What had
 // taken the longest: a factor multiplied as soon as it was asked for (the adding warps waited for its loads; now a warp of its own brings factors), and waits for
 // barriers that were over long since, 300 cycles each beside the MMAs (now asked one step ahead). A commit frees the stage and gives the sums over at once.
-// 256 tokens of 4,096 x 21,504 69.6 -> 55.0 us, 2,048 of 21,504 x 4,096 221 -> 198 us, 1,820 TFLOP/s. Tiles of 256 x 256 took the same time for the same work,
+// 256 tokens of 4,096 x 21,504 69.6 -> 55.0 us, 2,048 of 21,504 x 4,096 221 -> 197 us (1,830 TFLOP/s; 230 us in a long loop, where the power limit lowers the clock). Tiles of 256 x 256 took the same time for the same work,
 // one group a step 59.3 us, sixteen adding warps 63.5.
 //
 // Block 0 of the pair issues the MMAs; its `full` barriers count the bytes of both blocks' loads; commits arrive on both blocks' barriers; the partner's

@@ -1402,8 +1402,8 @@ def attention8(out, q, k_cache, v_cache, k_scales, v_scales, block_table, seq_sl
     table's rows have pages for; a longer one counts as that).
 
     A page that does not exist, or whose slot does not, reads as zeros; of ranges beyond the n rows nothing is read or written; a sequence shorter than its new
-    tokens gets results that mean nothing. What no token sees may hold any codes; a NaN code that some see reaches those alone. Long runs go through pages widened
-    to bfloat16: codes times scales that are no powers of two are rounded to it, and a NaN value that some rows of a run see may reach others of the run; their q
+    tokens gets results that mean nothing. What no token sees may hold any codes; a NaN code that some see reaches those alone. Long runs (the sizes given
+    decide) go through pages widened to bfloat16: codes times scales that are no powers of two are rounded to it, softmax weights have its 8 bits where others have 11, and a NaN value that some rows of a run see may reach others of the run; their q
     and out must be 16-byte aligned (others' 4-byte).
 
     Lengths, ranges, slots, table, and the pages before those of the new tokens are read while the kernel ahead may still run: they come from ``cache_write8``,
